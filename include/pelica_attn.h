@@ -281,6 +281,154 @@ int pelica_attn_qkv_rope_cache(const PelicaAttnDesc* desc, const PelicaRope* rop
                                const float* q_norm, const float* k_norm, float eps,
                                uint16_t* k_cache, uint16_t* v_cache, void* stream);
 
+/* ---- serving many requests from a paged cache --------------------------- */
+/* No counterpart in the reference, whose engines serve one request from one
+ * linear or ring cache.  A pool of pages holds the rows of all requests; a
+ * step is: pages_release / pages_append (lengths -> pages, slots,
+ * positions), paged_plan (once), then for each layer paged_qkv and paged.
+ * Everything a step needs to know about lengths is read on the GPU, so a
+ * captured step replays with new lengths. */
+
+/* most sequences of one step (rows of the page table) */
+#define PELICA_ATTN_PAGED_MAX_SEQ 4096
+
+/* One step's page bookkeeping.  Request s has cached_len[s] rows in the
+ * pages page_table[s][0 .. ceil(cached_len[s] / page_size)) and gets
+ * new_len[s] more.  The free list is a queue: page number i (counting from
+ * the beginning of time) is free_list[i % n_pages], those from free_state[0]
+ * (pages taken so far) to free_state[1] (pages given so far) are free. */
+typedef struct PelicaPageDesc {
+    int32_t n_seq;       /* 1 .. PELICA_ATTN_PAGED_MAX_SEQ */
+    int32_t n_tokens;    /* rows of slots, positions and token_seq */
+    int32_t page_size;   /* rows per page: a power of two, 8 .. 65536 */
+    int32_t n_pages;     /* pages of the pool = entries of free_list */
+    int32_t max_pages;   /* columns of page_table */
+} PelicaPageDesc;
+
+/* status of a request after pages_append */
+#define PELICA_ATTN_PAGES_OK 0
+#define PELICA_ATTN_PAGES_NONE 1   /* not enough free pages */
+#define PELICA_ATTN_PAGES_TABLE 2  /* more pages than page_table has columns */
+#define PELICA_ATTN_PAGES_ROWS 3   /* its tokens pass n_tokens */
+#define PELICA_ATTN_PAGES_LENGTH 4 /* a negative length, or a sum past 2^31 - 1 */
+
+/* Takes free pages for every request's new tokens, in request order, and
+ * appends them to its row of page_table (entries of pages it had stay as they
+ * are).  Writes q_start[n_seq + 1] (first row of each request's new tokens,
+ * packed in request order; requests with a negative length count none, and
+ * no entry passes n_tokens), seq_kv_len[n_seq] = cached + new, per row the
+ * slot (page * page_size + row in it), the position and the request
+ * (slots[n_tokens], positions[n_tokens], token_seq[n_tokens]; rows behind
+ * the last request: -1, 0, -1), status[n_seq], and free_out[2].
+ * A request that cannot be served keeps its pages and takes none; its
+ * seq_kv_len is 0 (attention skips it) and its rows' slots are -1 (the qkv
+ * step skips them).  When pages run out, every later request that needs one
+ * gets PELICA_ATTN_PAGES_NONE.  A page id outside the pool, from the table
+ * or the list, gives slot -1.  free_out must not overlap free_in: workgroups
+ * read the one while another writes the other. */
+int pelica_attn_pages_append(const PelicaPageDesc* desc, const int32_t* cached_len, const int32_t* new_len,
+                             int32_t* page_table, const int32_t* free_list, const int64_t* free_in,
+                             int64_t* free_out, int32_t* q_start, int32_t* seq_kv_len, int64_t* slots,
+                             int32_t* positions, int32_t* token_seq, int32_t* status, void* stream);
+
+/* Gives the pages of every request with ended[s] != 0 back to the free list,
+ * in (request, page) order: entries page_table[s][0 .. ceil(cached_len[s] /
+ * page_size)), which must be pages of the pool.  The table is not changed
+ * (set the request's cached length to 0).  When the list would hold more
+ * than n_pages nothing is given back.  n_tokens of the descriptor is not
+ * used.  free_out must not overlap free_in. */
+int pelica_attn_pages_release(const PelicaPageDesc* desc, const int32_t* ended, const int32_t* cached_len,
+                              const int32_t* page_table, int32_t* free_list, const int64_t* free_in,
+                              int64_t* free_out, void* stream);
+
+/* Shape and addressing of one layer's attention over the pages.  Row r of
+ * page p holds kv head h's hd values at p * page_stride + r * row_stride + h *
+ * head_stride (f16 values; the same for k and v).  Request s has the query rows
+ * q_start[s] .. q_start[s + 1) of q and out, token t of its T at position
+ * len - T + t of its len = seq_kv_len[s] keys, key j in page
+ * page_table[s][j / page_size].  A token sees the keys j with
+ * pos - window < j <= pos (window 0: all j <= pos), and every j <
+ * prefix_len[s].  Only entries of pages that hold a key some token sees are
+ * read through; one that is no page of the pool there makes outputs of that
+ * request NaN. */
+typedef struct PelicaPagedDesc {
+    int32_t n_head, n_kv, hd;   /* n_head % n_kv == 0; hd 64 or 128 */
+    int32_t n_seq;              /* 1 .. PELICA_ATTN_PAGED_MAX_SEQ */
+    int32_t n_tokens;           /* rows of q and out */
+    int32_t max_q;              /* most new tokens of one request (a request with more is skipped) */
+    int32_t page_size;          /* a power of two, 8 .. 65536 */
+    int32_t n_pages;            /* pages of the pool */
+    int32_t max_pages;          /* columns of page_table */
+    int32_t window;             /* sliding window in keys, 0 = all */
+    const int32_t* q_start;     /* device [n_seq + 1] */
+    const int32_t* seq_kv_len;  /* device [n_seq]; a request with len < T, or more keys than its table's row, is skipped */
+    const int32_t* page_table;  /* device [n_seq][max_pages] */
+    const int32_t* prefix_len;  /* device [n_seq], or NULL: no prefix */
+    const float* alibi;         /* device [n_head], or NULL: the score gets - alibi[h] * |pos - j| */
+    int64_t page_stride;        /* 0 = page_size * row_stride */
+    int64_t row_stride;         /* 0 = n_kv * hd */
+    int64_t head_stride;        /* 0 = hd */
+    int64_t q_token_stride;     /* values between tokens of q; 0 = n_head * hd */
+    int64_t out_token_stride;   /* values between tokens of out; 0 = n_head * hd */
+    float scale;                /* 0 = 1/sqrt(hd) */
+    float softcap;              /* c > 0: scores c tanh(s / c) (ahead of the alibi term); 0 = none */
+} PelicaPagedDesc;
+
+/* The work list of a step's attention, made on the GPU from q_start,
+ * seq_kv_len and prefix_len: which query rows and key ranges each workgroup
+ * takes.  One plan serves every pelica_attn_paged call of the step whose
+ * descriptor has the same n_head, n_kv, hd, n_seq, n_tokens, max_q, page
+ * sizes and counts, window and (NULL or not) prefix_len; calls with another
+ * one write nothing.  Make it again when lengths change (the same buffer
+ * will do).  plan: 16-byte aligned, pelica_attn_paged_plan_bytes bytes (0 on
+ * an invalid descriptor). */
+size_t pelica_attn_paged_plan_bytes(const PelicaPagedDesc* desc);
+int pelica_attn_paged_plan(const PelicaPagedDesc* desc, void* plan, size_t plan_bytes, void* stream);
+
+/* Attention of each request's new tokens over its pages: f16 queries and
+ * output, or f32 (_f32), whose products keep f32's precision (queries and
+ * probabilities as f16 hi + lo parts).  Softmax and sums in f32.  sinks:
+ * [n_head] natural-log logits or NULL.  Rows of skipped requests and behind
+ * the last one are left as they were.  Workspace (partials of key ranges;
+ * pelica_attn_paged_workspace_bytes, 0 if none is needed): contents need no
+ * initialisation; calls that share one must be ordered on one stream, in
+ * captured graphs too. */
+size_t pelica_attn_paged_workspace_bytes(const PelicaPagedDesc* desc);
+int pelica_attn_paged(const PelicaPagedDesc* desc, const void* plan, const uint16_t* q, const uint16_t* k_pages,
+                      const uint16_t* v_pages, const float* sinks, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int pelica_attn_paged_f32(const PelicaPagedDesc* desc, const void* plan, const float* q, const uint16_t* k_pages,
+                          const uint16_t* v_pages, const float* sinks, float* out, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The step before attention over pages: n_tokens rows of q ([n_head][hd]
+ * f32), k and v ([n_kv][hd] f32), row i's heads at i * token_stride (0: dense
+ * per tensor).  Per-head RMS norm of q and k (when q_norm / k_norm are
+ * given), rotary embedding with one position per axis: pair j turns by
+ * positions[pair_axis[j]][i] (axis a's positions at positions + a *
+ * axis_stride; axis_stride 0: one for all).  q goes to q_out (f32, may be q;
+ * or f16 when q_half is set) at i * q_out_stride, k and v rows rounded to f16
+ * into row slots[i] of the pages.  Rows whose slot is negative or past the
+ * pool are skipped and write nothing.  A position outside the rotary table
+ * gives NaN.  Of the descriptor: n_head, n_kv, hd (64, 128, 256), n_tokens,
+ * page_size, n_pages and the three strides. */
+typedef struct PelicaPagedRope {
+    int32_t rot;            /* rotated dims at the start of each head: even, <= hd; 0 = no rope */
+    int32_t neox;           /* 1: pairs (j, j + rot/2); 0: pairs (2j, 2j + 1) */
+    int32_t table_split;    /* 0: row = position, or n > 0: the two-level table (PelicaRope) */
+    int32_t table_rows;     /* rows in table */
+    const float* table;     /* device [table_rows][rot/2][2] (cos, sin) */
+    int32_t n_axes;         /* 1 .. 4 */
+    const uint8_t* pair_axis;  /* HOST [rot/2] axis of each pair, or NULL: all 0 */
+    const int32_t* positions;  /* device [n_axes][n_tokens] */
+    int64_t axis_stride;    /* values between axes of positions; 0 = all axes share one */
+} PelicaPagedRope;
+
+int pelica_attn_paged_qkv(const PelicaPagedDesc* desc, const PelicaPagedRope* rope, const float* q, const float* k,
+                          const float* v, int64_t token_stride, const float* q_norm, const float* k_norm, float eps,
+                          const int64_t* slots, void* q_out, int32_t q_half, int64_t q_out_stride, uint16_t* k_pages,
+                          uint16_t* v_pages, void* stream);
+
 /* ---- per-kernel GPU timing ------------------------------------------- */
 
 /* kernel ids of PelicaAttnProfRecord */
@@ -289,6 +437,11 @@ int pelica_attn_qkv_rope_cache(const PelicaAttnDesc* desc, const PelicaRope* rop
 #define PELICA_ATTN_PROF_PREFILL 3
 #define PELICA_ATTN_PROF_MERGE 4
 #define PELICA_ATTN_PROF_QKV 5
+#define PELICA_ATTN_PROF_PAGES 6
+#define PELICA_ATTN_PROF_PAGED_PLAN 7
+#define PELICA_ATTN_PROF_PAGED 8
+#define PELICA_ATTN_PROF_PAGED_JOIN 9
+#define PELICA_ATTN_PROF_PAGED_QKV 10
 
 typedef struct PelicaAttnProfRecord {
     int32_t kernel; /* PELICA_ATTN_PROF_* */

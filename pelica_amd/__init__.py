@@ -3,7 +3,8 @@
 The compute lives in ``lib/libpelica_attn.so`` (HIP kernels for gfx950 behind
 the C ABI declared in ``include/pelica_attn.h``).  ``pelica_amd.attn`` is the
 host-side binding: it loads that library (failing loudly when it is missing)
-and exposes every entry point on torch device tensors.
+and exposes every entry point on torch device tensors; ``pelica_amd.paged``
+does so for the calls over a paged cache.
 """
 from .attn import (  # noqa: F401
     AttnDesc,
@@ -31,7 +32,9 @@ from .attn import (  # noqa: F401
     token_stride,
     workspace_bytes,
 )
+from . import paged  # noqa: F401
 
+# (of pelica_amd.attn; a paged cache's calls are pelica_amd.paged's)
 __all__ = [
     "AttnDesc",
     "AttnError",

@@ -48,12 +48,21 @@ EXPORTS = (
     "pelica_attn_partials_merge",
     "pelica_attn_partials_merge_batch",
     "pelica_attn_qkv_rope_cache",
+    "pelica_attn_pages_append",
+    "pelica_attn_pages_release",
+    "pelica_attn_paged_plan_bytes",
+    "pelica_attn_paged_plan",
+    "pelica_attn_paged_workspace_bytes",
+    "pelica_attn_paged",
+    "pelica_attn_paged_f32",
+    "pelica_attn_paged_qkv",
     "pelica_attn_prof_enable",
     "pelica_attn_prof_read",
 )
 
 #: kernel ids of the per-kernel timing records
-PROF_KERNELS = {1: "decode_split", 2: "decode_combine", 3: "prefill", 4: "partials_merge", 5: "qkv_rope_cache"}
+PROF_KERNELS = {1: "decode_split", 2: "decode_combine", 3: "prefill", 4: "partials_merge", 5: "qkv_rope_cache",
+                6: "pages", 7: "paged_plan", 8: "paged", 9: "paged_join", 10: "paged_qkv"}
 
 
 class AttnError(RuntimeError):
@@ -124,6 +133,41 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PageDesc(ctypes.Structure):
+    """``PelicaPageDesc`` (field meanings in include/pelica_attn.h)."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_seq", "n_tokens", "page_size", "n_pages", "max_pages")]
+
+
+class PagedDesc(ctypes.Structure):
+    """``PelicaPagedDesc`` (field meanings in include/pelica_attn.h)."""
+
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("n_head", "n_kv", "hd", "n_seq", "n_tokens", "max_q", "page_size", "n_pages",
+                                       "max_pages", "window")]
+        + [(n, ctypes.c_void_p) for n in ("q_start", "seq_kv_len", "page_table", "prefix_len", "alibi")]
+        + [(n, ctypes.c_int64) for n in ("page_stride", "row_stride", "head_stride", "q_token_stride",
+                                         "out_token_stride")]
+        + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+    )
+
+
+class PagedRope(ctypes.Structure):
+    """``PelicaPagedRope`` (field meanings in include/pelica_attn.h)."""
+
+    _fields_ = [
+        ("rot", ctypes.c_int32),
+        ("neox", ctypes.c_int32),
+        ("table_split", ctypes.c_int32),
+        ("table_rows", ctypes.c_int32),
+        ("table", ctypes.c_void_p),
+        ("n_axes", ctypes.c_int32),
+        ("pair_axis", ctypes.c_char_p),
+        ("positions", ctypes.c_void_p),
+        ("axis_stride", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -183,6 +227,23 @@ def load_library() -> ctypes.CDLL:
     lib.pelica_attn_partials_merge.argtypes = [i32, i32, i32, vp, vp, vp, vp]
     lib.pelica_attn_partials_merge_batch.restype = ctypes.c_int
     lib.pelica_attn_partials_merge_batch.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp]
+    pd, gd = ctypes.POINTER(PageDesc), ctypes.POINTER(PagedDesc)
+    lib.pelica_attn_pages_append.restype = ctypes.c_int
+    lib.pelica_attn_pages_append.argtypes = [pd] + [vp] * 13
+    lib.pelica_attn_pages_release.restype = ctypes.c_int
+    lib.pelica_attn_pages_release.argtypes = [pd] + [vp] * 7
+    lib.pelica_attn_paged_plan_bytes.restype = sz
+    lib.pelica_attn_paged_plan_bytes.argtypes = [gd]
+    lib.pelica_attn_paged_plan.restype = ctypes.c_int
+    lib.pelica_attn_paged_plan.argtypes = [gd, vp, sz, vp]
+    lib.pelica_attn_paged_workspace_bytes.restype = sz
+    lib.pelica_attn_paged_workspace_bytes.argtypes = [gd]
+    for fn in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
+        fn.restype = ctypes.c_int
+        fn.argtypes = [gd, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.pelica_attn_paged_qkv.restype = ctypes.c_int
+    lib.pelica_attn_paged_qkv.argtypes = [gd, ctypes.POINTER(PagedRope), vp, vp, vp, ctypes.c_int64, vp, vp,
+                                          ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
     lib.pelica_attn_prof_enable.restype = ctypes.c_int
     lib.pelica_attn_prof_enable.argtypes = [ctypes.c_int]
     lib.pelica_attn_prof_read.restype = ctypes.c_int

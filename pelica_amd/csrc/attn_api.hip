@@ -10,6 +10,7 @@
 
 #include "../../include/pelica_attn.h"
 #include "attn_decode.hpp"
+#include "attn_error.hpp"
 #include "attn_merge.hpp"
 #include "attn_prefill.hpp"
 #include "attn_qkv.hpp"
@@ -19,6 +20,12 @@ namespace {
 
 thread_local char g_err[512] = "";
 
+}  // namespace
+
+namespace pelica {
+
+void clear_error() { g_err[0] = 0; }
+
 int fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
@@ -26,6 +33,12 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+
+}  // namespace pelica
+
+namespace {
+
+using pelica::fail;
 
 int env_int(const char* name, int dflt) {
     const char* s = getenv(name);

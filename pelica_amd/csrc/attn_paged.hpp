@@ -1,0 +1,74 @@
+// Launch parameters of the paged kernels (attn_pages.hip, attn_paged.hip,
+// attn_paged_qkv.hip).
+#pragma once
+#include "attn_common.hpp"
+#include "attn_paged_plan.hpp"
+
+namespace pelica {
+
+constexpr int kPagedMaxSeq = 4096;
+
+struct PagesParams {
+    const int32_t *cached, *fresh, *ended;
+    const int64_t* free_in;
+    int64_t* free_out;
+    int32_t *table, *list, *q_start, *kv_len, *positions, *token_seq, *status;
+    int64_t* slots;
+    int n_seq, n_tokens, page_log2, n_pages, max_pages;
+};
+hipError_t launch_pages_append(const PagesParams& p, hipStream_t st);
+hipError_t launch_pages_release(const PagesParams& p, hipStream_t st);
+
+struct PlanParams {
+    const int32_t *q_start, *kv_len, *prefix;
+    PlanHeader* head;
+    PlanJoin* joins;
+    PlanPiece* pieces;
+    int n_seq, n_tokens, max_q, hpk, hd, window, fill;
+    int64_t max_keys;
+    int max_joins, max_pieces;
+    bool split;  // no: every item is one piece
+    uint32_t sig;
+};
+hipError_t launch_paged_plan(const PlanParams& p, hipStream_t st);
+
+struct PagedParams {
+    const void* q;
+    const uint16_t *k, *v;
+    const PlanHeader* head;
+    const PlanPiece* pieces;
+    const int32_t* table;
+    const float *sinks, *alibi;
+    void* out;
+    float* ws_ml;               // [slot][n_kv][rows] x (max, sum), base-2 max
+    float* ws_o;                // [slot][n_kv][rows][hd]
+    const PlanJoin* joins;
+    int64_t page_b, head_b;     // bytes between pages, between kv heads of a row
+    int64_t q_tok, o_tok;       // values between tokens
+    uint32_t row_b, sig;        // bytes between rows of a page
+    int n_kv, hpk, n_pages, max_pages, page_log2, window, rows;
+    float qscale, cap;          // scale * log2 e; softcap (0: none)
+    // host side only
+    int hd, max_pieces, max_joins;
+    bool f32, wide;
+};
+hipError_t launch_paged(const PagedParams& p, hipStream_t st);
+hipError_t launch_paged_join(const PagedParams& p, hipStream_t st);
+
+struct PagedQkvParams {
+    const float *q, *k, *v, *q_norm, *k_norm, *table;
+    const int64_t* slots;
+    const int32_t* positions;
+    void* q_out;
+    uint16_t *k_pages, *v_pages;
+    int64_t tok_q, tok_kv, tok_o, axis_stride;
+    int64_t page_stride, row_stride, head_stride, n_slots;
+    int n_head, n_kv, n_tokens, rot, neox, table_split, covered, page_log2, n_axes;
+    float eps;
+    uint32_t axis[8];  // 2 bits a pair
+    int hd;            // host side only
+    bool half;
+};
+hipError_t launch_paged_qkv(const PagedQkvParams& p, hipStream_t st);
+
+}  // namespace pelica

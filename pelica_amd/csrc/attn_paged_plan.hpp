@@ -1,0 +1,110 @@
+// Plain arithmetic of the paged kernels, the same lines in the library, in its
+// kernels and in a host test: which keys a block of query rows walks, which rows
+// of a cache page a load may touch, how the work list is cut.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#ifdef __HIPCC__
+#define PELICA_HD __host__ __device__ __forceinline__
+#else
+#define PELICA_HD inline
+#endif
+
+namespace pelica {
+
+// Query rows of a request are (token, head of the kv head's group) pairs,
+// row = token * hpk + head.  A request of at most kNarrowRows rows is one item
+// whose four waves share the keys (narrow); others are cut into items of
+// wide_rows rows whose waves share the rows (wide).
+constexpr int kNarrowRows = 32;
+PELICA_HD constexpr int wide_rows(int hd) { return hd == 64 ? 256 : 128; }
+
+// The least cost of a piece of an item, in chunks a narrow workgroup walks
+// (32 keys a wave each); a wide workgroup's chunk counts kWideCost of them.
+constexpr int kWideCost = 4;
+constexpr int kMinPiece = 4;
+
+// 32-key chunks of the keys that any row of an item sees: its window's and
+// the causal ones [lo, kend), and the prefix's [0, pe).  Chunks count from
+// key 0 over the prefix, then (where a gap of whole chunks lies between) from
+// chunk n_pre at key lo_base.
+struct ItemKeys {
+    int n_pre, lo_base, n_chunks;
+    int lo, kend, pe;
+};
+
+PELICA_HD int imin(int a, int b) { return a < b ? a : b; }
+PELICA_HD int imax(int a, int b) { return a > b ? a : b; }
+
+// positions [pos_first, pos_last] of a request of len keys
+PELICA_HD ItemKeys item_keys(int pos_first, int pos_last, int len, int window, int prefix) {
+    ItemKeys k;
+    k.pe = imax(0, imin(prefix, len));
+    k.kend = pos_last + 1;
+    k.lo = window > 0 && pos_first >= window ? pos_first - window + 1 : 0;
+    const int lo32 = k.lo & ~31;
+    const int pre = (int)(((unsigned)k.pe + 31u) >> 5);
+    if (k.pe > 0 && pre < (lo32 >> 5)) {
+        k.n_pre = pre;
+        k.lo_base = lo32;
+        k.n_chunks = pre + (int)(((unsigned)(k.kend - lo32) + 31u) >> 5);
+    } else {
+        k.n_pre = 0;
+        k.lo_base = k.pe > 0 ? 0 : lo32;
+        k.n_chunks = (int)(((unsigned)(imax(k.kend, k.pe) - k.lo_base) + 31u) >> 5);
+    }
+    return k;
+}
+
+// first key of chunk c
+PELICA_HD int chunk_key(int c, int n_pre, int lo_base) { return c < n_pre ? 32 * c : lo_base + 32 * (c - n_pre); }
+
+// Of n consecutive keys from kg (all in one page), the rows [first, first +
+// count) that some row of the item may see: a load touches no others (they may
+// lie in a page that was given away, or hold anything).
+PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, int& count) {
+    const int a = imin(imax(pe - kg, 0), n);                         // of the prefix: [0, a)
+    const int b0 = imin(imax(lo - kg, 0), n), b1 = imin(imax(kend - kg, 0), n);
+    first = a > 0 ? 0 : b0;
+    const int end = b1 > b0 ? imax(a, b1) : a;
+    count = imax(end - first, 0);
+}
+
+// Pieces of an item of `cost` under the piece limit L (kMinPiece .. )
+PELICA_HD int item_pieces(int cost, int n_chunks, int L) {
+    const int k = (int)(((int64_t)cost + L - 1) / L);
+    return imax(1, imin(k, n_chunks));
+}
+
+// most items of a step: one for each request with tokens, and one for each
+// whole block of wide_rows rows
+inline int64_t plan_items(int64_t n_seq, int64_t n_tokens, int hpk, int hd) {
+    return (n_seq < n_tokens ? n_seq : n_tokens) + n_tokens * hpk / wide_rows(hd);
+}
+// pieces (per kv head) that fill the chip once: two workgroups a CU
+inline int plan_fill(int n_kv, int cus) {
+    const int n = (2 * cus + n_kv - 1) / n_kv;
+    return n < 1024 ? n : 1024;  // (the plan kernel holds one item a thread)
+}
+// most pieces: `fill` while the items are no more than that, else the items
+// and at most `fill` more
+inline int64_t plan_pieces(int64_t items, int fill) { return items <= fill ? fill : items + fill; }
+
+// the plan buffer: header, joins, pieces
+struct PlanHeader {
+    uint32_t sig;
+    int n_pieces, n_joins, pad[13];
+};
+struct PlanPiece {
+    int seq, q0, R, r0;        // request, its first row of q, its query rows, the item's first
+    int pos0, len, cb, ce;     // position of its first token, its keys; chunks [cb, ce)
+    int slot, n_pre, lo_base;  // partial slot, or -1: the item's only piece
+    int lo, kend, pe, pad[2];
+};
+struct PlanJoin {
+    int q0, R, r0, slot0, n_slots, pad[3];
+};
+static_assert(sizeof(PlanHeader) == 64 && sizeof(PlanPiece) == 64 && sizeof(PlanJoin) == 32, "plan layout");
+
+}  // namespace pelica

@@ -8,7 +8,10 @@
 
 namespace pelica {
 
-enum ProfKernel { kProfDecodeSplit = 1, kProfDecodeCombine = 2, kProfPrefill = 3, kProfMerge = 4, kProfQkv = 5 };
+enum ProfKernel {
+    kProfDecodeSplit = 1, kProfDecodeCombine = 2, kProfPrefill = 3, kProfMerge = 4, kProfQkv = 5,
+    kProfPages = 6, kProfPagedPlan = 7, kProfPaged = 8, kProfPagedJoin = 9, kProfPagedQkv = 10
+};
 
 bool prof_enabled();
 // opens a record (start event) for `kind` on `st`; returns a handle or -1

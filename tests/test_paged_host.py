@@ -1,0 +1,241 @@
+"""The paged calls without a GPU: the ctypes mirrors, the refusals of the C entry
+points and of the binding, and the address rules of the kernels walked key by key."""
+import ctypes
+import os
+import random
+import subprocess
+
+import pytest
+import torch
+
+from pelica_amd import attn, paged
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("name,cls", [("PelicaPageDesc", attn.PageDesc), ("PelicaPagedDesc", attn.PagedDesc),
+                                      ("PelicaPagedRope", attn.PagedRope)])
+def test_struct_layouts(name, cls, tmp_path):
+    src = tmp_path / "layout.c"
+    body = "".join(f'printf("{f} %zu\\n", offsetof({name}, {f}));\n' for f, _ in cls._fields_)
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "pelica_attn.h"\nint main(void) {\n' + body
+                   + f'printf("size %zu\\n", sizeof({name}));\nreturn 0;\n}}\n')
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)], check=True)
+    out = dict(x.split() for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines())
+    assert int(out["size"]) == ctypes.sizeof(cls)
+    for f, _ in cls._fields_:
+        assert int(out[f]) == getattr(cls, f).offset, f
+
+
+def test_constants_match_the_header():
+    text = open(os.path.join(ROOT, "include", "pelica_attn.h")).read()
+    assert f"#define PELICA_ATTN_PAGED_MAX_SEQ {paged.MAX_SEQ}\n" in text
+    for i, n in enumerate(("OK", "NONE", "TABLE", "ROWS", "LENGTH")):
+        assert f"#define PELICA_ATTN_PAGES_{n} {i}" in text
+
+
+A = 64  # an address that is aligned for everything and never read: the calls below end before a launch
+
+
+def _desc(**kw):
+    d = dict(n_head=8, n_kv=2, hd=64, n_seq=4, n_tokens=16, max_q=4, page_size=16, n_pages=100, max_pages=10, window=0,
+             q_start=A, seq_kv_len=A, page_table=A)
+    d.update(kw)
+    return attn.PagedDesc(**d)
+
+
+def _error(rc, code, word):
+    text = attn.load_library().pelica_attn_last_error().decode()
+    assert rc == code and word in text, (rc, text)
+
+
+BAD = [
+    (dict(n_kv=3), attn.EINVAL, "n_head"), (dict(n_head=0), attn.EINVAL, "n_head"), (dict(n_kv=-1), attn.EINVAL, "n_head"),
+    (dict(hd=96), attn.EUNSUPPORTED, "hd"), (dict(n_seq=0), attn.EINVAL, "n_seq"), (dict(n_seq=4097), attn.EINVAL, "n_seq"),
+    (dict(n_tokens=0), attn.EINVAL, "n_tokens"), (dict(n_tokens=(1 << 20) + 1), attn.EINVAL, "n_tokens"),
+    (dict(max_q=0), attn.EINVAL, "max_q"), (dict(max_q=17), attn.EINVAL, "max_q"),
+    (dict(page_size=4), attn.EUNSUPPORTED, "page_size"), (dict(page_size=24), attn.EUNSUPPORTED, "page_size"),
+    (dict(page_size=1 << 17), attn.EUNSUPPORTED, "page_size"), (dict(page_size=0), attn.EUNSUPPORTED, "page_size"),
+    (dict(page_size=-16), attn.EUNSUPPORTED, "page_size"),
+    (dict(n_pages=0), attn.EINVAL, "n_pages"), (dict(max_pages=0), attn.EINVAL, "max_pages"),
+    (dict(max_pages=(1 << 26) + 1), attn.EINVAL, "max_pages"), (dict(window=-1), attn.EINVAL, "window"),
+    (dict(scale=-1.0), attn.EINVAL, "scale"), (dict(scale=float("nan")), attn.EINVAL, "scale"),
+    (dict(scale=float("inf")), attn.EINVAL, "scale"), (dict(softcap=-1.0), attn.EINVAL, "softcap"),
+    (dict(softcap=float("nan")), attn.EINVAL, "softcap"), (dict(row_stride=60), attn.EINVAL, "strides"),
+    (dict(row_stride=132), attn.EINVAL, "strides"), (dict(head_stride=4), attn.EINVAL, "strides"),
+    (dict(page_stride=-8), attn.EINVAL, "strides"), (dict(row_stride=1 << 24), attn.EUNSUPPORTED, "strides"),
+    (dict(q_start=None), attn.EINVAL, "NULL"), (dict(seq_kv_len=None), attn.EINVAL, "NULL"),
+    (dict(page_table=None), attn.EINVAL, "NULL"),
+]
+
+
+@pytest.mark.parametrize("kw,code,word", BAD, ids=[str(b[0]) for b in BAD])
+def test_bad_descriptors(kw, code, word):
+    lib, d = attn.load_library(), _desc(**kw)
+    assert lib.pelica_attn_paged_plan_bytes(ctypes.byref(d)) == 0
+    assert word in lib.pelica_attn_last_error().decode()
+    assert lib.pelica_attn_paged_workspace_bytes(ctypes.byref(d)) == 0
+    _error(lib.pelica_attn_paged_plan(ctypes.byref(d), A, 1 << 30, None), code, word)
+    for f in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
+        _error(f(ctypes.byref(d), A, A, A, A, None, A, A, 1 << 40, None), code, word)
+
+
+def test_null_and_misaligned_arguments():
+    lib, d = attn.load_library(), _desc(max_q=16)
+    ref = ctypes.byref(d)
+    need = lib.pelica_attn_paged_plan_bytes(ref)
+    _error(lib.pelica_attn_paged_plan(ref, None, need, None), attn.EINVAL, "plan")
+    _error(lib.pelica_attn_paged_plan(ref, A + 4, need, None), attn.EINVAL, "plan")
+    _error(lib.pelica_attn_paged_plan(ref, A, need - 1, None), attn.EWORKSPACE, "plan")
+    _error(lib.pelica_attn_paged_plan(None, A, need, None), attn.EINVAL, "desc")
+    ws = lib.pelica_attn_paged_workspace_bytes(ref)
+    assert ws > 0
+    good = [A, A, A, A, None, A, A, ws, None]
+    for f in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
+        for i in (0, 1, 2, 3, 5):
+            _error(f(ref, *[None if j == i else x for j, x in enumerate(good)]), attn.EINVAL, "NULL")
+            _error(f(ref, *[A + 8 if j == i else x for j, x in enumerate(good)]), attn.EINVAL, "aligned")
+        _error(f(ref, *[None if j == 6 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
+        _error(f(ref, *[ws - 1 if j == 7 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
+    for kw in (dict(q_token_stride=8), dict(out_token_stride=511), dict(q_token_stride=516), dict(out_token_stride=1 << 31)):
+        d = _desc(max_q=16, **kw)
+        _error(lib.pelica_attn_paged(ctypes.byref(d), *good), attn.EINVAL, "stride")
+
+
+def test_pages_arguments():
+    lib = attn.load_library()
+    good = attn.PageDesc(4, 16, 16, 100, 10)
+    args = [A, A, A, A, 128, 256, A, A, A, A, A, A, None]
+    for i in range(12):
+        _error(lib.pelica_attn_pages_append(ctypes.byref(good), *[None if j == i else x for j, x in enumerate(args)]),
+               attn.EINVAL, "NULL")
+        _error(lib.pelica_attn_pages_append(ctypes.byref(good), *[x + 2 if j == i else x for j, x in enumerate(args)]),
+               attn.EINVAL, "aligned")
+    for out in (120, 128, 136):
+        _error(lib.pelica_attn_pages_append(ctypes.byref(good), *[out if j == 5 else x for j, x in enumerate(args)]),
+               attn.EINVAL, "overlaps")
+    rel = [A, A, A, A, 128, 256, None]
+    for i in range(6):
+        _error(lib.pelica_attn_pages_release(ctypes.byref(good), *[None if j == i else x for j, x in enumerate(rel)]),
+               attn.EINVAL, "NULL")
+    _error(lib.pelica_attn_pages_release(ctypes.byref(good), A, A, A, A, 128, 128, None), attn.EINVAL, "overlaps")
+    for bad, code, word in (((0, 16, 16, 100, 10), attn.EINVAL, "n_seq"), ((4097, 16, 16, 100, 10), attn.EINVAL, "n_seq"),
+                            ((4, 16, 12, 100, 10), attn.EUNSUPPORTED, "page_size"),
+                            ((4, 16, 16, 0, 10), attn.EINVAL, "n_pages"), ((4, 16, 16, 100, 0), attn.EINVAL, "max_pages")):
+        d = attn.PageDesc(*bad)
+        _error(lib.pelica_attn_pages_append(ctypes.byref(d), *args), code, word)
+        _error(lib.pelica_attn_pages_release(ctypes.byref(d), *rel), code, word)
+    for n in (0, (1 << 20) + 1):
+        d = attn.PageDesc(4, n, 16, 100, 10)
+        _error(lib.pelica_attn_pages_append(ctypes.byref(d), *args), attn.EINVAL, "n_tokens")
+
+
+def test_qkv_arguments():
+    lib = attn.load_library()
+    args = [A, A, A, 0, None, None, 1e-6, A, 128, 0, 0, A, A, None]
+
+    def call(d=None, rope=None, **at):
+        d = d or _desc(hd=128)
+        a = [at.get(f"a{i}", x) for i, x in enumerate(args)]
+        return lib.pelica_attn_paged_qkv(ctypes.byref(d), None if rope is None else ctypes.byref(rope), *a)
+
+    for i in (0, 1, 2, 7, 8, 11, 12):
+        _error(call(**{f"a{i}": None}), attn.EINVAL, "NULL")
+        _error(call(**{f"a{i}": A + 4}), attn.EINVAL, "aligned")
+    _error(call(a4=A + 8), attn.EINVAL, "aligned")
+    _error(call(a3=100), attn.EINVAL, "token_stride")
+    _error(call(a3=1026), attn.EINVAL, "token_stride")
+    _error(call(a10=1000), attn.EINVAL, "q_out_stride")
+    _error(call(a8=A, a9=1), attn.EINVAL, "q_out")
+    _error(call(a6=float("nan")), attn.EINVAL, "eps")
+    _error(call(_desc(hd=96)), attn.EUNSUPPORTED, "hd")
+    _error(call(_desc(hd=128, page_size=7)), attn.EUNSUPPORTED, "page_size")
+    _error(call(_desc(hd=128, n_tokens=0)), attn.EINVAL, "n_tokens")
+    pair = bytes([0] * 63 + [3])
+    base = dict(rot=128, neox=1, table_split=0, table_rows=100, table=A, n_axes=3, pair_axis=None, positions=A,
+                axis_stride=16)
+    for kw, word in ((dict(rot=7), "rot"), (dict(rot=130), "rot"), (dict(rot=-2), "rot"), (dict(table=None), "table"),
+                     (dict(table=A + 4), "table"), (dict(table_rows=0), "table"), (dict(table_split=10), "two-level"),
+                     (dict(n_axes=0), "n_axes"), (dict(n_axes=5), "n_axes"), (dict(positions=None), "positions"),
+                     (dict(axis_stride=15), "axis_stride"), (dict(pair_axis=pair), "axis 3")):
+        _error(call(rope=attn.PagedRope(**{**base, **kw})), attn.EINVAL, word)
+
+
+def test_the_binding_refuses_cpu_tensors_and_wrong_types():
+    i = torch.zeros(4, dtype=torch.int32)
+    for f in (lambda: paged.pages_append(i, i, i.view(2, 2), i, torch.zeros(2, dtype=torch.int64), page_size=16, step=None),
+              lambda: paged.PagedPlan(i, i, i.view(2, 2), n_head=1, n_kv=1, hd=64, page_size=16, n_pages=4, n_tokens=4, max_q=1),
+              lambda: paged.paged_qkv(*[torch.zeros(1, 1, 64)] * 3, i, i, i)):
+        with pytest.raises(attn.AttnError) as e:
+            f()
+        assert e.value.code == attn.EINVAL
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    so = tmp_path_factory.mktemp("plan") / "plan.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-o", str(so),
+                    os.path.join(ROOT, "tests", "paged_plan_shim.cpp")], check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.plan_items_of.restype = ctypes.c_int64
+    lib.plan_items_of.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+    return lib
+
+
+def _seen(pos, window, pe):
+    lo = pos - window + 1 if window and pos >= window else 0
+    return set(range(lo, pos + 1)) | set(range(pe))
+
+
+def test_an_items_chunks_hold_every_key_its_rows_see_once(rules):
+    r = random.Random(1)
+    out6, out2 = (ctypes.c_int * 6)(), (ctypes.c_int * 2)()
+    for _ in range(3000):
+        length = r.randint(1, 700)
+        first = r.randint(0, length - 1)
+        last = r.randint(first, min(length - 1, first + r.choice((0, 3, 40))))
+        window = r.choice((0, 0, 1, 5, 32, 64, 300))
+        prefix = r.choice((0, 0, 1, 31, 32, 33, 200, 1000))
+        rules.item_keys_of(first, last, length, window, prefix, out6)
+        n_pre, lo_base, n_chunks, lo, kend, pe = out6
+        assert pe == min(prefix, length) and kend == last + 1
+        want = set().union(*(_seen(p, window, pe) for p in range(first, last + 1)))
+        got = []
+        for c in range(n_chunks):
+            key = rules.chunk_key_of(c, n_pre, lo_base)
+            assert key % 32 == 0
+            for n in (4, 8):  # rows of a load at head dim 128, 64
+                touched = []
+                for kg in range(key, key + 32, n):
+                    rules.group_rows_of(kg, n, lo, kend, pe, out2)
+                    f, cnt = out2
+                    assert 0 <= f and f + cnt <= n
+                    rows = list(range(kg + f, kg + f + cnt))
+                    # every wanted row, none past the request's keys, and what lies between the prefix
+                    # and the window within one group (of one page) only
+                    assert set(range(kg, kg + n)) & want <= set(rows)
+                    assert all(x in want or (kg <= pe - 1 < kg + n and x < kend) for x in rows)
+                    assert not rows or rows[-1] < max(kend, pe)
+                    touched += rows
+            got += [x for x in touched if x in want]
+        assert len(got) == len(set(got)) and set(got) == want
+
+
+def test_pieces_of_an_item(rules):
+    for cost, chunks, L in ((1, 1, 4), (4, 4, 4), (5, 5, 4), (400, 100, 4), (400, 100, 37), (7, 7, 1 << 30)):
+        k = rules.item_pieces_of(cost, chunks, L)
+        assert 1 <= k <= chunks and (k == chunks or k * L >= cost)
+        cuts = [chunks * i // k for i in range(k + 1)]
+        assert cuts[0] == 0 and cuts[-1] == chunks and all(a < b for a, b in zip(cuts, cuts[1:]))
+
+
+def test_the_bound_on_items_holds(rules):
+    r = random.Random(2)
+    for _ in range(500):
+        hpk, hd = r.choice((1, 2, 3, 8, 16, 71)), r.choice((64, 128))
+        new = [r.choice((0, 1, 2, 5, 40, 300)) for _ in range(r.randint(1, 40))]
+        W = 256 if hd == 64 else 128
+        items = sum(1 if n * hpk <= 32 else -(-n * hpk // W) for n in new if n)
+        if sum(new):
+            assert items <= rules.plan_items_of(len(new), sum(new), hpk, hd)
