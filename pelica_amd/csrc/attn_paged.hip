@@ -27,6 +27,7 @@
 // see: what lies behind is not touched and reads as zeros.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "attn_paged.hpp"
 #include "attn_prof.hpp"
@@ -36,6 +37,7 @@ namespace pelica {
 namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 
 constexpr int kNW = 4;  // waves of a workgroup
 constexpr int kBufFlags = 0x00020000;  // 32-bit raw buffer
@@ -64,6 +66,16 @@ __device__ __forceinline__ int v_slot(int k, int p) {
     return k * (HD * 2) + ((p ^ ((k & 3) << 1)) << 4);
 }
 
+// f(0) .. f(N - 1), the indexes as types
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled_(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    unrolled_(f, std::make_integer_sequence<int, N>{});
+}
+
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -79,11 +91,151 @@ __device__ __forceinline__ void lds_done() {
     __asm__ volatile("" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t lds_byte(const char* p) {
+    return (uint32_t)(size_t)(__attribute__((address_space(3))) const char*)p;
+}
+
 // a table entry as a scalar load
 __device__ __forceinline__ int table_entry(const int32_t* t, size_t i) {
     typedef const __attribute__((address_space(4))) int32_t* cptr;
     return *(cptr)(reinterpret_cast<uintptr_t>(t + i));
 }
+
+// V^T of 16 keys from row `key` of a tile, dims 32 dt .. + 31, as the A operand
+// of the PV product: lanes of 16-lane group G read keys 4 h2 + r4 (+ 8) at dims
+// 16 (G & 1) + 4 q4, and the read transposes
+template <int HD>
+__device__ __forceinline__ half8 v_operand(const char* vt, int key, int dt, int lane) {
+    const int G = lane >> 4, r4 = (lane & 15) >> 2, q4 = lane & 3;
+    const int k = key + 4 * (lane >> 5) + r4, dim = 32 * dt + 16 * (G & 1) + 4 * q4;
+    const _Float16* a0 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(k, dim >> 3) + ((dim & 7) << 1));
+    const _Float16* a1 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(k + 8, dim >> 3) + ((dim & 7) << 1));
+    return cat8(lds_read_tr(a0), lds_read_tr(a1));
+}
+
+// A chunk that some rows see in part may hold infinities or NaN in rows of V
+// that they do not see, and 0 times those is NaN.  Where it does, they are
+// taken out of the tile (clean_chunk: whether any were there) and added after
+// the last chunk to the rows that see them (add_special).  The waves of a wide
+// workgroup may clean a chunk at once: each has written zeros over what it
+// found before it reads the chunk.
+__device__ __forceinline__ bool is_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; }
+
+// Whether a row sees a key: its own span of keys from lo on, or the prefix
+__device__ __forceinline__ bool sees(int key, int pe, int lo, unsigned span) {
+    return (key < pe) | ((unsigned)(key - lo) <= span);
+}
+
+template <int HD>
+__device__ __forceinline__ bool clean_chunk(char* vt, int lane) {
+    char* const at = vt + 16 * lane;
+    float a = 0.f;  // (any infinity or NaN times 0)
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+        const half8 x = *reinterpret_cast<const half8*>(at + 1024 * i);
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) a = __builtin_amdgcn_fdot2(half2{x[k], x[k + 1]}, half2{0, 0}, a, false);
+    }
+    if (__builtin_amdgcn_ballot_w64(a != 0.f) == 0) return false;
+#pragma unroll 1
+    for (int i = 0; i < HD / 16; ++i) {
+        half8 x = *reinterpret_cast<const half8*>(at + 1024 * i);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = is_finite(x[k]) ? x[k] : (_Float16)0;
+        *reinterpret_cast<half8*>(at + 1024 * i) = x;
+    }
+    lds_done();
+    return true;
+}
+
+// the chunk at key kb
+template <int HD, int RT>
+__device__ __forceinline__ void add_special(const PagedParams& p, const PlanPiece& z, uint64_t vbase, const int32_t* table,
+                                            int kb, int h2, const int (&lor)[RT], const unsigned (&span)[RT],
+                                            float16v (&o)[HD / 32][RT]) {
+#pragma unroll 1
+    for (int key = kb; key < kb + 32; ++key) {
+        int first, count;
+        group_rows(key, 1, z.lo, z.kend, z.pe, first, count);
+        if (count == 0) continue;
+        const unsigned id = min((unsigned)table_entry(table, key >> p.page_log2), (unsigned)p.n_pages - 1u);
+        const char* const src = reinterpret_cast<const char*>(vbase + (uint64_t)id * (uint64_t)p.page_b +
+                                                              (uint64_t)(key & ((1 << p.page_log2) - 1)) * p.row_b);
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const half4 x = *reinterpret_cast<const half4*>(src + 2 * (32 * dt + 8 * i4 + 4 * h2));
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const bool seen = sees(key, z.pe, lor[rt], span[rt]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[dt][rt][4 * i4 + i] += (seen & !is_finite(x[i])) ? (float)x[i] : 0.f;
+                }
+            }
+    }
+}
+
+// The cache rows of one kv head: a wave fills runs of 8 consecutive rows of a
+// tile, which lie in one page (pages are at least 8 rows).  A run's address is
+// scalar: its table entry, in 64 bits; a lane adds its row and piece, a
+// constant.
+template <int HD>
+struct CacheRows {
+    static constexpr int PPR = HD / 8, RPI = 64 / PPR, IPR = 8 / RPI;  // pieces a row; rows, instructions of a run
+    const PagedParams& p;
+    const PlanPiece& z;
+    uint64_t k, v;            // the head's rows of page 0
+    const int32_t* table;     // the request's row
+    int last, bad = 0;        // last key that a row sees; a page of a wanted key is none of the pool's
+    uint32_t klane[IPR], vlane[IPR];
+
+    struct Run {
+        uint64_t off;         // bytes to the first row wanted
+        uint32_t nrec, skip;  // bytes of the rows wanted, bytes of the run ahead of them
+    };
+
+    __device__ __forceinline__ CacheRows(const PagedParams& p_, const PlanPiece& z_, int kvh, int lane) : p(p_), z(z_) {
+        k = reinterpret_cast<uintptr_t>(p.k) + (uint64_t)kvh * p.head_b;
+        v = reinterpret_cast<uintptr_t>(p.v) + (uint64_t)kvh * p.head_b;
+        table = p.table + (size_t)z.seq * p.max_pages;
+        last = imax(z.kend, z.pe) - 1;
+        const int lrow = lane / PPR, phys = lane % PPR;
+#pragma unroll
+        for (int j = 0; j < IPR; ++j) {
+            const int row = RPI * j + lrow;  // (the pieces' swizzle, see k_slot and v_slot)
+            klane[j] = (uint32_t)row * p.row_b + 16u * (phys ^ (row & 7));
+            vlane[j] = (uint32_t)row * p.row_b + 16u * (phys ^ ((row & 3) << 1));
+            __asm__("" : "+v"(klane[j]), "+v"(vlane[j]));  // (else taken apart again at each use)
+        }
+    }
+    __device__ __forceinline__ int entry(int key) const { return table_entry(table, imin(key, last) >> p.page_log2); }
+    // keys key .. key + 7; none are wanted unless `any`
+    __device__ __forceinline__ Run run(int key, bool any, int id) {
+        int first, count;
+        group_rows(key, 8, z.lo, z.kend, z.pe, first, count);
+        count = any ? count : 0;
+        bad |= count > 0 ? (unsigned)id >= (unsigned)p.n_pages : 0;
+        const unsigned page = min((unsigned)id, (unsigned)p.n_pages - 1u);
+        Run r;
+        r.skip = (uint32_t)first * p.row_b;
+        r.nrec = (uint32_t)count * p.row_b;
+        r.off = (uint64_t)page * (uint64_t)p.page_b + (uint32_t)((key & ((1 << p.page_log2) - 1)) * p.row_b) + r.skip;
+        return r;
+    }
+    // instruction j of a run into 1 KB of LDS at byte `to`
+    template <bool V>
+    __device__ __forceinline__ void load(const Run& r, int j, uint32_t to) const {
+        const uint64_t base = (V ? v : k) + r.off;
+        const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32), r.nrec, (uint32_t)kBufFlags};
+        uint32_t saved;
+        __asm__ volatile(
+            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+            "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "s"(to), "v"((V ? vlane[j] : klane[j]) - r.skip), "s"(rs));
+    }
+};
 
 template <int HD, int RT, int KG>
 struct PagedShape {
@@ -93,25 +245,59 @@ struct PagedShape {
     static constexpr int CPT = TK / 32;
     static constexpr int NB = KG == 1 ? 2 : HD == 64 ? 2 : 1;  // buffers of K (and of V) a group
     static constexpr int TILE = TK * HD * 2;
-    static constexpr int RPI = 64 / PPR;                 // rows of a load instruction
-    static constexpr int WI = TK / RPI / NWG;            // its instructions a wave and tile
+    static constexpr int NR = TK / NWG / 8;              // runs of 8 rows a wave fills of a tile
+    static constexpr int WI = NR * CacheRows<HD>::IPR;   // load instructions of these
     static constexpr int STREAM = KG * 2 * NB * TILE;
     static constexpr int MERGE = KG > 1 ? kNW * DT * RT * 64 * 64 + kNW * RT * 64 * 8 : 0;
     static constexpr int LDS = STREAM > MERGE ? STREAM : MERGE;
 };
 
+// What a row's state (max M, sum L, both of the keys only) is multiplied by for
+// the output: the sink joins here, last, so that probabilities are relative
+// to the keys' max and keep their bits however large the sink is.
+__device__ __forceinline__ float row_weight(const PagedParams& p, int h, float M, float L) {
+    if (!p.sinks) return 1.f / L;
+    const float sk = p.sinks[h] * kLog2e, top = fmaxf(M, sk), f = fast_exp2(M - top);
+    return f / (L * f + fast_exp2(sk - top));
+}
+
+// Where row rl of the piece's item goes: its output, or the partial sums of a
+// split item's piece
+template <int HD, bool F32>
+struct RowOut {
+    char* at;
+    bool part;
+    __device__ __forceinline__ RowOut(const PagedParams& p, const PlanPiece& z, int kvh, int rl) {
+        part = z.slot >= 0;
+        const int r = z.r0 + rl, t = r / p.hpk, h = kvh * p.hpk + r - t * p.hpk;
+        at = part ? reinterpret_cast<char*>(p.ws_o + ((size_t)(z.slot * p.n_kv + kvh) * p.rows + rl) * HD)
+                  : static_cast<char*>(p.out) + ((size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD) * (F32 ? 4 : 2);
+    }
+    // 4 dims from d on
+    __device__ __forceinline__ void store(int d, const float4v& x, float w) const {
+        if (F32 || part) *reinterpret_cast<float4v*>(at + 4 * d) = part ? x : x * w;
+        else *reinterpret_cast<half4*>(at + 2 * d) =
+            half4{(_Float16)(x[0] * w), (_Float16)(x[1] * w), (_Float16)(x[2] * w), (_Float16)(x[3] * w)};
+    }
+};
+__device__ __forceinline__ void store_sum(const PagedParams& p, const PlanPiece& z, int kvh, int rl, float M, float L) {
+    reinterpret_cast<float2*>(p.ws_ml)[(size_t)(z.slot * p.n_kv + kvh) * p.rows + rl] = make_float2(M, L);
+}
+
 template <int HD, int RT, int KG, bool F32, bool SC>
 __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S = PagedShape<HD, RT, KG>;
-    constexpr int KS = S::KS, DT = S::DT, PPR = S::PPR, NWG = S::NWG, CPT = S::CPT, NB = S::NB;
-    constexpr int TILE = S::TILE, RPI = S::RPI, WI = S::WI;
+    constexpr int KS = S::KS, DT = S::DT, NWG = S::NWG, CPT = S::CPT, NB = S::NB;
+    constexpr int TILE = S::TILE, NR = S::NR, WI = S::WI;
+    using Rows = CacheRows<HD>;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int h2 = lane >> 5, c32 = lane & 31;
     const int kg = wave / NWG, wr = wave % NWG;
 
     // rows: the queries as the B operand (column c32 of each 32-row tile)
     half8 qh[RT][KS], ql[F32 ? RT : 1][F32 ? KS : 1];
-    int posr[RT], lor[RT];
+    int posr[RT], lor[RT];  // position, first key of the window
+    unsigned span[RT];      // keys behind that one that the row sees
     bool valid[RT];
     float slope[RT];
     constexpr int QES = F32 ? 4 : 2;
@@ -139,8 +325,10 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
             }
         }
         const int pos = z.pos0 + t;
-        posr[rt] = valid[rt] ? pos : -1;
+        posr[rt] = pos;
         lor[rt] = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+        span[rt] = (unsigned)(pos - lor[rt]);
+        if (!valid[rt]) lor[rt] = INT32_MAX, span[rt] = 0;  // (sees none)
         slope[rt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
     }
     // every row sees the keys [lo_all, hi_all] and those below z.pe
@@ -154,66 +342,41 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
     for (int rt = 0; rt < RT; ++rt) {
         m[rt] = -INFINITY;
         l[rt] = 0.f;
-        if (p.sinks && z.slot < 0 && kg == 0) {  // (a split item's sink joins with its pieces)
-            const int rc = min(z.r0 + (wr * RT + rt) * 32 + c32, z.R - 1);
-            m[rt] = p.sinks[kvh * p.hpk + rc % p.hpk] * kLog2e;
-            l[rt] = h2 == 0 ? 1.f : 0.f;
-        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt][rt] = float16v{};
     }
 
-    // Cache rows: instruction i of this wave fills rows RPI (NWG i + wr) .. of a
-    // tile.  lane constants: the row within the group and the piece that the
-    // swizzled layout puts in the lane's slot (RPI divides 8, so the slot's
-    // key & 7 is the row's within 8)
     char* const kbuf = lds + kg * 2 * NB * TILE;
     char* const vbuf = kbuf + NB * TILE;
-    const int lrow = lane / PPR, phys = lane % PPR;
-    const char* const kbase = reinterpret_cast<const char*>(p.k) + (size_t)kvh * p.head_b;
-    const char* const vbase = reinterpret_cast<const char*>(p.v) + (size_t)kvh * p.head_b;
-    const size_t trow = (size_t)z.seq * p.max_pages;
-    bool bad = false;
-    // one group: K or V rows of tile keys kt .. of chunk-relative row r0g
-    struct Group {
-        int64_t off;     // bytes from the head's base to the first row wanted
-        uint32_t skip;   // bytes ahead of it within the group
-        uint32_t nrec;   // bytes of rows wanted
-    };
-    auto group = [&](int c, int row) {  // chunk c, first row within the chunk
-        Group g;
-        const int key = chunk_key(c, z.n_pre, z.lo_base) + row;
-        int first, count;
-        group_rows(key, RPI, z.lo, z.kend, z.pe, first, count);
-        if (c >= z.ce) count = 0;
-        g.skip = (uint32_t)first * p.row_b;
-        g.nrec = (uint32_t)count * p.row_b;
-        g.off = 0;
-        if (count > 0) {
-            const int id = table_entry(p.table, trow + (key >> p.page_log2));
-            bad |= (unsigned)id >= (unsigned)p.n_pages;
-            const int page = min(max(id, 0), p.n_pages - 1);
-            g.off = (int64_t)page * p.page_b + (int64_t)((key & ((1 << p.page_log2) - 1)) + first) * p.row_b;
-        }
-        return g;
-    };
-    auto load = [&](const char* base, const Group& g, char* dst, int i, bool is_v) {
-        const int row = RPI * (NWG * i + wr) + lrow;  // within the tile
-        const int piece = is_v ? phys ^ ((row & 3) << 1) : phys ^ (row & 7);
-        const __amdgpu_buffer_rsrc_t rs =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(base + g.off), (short)0, (int)g.nrec, kBufFlags);
-        lds_dma16_untracked(rs, (uint32_t)lrow * p.row_b + 16u * piece - g.skip, dst + 1024 * (NWG * i + wr));
-    };
+    Rows rows(p, z, kvh, lane);
+    const uint32_t lds_at = lds_byte(lds);
     // tile t of this key group: its first chunk
     auto tile_chunk = [&](int t) { return KG > 1 ? z.cb + kg + KG * t : z.cb + CPT * t; };
-    auto load_tile = [&](int t, bool is_v) {
-        char* const dst = (is_v ? vbuf : kbuf) + (t % NB) * TILE;
-#pragma unroll
-        for (int i = 0; i < WI; ++i) {
-            const int row = RPI * (NWG * i + wr);
-            load(is_v ? vbase : kbase, group(tile_chunk(t) + row / 32, row % 32), dst, i, is_v);
-        }
+    // run r of this wave: its first row of a tile, its first key
+    constexpr int WR = 8 * NR;  // rows a wave fills
+    auto run_key = [&](int t, int r) {
+        const int row = WR * wr + 8 * r;
+        return chunk_key(tile_chunk(t) + row / 32, z.n_pre, z.lo_base) + row % 32;
     };
+    auto fetch = [&](int t, int (&id)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t, r));
+    };
+    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+            run[r] = rows.run(run_key(t, r), tile_chunk(t) + (WR * wr + 8 * r) / 32 < z.ce, id[r]);
+    };
+    auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
+        constexpr bool V = decltype(is_v)::value;
+        const uint32_t to = lds_at + kg * 2 * NB * TILE + (V ? NB * TILE : 0) + (t % NB) * TILE + WR * HD * 2 * wr;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int j = 0; j < Rows::IPR; ++j) rows.template load<V>(run[r], j, to + 1024 * (Rows::IPR * r + j));
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
     const int n = z.ce - z.cb;
     const int n_tiles = KG > 1 ? (n - kg + KG - 1) / KG : (n + CPT - 1) / CPT;  // (kg <= n + KG - 1: >= 0)
 
@@ -261,7 +424,7 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
                 const int key = kb + 8 * (i / 4) + 4 * h2 + i % 4;
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    if (!(key < z.pe || (key >= lor[rt] && key <= posr[rt]))) s[rt][i] = -INFINITY;
+                    s[rt][i] = sees(key, z.pe, lor[rt], span[rt]) ? s[rt][i] : -INFINITY;
             }
         }
     };
@@ -300,16 +463,11 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
         }
     };
     auto pv = [&](const char* vt, int sub, const half8 (&ph)[2][RT], const half8 (&pl)[2][RT]) {
-        const int G = lane >> 4, r4 = (lane & 15) >> 2, q4 = lane & 3;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                // lanes of 16-lane group G: keys 16 w + 4 h2 + r4 (+ 8), dims 32 dt + 16 (G & 1) + 4 q4
-                const int key = 32 * sub + 16 * w + 4 * h2 + r4, dim = 32 * dt + 16 * (G & 1) + 4 * q4;
-                const _Float16* a0 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(key, dim >> 3) + ((dim & 7) << 1));
-                const _Float16* a1 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(key + 8, dim >> 3) + ((dim & 7) << 1));
-                const half8 va = cat8(lds_read_tr(a0), lds_read_tr(a1));
+                const half8 va = v_operand<HD>(vt, 32 * sub + 16 * w, dt, lane);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     o[dt][rt] = mfma32(va, ph[w][rt], o[dt][rt]);
@@ -318,100 +476,62 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
             }
         }
     };
-
-    // A chunk that some rows see in part may hold infinities or NaN in rows of
-    // V that they do not see, and 0 times those is NaN.  Where it does, they
-    // are taken out of the tile here and added after the last chunk to the rows
-    // that see them.
     auto partly_seen = [&](int c) {
         const int kb = chunk_key(c, z.n_pre, z.lo_base);
         return pos_last > hi_all && !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all));
     };
-    auto finite = [](_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; };
     bool special = false;
-    auto clean = [&](char* vt, int sub) {
-        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-        char* const at = vt + 64 * HD * sub + 16 * lane;
-        float a = 0.f;  // (any infinity or NaN times 0)
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-            const half8 x = *reinterpret_cast<const half8*>(at + 1024 * i);
-#pragma unroll
-            for (int k = 0; k < 8; k += 2) a = __builtin_amdgcn_fdot2(half2{x[k], x[k + 1]}, half2{0, 0}, a, false);
-        }
-        if (__builtin_amdgcn_ballot_w64(a != 0.f) == 0) return;
-        special = true;
-        // (the waves of a wide workgroup may do so at once: each writes zeros
-        // over what it finds before it reads the tile)
-#pragma unroll 1
-        for (int i = 0; i < HD / 16; ++i) {
-            half8 x = *reinterpret_cast<const half8*>(at + 1024 * i);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = finite(x[k]) ? x[k] : (_Float16)0;
-            *reinterpret_cast<half8*>(at + 1024 * i) = x;
-        }
-        lds_done();
-    };
-    auto add_special = [&](int c) {
-        const int kb = chunk_key(c, z.n_pre, z.lo_base);
-#pragma unroll 1
-        for (int key = kb; key < kb + 32; ++key) {
-            int first, count;
-            group_rows(key, 1, z.lo, z.kend, z.pe, first, count);
-            if (count == 0) continue;
-            const int id = min(max(table_entry(p.table, trow + (key >> p.page_log2)), 0), p.n_pages - 1);
-            const char* const src = vbase + (int64_t)id * p.page_b + (int64_t)(key & ((1 << p.page_log2) - 1)) * p.row_b;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                    const half4 x = *reinterpret_cast<const half4*>(src + 2 * (32 * dt + 8 * i4 + 4 * h2));
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        const bool sees = key < z.pe || (key >= lor[rt] && key <= posr[rt]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (sees && !finite(x[i])) o[dt][rt][4 * i4 + i] += (float)x[i];
-                    }
-                }
-        }
-    };
 
     half8 ph[2][RT], pl[2][RT];
     float16v s[RT];
     if constexpr (KG > 1) {
         // requests in order K0 V0 (K1 V1): ahead of a tile's wait stand the
-        // 2 NB - 1 tiles after it (past the last one: empty requests)
+        // 2 NB - 1 tiles after it (past the last one: empty requests); table
+        // entries a tile earlier
         constexpr int AHEAD = WI * (2 * NB - 1);
+        int id[NR];
+        typename Rows::Run run[NR];
+        fetch(0, id);
 #pragma unroll
         for (int t = 0; t < NB; ++t) {
-            load_tile(t, false);
-            load_tile(t, true);
+            place(t, id, run);
+            fetch(t + 1, id);
+            load_tile(t, run, K_{});
+            load_tile(t, run, V_{});
         }
         for (int t = 0; t < n_tiles; ++t) {
             const int c = tile_chunk(t);
             wait_loads<AHEAD>();
             scores(kbuf + (t % NB) * TILE, 0, c, s);
             lds_done();
-            load_tile(t + NB, false);
+            place(t + NB, id, run);
+            fetch(t + NB + 1, id);
+            load_tile(t + NB, run, K_{});
             transform(c, s);
             softmax(s, ph, pl);
             wait_loads<AHEAD>();
-            if (partly_seen(c)) clean(vbuf + (t % NB) * TILE, 0);
+            if (partly_seen(c)) special |= clean_chunk<HD>(vbuf + (t % NB) * TILE, lane);
             pv(vbuf + (t % NB) * TILE, 0, ph, pl);
             lds_done();
-            load_tile(t + NB, true);
+            load_tile(t + NB, run, V_{});
         }
         wait_loads<0>();
     } else {
-        load_tile(0, false);
-        load_tile(0, true);
+        int id[NR];
+        typename Rows::Run run[NR];
+        fetch(0, id);
+        place(0, id, run);
+        fetch(1, id);
+        load_tile(0, run, K_{});
+        load_tile(0, run, V_{});
         for (int t = 0; t < n_tiles; ++t) {
             wait_loads<0>();
             __syncthreads();  // tile t is there, and no wave reads tile t - 1
             if (t + 1 < n_tiles) {
-                load_tile(t + 1, false);
-                load_tile(t + 1, true);
+                place(t + 1, id, run);
+                fetch(t + 2, id);
+                load_tile(t + 1, run, K_{});
+                load_tile(t + 1, run, V_{});
             }
 #pragma unroll
             for (int sub = 0; sub < CPT; ++sub) {
@@ -420,42 +540,21 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
                 scores(kbuf + (t % NB) * TILE, sub, c, s);
                 transform(c, s);
                 softmax(s, ph, pl);
-                if (partly_seen(c)) clean(vbuf + (t % NB) * TILE, sub);
+                if (partly_seen(c)) special |= clean_chunk<HD>(vbuf + (t % NB) * TILE + 64 * HD * sub, lane);
                 pv(vbuf + (t % NB) * TILE, sub, ph, pl);
             }
         }
     }
-    const bool any_bad = __syncthreads_or(bad);  // (and every wave is done with the tiles)
+    const bool any_bad = __syncthreads_or(rows.bad);  // (and every wave is done with the tiles)
     if (KG == 1) special = __syncthreads_or(special);
     if (special)
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t)
 #pragma unroll 1
             for (int c = tile_chunk(t); c < min(tile_chunk(t) + CPT, z.ce); ++c)
-                if (partly_seen(c)) add_special(c);
+                if (partly_seen(c))
+                    add_special<HD, RT>(p, z, rows.v, rows.table, chunk_key(c, z.n_pre, z.lo_base), h2, lor, span, o);
 
-    // a row's final state: (M, L), and 4 consecutive dims at 32 dt + 8 i4 + 4 h2
-    const size_t part = (size_t)(z.slot * p.n_kv + kvh) * p.rows;
-    auto store_ml = [&](int rl, float M, float L) {
-        reinterpret_cast<float2*>(p.ws_ml)[part + rl] = make_float2(M, any_bad ? NAN : L);
-    };
-    auto store4 = [&](int rl, int dt, int i4, float4v x, float inv) {
-        const int d = 32 * dt + 8 * i4 + 4 * h2;
-        if (z.slot >= 0) {
-            *reinterpret_cast<float4v*>(p.ws_o + (part + rl) * HD + d) = x;
-            return;
-        }
-        if (any_bad) inv = NAN;
-        x *= inv;
-        const int r = z.r0 + rl;
-        const size_t at = (size_t)(z.q0 + r / p.hpk) * p.o_tok + (size_t)(kvh * p.hpk + r % p.hpk) * HD + d;
-        if constexpr (F32) {
-            *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at) = x;
-        } else {
-            *reinterpret_cast<half4*>(static_cast<uint16_t*>(p.out) + at) =
-                half4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-        }
-    };
     if constexpr (KG > 1) {
         // the waves' states through LDS, merged in wave order: wave g takes
         // the output tiles g, g + KG, ...
@@ -485,8 +584,10 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
             w[g] = fast_exp2(ml[g].x - ms);  // 0 where the wave saw no key
             L += ml[g].y * w[g];
         }
-        const float inv = 1.f / L;
-        if (z.slot >= 0 && wave == 0 && h2 == 0) store_ml(c32, M, L);
+        if (any_bad) L = NAN;
+        const float inv = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + c32) % p.hpk, M, L) : 1.f;
+        if (z.slot >= 0 && wave == 0 && h2 == 0) store_sum(p, z, kvh, c32, M, L);
+        const RowOut<HD, F32> to(p, z, kvh, c32);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             if (dt % KG != kg) continue;
@@ -495,27 +596,354 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
                 float4v x = so[(dt * 4 + i4) * 64 + lane] * w[0];
 #pragma unroll
                 for (int g = 1; g < KG; ++g) x += so[((g * DT + dt) * 4 + i4) * 64 + lane] * w[g];
-                store4(c32, dt, i4, x, inv);
+                to.store(32 * dt + 8 * i4 + 4 * h2, x, inv);
             }
         }
     } else {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const float L = half_sum(l[rt]);
+            const float L = any_bad ? NAN : half_sum(l[rt]);
             if (!valid[rt]) continue;
             const int rl = (wr * RT + rt) * 32 + c32;
-            if (z.slot >= 0 && h2 == 0) store_ml(rl, m[rt], L);
+            if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
+            const float w = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + rl) % p.hpk, m[rt], L) : 1.f;
+            const RowOut<HD, F32> to(p, z, kvh, rl);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int i4 = 0; i4 < 4; ++i4)
-                    store4(rl, dt, i4,
-                           float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]},
-                           1.f / L);
+                    to.store(32 * dt + 8 * i4 + 4 * h2,
+                             float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
         }
     }
 }
 
+// The wide item with f16 queries, as a software pipeline over 32-key chunks:
+// while the softmax of chunk c runs on the vector ALUs, the matrix cores take
+// QK^T of chunk c + 1 and PV of chunk c - 1, one MFMA at a time between the
+// softmax's instructions.  P = 2^(x - m) with a max m that moves only when a
+// chunk's row sum passes 2^14 (below it nothing overflowed f16, and keys far
+// below m are negligible beside the one m was taken from), or is not set yet:
+// then the wave takes the chunk's max, rescales O and the sum, and
+// recomputes P.
+//
+// K and V tiles of 64 keys, double-buffered; K runs a tile ahead of V.  In
+// step c = 2 t + 1 the loads of K tile t + 2 and V tile t + 1 go out between
+// the MFMAs (in a burst ahead of them a wave stalls at each); the barrier after
+// step 2 t orders them behind the last reads of their buffers and ahead of
+// their first.  A tile's table entries are loaded a step before its loads.
+template <int HD, int RT, bool SC>
+__device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
+    using S_ = PagedShape<HD, RT, 1>;
+    constexpr int KS = S_::KS, DT = S_::DT, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
+    using Rows = CacheRows<HD>;
+    constexpr int IPR = Rows::IPR;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int h2 = lane >> 5, c32 = lane & 31;
+    char* const kbuf = lds;
+    char* const vbuf = lds + 2 * TILE;
+    const int n = z.ce - z.cb;
+
+    Rows rows(p, z, kvh, lane);
+    // this wave fills rows 16 wave .. + 15 of a tile: two runs of one chunk
+    const uint32_t to_k = lds_byte(lds) + 16 * HD * 2 * wave, to_v = to_k + 2 * TILE;
+    auto run_key = [&](int t, int r) {
+        return chunk_key(z.cb + 2 * t + (wave >> 1), z.n_pre, z.lo_base) + 16 * (wave & 1) + 8 * r;
+    };
+    auto wanted = [&](int t) { return 2 * t + (wave >> 1) < n; };
+    // the first tiles, then the queries beside them
+    int id[NR];                            // table entries of the next K tile to request
+    typename Rows::Run rk[NR], rv[NR];     // runs of the K tile and the V tile to request
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        rk[r] = rows.run(run_key(0, r), wanted(0), rows.entry(run_key(0, r)));
+        rv[r] = rows.run(run_key(1, r), wanted(1), rows.entry(run_key(1, r)));
+    }
+#pragma unroll
+    for (int x = 0; x < WI; ++x) rows.template load<false>(rk[x / IPR], x % IPR, to_k + 1024 * x);
+#pragma unroll
+    for (int x = 0; x < WI; ++x) rows.template load<true>(rk[x / IPR], x % IPR, to_v + 1024 * x);
+#pragma unroll
+    for (int x = 0; x < WI; ++x) rows.template load<false>(rv[x / IPR], x % IPR, to_k + TILE + 1024 * x);
+    // (the first step's empty PV product reads V tile 1's buffer)
+#pragma unroll
+    for (int i = 0; i < TILE / (16 * 64 * kNW); ++i)
+        *reinterpret_cast<u32x4*>(vbuf + TILE + 16 * (64 * wave + lane + 64 * kNW * i)) = u32x4{0, 0, 0, 0};
+
+    half8 qb[RT][KS];
+    int posr[RT], lor[RT];  // position, first key of the window
+    unsigned span[RT];      // keys behind that one that the row sees
+    bool valid[RT];
+    float slope[RT], m[RT], l[RT];
+    float16v o[DT][RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = z.r0 + (wave * RT + rt) * 32 + c32;
+        valid[rt] = r < z.R;
+        const int rc = min(r, z.R - 1), t = rc / p.hpk, h = kvh * p.hpk + rc % p.hpk;
+        const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * h2) * 2;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qb[rt][ks] = load16(src + 32 * ks);
+        const int pos = z.pos0 + t;
+        posr[rt] = pos;
+        lor[rt] = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+        span[rt] = (unsigned)(pos - lor[rt]);
+        if (!valid[rt]) lor[rt] = INT32_MAX, span[rt] = 0;  // (sees none)
+        slope[rt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
+        m[rt] = valid[rt] ? -INFINITY : 0.f;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][rt] = float16v{};
+    }
+    const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
+    const int hi_all = z.pos0 + z.r0 / p.hpk, pos_last = z.pos0 + r_last / p.hpk;
+    const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
+
+    // a chunk that not every row sees whole; its V rows may hold infinities or
+    // NaN that some rows do not see (see paged_body)
+    auto key_of = [&](int c) { return chunk_key(z.cb + c, z.n_pre, z.lo_base); };
+    auto partly = [&](int kb) { return !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all)); };
+    bool special = false;
+
+    // S^T of the first chunk
+    auto v_chunk = [&](int c) { return vbuf + ((c >> 1) & 1) * TILE + 64 * HD * (c & 1); };
+
+    float16v s_a[RT], s_b[RT];
+    half8 p_a[2][RT], p_b[2][RT];
+    const float qs = SC ? 1.f : p.qscale;
+
+    auto step = [&](auto par, int c, float16v (&s_cur)[RT], float16v (&s_nxt)[RT], const half8 (&p_prv)[2][RT],
+                    half8 (&p_cur)[2][RT]) {
+        constexpr int PAR = decltype(par)::value;
+        const int t = c >> 1;
+        const int kb = key_of(c);
+        if constexpr ((PAR & 1) == 0) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t + 2, r));
+        } else {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) rk[r] = rows.run(run_key(t + 2, r), wanted(t + 2), id[r]);
+        }
+        if (c > 0 && pos_last > hi_all && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
+        auto load_nth = [&](auto x_) {
+            constexpr int x = decltype(x_)::value;
+            if constexpr (x < WI)  // K tile t + 2
+                rows.template load<false>(rk[x / IPR], x % IPR, to_k + ((PAR >> 1) & 1) * TILE + 1024 * x);
+            else  // V tile t + 1
+                rows.template load<true>(rv[x / IPR - NR], x % IPR, to_v + (((PAR >> 1) + 1) & 1) * TILE + 1024 * (x - WI));
+        };
+        if constexpr (SC) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (p.cap > 0.f) {
+                    // cap tanh(y / cap), tanh(y) = 1 - 2 / (1 + e^(2 y))
+                    const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s_cur[rt][i] = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s_cur[rt][i] * f));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s_cur[rt][i] *= p.qscale;
+                }
+                if (p.alibi) {
+                    const float d = (float)(posr[rt] - kb - 4 * h2);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s_cur[rt][i] -= slope[rt] * fabsf(d - (float)(8 * (i / 4) + i % 4));
+                }
+            }
+        }
+        if (partly(kb)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = kb + 8 * (i / 4) + 4 * h2 + i % 4;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    s_cur[rt][i] = sees(key, z.pe, lor[rt], span[rt]) ? s_cur[rt][i] : -INFINITY;
+            }
+        }
+        // operands: KS pieces of K (chunk c + 1), then 2 DT of V^T (chunk
+        // c - 1), each read two ahead of its first MFMA
+        constexpr int NOPD = KS + 2 * DT, NM = KS * RT + 2 * DT * RT;
+        half8 opd[NOPD];
+        const char* const kt = kbuf + (((PAR + 1) >> 1) & 1) * TILE;
+        const char* const vt = vbuf + (((PAR + 3) >> 1) & 1) * TILE;
+        const int krow = 32 * ((PAR + 1) & 1) + c32;
+        auto read_opd = [&](auto r_) {
+            constexpr int r = decltype(r_)::value;
+            if constexpr (r < KS) {
+                opd[r] = *reinterpret_cast<const half8*>(kt + k_slot<HD>(krow, 2 * r + h2));
+            } else {
+                constexpr int w = (r - KS) / DT, dt = (r - KS) % DT;
+                opd[r] = v_operand<HD>(vt, 32 * ((PAR + 3) & 1) + 16 * w, dt, lane);
+            }
+        };
+        read_opd(std::integral_constant<int, 0>{});
+        read_opd(std::integral_constant<int, 1>{});
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s_nxt[rt] = float16v{};
+        // The softmax's stages (x - m, exp2, f16 pairs, row sum) are skewed by a
+        // slot (an MFMA) each, NS / NM scores a slot.
+        constexpr int NS = 16 * RT, NP = NS / 2, S = NS / NM;
+        static_assert(NS % NM == 0, "whole scores a slot");
+        constexpr int NLD = (PAR & 1) ? 2 * WI : 0;
+        constexpr int LSL = HD == 128 ? NM : NM / 2;  // slots the loads go out in
+        float ms[RT], acc[RT][2], e[NS];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            ms[rt] = m[rt] == -INFINITY ? 0.f : m[rt];
+            acc[rt][0] = acc[rt][1] = 0.f;
+        }
+        auto op_fma = [&](int i) {
+            if (i < NS) s_cur[i / 16][i % 16] = __builtin_fmaf(s_cur[i / 16][i % 16], qs, -ms[i / 16]);
+        };
+        auto op_exp = [&](int i) {
+            if (i < NS) e[i] = fast_exp2(s_cur[i / 16][i % 16]);
+        };
+        auto op_pack = [&](int k) {
+            const int rt = k / 8, i = 2 * (k % 8);
+            p_cur[i / 8][rt][i % 8] = (_Float16)e[2 * k];
+            p_cur[i / 8][rt][i % 8 + 1] = (_Float16)e[2 * k + 1];
+        };
+        auto op_sum = [&](int k) {
+            const int rt = k / 8, i = 2 * (k % 8);
+            acc[rt][k & 1] = __builtin_amdgcn_fdot2(half2{p_cur[i / 8][rt][i % 8], p_cur[i / 8][rt][i % 8 + 1]},
+                                                    half2{1, 1}, acc[rt][k & 1], false);
+        };
+        // pairs whose exp2s are done after slot u
+        auto ready = [](int u) { return u < 0 ? 0 : (S * (u + 1)) / 2; };
+#pragma unroll
+        for (int j = 0; j < S; ++j) op_fma(j);
+        unrolled<NM>([&](auto u_) {
+            constexpr int u = decltype(u_)::value;
+            constexpr bool of_k = u < KS * RT;
+            constexpr int r = u / RT, rt = u % RT;
+            if constexpr (rt == 0 && r + 2 < NOPD) read_opd(std::integral_constant<int, r + 2>{});
+            unrolled<NLD>([&](auto i) {
+                if constexpr (decltype(i)::value * LSL / NLD == u) load_nth(i);
+            });
+            if constexpr (of_k) {
+                s_nxt[rt] = mfma32(opd[r], qb[rt][r], s_nxt[rt]);
+            } else {
+                constexpr int w = (r - KS) / DT, dt = (r - KS) % DT;
+                o[dt][rt] = mfma32(opd[r], p_prv[w][rt], o[dt][rt]);
+            }
+#pragma unroll
+            for (int k = ready(u - 3); k < ready(u - 2); ++k) op_sum(k);
+#pragma unroll
+            for (int k = ready(u - 2); k < ready(u - 1); ++k) op_pack(k);
+#pragma unroll
+            for (int j = 0; j < S; ++j) op_exp(S * u + j);
+#pragma unroll
+            for (int j = 0; j < S; ++j) op_fma(S * (u + 1) + j);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+#pragma unroll
+        for (int k = ready(NM - 2); k < NP; ++k) op_pack(k);
+#pragma unroll
+        for (int k = ready(NM - 3); k < NP; ++k) op_sum(k);
+        float ls[RT];
+        bool redo = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            ls[rt] = acc[rt][0] + acc[rt][1];
+            redo |= !(ls[rt] <= 16384.f) || m[rt] == -INFINITY;
+        }
+        if (__builtin_amdgcn_ballot_w64(redo)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float x = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x = fmaxf(x, s_cur[rt][i]);
+                const float mn = fmaxf(m[rt], half_max(x) + ms[rt]);
+                if (mn > m[rt]) {
+                    const float cf = fast_exp2(m[rt] - mn);  // 0 while m was -inf
+                    l[rt] *= cf;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[dt][rt] *= cf;
+                    m[rt] = mn;
+                }
+                const float shift = ms[rt] - (m[rt] == -INFINITY ? 0.f : m[rt]);
+                float a = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p_cur[i / 8][rt][i % 8] = (_Float16)fast_exp2(s_cur[rt][i] + shift);
+                    a += (float)p_cur[i / 8][rt][i % 8];
+                }
+                ls[rt] = a;
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) l[rt] += ls[rt];
+        if constexpr (PAR & 1) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) rv[r] = rk[r];
+        } else {
+            wait_loads<0>();
+            __syncthreads();
+        }
+    };
+
+    wait_loads<0>();
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) s_a[rt] = float16v{};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const half8 ka = *reinterpret_cast<const half8*>(kbuf + k_slot<HD>(c32, 2 * ks + h2));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s_a[rt] = mfma32(ka, qb[rt][ks], s_a[rt]);
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) p_b[w][rt] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+    using P0 = std::integral_constant<int, 0>;
+    using P1 = std::integral_constant<int, 1>;
+    using P2 = std::integral_constant<int, 2>;
+    using P3 = std::integral_constant<int, 3>;
+    int c = 0;
+    for (; c + 4 <= n; c += 4) {
+        step(P0{}, c, s_a, s_b, p_b, p_a);
+        step(P1{}, c + 1, s_b, s_a, p_a, p_b);
+        step(P2{}, c + 2, s_a, s_b, p_b, p_a);
+        step(P3{}, c + 3, s_b, s_a, p_a, p_b);
+    }
+    const int rem = n - c;
+    if (rem >= 1) step(P0{}, c, s_a, s_b, p_b, p_a);
+    if (rem >= 2) step(P1{}, c + 1, s_b, s_a, p_a, p_b);
+    if (rem >= 3) step(P2{}, c + 2, s_a, s_b, p_b, p_a);
+    wait_loads<0>();  // (what was requested past the last tile)
+    if (pos_last > hi_all && partly(key_of(n - 1))) special |= clean_chunk<HD>(v_chunk(n - 1), lane);
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const half8 va = v_operand<HD>(v_chunk(n - 1), 16 * w, dt, lane);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[dt][rt] = mfma32(va, (n & 1) ? p_a[w][rt] : p_b[w][rt], o[dt][rt]);
+        }
+    const bool any_bad = __syncthreads_or(rows.bad);
+    if (__syncthreads_or(special))
+#pragma unroll 1
+        for (int i = 0; i < n; ++i)
+            if (partly(key_of(i))) add_special<HD, RT>(p, z, rows.v, rows.table, key_of(i), h2, lor, span, o);
+
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float L = any_bad ? NAN : half_sum(l[rt]);
+        if (!valid[rt]) continue;
+        const int rl = (wave * RT + rt) * 32 + c32;
+        if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
+        const float w = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + rl) % p.hpk, m[rt], L) : 1.f;
+        const RowOut<HD, false> to(p, z, kvh, rl);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+                to.store(32 * dt + 8 * i4 + 4 * h2,
+                         float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
+    }
+}
 template <int HD, bool F32, bool SC, bool WIDE>
 __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedParams p) {
     constexpr int RT = HD == 64 ? 2 : 1;
@@ -524,38 +952,48 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int id = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
     if (p.head->sig != p.sig || id >= p.head->n_pieces) return;
     const PlanPiece z = p.pieces[id];
-    if (WIDE && z.R > kNarrowRows) paged_body<HD, RT, 1, F32, SC>(p, z, kvh, lds);
-    else paged_body<HD, 1, kNW, F32, SC>(p, z, kvh, lds);
+    if (WIDE && z.R > kNarrowRows) {
+        if constexpr (F32) paged_body<HD, RT, 1, true, SC>(p, z, kvh, lds);
+        else wide_body<HD, RT, SC>(p, z, kvh, lds);
+    } else paged_body<HD, 1, kNW, F32, SC>(p, z, kvh, lds);
 }
 
-// The pieces of a split item, joined in key order with the sink: per row
-// (M, L, O) of each slot, weights 2^(M_i - M).  WPR waves a row: HD / 4 lanes
-// hold 4 dims each, the other lane groups and waves take slots in turn and
-// meet through lane exchanges and LDS in a fixed order.
+// The pieces of a split item, joined with the sink: per row (M, L, O) of each
+// slot, weights 2^(M_i - M).  HD / 4 lanes hold a row's dims, 4 each; a wave's
+// lane groups (and WPR waves) take one row's slots in turn and meet through
+// lane exchanges and LDS in a fixed order, or, where the slots are few, a
+// row each.  Bound by the partials' bytes, and for single tokens by its two
+// round trips (plan, partials) behind the attention kernel.
 template <int HD, bool F32, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
-    constexpr int LPR = HD / 4, GPW = 64 / LPR, PH = GPW * WPR, U = 8;
+    constexpr int LPR = HD / 4, GPW = 64 / LPR, U = 4;
     __shared__ float st[WPR > 1 ? WPR : 1][64][6];
     const int j = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
     if (p.head->sig != p.sig || j >= p.head->n_joins) return;
     const PlanJoin z = p.joins[j];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = 4 * (lane % LPR);
-    const int ph = (WPR > 1 ? wave * GPW : 0) + lane / LPR;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = 4 * (lane % LPR), grp = lane / LPR;
     const int rows = min(z.R - z.r0, p.rows);
-    for (int r = WPR > 1 ? (int)blockIdx.y : (int)blockIdx.y * (4 / WPR) + wave; r < rows;
-         r += (WPR > 1 ? 1 : 4) * (int)gridDim.y) {
+    const bool spread = WPR > 1 || z.n_slots > 8;  // a row's slots over the lane groups
+    const int ph = WPR > 1 ? wave * GPW + grp : spread ? grp : 0, n_ph = WPR > 1 ? GPW * WPR : spread ? GPW : 1;
+    const int per_wave = spread ? 1 : GPW;  // rows
+    const int step = WPR > 1 ? (int)gridDim.y : (int)gridDim.y * 4 * per_wave;
+    for (int r0 = WPR > 1 ? (int)blockIdx.y : ((int)blockIdx.y * 4 + wave) * per_wave; r0 < rows; r0 += step) {
+        const int r = min(r0 + (spread ? 0 : grp), rows - 1);
         float m = -INFINITY, l = 0.f;
         float4v o = {};
-        for (int s0 = ph; s0 < z.n_slots; s0 += PH * U) {
+        for (int s0 = 0; s0 < z.n_slots; s0 += n_ph * U) {
             float2 ml[U];
             float4v v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int sl = s0 + PH * u;
-                const size_t at = ((size_t)(z.slot0 + min(sl, z.n_slots - 1)) * p.n_kv + kvh) * p.rows + r;
-                ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[at];
-                v[u] = *reinterpret_cast<const float4v*>(p.ws_o + at * HD + d);
-                if (sl >= z.n_slots) ml[u] = make_float2(-INFINITY, 0.f);
+                const int sl = s0 + ph + n_ph * u;
+                ml[u] = make_float2(-INFINITY, 0.f);
+                v[u] = float4v{};
+                if (sl < z.n_slots) {
+                    const size_t at = ((size_t)(z.slot0 + sl) * p.n_kv + kvh) * p.rows + r;
+                    ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[at];
+                    v[u] = *reinterpret_cast<const float4v*>(p.ws_o + at * HD + d);
+                }
             }
             float mb = m;
 #pragma unroll
@@ -571,16 +1009,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
             }
             m = mb;
         }
-        // the lane groups of a wave, then the waves
+        if (spread) {
 #pragma unroll
-        for (int off = LPR; off < 64; off <<= 1) {
-            const float m2 = __shfl_xor(m, off, 64), l2 = __shfl_xor(l, off, 64);
-            const float M = fmaxf(m, m2), ms = M == -INFINITY ? 0.f : M;
-            const float a = fast_exp2(m - ms), b = fast_exp2(m2 - ms);
-            l = l * a + l2 * b;
+            for (int off = LPR; off < 64; off <<= 1) {
+                const float m2 = __shfl_xor(m, off, 64), l2 = __shfl_xor(l, off, 64);
+                const float M = fmaxf(m, m2), ms = M == -INFINITY ? 0.f : M;
+                const float a = fast_exp2(m - ms), b = fast_exp2(m2 - ms);
+                l = l * a + l2 * b;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * a + __shfl_xor(o[i], off, 64) * b;
-            m = M;
+                for (int i = 0; i < 4; ++i) o[i] = o[i] * a + __shfl_xor(o[i], off, 64) * b;
+                m = M;
+            }
         }
         if (WPR > 1) {
             __syncthreads();
@@ -604,15 +1043,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
             }
             m = M;
         }
-        const int rr = z.r0 + r, h = kvh * p.hpk + rr % p.hpk;
-        if (p.sinks) {
-            const float sk = p.sinks[h] * kLog2e, M = fmaxf(m, sk), f = fast_exp2(m - M);
-            l = l * f + fast_exp2(sk - M);
-            o *= f;
-        }
-        if (lane >= LPR) continue;
-        o *= 1.f / l;
-        const size_t at = (size_t)(z.q0 + rr / p.hpk) * p.o_tok + (size_t)h * HD + d;
+        if (spread ? lane >= LPR : r0 + grp >= rows) continue;
+        const int rr = z.r0 + r, t = rr / p.hpk, h = kvh * p.hpk + rr - t * p.hpk;
+        o *= row_weight(p, h, m, l);
+        const size_t at = (size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD + d;
         if constexpr (F32) {
             *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at) = o;
         } else {
@@ -656,7 +1090,7 @@ hipError_t launch_paged_join(const PagedParams& p, hipStream_t st) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool F32 = decltype(f32)::value;
         const unsigned x = (unsigned)p.max_joins * p.n_kv;
-        if (p.wide) hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1>), dim3(x, 8), dim3(256), 0, st, p);
+        if (p.wide) hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1>), dim3(x, 16), dim3(256), 0, st, p);
         else hipLaunchKernelGGL((paged_join_kernel<HD, F32, 4>), dim3(x, std::min(p.rows, 32)), dim3(256), 0, st, p);
         return hipGetLastError();
     });

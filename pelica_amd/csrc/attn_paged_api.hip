@@ -59,8 +59,8 @@ int check_pool(const PelicaPagedDesc* d, int piece) {
     if (rs < d->hd || hs < d->hd || ps < d->hd || rs % piece || hs % piece || ps % piece)
         return fail(PELICA_ATTN_EINVAL, "page, row and head strides (%lld, %lld, %lld): at least hd, whole %d-byte pieces",
                     (long long)ps, (long long)rs, (long long)hs, 2 * piece);
-    // (a load's rows are addressed with 32-bit byte offsets, a page with 64)
-    if (rs >= 1 << 24 || hs >= 1LL << 40 || ps >= 1LL << 40)
+    // (a page's rows are addressed with 32-bit byte offsets, a page with 64)
+    if (rs >= 1 << 24 || rs * d->page_size >= 1LL << 31 || hs >= 1LL << 40 || ps >= 1LL << 40)
         return fail(PELICA_ATTN_EUNSUPPORTED, "page, row and head strides (%lld, %lld, %lld) too large", (long long)ps,
                     (long long)rs, (long long)hs);
     return PELICA_ATTN_OK;

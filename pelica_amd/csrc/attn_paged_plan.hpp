@@ -63,9 +63,20 @@ PELICA_HD int chunk_key(int c, int n_pre, int lo_base) { return c < n_pre ? 32 *
 // Of n consecutive keys from kg (all in one page), the rows [first, first +
 // count) that some row of the item may see: a load touches no others (they may
 // lie in a page that was given away, or hold anything).
+// x between 0 and n, on the scalar unit: as a minimum of a maximum the compiler
+// makes it a vector instruction, and every address that follows with it
+PELICA_HD int clamp_to(int x, int n) {
+#ifdef __HIP_DEVICE_COMPILE__
+    int y;
+    __asm__("s_max_i32 %0, %1, 0" : "=s"(y) : "s"(x) : "scc");
+    return imin(y, n);
+#else
+    return imin(imax(x, 0), n);
+#endif
+}
 PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, int& count) {
-    const int a = imin(imax(pe - kg, 0), n);                         // of the prefix: [0, a)
-    const int b0 = imin(imax(lo - kg, 0), n), b1 = imin(imax(kend - kg, 0), n);
+    const int a = clamp_to(pe - kg, n);  // of the prefix: [0, a)
+    const int b0 = clamp_to(lo - kg, n), b1 = clamp_to(kend - kg, n);
     first = a > 0 ? 0 : b0;
     const int end = b1 > b0 ? imax(a, b1) : a;
     count = imax(end - first, 0);
