@@ -27,7 +27,8 @@ struct PlanParams {
     int n_seq, n_tokens, max_q, hpk, hd, window, fill;
     int64_t max_keys;
     int max_joins, max_pieces;
-    bool split;  // no: every item is one piece
+    int max_slots;  // most pieces of split items
+    bool split;     // no: every item is one piece
     uint32_t sig;
 };
 hipError_t launch_paged_plan(const PlanParams& p, hipStream_t st);

@@ -100,7 +100,6 @@ PagedPlan plan_of(const PelicaPagedDesc* d) {
     x.fill = pelica::plan_fill(d->n_kv, device_cus());
     const int64_t items = x.wide ? pelica::plan_items(d->n_seq, d->n_tokens, x.hpk, d->hd)
                                  : std::min(d->n_seq, d->n_tokens);
-    x.max_pieces = pelica::plan_pieces(items, x.fill);
     x.rows = x.wide ? pelica::wide_rows(d->hd)
                     : std::min(pelica::kNarrowRows, d->max_q * x.hpk);
     // a step whose items are at most two chunks a wave (window layers) is not
@@ -108,12 +107,13 @@ PagedPlan plan_of(const PelicaPagedDesc* d) {
     const int64_t keys = (int64_t)d->max_pages * d->page_size;
     const int64_t span = d->window > 0 && !d->prefix_len ? std::min(keys, (int64_t)d->window + d->max_q - 1) : keys;
     x.split = x.wide || span / 32 + 2 > 8;
-    x.max_joins = x.split ? (int)std::max<int64_t>(1, std::min<int64_t>(items, x.fill / 2)) : 0;
+    x.max_pieces = x.split ? pelica::plan_pieces(items, x.fill) : items;
+    x.max_joins = x.split ? (int)std::min<int64_t>(items, pelica::plan_slots(x.fill) / 2) : 0;
     auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
     x.join_at = 64;
     x.piece_at = 64 + (((size_t)x.max_joins * sizeof(pelica::PlanJoin) + 63) & ~(size_t)63);
     x.bytes = x.piece_at + (size_t)x.max_pieces * sizeof(pelica::PlanPiece);
-    const size_t slots = x.split ? (size_t)x.fill * d->n_kv * x.rows : 0;
+    const size_t slots = x.split ? (size_t)pelica::plan_slots(x.fill) * d->n_kv * x.rows : 0;
     x.ml_bytes = al(slots * 8);
     x.ws_bytes = x.split ? x.ml_bytes + al(slots * d->hd * 4) : 0;
     // what a plan depends on (FNV-1a)
@@ -289,6 +289,7 @@ int pelica_attn_paged_plan(const PelicaPagedDesc* d, void* plan, size_t plan_byt
     p.max_pieces = (int)x.max_pieces;
     p.sig = x.sig;
     p.split = x.split;
+    p.max_slots = pelica::plan_slots(x.fill);
     const hipError_t e = pelica::launch_paged_plan(p, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_plan launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;

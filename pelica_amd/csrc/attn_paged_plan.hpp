@@ -2,6 +2,8 @@
 // kernels and in a host test: which keys a block of query rows walks, which rows
 // of a cache page a load may touch, how the work list is cut.
 #pragma once
+#include <math.h>
+
 #include <cstddef>
 #include <cstdint>
 
@@ -20,10 +22,28 @@ namespace pelica {
 constexpr int kNarrowRows = 32;
 PELICA_HD constexpr int wide_rows(int hd) { return hd == 64 ? 256 : 128; }
 
-// The least cost of a piece of an item, in chunks a narrow workgroup walks
-// (32 keys a wave each); a wide workgroup's chunk counts kWideCost of them.
-constexpr int kWideCost = 4;
+// Costs of the work list, in the time a narrow workgroup's wave takes for a
+// chunk of 32 keys (~0.45 us): a wide workgroup's chunk (1.3 us at both head
+// dims, two workgroups a CU), the least cost of a piece, a piece's start and
+// end, and the partials that a split item's piece writes and the join reads.
+constexpr int kWideCost = 3;
 constexpr int kMinPiece = 4;
+struct PlanCost {
+    // a piece's own time, and what it takes of the whole chip's
+    static PELICA_HD float piece(bool wide, int chunks) {
+        return (float)(wide ? kWideCost * chunks + 10 : ((chunks + 3) & ~3) + 10);  // (four waves share a narrow one's)
+    }
+    static PELICA_HD float share(bool wide, int chunks, bool split) {
+        return piece(wide, chunks) + (split ? wide ? 20.f : 1.f : 0.f);
+    }
+    // the step: pieces that all run at once end with the longest, which
+    // runs faster once its neighbour is done; more than that fill the gaps
+    static PELICA_HD float step(float mean, float longest, bool at_once) {
+        if (at_once) return mean + 0.6f * (longest - mean);
+        const float a = mean + 0.05f * longest, b = 0.65f * longest;
+        return a > b ? a : b;
+    }
+};
 
 // 32-key chunks of the keys that any row of an item sees: its window's and
 // the causal ones [lo, kend), and the prefix's [0, pe).  Chunks count from
@@ -82,10 +102,10 @@ PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, i
     count = imax(end - first, 0);
 }
 
-// Pieces of an item of `cost` under the piece limit L (kMinPiece .. )
-PELICA_HD int item_pieces(int cost, int n_chunks, int L) {
-    const int k = (int)(((int64_t)cost + L - 1) / L);
-    return imax(1, imin(k, n_chunks));
+// Pieces of an item of `cost` where a piece's may be 1 / inv_limit
+PELICA_HD int item_pieces(int cost, int n_chunks, float inv_limit) {
+    const float k = ceilf((float)cost * inv_limit);
+    return k >= (float)n_chunks ? n_chunks : imax(1, (int)k);
 }
 
 // most items of a step: one for each request with tokens, and one for each
@@ -96,11 +116,12 @@ inline int64_t plan_items(int64_t n_seq, int64_t n_tokens, int hpk, int hd) {
 // pieces (per kv head) that fill the chip once: two workgroups a CU
 inline int plan_fill(int n_kv, int cus) {
     const int n = (2 * cus + n_kv - 1) / n_kv;
-    return n < 1024 ? n : 1024;  // (the plan kernel holds one item a thread)
+    return n > 1 ? n : 1;
 }
-// most pieces: `fill` while the items are no more than that, else the items
-// and at most `fill` more
-inline int64_t plan_pieces(int64_t items, int fill) { return items <= fill ? fill : items + fill; }
+// most pieces that split items have together (each a slot of partials), and
+// most pieces of a step
+inline int plan_slots(int fill) { return 2 * fill; }
+inline int64_t plan_pieces(int64_t items, int fill) { return items + plan_slots(fill); }
 
 // the plan buffer: header, joins, pieces
 struct PlanHeader {

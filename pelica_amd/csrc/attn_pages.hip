@@ -15,26 +15,93 @@ namespace pelica {
 
 namespace {
 
-// Exclusive sum of one value per thread over the workgroup (NT threads),
-// and the whole sum.
-template <int NT, typename T>
-__device__ __forceinline__ T block_scan(T x, T* part, T& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T sum = x;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T y = __shfl_up(sum, off, 64);
-        if (lane >= off) sum += y;
-    }
-    __syncthreads();  // (part of the scan before is read)
+// A lane's value from another of the wave by a data-parallel move (DPP):
+// row_shr 1, 2, 4, 8 within 16 lanes, then the last lane of a row, or of two,
+// to the rows after it.  A few cycles each; a shuffle goes through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int old, int x) {
+    return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xF, false);
+}
+// inclusive sums over the wave's lanes
+__device__ __forceinline__ int wave_scan(int x) {
+    x += dpp<0x111, 0xF>(0, x);
+    x += dpp<0x112, 0xF>(0, x);
+    x += dpp<0x114, 0xF>(0, x);
+    x += dpp<0x118, 0xF>(0, x);
+    x += dpp<0x142, 0xA>(0, x);
+    x += dpp<0x143, 0xC>(0, x);
+    return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+template <typename F>
+__device__ __forceinline__ float wave_fold(float x, F f) {
+    auto at = [&](auto moved) { x = f(x, __uint_as_float(moved(__float_as_uint(x)))); };
+    at([](int v) { return dpp<0x111, 0xF>(v, v); });
+    at([](int v) { return dpp<0x112, 0xF>(v, v); });
+    at([](int v) { return dpp<0x114, 0xF>(v, v); });
+    at([](int v) { return dpp<0x118, 0xF>(v, v); });
+    at([](int v) { return dpp<0x142, 0xA>(v, v); });
+    at([](int v) { return dpp<0x143, 0xC>(v, v); });
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    // (a fold would add what a lane without a source keeps)
+    auto at = [&](auto moved) { x += __uint_as_float(moved(__float_as_uint(x))); };
+    at([](int v) { return dpp<0x111, 0xF>(0, v); });
+    at([](int v) { return dpp<0x112, 0xF>(0, v); });
+    at([](int v) { return dpp<0x114, 0xF>(0, v); });
+    at([](int v) { return dpp<0x118, 0xF>(0, v); });
+    at([](int v) { return dpp<0x142, 0xA>(0, v); });
+    at([](int v) { return dpp<0x143, 0xC>(0, v); });
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+
+// Exclusive sum of one value per thread over the workgroup (NT threads), and
+// the whole sum; part: NT / 64 values of its own for each call.
+template <int NT>
+__device__ __forceinline__ int block_scan(int x, int* part, int& total) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sum = wave_scan(x);
     if (lane == 63) part[wave] = sum;
     __syncthreads();
-    T before = 0, all = 0;
+    const int waves = wave_scan(lane < NT / 64 ? part[lane] : 0);
+    total = __builtin_amdgcn_readlane(waves, NT / 64 - 1);
+    return (wave > 0 ? __builtin_amdgcn_readlane(waves, wave > 0 ? wave - 1 : 0) : 0) + sum - x;
+}
+
+// The same where a wave's sum fits 32 bits and the workgroup's may not.
+template <int NT>
+__device__ __forceinline__ int64_t block_scan_long(int x, int* part, int64_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sum = wave_scan(x);
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    int64_t before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-        const T v = part[w];
-        if (w < wave) before += v;
-        all += v;
+        before += w < wave ? part[w] : 0;
+        all += part[w];
+    }
+    total = all;
+    return before + sum - x;
+}
+// The same for any values.
+template <int NT>
+__device__ __forceinline__ int64_t block_scan_any(int64_t x, int64_t* part, int64_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t sum = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t y = __shfl_up(sum, off, 64);
+        if (lane >= off) sum += y;
+    }
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        before += w < wave ? part[w] : 0;
+        all += part[w];
     }
     total = all;
     return before + sum - x;
@@ -52,103 +119,119 @@ __device__ __forceinline__ int find_last(const T* a, int n, T x) {
     return lo;
 }
 
+// place of a queue's entry number x in its ring
+__device__ __forceinline__ int64_t queue_at(int64_t x, int n) {
+    const int64_t r = x % n;
+    return r < 0 ? r + n : r;
+}
+
 constexpr int kPagesThreads = 256;
 
 __global__ __launch_bounds__(kPagesThreads) void pages_append_kernel(PagesParams p) {
-    __shared__ int qs[kPagedMaxSeq + 1];       // first row of each request
-    __shared__ int64_t first[kPagedMaxSeq + 1];  // its first new page's number within the step
-    __shared__ int64_t part[kPagesThreads / 64];
-    __shared__ int64_t served_end;
+    __shared__ int len[kPagedMaxSeq], add[kPagedMaxSeq];  // cached and new tokens of each request
+    __shared__ int qs[kPagedMaxSeq + 1];     // its first row
+    __shared__ int first[kPagedMaxSeq + 1];  // its first new page's number within the step
+    __shared__ int part[2 * kPagesThreads / 64];
+    __shared__ int served_end;
     const int tid = threadIdx.x;
+    // (whatever the state holds, no entry outside the list is touched)
+    const int64_t taken = p.free_in[0], given = p.free_in[1], avail = min<int64_t>(given - taken, p.n_pages);
+    if (tid == 0) served_end = 0;
+    for (int s = tid; s < p.n_seq; s += kPagesThreads) {
+        len[s] = p.cached[s];
+        add[s] = p.fresh[s];
+    }
+    __syncthreads();
+
     const int per = (p.n_seq + kPagesThreads - 1) / kPagesThreads;
     const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
-    const int64_t taken = p.free_in[0], avail = p.free_in[1] - taken;
-    const int64_t psz = 1LL << p.page_log2;
-    if (tid == 0) served_end = 0;
-
-    // rows and pages of this thread's requests
     struct Need {
-        int64_t c, n, have, pages;
-        int status;
+        int c, n, have, pages, status;
     };
+    // (n is cut off behind the last row, at 2^20 + 1 at most: such a request is
+    // refused, and 1024 of them, a wave's, sum to less than 2^31)
     auto look = [&](int s) {
         Need x;
-        const int c = p.cached[s], n = p.fresh[s];
-        x.status = c < 0 || n < 0 || (int64_t)c + n > INT32_MAX ? 4 : 0;
+        const int c = len[s], n = add[s];
+        const int64_t sum = (int64_t)c + n;
+        x.status = c < 0 || n < 0 || sum > INT32_MAX ? 4 : 0;
         x.c = x.status ? 0 : c;
-        x.n = n < 0 ? 0 : n;
-        x.have = (x.c + psz - 1) >> p.page_log2;
-        const int64_t want = (x.c + x.n + psz - 1) >> p.page_log2;
-        if (!x.status && want > p.max_pages) x.status = 2;
+        x.n = min(max(n, 0), p.n_tokens + 1);
+        const int64_t psz = 1LL << p.page_log2;
+        x.have = (int)((x.c + psz - 1) >> p.page_log2);
+        const int want = (int)((x.c + (int64_t)x.n + psz - 1) >> p.page_log2);
+        if (!x.status && (sum + psz - 1) >> p.page_log2 > p.max_pages) x.status = 2;
         x.pages = x.status ? 0 : want - x.have;
         return x;
     };
-    int64_t rows = 0;
-    for (int s = s0; s < s1; ++s) rows += look(s).n;
-    int64_t all_rows, all_pages;
-    int64_t row = block_scan<kPagesThreads>(rows, part, all_rows);
-    int64_t pages = 0;
-    {
-        int64_t r = row;
-        for (int s = s0; s < s1; ++s) {
-            const Need x = look(s);
-            r += x.n;
-            pages += r > p.n_tokens ? 0 : x.pages;  // (a request whose rows do not fit takes none)
-        }
+    // rows and pages of the requests before.  Rows run out for a request and
+    // every later one that has any, so that pages counted for it are no one
+    // else's loss.
+    int rows = 0, pages = 0;
+    for (int s = s0; s < s1; ++s) {
+        const Need x = look(s);
+        rows += x.n;
+        pages += x.pages;
     }
-    int64_t page = block_scan<kPagesThreads>(pages, part, all_pages);
+    int64_t all_rows, all_pages;
+    int64_t row = block_scan_long<kPagesThreads>(rows, part, all_rows);
+    int64_t page = block_scan_long<kPagesThreads>(pages, part + kPagesThreads / 64, all_pages);
+    int served = 0;
     for (int s = s0; s < s1; ++s) {
         Need x = look(s);
         qs[s] = (int)min<int64_t>(row, p.n_tokens);
+        first[s] = (int)page;
         row += x.n;
-        if (row > p.n_tokens && x.n > 0 && x.status == 0) x.status = 3;
-        if (x.status == 3) x.pages = 0;
-        first[s] = page;
         page += x.pages;
-        if (x.status == 0 && x.pages > 0 && page > avail) x.status = 1;
-        if (x.status == 0 && x.pages > 0) atomicMax((unsigned long long*)&served_end, (unsigned long long)page);
-        // (the requests that go unserved for want of pages are those behind avail)
+        if (x.status == 0 && x.n > 0 && row > p.n_tokens) x.status = 3;
+        if (x.status == 0 && x.pages > 0) {
+            if (page > avail) x.status = 1;
+            else served = (int)page;
+        }
         if (blockIdx.x == 0) {
             p.q_start[s] = qs[s];
-            p.kv_len[s] = x.status ? 0 : (int)(x.c + x.n);
+            p.kv_len[s] = x.status ? 0 : x.c + x.n;
             p.status[s] = x.status;
         }
     }
+    // (the requests that get their pages are the first ones that need any)
+    if (served > 0) atomicMax(&served_end, served);
     if (tid == 0) {
         qs[p.n_seq] = (int)min<int64_t>(all_rows, p.n_tokens);
-        first[p.n_seq] = all_pages;
+        first[p.n_seq] = (int)all_pages;
     }
     __syncthreads();
     if (blockIdx.x == 0 && tid == 0) {
         p.q_start[p.n_seq] = qs[p.n_seq];
         p.free_out[0] = taken + served_end;
-        p.free_out[1] = taken + avail;
+        p.free_out[1] = given;
     }
     // page number i of the step, a queue entry
-    auto entry = [&](int64_t i) {
-        const int id = p.list[(taken + i) % p.n_pages];
+    const int64_t begin = queue_at(taken, p.n_pages);
+    auto entry = [&](int i) {
+        int64_t j = begin + i;
+        if (j >= p.n_pages) j -= p.n_pages;  // (fewer pages than the queue has are taken)
+        const int id = p.list[j];
         return (unsigned)id < (unsigned)p.n_pages ? id : -1;
     };
+    const int nt = gridDim.x * kPagesThreads, g = blockIdx.x * kPagesThreads + tid;
     // new pages into the table
-    const int64_t nt = (int64_t)gridDim.x * kPagesThreads, g = (int64_t)blockIdx.x * kPagesThreads + tid;
-    for (int64_t i = g; i < served_end; i += nt) {
+    for (int i = g; i < served_end; i += nt) {
         const int s = find_last(first, p.n_seq, i);
-        const Need x = look(s);
-        p.table[(size_t)s * p.max_pages + x.have + (i - first[s])] = entry(i);
+        const int have = (int)(((int64_t)len[s] + (1LL << p.page_log2) - 1) >> p.page_log2);
+        p.table[(size_t)s * p.max_pages + have + (i - first[s])] = entry(i);
     }
     // rows
-    for (int64_t i = g; i < p.n_tokens; i += nt) {
+    for (int i = g; i < p.n_tokens; i += nt) {
         int64_t slot = -1;
         int pos = 0, seq = -1;
         if (i < qs[p.n_seq]) {
-            const int s = find_last(qs, p.n_seq, (int)i);
+            const int s = find_last(qs, p.n_seq, i);
             const Need x = look(s);
-            const int64_t at = x.c + (i - qs[s]);
-            pos = (int)at;
+            pos = x.c + (i - qs[s]);
             seq = s;
-            const bool fits = x.status == 0 && qs[s] + x.n <= p.n_tokens;
-            if (fits && (x.pages == 0 || first[s] + x.pages <= avail)) {
-                const int64_t j = at >> p.page_log2;
+            if (x.status == 0 && qs[s] + x.n <= p.n_tokens && (x.pages == 0 || first[s] + x.pages <= avail)) {
+                const int j = pos >> p.page_log2;
                 int id;
                 if (j < x.have) {
                     id = p.table[(size_t)s * p.max_pages + j];
@@ -156,7 +239,7 @@ __global__ __launch_bounds__(kPagesThreads) void pages_append_kernel(PagesParams
                 } else {
                     id = entry(first[s] + j - x.have);
                 }
-                if (id >= 0) slot = ((int64_t)id << p.page_log2) + (at & (psz - 1));
+                if (id >= 0) slot = ((int64_t)id << p.page_log2) + (pos & ((1 << p.page_log2) - 1));
             }
         }
         p.slots[i] = slot;
@@ -166,84 +249,97 @@ __global__ __launch_bounds__(kPagesThreads) void pages_append_kernel(PagesParams
 }
 
 __global__ __launch_bounds__(kPagesThreads) void pages_release_kernel(PagesParams p) {
+    __shared__ int count[kPagedMaxSeq];  // pages each request gives back
     __shared__ int64_t first[kPagedMaxSeq + 1];
     __shared__ int64_t part[kPagesThreads / 64];
     const int tid = threadIdx.x;
-    const int per = (p.n_seq + kPagesThreads - 1) / kPagesThreads;
-    const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
     const int64_t taken = p.free_in[0], given = p.free_in[1];
-    auto held = [&](int s) -> int64_t {
-        if (p.ended[s] == 0 || p.cached[s] <= 0) return 0;
-        return min<int64_t>(((int64_t)p.cached[s] + (1LL << p.page_log2) - 1) >> p.page_log2, p.max_pages);
-    };
-    int64_t n = 0, total;
-    for (int s = s0; s < s1; ++s) n += held(s);
-    int64_t at = block_scan<kPagesThreads>(n, part, total);
-    for (int s = s0; s < s1; ++s) {
-        first[s] = at;
-        at += held(s);
+    for (int s = tid; s < p.n_seq; s += kPagesThreads) {
+        const int64_t held = ((int64_t)p.cached[s] + (1LL << p.page_log2) - 1) >> p.page_log2;
+        count[s] = p.ended[s] == 0 || p.cached[s] <= 0 ? 0 : (int)min<int64_t>(held, p.max_pages);
     }
     __syncthreads();
-    if (given - taken + total > p.n_pages) total = 0;
+    const int per = (p.n_seq + kPagesThreads - 1) / kPagesThreads;
+    const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
+    int64_t n = 0, total;
+    for (int s = s0; s < s1; ++s) n += count[s];
+    int64_t at = block_scan_any<kPagesThreads>(n, part, total);
+    for (int s = s0; s < s1; ++s) {
+        first[s] = at;
+        at += count[s];
+    }
+    __syncthreads();
+    if (given - taken + total > p.n_pages || total > p.n_pages) total = 0;
     if (blockIdx.x == 0 && tid == 0) {
         p.free_out[0] = taken;
         p.free_out[1] = given + total;
     }
+    const int64_t begin = queue_at(given, p.n_pages);
     for (int64_t i = (int64_t)blockIdx.x * kPagesThreads + tid; i < total; i += (int64_t)gridDim.x * kPagesThreads) {
         const int s = find_last(first, p.n_seq, i);
-        p.list[(given + i) % p.n_pages] = p.table[(size_t)s * p.max_pages + (i - first[s])];
+        const int64_t j = begin + i;
+        p.list[j >= p.n_pages ? j - p.n_pages : j] = p.table[(size_t)s * p.max_pages + (i - first[s])];
     }
 }
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanItems = 4096;  // items whose costs are weighed against each other
+
+constexpr int kBuckets = 128;     // of pieces' costs, four to a doubling, narrow and wide
 
 // The work list.  Items (requests' blocks of query rows) cost the chunks they
-// walk; where the items are fewer than fill the chip, the smallest piece
-// limit is taken whose pieces are no more than fill it, so that all
-// workgroups end together; else only items of over twice the mean share are
-// cut.  An item's pieces are equal in chunks.
+// walk; an item of k pieces is cut into equal ranges of them by a limit on a
+// piece's cost.  Limits are weighed, a wave each, by the time that the step
+// would take (PlanCost).
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) {
-    __shared__ int item0[kPagedMaxSeq + 1];     // first item of each request
-    __shared__ int64_t part[kPlanThreads / 64];
-    __shared__ int piece0[kPlanThreads + 1], slot0[kPlanThreads];
-    const int tid = threadIdx.x;
-    const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads;
-    const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
+    __shared__ int item0[kPagedMaxSeq + 1];  // first item of each request
+    __shared__ int q0[kPagedMaxSeq + 1], kv[kPagedMaxSeq], pre[kPagedMaxSeq];  // q_start, kv_len, prefix
+    __shared__ int costs[kPlanItems];
+    __shared__ int part[4][kPlanWaves];
+    __shared__ float est[2][kPlanWaves], limit[2][kPlanWaves];
+    __shared__ int at_bucket[kBuckets];
+    __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int W = wide_rows(p.hd);
+    for (int s = tid; s <= p.n_seq; s += kPlanThreads) {
+        q0[s] = p.q_start[s];
+        if (s < p.n_seq) {
+            kv[s] = p.kv_len[s];
+            pre[s] = p.prefix ? p.prefix[s] : 0;
+        }
+    }
+    if (tid < kBuckets) at_bucket[tid] = 0;
+    __syncthreads();
 
-    struct Seq {
-        int q0, T, len, prefix;
+    // tokens of a request; 0: no item (none, or lengths that do not fit together)
+    auto tokens = [&](int s) {
+        const int64_t a = q0[s], b = q0[s + 1], T = b - a;
+        const bool ok = a >= 0 && b <= p.n_tokens && T > 0 && T <= p.max_q && kv[s] >= T && kv[s] <= p.max_keys;
+        return ok ? (int)T : 0;
     };
-    // T = 0: no item (no tokens, or lengths that do not fit together)
-    auto seq = [&](int s) {
-        Seq x;
-        x.q0 = p.q_start[s];
-        const int64_t q1 = p.q_start[s + 1];
-        x.len = p.kv_len[s];
-        x.prefix = p.prefix ? p.prefix[s] : 0;
-        const int64_t T = q1 - x.q0;
-        const bool ok = x.q0 >= 0 && q1 <= p.n_tokens && T > 0 && T <= p.max_q && x.len >= T && x.len <= p.max_keys;
-        x.T = ok ? (int)T : 0;
-        return x;
-    };
-    auto items_of = [&](const Seq& x) {
-        const int R = x.T * p.hpk;
+    auto items_of = [&](int T) {
+        const int R = T * p.hpk;
         return R <= kNarrowRows ? (R > 0 ? 1 : 0) : (R + W - 1) / W;
     };
-    int64_t n = 0, total;
-    for (int s = s0; s < s1; ++s) n += items_of(seq(s));
-    int64_t at = block_scan<kPlanThreads>(n, part, total);
-    const int n_items = (int)total;
+    const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads;
+    const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
+    int n = 0, n_items;
+    for (int s = s0; s < s1; ++s) n += items_of(tokens(s));
+    int at = block_scan<kPlanThreads>(n, part[0], n_items);
     for (int s = s0; s < s1; ++s) {
-        item0[s] = (int)at;
-        at += items_of(seq(s));
+        item0[s] = at;
+        at += items_of(tokens(s));
     }
     if (tid == 0) item0[p.n_seq] = n_items;
     __syncthreads();
 
+    // r / hpk (r < 2^30), as (r + 1/2) / hpk in f64: at least 1 / (2 hpk) from
+    // a whole number, hpk <= 2^16
+    const double inv_hpk = 1.0 / p.hpk;
+    auto token = [&](int r) { return (int)(((double)r + 0.5) * inv_hpk); };
     struct Item {
-        Seq q;
-        int s, r0, R, cost;
+        int s, T, r0, R, cost;
         ItemKeys k;
     };
     auto item = [&](int i) {
@@ -251,110 +347,168 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         // (requests without items share their first item with the next one:
         // the last of them is the one that has it)
         x.s = find_last(item0, p.n_seq, i);
-        x.q = seq(x.s);
-        x.R = x.q.T * p.hpk;
+        x.T = tokens(x.s);
+        x.R = x.T * p.hpk;
         const bool narrow = x.R <= kNarrowRows;
-        // a prompt's last block, the longest, first
-        x.r0 = narrow ? 0 : (item0[x.s + 1] - 1 - i) * W;
+        x.r0 = narrow ? 0 : (i - item0[x.s]) * W;
         const int rows = narrow ? x.R : imin(W, x.R - x.r0);
-        const int pos0 = x.q.len - x.q.T;
-        x.k = item_keys(pos0 + x.r0 / p.hpk, pos0 + (x.r0 + rows - 1) / p.hpk, x.q.len, p.window, x.q.prefix);
+        const int pos0 = kv[x.s] - x.T;
+        x.k = item_keys(pos0 + token(x.r0), pos0 + token(x.r0 + rows - 1), kv[x.s], p.window, pre[x.s]);
         x.cost = x.k.n_chunks * (narrow ? 1 : kWideCost);
         return x;
     };
+    // this thread's first item, the only one of most steps
+    const Item own = tid < n_items ? item(tid) : Item{};
+    auto item_at = [&](int i) { return i < kPlanThreads ? own : item(i); };
 
-    int64_t cost = 0;
-    Item mine{};
-    for (int i = tid; i < n_items; i += kPlanThreads) {
-        mine = item(i);
-        cost += mine.cost;
-    }
-    block_scan<kPlanThreads>(cost, part, total);
-    int64_t L = kMinPiece;
+    auto piece = [&](const Item& y, int of, int nth, int slot) {
+        PlanPiece z;
+        z.seq = y.s;
+        z.q0 = q0[y.s];
+        z.R = y.R;
+        z.r0 = y.r0;
+        z.pos0 = kv[y.s] - y.T;
+        z.len = kv[y.s];
+        z.cb = (int)((int64_t)y.k.n_chunks * nth / of);
+        z.ce = (int)((int64_t)y.k.n_chunks * (nth + 1) / of);
+        z.slot = slot;
+        z.n_pre = y.k.n_pre;
+        z.lo_base = y.k.lo_base;
+        z.lo = y.k.lo;
+        z.kend = y.k.kend;
+        z.pe = y.k.pe;
+        z.pad[0] = z.pad[1] = 0;
+        return z;
+    };
+    auto header = [&](int pieces, int joins) {
+        PlanHeader h{};
+        h.sig = p.sig;
+        h.n_pieces = min(pieces, p.max_pieces);
+        h.n_joins = min(joins, p.max_joins);
+        return h;
+    };
+    // Narrow pieces start first, longest first: they wait for memory while
+    // the wide ones beside them keep the matrix cores busy
+    auto bucket_of = [&](const Item& x, int k) {
+        const int c = min(kBuckets / 2 - 1, max(0, (int)(__float_as_uint((float)x.cost / (float)k) >> 21) - (127 << 2)));
+        return (x.R <= kNarrowRows ? kBuckets / 2 - 1 : kBuckets - 1) - c;
+    };
+    // a step that is not split: an item a piece, in order
     if (!p.split) {
-        L = INT32_MAX;
-    } else if (n_items > p.fill) {
-        L = max<int64_t>(kMinPiece, 2 * ((total + p.fill - 1) / p.fill));
-    } else if (n_items > 0) {
-        // (fill <= kPlanThreads: one item a thread)
-        // (at total / (fill - items) the pieces, at most total / L + items, fit)
-        int64_t lo = max<int64_t>(kMinPiece, (total + p.fill - 1) / p.fill);
-        int64_t hi = max(lo, p.fill > n_items ? (total + p.fill - n_items - 1) / (p.fill - n_items) : total);
-        lo = min<int64_t>(lo, INT32_MAX);
-        hi = min<int64_t>(hi, INT32_MAX);
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) >> 1;
-            int64_t pieces;
-            block_scan<kPlanThreads>((int64_t)(tid < n_items ? item_pieces(mine.cost, mine.k.n_chunks, (int)mid) : 0), part, pieces);
-            if (pieces <= p.fill) hi = mid;
-            else lo = mid + 1;
-        }
-        L = lo;
+        for (int i = tid; i < n_items; i += kPlanThreads)
+            if (i < p.max_pieces) p.pieces[i] = piece(item_at(i), 1, 0, -1);
+        if (tid == 0) *p.head = header(n_items, 0);
+        return;
     }
-    L = min<int64_t>(L, INT32_MAX);
 
-    int base_piece = 0, base_slot = 0, base_join = 0;
+    float inv_limit = 0.f;  // (no limit)
+    if (n_items > 0 && n_items <= kPlanItems) {
+        // (a wide item's cost is negative: kWideCost a chunk, and a multiple)
+        for (int i = tid; i < n_items; i += kPlanThreads) {
+            const Item x = item_at(i);
+            costs[i] = x.R <= kNarrowRows ? x.cost : -x.cost;
+        }
+        __syncthreads();
+        float total = 0.f;
+        for (int i = lane; i < n_items; i += 64) total += (float)abs(costs[i]);
+        const float share = fmaxf(wave_sum(total) / (float)p.fill, (float)kMinPiece);
+        // wave w's limit: 0.5 .. 3 shares, the last wave's none; then finer about
+        // the best
+        float step = 2.58f / (kPlanWaves - 2);
+        float mine = wave == kPlanWaves - 1 ? 1e9f : share * 0.5f * fast_exp2((float)wave * step);
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+            mine = fmaxf(mine, (float)kMinPiece);
+            const float inv = 1.f / mine;
+            float time = 0.f, longest = 0.f;
+            int pieces = 0, slots = 0;
+            for (int i = lane; i < n_items; i += 64) {
+                const int c = abs(costs[i]);
+                const bool wide = costs[i] < 0;
+                const int chunks = wide ? c / kWideCost : c;
+                const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
+                time += PlanCost::share(wide, m, k > 1) * (float)k;
+                longest = fmaxf(longest, PlanCost::piece(wide, m));
+                pieces += k;
+                slots += k > 1 ? k : 0;
+            }
+            time = wave_sum(time);
+            longest = wave_fold(longest, [](float a, float b) { return fmaxf(a, b); });
+            pieces = wave_sum(pieces);
+            slots = wave_sum(slots);
+            if (lane == 0) {
+                est[round][wave] = slots <= p.max_slots
+                                       ? PlanCost::step(time / (float)p.fill, longest, pieces <= p.fill) : INFINITY;
+                limit[round][wave] = mine;
+            }
+            __syncthreads();
+            float best = INFINITY, l0 = 1e9f;
+#pragma unroll
+            for (int w = 0; w < kPlanWaves; ++w) {
+                const float e = est[round][w];
+                l0 = e < best ? limit[round][w] : l0;
+                best = fminf(best, e);
+            }
+            // (the last wave's limit splits nothing, and is always one to take)
+            if (round == 0) mine = l0 >= 1e9f ? l0 : l0 * fast_exp2(step * (2.f / kPlanWaves) * (float)(wave - kPlanWaves / 2));
+            else inv_limit = 1.f / l0;
+        }
+    }
+
+    // where each bucket's pieces begin
+    for (int i = tid; i < n_items; i += kPlanThreads) {
+        const Item x = item_at(i);
+        const int k = item_pieces(x.cost, x.k.n_chunks, inv_limit);
+        atomicAdd(&at_bucket[bucket_of(x, k)], k);
+    }
+    __syncthreads();
+    if (wave == 0) {
+        static_assert(kBuckets == 128, "two buckets a lane");
+        const int a = at_bucket[2 * lane], b = at_bucket[2 * lane + 1], sum = wave_scan(a + b);
+        at_bucket[2 * lane] = sum - a - b;
+        at_bucket[2 * lane + 1] = sum - b;
+    }
+    __syncthreads();
+
+    int n_pieces = 0, base_slot = 0, base_join = 0;
     for (int b = 0; b < n_items; b += kPlanThreads) {
         const int i = b + tid;
         Item x{};
         int k = 0;
         if (i < n_items) {
-            x = item(i);
-            k = item_pieces(x.cost, x.k.n_chunks, (int)L);
+            x = item_at(i);
+            k = item_pieces(x.cost, x.k.n_chunks, inv_limit);
         }
-        // pieces, split pieces and split items of the items before, packed
-        int64_t all;
-        const int64_t mine3 = k | (k > 1 ? (int64_t)k << 24 | (int64_t)1 << 48 : 0);
-        const int64_t sum = block_scan<kPlanThreads>(mine3, part, all);
-        const int pc = base_piece + (int)(sum & 0xFFFFFF), sl = base_slot + (int)((sum >> 24) & 0xFFFFFF),
-                  jn = base_join + (int)(sum >> 48);
+        // pieces of the items before, and split items' pieces and items
+        int all, slots, joins;
+        const int pc = block_scan<kPlanThreads>(k, part[1], all);
+        const int sl = base_slot + block_scan<kPlanThreads>(k > 1 ? k : 0, part[2], slots);
+        const int jn = base_join + block_scan<kPlanThreads>(k > 1 ? 1 : 0, part[3], joins);
         piece0[tid] = pc;
+        place[tid] = k > 0 ? atomicAdd(&at_bucket[bucket_of(x, k)], k) : 0;
         slot0[tid] = k > 1 ? sl : -1;
-        if (tid == 0) piece0[kPlanThreads] = base_piece + (int)(all & 0xFFFFFF);
-        if (k > 1 && jn < p.max_joins) p.joins[jn] = PlanJoin{x.q.q0, x.R, x.r0, sl, k, {}};
+        if (k > 1 && jn < p.max_joins) p.joins[jn] = PlanJoin{q0[x.s], x.R, x.r0, sl, k, {}};
         __syncthreads();
-        const int n_here = min(kPlanThreads, n_items - b), end = piece0[kPlanThreads];
-        for (int j = base_piece + tid; j < end && j < p.max_pieces; j += kPlanThreads) {
+        const int n_here = min(kPlanThreads, n_items - b);
+        for (int j = tid; j < all; j += kPlanThreads) {
             const int t = find_last(piece0, n_here, j);
             const Item y = item(b + t);
-            const int of = item_pieces(y.cost, y.k.n_chunks, (int)L), at_ = j - piece0[t];
-            PlanPiece z;
-            z.seq = y.s;
-            z.q0 = y.q.q0;
-            z.R = y.R;
-            z.r0 = y.r0;
-            z.pos0 = y.q.len - y.q.T;
-            z.len = y.q.len;
-            z.cb = (int)((int64_t)y.k.n_chunks * at_ / of);
-            z.ce = (int)((int64_t)y.k.n_chunks * (at_ + 1) / of);
-            z.slot = slot0[t] < 0 ? -1 : slot0[t] + at_;
-            z.n_pre = y.k.n_pre;
-            z.lo_base = y.k.lo_base;
-            z.lo = y.k.lo;
-            z.kend = y.k.kend;
-            z.pe = y.k.pe;
-            z.pad[0] = z.pad[1] = 0;
-            p.pieces[j] = z;
+            const int of = item_pieces(y.cost, y.k.n_chunks, inv_limit), nth = j - piece0[t];
+            if (place[t] + nth < p.max_pieces)
+                p.pieces[place[t] + nth] = piece(y, of, nth, slot0[t] < 0 ? -1 : slot0[t] + nth);
         }
-        base_piece = end;
-        base_slot += (int)((all >> 24) & 0xFFFFFF);
-        base_join += (int)(all >> 48);
+        n_pieces += all;
+        base_slot += slots;
+        base_join += joins;
         __syncthreads();
     }
-    if (tid == 0) {
-        PlanHeader h{};
-        h.sig = p.sig;
-        h.n_pieces = min(base_piece, p.max_pieces);
-        h.n_joins = min(base_join, p.max_joins);
-        *p.head = h;
-    }
+    if (tid == 0) *p.head = header(n_pieces, base_join);
 }
 
 }  // namespace
 
 hipError_t launch_pages_append(const PagesParams& p, hipStream_t st) {
-    // a workgroup for each 1024 rows (its scan is paid once for them)
-    const int grid = p.n_tokens <= 1024 ? 1 : min((p.n_tokens + 1023) / 1024, 256);
+    const int grid = min((p.n_tokens + kPagesThreads - 1) / kPagesThreads, 256);
     ProfScope ps(kProfPages, st);
     hipLaunchKernelGGL(pages_append_kernel, dim3(grid), dim3(kPagesThreads), 0, st, p);
     return hipGetLastError();
@@ -362,7 +516,7 @@ hipError_t launch_pages_append(const PagesParams& p, hipStream_t st) {
 
 hipError_t launch_pages_release(const PagesParams& p, hipStream_t st) {
     ProfScope ps(kProfPages, st);
-    hipLaunchKernelGGL(pages_release_kernel, dim3(p.n_seq <= 64 ? 1 : 8), dim3(kPagesThreads), 0, st, p);
+    hipLaunchKernelGGL(pages_release_kernel, dim3(p.n_seq <= 64 ? 4 : 16), dim3(kPagesThreads), 0, st, p);
     return hipGetLastError();
 }
 

@@ -39,16 +39,24 @@ def _need(ok, message: str) -> None:
         raise AttnError(EINVAL, message)
 
 
-_device = None
+_torch = None
+_device = None  # () -> the current device's index
+
+
+def _start():
+    """The names that a call looks up."""
+    global _torch, _device
+    import torch
+
+    _device = torch._C._cuda_getDevice if torch.cuda.is_available() else lambda: -1
+    _torch = torch
+    return torch
 
 
 def _check(name: str, t, dtype, dim: Optional[int] = None, dense: bool = True):
     """A tensor argument: its type, dims, layout, and that it is on the current device."""
-    global _device
-    if _device is None:
-        import torch
-
-        _device = torch._C._cuda_getDevice if torch.cuda.is_available() else lambda: -1
+    if _torch is None:
+        _start()
     if t.dtype is not dtype or not t.is_cuda or (dim is not None and t.dim() != dim) or (
             dense and not t.is_contiguous()) or t.get_device() != _device():
         raise AttnError(EINVAL, f"{name}: a {'contiguous ' if dense else ''}{dtype} tensor"
@@ -84,22 +92,33 @@ class PageStep:
         self.positions = torch.zeros(n_tokens, **i32)
         self.token_seq = torch.full((n_tokens,), -1, **i32)
         self.free_state = torch.zeros(2, dtype=torch.int64, device=device)
+        self.device = self.slots.get_device()
         self._out = tuple(t.data_ptr() for t in (self.free_state, self.q_start, self.seq_kv_len, self.slots,
                                                  self.positions, self.token_seq, self.status))
 
 
-def _page_args(lens, page_table, free_list, free_state, page_size, n_tokens):
+def _pages_ok(dev, n_seq, a, b, page_table, free_list, free_state) -> bool:
+    i32 = _torch.int32
+    return (a.dtype is i32 and b.dtype is i32 and page_table.dtype is i32 and free_list.dtype is i32
+            and free_state.dtype is _torch.int64 and a.get_device() == dev and b.get_device() == dev
+            and page_table.get_device() == dev and free_list.get_device() == dev and free_state.get_device() == dev
+            and a.dim() == 1 and b.dim() == 1 and free_list.dim() == 1 and a.numel() == n_seq and b.numel() == n_seq
+            and free_state.numel() == 2 and a.is_contiguous() and b.is_contiguous() and page_table.is_contiguous()
+            and free_list.is_contiguous() and free_state.is_contiguous())
+
+
+def _refuse_pages(lens, page_table, free_list, free_state):
+    """Names what is wrong with the arguments of a call over pages."""
     import torch
 
-    n_seq = page_table.shape[0]
     _check("page_table", page_table, torch.int32, 2)
     _check("free_list", free_list, torch.int32, 1)
     _check("free_state", free_state, torch.int64, 1)
     _need(free_state.numel() == 2, "free_state: two values")
     for name, t in lens:
         _check(name, t, torch.int32, 1)
-        _need(t.numel() == n_seq, f"{name}: one value for each of the {n_seq} rows of page_table")
-    return PageDesc(n_seq, n_tokens, page_size, free_list.numel(), page_table.shape[1])
+        _need(t.numel() == page_table.shape[0], f"{name}: one value for each of the {page_table.shape[0]} rows of page_table")
+    raise AttnError(EINVAL, "arguments of a call over pages")
 
 
 def pages_append(cached_len, new_len, page_table, free_list, free_state, *, page_size: int,
@@ -110,19 +129,27 @@ def pages_append(cached_len, new_len, page_table, free_list, free_state, *, page
     [n_pages] and its queue ends ``free_state`` int64 [2].  Returns ``step``, or
     a new PageStep of ``n_tokens`` rows; its ``free_state`` is the next call's
     (of another PageStep: a call's may not be its own input)."""
+    if _torch is None:
+        _start()
+    _need(page_table.dim() == 2, "page_table: [n_seq, max_pages]")
+    n_seq, max_pages = page_table.shape
+    dev = _device()
+    if not _pages_ok(dev, n_seq, cached_len, new_len, page_table, free_list, free_state):
+        _refuse_pages((("cached_len", cached_len), ("new_len", new_len)), page_table, free_list, free_state)
     if step is None:
         _need(n_tokens is not None, "n_tokens or step is needed")
         with _on(stream):
-            step = PageStep(page_table.shape[0], n_tokens, page_table.device)
-    _need(n_tokens is None or n_tokens == step.n_tokens, "n_tokens is the step's")
-    desc = _page_args((("cached_len", cached_len), ("new_len", new_len)), page_table, free_list, free_state, page_size,
-                      step.n_tokens)
-    _need(step.n_seq == desc.n_seq, "step: made for another number of requests")
-    _need(step.q_start.device == page_table.device, "step: on another device")
-    lib = attn.load_library()
-    attn._check(lib.pelica_attn_pages_append(ctypes.byref(desc), cached_len.data_ptr(), new_len.data_ptr(),
-                                             page_table.data_ptr(), free_list.data_ptr(), free_state.data_ptr(),
-                                             *step._out, attn._stream_ptr(stream)))
+            step = PageStep(n_seq, n_tokens, page_table.device)
+    if step.n_seq != n_seq or step.device != dev or not (n_tokens is None or n_tokens == step.n_tokens):
+        raise AttnError(EINVAL, f"step: made for {step.n_seq} requests and {step.n_tokens} rows on device {step.device}, "
+                                f"called with {n_seq}, {n_tokens} on {dev}")
+    desc = PageDesc(n_seq, step.n_tokens, page_size, free_list.numel(), max_pages)
+    lib = attn._lib or attn.load_library()
+    rc = lib.pelica_attn_pages_append(ctypes.byref(desc), cached_len.data_ptr(), new_len.data_ptr(),
+                                      page_table.data_ptr(), free_list.data_ptr(), free_state.data_ptr(), *step._out,
+                                      attn._stream_ptr(stream))
+    if rc:
+        attn._check(rc)
     return step
 
 
@@ -131,40 +158,43 @@ def pages_release(ended, cached_len, page_table, free_list, free_state, *, page_
     """Gives the pages of the requests with ``ended[s] != 0`` back to the free
     list (pelica_attn_pages_release).  Returns ``free_out``, the queue ends
     after it (int64 [2], another tensor than ``free_state``)."""
-    import torch
-
+    if _torch is None:
+        _start()
+    _need(page_table.dim() == 2, "page_table: [n_seq, max_pages]")
+    n_seq, max_pages = page_table.shape
+    if not _pages_ok(_device(), n_seq, ended, cached_len, page_table, free_list, free_state):
+        _refuse_pages((("ended", ended), ("cached_len", cached_len)), page_table, free_list, free_state)
     if free_out is None:
         with _on(stream):
-            free_out = torch.empty_like(free_state)
-    _check("free_out", free_out, torch.int64, 1)
+            free_out = _torch.empty_like(free_state)
+    _check("free_out", free_out, _torch.int64, 1)
     _need(free_out.numel() == 2, "free_out: two values")
-    desc = _page_args((("ended", ended), ("cached_len", cached_len)), page_table, free_list, free_state, page_size, 1)
-    lib = attn.load_library()
-    attn._check(lib.pelica_attn_pages_release(ctypes.byref(desc), ended.data_ptr(), cached_len.data_ptr(),
-                                              page_table.data_ptr(), free_list.data_ptr(), free_state.data_ptr(),
-                                              free_out.data_ptr(), attn._stream_ptr(stream)))
+    desc = PageDesc(n_seq, 1, page_size, free_list.numel(), max_pages)
+    lib = attn._lib or attn.load_library()
+    rc = lib.pelica_attn_pages_release(ctypes.byref(desc), ended.data_ptr(), cached_len.data_ptr(),
+                                       page_table.data_ptr(), free_list.data_ptr(), free_state.data_ptr(),
+                                       free_out.data_ptr(), attn._stream_ptr(stream))
+    if rc:
+        attn._check(rc)
     return free_out
 
 
-def _pool(name, t, shape=None):
-    """The strides of a pool of pages: (page, row, head)."""
-    import torch
-
-    _check(name, t, torch.float16, 4, dense=False)
-    st = t.stride()
-    _need(st[3] == 1 and (shape is None or t.shape == shape), f"{name}: [n_pages, page_size, n_kv, hd] pages whose hd "
-          f"values are contiguous, alike for k and v; got {tuple(t.shape)} strides {tuple(st)}")
+def _pools(k_pages, v_pages, dev):
+    """The strides of both pools of pages: (page, row, head)."""
+    st = k_pages.stride()
+    if not (k_pages.dtype is _torch.float16 and v_pages.dtype is _torch.float16 and len(st) == 4 and st[3] == 1
+            and v_pages.stride() == st and k_pages.shape == v_pages.shape and k_pages.get_device() == dev
+            and v_pages.get_device() == dev):
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _check(name, t, _torch.float16, 4, dense=False)
+        raise AttnError(EINVAL, "k_pages and v_pages: [n_pages, page_size, n_kv, hd] pages whose hd values are contiguous, "
+                                f"one layout for both; got {tuple(k_pages.shape)} strides {tuple(st)} and "
+                                f"{tuple(v_pages.shape)} strides {tuple(v_pages.stride())}")
     # (a dim of one has no stride of its own)
-    return st[0] if t.shape[0] > 1 else 0, st[1], st[2] if t.shape[2] > 1 else 0
+    return st[0] if k_pages.shape[0] > 1 else 0, st[1], st[2] if k_pages.shape[2] > 1 else 0
 
 
-def _pools(k_pages, v_pages):
-    a, b = _pool("k_pages", k_pages), _pool("v_pages", v_pages, k_pages.shape)
-    _need(a == b, f"k_pages and v_pages: one layout for both, got strides {a} and {b}")
-    return a
-
-
-def _rows(name, t, dim=3):
+def _rows(name, t):
     """The stride of token rows [n, heads, hd] (0: dense)."""
     if t.is_contiguous():
         return 0
@@ -202,6 +232,9 @@ class PagedPlan:
         if n == 0:
             raise AttnError(EINVAL, lib.pelica_attn_last_error().decode(errors="replace"))
         self.device = page_table.device
+        self._dev = page_table.get_device()
+        self._q_shape = (n_tokens, n_head, hd)
+        self._page_shape = (n_pages, page_size, n_kv, hd)
         with _on(stream):
             self.buffer = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.workspace_bytes = lib.pelica_attn_paged_workspace_bytes(ctypes.byref(self.desc))
@@ -209,9 +242,12 @@ class PagedPlan:
 
     def update(self, stream=None) -> "PagedPlan":
         """Make the work list from the arrays' present contents."""
-        _check("page_table", self._keep[2], self._keep[2].dtype)
-        attn._check(attn.load_library().pelica_attn_paged_plan(ctypes.byref(self.desc), self.buffer.data_ptr(),
-                                                               self.buffer.numel(), attn._stream_ptr(stream)))
+        if _device() != self._dev:
+            raise AttnError(EINVAL, f"the plan is on device {self._dev}, the current device is {_device()}")
+        rc = (attn._lib or attn.load_library()).pelica_attn_paged_plan(
+            ctypes.byref(self.desc), self.buffer.data_ptr(), self.buffer.numel(), attn._stream_ptr(stream))
+        if rc:
+            attn._check(rc)
         return self
 
     def new_workspace(self):
@@ -230,43 +266,56 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
     distance bias; ``softcap`` c: scores c tanh(s / c).  Returns q's type;
     rows of requests without tokens or with lengths that do not fit, and rows
     behind the last, are left as they were (undefined in a new ``out``)."""
-    import torch
-
-    d = plan.desc
-    f32 = q.dtype is torch.float32
-    _need(f32 or q.dtype is torch.float16, f"q: f16 or f32, got {q.dtype}")
-    shape = (d.n_tokens, d.n_head, d.hd)
-    _check("q", q, q.dtype, 3, dense=False)
-    _need(q.shape == shape, f"q: {shape} as planned, got {tuple(q.shape)}")
-    page, row, head = _pools(k_pages, v_pages)
-    _need(k_pages.shape == (d.n_pages, d.page_size, d.n_kv, d.hd),
-          f"k_pages: {(d.n_pages, d.page_size, d.n_kv, d.hd)} as planned, got {tuple(k_pages.shape)}")
+    torch, dev, shape = _torch, plan._dev, plan._q_shape
+    dtype = q.dtype
+    f32 = dtype is torch.float32
+    if not ((f32 or dtype is torch.float16) and q.shape == shape and q.get_device() == dev and dev == _device()):
+        _need(f32 or dtype is torch.float16, f"q: f16 or f32, got {dtype}")
+        _check("q", q, dtype, 3, dense=False)
+        _need(q.shape == shape, f"q: {shape} as planned, got {tuple(q.shape)}")
+        raise AttnError(EINVAL, f"the plan is on device {dev}, q on {q.device}")
+    page, row, head = _pools(k_pages, v_pages, dev)
+    if k_pages.shape != plan._page_shape:
+        raise AttnError(EINVAL, f"k_pages: {plan._page_shape} as planned, got {tuple(k_pages.shape)}")
     if out is None:
         with _on(stream):
-            out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    else:
-        _check("out", out, q.dtype, 3, dense=False)
-        _need(out.shape == shape, f"out: {shape}, got {tuple(out.shape)}")
+            out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif not (out.dtype is dtype and out.shape == shape and out.get_device() == dev):
+        _check("out", out, dtype, 3, dense=False)
+        raise AttnError(EINVAL, f"out: {shape}, got {tuple(out.shape)}")
     for name, t in (("sinks", sinks), ("alibi", alibi)):
-        if t is not None:
+        if t is not None and not (t.dtype is torch.float32 and t.get_device() == dev and t.shape == shape[1:2]
+                                  and t.is_contiguous()):
             _check(name, t, torch.float32, 1)
-            _need(t.numel() == d.n_head, f"{name}: one value for each of the {d.n_head} heads")
-    if plan.workspace_bytes and (workspace is None or workspace.numel() * workspace.element_size() < plan.workspace_bytes):
-        with _on(stream):
-            workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device)
-    elif workspace is not None:
-        _check("workspace", workspace, workspace.dtype)
-    x = PagedDesc.from_buffer_copy(d)
-    x.alibi = attn._ptr(alibi)
+            raise AttnError(EINVAL, f"{name}: one value for each of the {shape[1]} heads")
+    need, ws, ws_bytes = plan.workspace_bytes, None, 0
+    if need:
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            with _on(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws_bytes = need
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            _check("workspace", workspace, workspace.dtype)
+        ws = workspace.data_ptr()
+    x = PagedDesc.from_buffer_copy(plan.desc)
+    if alibi is not None:
+        x.alibi = alibi.data_ptr()
     x.page_stride, x.row_stride, x.head_stride = page, row, head
-    x.q_token_stride, x.out_token_stride = _rows("q", q), _rows("out", out)
-    x.scale, x.softcap = 0.0 if scale is None else float(scale), float(softcap)
-    lib = attn.load_library()
-    fn = lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged
-    attn._check(fn(ctypes.byref(x), plan.buffer.data_ptr(), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                   attn._ptr(sinks), out.data_ptr(), attn._ptr(workspace),
-                   0 if workspace is None else workspace.numel() * workspace.element_size(),
-                   attn._stream_ptr(stream)))
+    if not q.is_contiguous():
+        x.q_token_stride = _rows("q", q)
+    if not out.is_contiguous():
+        x.out_token_stride = _rows("out", out)
+    if scale is not None:
+        x.scale = scale
+    if softcap:
+        x.softcap = softcap
+    lib = attn._lib
+    rc = (lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged)(
+        ctypes.byref(x), plan.buffer.data_ptr(), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws, ws_bytes, attn._stream_ptr(stream))
+    if rc:
+        attn._check(rc)
     return out
 
 
@@ -292,51 +341,73 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
     [n_tokens, n_kv, hd], contiguous or views into one buffer of token rows.
     Returns ``out`` (f32, may be q; or f16), by default a new f32 tensor (its
     skipped rows undefined)."""
-    import torch
-
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check(name, t, torch.float32, 3, dense=False)
-    T, n_head, hd = q.shape
-    n_kv = k.shape[1]
-    _need(k.shape == v.shape == (T, n_kv, hd), f"k and v: [{T}, n_kv, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    page, row, head = _pools(k_pages, v_pages)
-    _need(k_pages.shape[2:] == (n_kv, hd), f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
-    st = {_rows(name, t) for name, t in (("q", q), ("k", k), ("v", v))}
-    _need(len(st) == 1, "q, k and v: all contiguous, or views into rows of one stride")
-    _check("slots", slots, torch.int64, 1)
-    _need(slots.numel() == T, f"slots: one for each of the {T} rows")
+    if _torch is None:
+        _start()
+    f32, dev = _torch.float32, _device()
+    shape, kv_shape = q.shape, k.shape
+    if not (q.dtype is f32 and k.dtype is f32 and v.dtype is f32 and len(shape) == 3 and len(kv_shape) == 3
+            and v.shape == kv_shape and kv_shape[0] == shape[0] and kv_shape[2] == shape[2]
+            and q.get_device() == dev and k.get_device() == dev and v.get_device() == dev):
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            _check(name, t, f32, 3, dense=False)
+        raise AttnError(EINVAL, f"q, k, v: [n_tokens, heads, hd], k and v alike; got {tuple(shape)}, {tuple(kv_shape)} and "
+                                f"{tuple(v.shape)}")
+    T, n_head, hd = shape
+    n_kv = kv_shape[1]
+    page, row, head = _pools(k_pages, v_pages, dev)
+    n_pages, page_size, heads, dims = k_pages.shape
+    if heads != n_kv or dims != hd:
+        raise AttnError(EINVAL, f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
+    stride = _rows("q", q)
+    if _rows("k", k) != stride or _rows("v", v) != stride:
+        raise AttnError(EINVAL, "q, k and v: all contiguous, or views into rows of one stride")
+    if not (slots.dtype is _torch.int64 and slots.get_device() == dev and slots.dim() == 1 and slots.numel() == T
+            and slots.is_contiguous()):
+        _check("slots", slots, _torch.int64, 1)
+        raise AttnError(EINVAL, f"slots: one for each of the {T} rows")
     if out is None:
         with _on(stream):
-            out = torch.empty((T, n_head, hd), dtype=torch.float32, device=q.device)
-    _need(out.dtype in (torch.float16, torch.float32), f"out: f16 or f32, got {out.dtype}")
-    _check("out", out, out.dtype, 3, dense=False)
-    _need(out.shape == q.shape, f"out: {tuple(q.shape)}, got {tuple(out.shape)}")
+            out = _torch.empty(shape, dtype=f32, device=q.device)
+    half = out.dtype is _torch.float16
+    if not ((half or out.dtype is f32) and out.shape == shape and out.get_device() == dev):
+        _need(out.dtype in (_torch.float16, f32), f"out: f16 or f32, got {out.dtype}")
+        _check("out", out, out.dtype, 3, dense=False)
+        raise AttnError(EINVAL, f"out: {tuple(shape)}, got {tuple(out.shape)}")
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None:
-            _check(name, t, torch.float32, 1)
-            _need(t.numel() == hd, f"{name}: {hd} weights")
+        if t is not None and not (t.dtype is f32 and t.get_device() == dev and t.numel() == hd and t.is_contiguous()):
+            _check(name, t, f32, 1)
+            raise AttnError(EINVAL, f"{name}: {hd} weights")
     rp = None
     if table is not None:
-        _check("table", table, torch.float32, 3)
         rot = rot or 2 * table.shape[1]
-        _need(table.shape[1:] == (rot // 2, 2), f"table: [rows, {rot // 2}, 2], got {tuple(table.shape)}")
+        if not (table.dtype is f32 and table.get_device() == dev and table.dim() == 3 and 2 * table.shape[1] == rot
+                and table.shape[2] == 2 and table.is_contiguous()):
+            _check("table", table, f32, 3)
+            raise AttnError(EINVAL, f"table: [rows, {rot // 2}, 2], got {tuple(table.shape)}")
         _need(positions is not None, "positions are needed with a table")
-        _check("positions", positions, torch.int32)
-        _need(positions.dim() in (1, 2) and positions.shape[-1] == T, f"positions: [{T}] or [n_axes, {T}]")
         n_axes = positions.shape[0] if positions.dim() == 2 else 1
-        _need(n_axes == 1 or pair_axis is not None, "pair_axis is needed with more than one axis")
+        if not (positions.dtype is _torch.int32 and positions.get_device() == dev and positions.numel() == n_axes * T
+                and positions.shape[-1] == T and positions.is_contiguous()):
+            _check("positions", positions, _torch.int32)
+            raise AttnError(EINVAL, f"positions: [{T}] or [n_axes, {T}], got {tuple(positions.shape)}")
         axes = None
         if pair_axis is not None:
-            _need(len(pair_axis) == rot // 2 and all(0 <= a < n_axes for a in pair_axis),
-                  f"pair_axis: an axis below {n_axes} for each of the {rot // 2} pairs")
-            axes = bytes(pair_axis)
-        rp = PagedRope(rot, 1 if neox else 0, table_split, table.shape[0], table.data_ptr(), n_axes, axes,
-                       positions.data_ptr(), T)
-    d = PagedDesc(n_head=n_head, n_kv=n_kv, hd=hd, n_tokens=T, page_size=k_pages.shape[1], n_pages=k_pages.shape[0],
-                  page_stride=page, row_stride=row, head_stride=head)
-    attn._check(attn.load_library().pelica_attn_paged_qkv(
-        ctypes.byref(d), None if rp is None else ctypes.byref(rp), q.data_ptr(), k.data_ptr(), v.data_ptr(), st.pop(),
-        attn._ptr(q_norm), attn._ptr(k_norm), eps, slots.data_ptr(), out.data_ptr(),
-        1 if out.dtype is torch.float16 else 0, _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(),
-        attn._stream_ptr(stream)))
+            try:
+                axes = bytes(pair_axis)  # (the call checks them against n_axes)
+            except (TypeError, ValueError) as e:
+                raise AttnError(EINVAL, f"pair_axis: an axis below {n_axes} for each pair: {e}") from None
+            _need(len(axes) == rot // 2, f"pair_axis: an axis for each of the {rot // 2} pairs")
+        _need(n_axes == 1 or axes is not None, "pair_axis is needed with more than one axis")
+        rp = ctypes.byref(PagedRope(rot, 1 if neox else 0, table_split, table.shape[0], table.data_ptr(), n_axes, axes,
+                                    positions.data_ptr(), T))
+    # (in the order of PagedDesc._fields_)
+    d = PagedDesc(n_head, n_kv, hd, 0, T, 0, page_size, n_pages, 0, 0, None, None, None, None, None, page, row, head)
+    lib = attn._lib or attn.load_library()
+    rc = lib.pelica_attn_paged_qkv(
+        ctypes.byref(d), rp, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride,
+        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+        slots.data_ptr(), out.data_ptr(), half, _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(),
+        attn._stream_ptr(stream))
+    if rc:
+        attn._check(rc)
     return out

@@ -223,11 +223,17 @@ def test_an_items_chunks_hold_every_key_its_rows_see_once(rules):
 
 
 def test_pieces_of_an_item(rules):
-    for cost, chunks, L in ((1, 1, 4), (4, 4, 4), (5, 5, 4), (400, 100, 4), (400, 100, 37), (7, 7, 1 << 30)):
-        k = rules.item_pieces_of(cost, chunks, L)
-        assert 1 <= k <= chunks and (k == chunks or k * L >= cost)
-        cuts = [chunks * i // k for i in range(k + 1)]
-        assert cuts[0] == 0 and cuts[-1] == chunks and all(a < b for a, b in zip(cuts, cuts[1:]))
+    rules.item_pieces_of.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_float]
+    r = random.Random(3)
+    for _ in range(2000):
+        chunks = r.choice((1, 2, 5, 100, 5000, 1 << 25))
+        cost = chunks * r.choice((1, 3))
+        limit = r.choice((4.0, 4.7, 37.2, 1000.5, 1e9))
+        k = rules.item_pieces_of(cost, chunks, limit)
+        # (in f32: a piece may pass the limit by its roundings)
+        assert 1 <= k <= chunks and (k == chunks or k * limit * (1 + 2 ** -21) >= cost)
+        cuts = [chunks * i // k for i in range(min(k, 300) + 1)]
+        assert cuts[0] == 0 and all(a < b for a, b in zip(cuts, cuts[1:])) and chunks * k // k == chunks
 
 
 def test_the_bound_on_items_holds(rules):
