@@ -294,6 +294,52 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
     const int h2 = lane >> 5, c32 = lane & 31;
     const int kg = wave / NWG, wr = wave % NWG;
 
+    char* const kbuf = lds + kg * 2 * NB * TILE;
+    char* const vbuf = kbuf + NB * TILE;
+    Rows rows(p, z, kvh, lane);
+    const uint32_t lds_at = lds_byte(lds);
+    // tile t of this key group: its first chunk
+    auto tile_chunk = [&](int t) { return KG > 1 ? z.cb + kg + KG * t : z.cb + CPT * t; };
+    // run r of this wave: its first row of a tile, its first key
+    constexpr int WR = 8 * NR;  // rows a wave fills
+    auto run_key = [&](int t, int r) {
+        const int row = WR * wr + 8 * r;
+        return chunk_key(tile_chunk(t) + row / 32, z.n_pre, z.lo_base) + row % 32;
+    };
+    auto fetch = [&](int t, int (&id)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t, r));
+    };
+    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+            run[r] = rows.run(run_key(t, r), tile_chunk(t) + (WR * wr + 8 * r) / 32 < z.ce, id[r]);
+    };
+    auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
+        constexpr bool V = decltype(is_v)::value;
+        const uint32_t to = lds_at + kg * 2 * NB * TILE + (V ? NB * TILE : 0) + (t % NB) * TILE + WR * HD * 2 * wr;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int j = 0; j < Rows::IPR; ++j) rows.template load<V>(run[r], j, to + 1024 * (Rows::IPR * r + j));
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
+    const int n = z.ce - z.cb;
+    const int n_tiles = KG > 1 ? (n - kg + KG - 1) / KG : (n + CPT - 1) / CPT;  // (kg <= n + KG - 1: >= 0)
+    // the first tiles are requested ahead of the queries, whose use waits for
+    // all that was requested before it
+    int id[NR];  // table entries of the next tile to request
+    typename Rows::Run run[NR];
+    fetch(0, id);
+#pragma unroll
+    for (int t = 0; t < (KG > 1 ? NB : 1); ++t) {
+        place(t, id, run);
+        fetch(t + 1, id);
+        load_tile(t, run, K_{});
+        load_tile(t, run, V_{});
+    }
+
     // rows: the queries as the B operand (column c32 of each 32-row tile)
     half8 qh[RT][KS], ql[F32 ? RT : 1][F32 ? KS : 1];
     int posr[RT], lor[RT];  // position, first key of the window
@@ -346,39 +392,6 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
         for (int dt = 0; dt < DT; ++dt) o[dt][rt] = float16v{};
     }
 
-    char* const kbuf = lds + kg * 2 * NB * TILE;
-    char* const vbuf = kbuf + NB * TILE;
-    Rows rows(p, z, kvh, lane);
-    const uint32_t lds_at = lds_byte(lds);
-    // tile t of this key group: its first chunk
-    auto tile_chunk = [&](int t) { return KG > 1 ? z.cb + kg + KG * t : z.cb + CPT * t; };
-    // run r of this wave: its first row of a tile, its first key
-    constexpr int WR = 8 * NR;  // rows a wave fills
-    auto run_key = [&](int t, int r) {
-        const int row = WR * wr + 8 * r;
-        return chunk_key(tile_chunk(t) + row / 32, z.n_pre, z.lo_base) + row % 32;
-    };
-    auto fetch = [&](int t, int (&id)[NR]) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t, r));
-    };
-    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-            run[r] = rows.run(run_key(t, r), tile_chunk(t) + (WR * wr + 8 * r) / 32 < z.ce, id[r]);
-    };
-    auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
-        constexpr bool V = decltype(is_v)::value;
-        const uint32_t to = lds_at + kg * 2 * NB * TILE + (V ? NB * TILE : 0) + (t % NB) * TILE + WR * HD * 2 * wr;
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int j = 0; j < Rows::IPR; ++j) rows.template load<V>(run[r], j, to + 1024 * (Rows::IPR * r + j));
-    };
-    using K_ = std::false_type;
-    using V_ = std::true_type;
-    const int n = z.ce - z.cb;
-    const int n_tiles = KG > 1 ? (n - kg + KG - 1) / KG : (n + CPT - 1) / CPT;  // (kg <= n + KG - 1: >= 0)
 
     // chunk c's scores: S^T, then in the log2 domain, masked
     auto scores = [&](const char* kt, int sub, int c, float16v (&s)[RT]) {
@@ -489,16 +502,6 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
         // 2 NB - 1 tiles after it (past the last one: empty requests); table
         // entries a tile earlier
         constexpr int AHEAD = WI * (2 * NB - 1);
-        int id[NR];
-        typename Rows::Run run[NR];
-        fetch(0, id);
-#pragma unroll
-        for (int t = 0; t < NB; ++t) {
-            place(t, id, run);
-            fetch(t + 1, id);
-            load_tile(t, run, K_{});
-            load_tile(t, run, V_{});
-        }
         for (int t = 0; t < n_tiles; ++t) {
             const int c = tile_chunk(t);
             wait_loads<AHEAD>();
@@ -517,13 +520,6 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
         }
         wait_loads<0>();
     } else {
-        int id[NR];
-        typename Rows::Run run[NR];
-        fetch(0, id);
-        place(0, id, run);
-        fetch(1, id);
-        load_tile(0, run, K_{});
-        load_tile(0, run, V_{});
         for (int t = 0; t < n_tiles; ++t) {
             wait_loads<0>();
             __syncthreads();  // tile t is there, and no wave reads tile t - 1
@@ -950,8 +946,12 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     constexpr int LN = PagedShape<HD, 1, kNW>::LDS, LW = WIDE ? PagedShape<HD, RT, 1>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char lds[LN > LW ? LN : LW];
     const int id = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
-    if (p.head->sig != p.sig || id >= p.head->n_pieces) return;
+    // (the piece beside the header, not after it: one round trip)
     const PlanPiece z = p.pieces[id];
+    const uint32_t sig = p.head->sig;
+    const int n_pieces = p.head->n_pieces;
+    __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces));
+    if (sig != p.sig || id >= n_pieces) return;
     if (WIDE && z.R > kNarrowRows) {
         if constexpr (F32) paged_body<HD, RT, 1, true, SC>(p, z, kvh, lds);
         else wide_body<HD, RT, SC>(p, z, kvh, lds);
@@ -969,8 +969,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     constexpr int LPR = HD / 4, GPW = 64 / LPR, U = 4;
     __shared__ float st[WPR > 1 ? WPR : 1][64][6];
     const int j = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
-    if (p.head->sig != p.sig || j >= p.head->n_joins) return;
     const PlanJoin z = p.joins[j];
+    const uint32_t sig = p.head->sig;
+    const int n_joins = p.head->n_joins;
+    __asm__ volatile("" ::"s"(z.q0), "s"(z.slot0), "s"(sig), "s"(n_joins));
+    if (sig != p.sig || j >= n_joins) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = 4 * (lane % LPR), grp = lane / LPR;
     const int rows = min(z.R - z.r0, p.rows);
     const bool spread = WPR > 1 || z.n_slots > 8;  // a row's slots over the lane groups

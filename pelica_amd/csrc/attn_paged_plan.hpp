@@ -36,13 +36,10 @@ struct PlanCost {
     static PELICA_HD float share(bool wide, int chunks, bool split) {
         return piece(wide, chunks) + (split ? wide ? 20.f : 1.f : 0.f);
     }
-    // the step: pieces that all run at once end with the longest, which
-    // runs faster once its neighbour is done; more than that fill the gaps
-    static PELICA_HD float step(float mean, float longest, bool at_once) {
-        if (at_once) return mean + 0.6f * (longest - mean);
-        const float a = mean + 0.05f * longest, b = 0.65f * longest;
-        return a > b ? a : b;
-    }
+    // the step: the chip's mean, or a slot with `last` to do (its one piece, or
+    // the pieces that have to share a slot), which runs faster once its
+    // neighbours are done
+    static PELICA_HD float step(float mean, float last) { return last > mean ? mean + 0.6f * (last - mean) : mean; }
 };
 
 // 32-key chunks of the keys that any row of an item sees: its window's and

@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     __shared__ int costs[kPlanItems];
     __shared__ int part[4][kPlanWaves];
     __shared__ float est[2][kPlanWaves], limit[2][kPlanWaves];
-    __shared__ int at_bucket[kBuckets];
+    __shared__ int at_bucket[kBuckets], hist[kPlanWaves][64];
     __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int W = wide_rows(p.hd);
@@ -436,9 +436,29 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
             longest = wave_fold(longest, [](float a, float b) { return fmaxf(a, b); });
             pieces = wave_sum(pieces);
             slots = wave_sum(slots);
+            float last = longest;
+            if (pieces > p.fill) {
+                // Of more than g `fill` pieces, the g + 1 that share a slot are
+                // at least as long as number g `fill` + 1 (longest first).  A
+                // histogram of the lengths, in 64ths of the longest, finds it.
+                hist[wave][lane] = 0;
+                const float scale = 63.99f / longest;
+                for (int i = lane; i < n_items; i += 64) {
+                    const int c = abs(costs[i]);
+                    const bool wide = costs[i] < 0;
+                    const int chunks = wide ? c / kWideCost : c;
+                    const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
+                    atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m) * scale)], k);
+                }
+                __builtin_amdgcn_wave_barrier();
+                const int have = hist[wave][lane], longer = pieces - wave_scan(have) + have;  // as long as this bucket's
+                for (int g = 1; g <= 3 && pieces > g * p.fill; ++g) {
+                    const int b = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(longer > g * p.fill) | 1);
+                    last = fmaxf(last, (float)(g + 1) * ((float)b + 0.5f) / scale);
+                }
+            }
             if (lane == 0) {
-                est[round][wave] = slots <= p.max_slots
-                                       ? PlanCost::step(time / (float)p.fill, longest, pieces <= p.fill) : INFINITY;
+                est[round][wave] = slots <= p.max_slots ? PlanCost::step(time / (float)p.fill, last) : INFINITY;
                 limit[round][wave] = mine;
             }
             __syncthreads();
