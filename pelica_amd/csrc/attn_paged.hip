@@ -54,16 +54,26 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// LDS byte of 16-byte piece p of key row k of a K tile (XOR-swizzled: 32 rows'
-// same piece spreads over the banks), and of a V tile (the transposing reads of
-// 4 rows' 16 dims do).
+// LDS byte of 16-byte piece p of key row k of a K tile: pieces XOR-swizzled so
+// that 16 consecutive rows' same piece, which 16 lanes read at once, lie in 64
+// banks (a row of 128 bytes is half of them).
+template <int HD>
+__device__ __forceinline__ constexpr int k_swizzle(int k) {
+    return HD == 64 ? (k >> 1) & 7 : k & 15;
+}
 template <int HD>
 __device__ __forceinline__ int k_slot(int k, int p) {
-    return k * (HD * 2) + ((p ^ (k & 7)) << 4);
+    return k * (HD * 2) + ((p ^ k_swizzle<HD>(k)) << 4);
+}
+// ... and of a V tile, whose transposing reads take 4 rows' 16 dims a 16-lane
+// group, the groups rows 4 apart (or dims 16 apart).
+template <int HD>
+__device__ __forceinline__ constexpr int v_swizzle(int k) {
+    return HD == 64 ? ((k & 3) ^ ((k >> 2) & 1)) << 1 : (k & 7) << 1;
 }
 template <int HD>
 __device__ __forceinline__ int v_slot(int k, int p) {
-    return k * (HD * 2) + ((p ^ ((k & 3) << 1)) << 4);
+    return k * (HD * 2) + ((p ^ v_swizzle<HD>(k)) << 4);
 }
 
 // f(0) .. f(N - 1), the indexes as types
@@ -148,19 +158,87 @@ __device__ __forceinline__ bool clean_chunk(char* vt, int lane) {
     return true;
 }
 
-// the chunk at key kb
+// The cache rows of one kv head: a wave fills runs of 8 consecutive rows of a
+// tile, which lie in one page (pages are at least 8 rows).  A run's address is
+// scalar: its table entry, in 64 bits; a lane adds its row and piece, a
+// constant.
+template <int HD>
+struct CacheRows {
+    static constexpr int PPR = HD / 8, RPI = 64 / PPR, IPR = 8 / RPI;  // pieces a row; rows, instructions of a run
+    const PagedParams& p;
+    const PlanPiece& z;
+    uint64_t k, v;            // the head's rows of page 0
+    const int32_t* table;     // the request's row
+    int last, bad = 0;        // last key that a row sees; a page of a wanted key is none of the pool's
+    uint32_t klane[2][IPR], vlane[IPR];  // (K's by the run's parity)
+
+    struct Run {
+        uint64_t off;         // bytes to the first row wanted
+        uint32_t nrec, skip;  // bytes of the rows wanted, bytes of the run ahead of them
+    };
+
+    __device__ __forceinline__ CacheRows(const PagedParams& p_, const PlanPiece& z_, int kvh, int lane) : p(p_), z(z_) {
+        k = reinterpret_cast<uintptr_t>(p.k) + (uint64_t)kvh * p.head_b;
+        v = reinterpret_cast<uintptr_t>(p.v) + (uint64_t)kvh * p.head_b;
+        table = p.table + (size_t)z.seq * p.max_pages;
+        last = imax(z.kend, z.pe) - 1;
+        const int lrow = lane / PPR, phys = lane % PPR;
+#pragma unroll
+        for (int j = 0; j < IPR; ++j) {
+            const int row = RPI * j + lrow;
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                klane[odd][j] = (uint32_t)row * p.row_b + 16u * (phys ^ k_swizzle<HD>(8 * odd + row));
+                __asm__("" : "+v"(klane[odd][j]));  // (else taken apart again at each use)
+            }
+            vlane[j] = (uint32_t)row * p.row_b + 16u * (phys ^ v_swizzle<HD>(row));
+            __asm__("" : "+v"(vlane[j]));
+        }
+    }
+    __device__ __forceinline__ int entry(int key) const { return table_entry(table, imin(key, last) >> p.page_log2); }
+    __device__ __forceinline__ const char* v_row(int key) const {
+        const unsigned page = min((unsigned)entry(key), (unsigned)p.n_pages - 1u);
+        return reinterpret_cast<const char*>(v + (uint64_t)page * (uint64_t)p.page_b +
+                                             (uint32_t)((key & ((1 << p.page_log2) - 1)) * p.row_b));
+    }
+    // keys key .. key + 7; none are wanted unless `any`
+    __device__ __forceinline__ Run run(int key, bool any, int id) {
+        int first, count;
+        group_rows(key, 8, z.lo, z.kend, z.pe, first, count);
+        count = any ? count : 0;
+        bad |= count > 0 ? (unsigned)id >= (unsigned)p.n_pages : 0;
+        const unsigned page = min((unsigned)id, (unsigned)p.n_pages - 1u);
+        Run r;
+        r.skip = (uint32_t)first * p.row_b;
+        r.nrec = (uint32_t)count * p.row_b;
+        r.off = (uint64_t)page * (uint64_t)p.page_b + (uint32_t)((key & ((1 << p.page_log2) - 1)) * p.row_b) + r.skip;
+        return r;
+    }
+    // instruction j of a run (an odd or even one of its tile) into 1 KB of LDS
+    // at byte `to`
+    template <bool V>
+    __device__ __forceinline__ void load(const Run& r, int odd, int j, uint32_t to) const {
+        const uint64_t base = (V ? v : k) + r.off;
+        const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32), r.nrec, (uint32_t)kBufFlags};
+        uint32_t saved;
+        __asm__ volatile(
+            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+            "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "s"(to), "v"((V ? vlane[j] : klane[odd][j]) - r.skip), "s"(rs));
+    }
+};
+
+// (see clean_chunk) of the chunk at key kb, to the rows of 32-row tiles
 template <int HD, int RT>
-__device__ __forceinline__ void add_special(const PagedParams& p, const PlanPiece& z, uint64_t vbase, const int32_t* table,
-                                            int kb, int h2, const int (&lor)[RT], const unsigned (&span)[RT],
-                                            float16v (&o)[HD / 32][RT]) {
+__device__ __forceinline__ void add_special(const PlanPiece& z, const CacheRows<HD>& rows, int kb, int h2,
+                                            const int (&lor)[RT], const unsigned (&span)[RT], float16v (&o)[HD / 32][RT]) {
 #pragma unroll 1
     for (int key = kb; key < kb + 32; ++key) {
         int first, count;
         group_rows(key, 1, z.lo, z.kend, z.pe, first, count);
         if (count == 0) continue;
-        const unsigned id = min((unsigned)table_entry(table, key >> p.page_log2), (unsigned)p.n_pages - 1u);
-        const char* const src = reinterpret_cast<const char*>(vbase + (uint64_t)id * (uint64_t)p.page_b +
-                                                              (uint64_t)(key & ((1 << p.page_log2) - 1)) * p.row_b);
+        const char* const src = rows.v_row(key);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
@@ -176,90 +254,37 @@ __device__ __forceinline__ void add_special(const PagedParams& p, const PlanPiec
     }
 }
 
-// The cache rows of one kv head: a wave fills runs of 8 consecutive rows of a
-// tile, which lie in one page (pages are at least 8 rows).  A run's address is
-// scalar: its table entry, in 64 bits; a lane adds its row and piece, a
-// constant.
+// A wide item's tiles: 64 keys, two buffers each of K and V, of whose rows a
+// wave fills 16.
 template <int HD>
-struct CacheRows {
-    static constexpr int PPR = HD / 8, RPI = 64 / PPR, IPR = 8 / RPI;  // pieces a row; rows, instructions of a run
-    const PagedParams& p;
-    const PlanPiece& z;
-    uint64_t k, v;            // the head's rows of page 0
-    const int32_t* table;     // the request's row
-    int last, bad = 0;        // last key that a row sees; a page of a wanted key is none of the pool's
-    uint32_t klane[IPR], vlane[IPR];
-
-    struct Run {
-        uint64_t off;         // bytes to the first row wanted
-        uint32_t nrec, skip;  // bytes of the rows wanted, bytes of the run ahead of them
-    };
-
-    __device__ __forceinline__ CacheRows(const PagedParams& p_, const PlanPiece& z_, int kvh, int lane) : p(p_), z(z_) {
-        k = reinterpret_cast<uintptr_t>(p.k) + (uint64_t)kvh * p.head_b;
-        v = reinterpret_cast<uintptr_t>(p.v) + (uint64_t)kvh * p.head_b;
-        table = p.table + (size_t)z.seq * p.max_pages;
-        last = imax(z.kend, z.pe) - 1;
-        const int lrow = lane / PPR, phys = lane % PPR;
-#pragma unroll
-        for (int j = 0; j < IPR; ++j) {
-            const int row = RPI * j + lrow;  // (the pieces' swizzle, see k_slot and v_slot)
-            klane[j] = (uint32_t)row * p.row_b + 16u * (phys ^ (row & 7));
-            vlane[j] = (uint32_t)row * p.row_b + 16u * (phys ^ ((row & 3) << 1));
-            __asm__("" : "+v"(klane[j]), "+v"(vlane[j]));  // (else taken apart again at each use)
-        }
-    }
-    __device__ __forceinline__ int entry(int key) const { return table_entry(table, imin(key, last) >> p.page_log2); }
-    // keys key .. key + 7; none are wanted unless `any`
-    __device__ __forceinline__ Run run(int key, bool any, int id) {
-        int first, count;
-        group_rows(key, 8, z.lo, z.kend, z.pe, first, count);
-        count = any ? count : 0;
-        bad |= count > 0 ? (unsigned)id >= (unsigned)p.n_pages : 0;
-        const unsigned page = min((unsigned)id, (unsigned)p.n_pages - 1u);
-        Run r;
-        r.skip = (uint32_t)first * p.row_b;
-        r.nrec = (uint32_t)count * p.row_b;
-        r.off = (uint64_t)page * (uint64_t)p.page_b + (uint32_t)((key & ((1 << p.page_log2) - 1)) * p.row_b) + r.skip;
-        return r;
-    }
-    // instruction j of a run into 1 KB of LDS at byte `to`
-    template <bool V>
-    __device__ __forceinline__ void load(const Run& r, int j, uint32_t to) const {
-        const uint64_t base = (V ? v : k) + r.off;
-        const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32), r.nrec, (uint32_t)kBufFlags};
-        uint32_t saved;
-        __asm__ volatile(
-            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
-            "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-            : "=&s"(saved)
-            : "s"(to), "v"((V ? vlane[j] : klane[j]) - r.skip), "s"(rs));
-    }
+struct WideShape {
+    static constexpr int RT = HD == 64 ? 2 : 1;  // row tiles of 32 a wave
+    static constexpr int KS = HD / 16, DT = HD / 32;
+    static constexpr int TILE = 64 * HD * 2;
+    static constexpr int NR = 2, WI = NR * CacheRows<HD>::IPR;  // runs of 8 rows, load instructions
+    static constexpr int LDS = 4 * TILE;
 };
-
-template <int HD, int RT, int KG>
-struct PagedShape {
-    static constexpr int KS = HD / 16, DT = HD / 32, PPR = HD / 8;
-    static constexpr int NWG = kNW / KG;                 // waves of a key group
-    static constexpr int TK = KG == 1 ? 64 : 32;         // keys a tile
-    static constexpr int CPT = TK / 32;
-    static constexpr int NB = KG == 1 ? 2 : HD == 64 ? 2 : 1;  // buffers of K (and of V) a group
-    static constexpr int TILE = TK * HD * 2;
-    static constexpr int NR = TK / NWG / 8;              // runs of 8 rows a wave fills of a tile
-    static constexpr int WI = NR * CacheRows<HD>::IPR;   // load instructions of these
-    static constexpr int STREAM = KG * 2 * NB * TILE;
-    static constexpr int MERGE = KG > 1 ? kNW * DT * RT * 64 * 64 + kNW * RT * 64 * 8 : 0;
+// A narrow item's: 32 keys, each wave's own; at head dim 64 two buffers.
+template <int HD, int NT>
+struct NarrowShape {
+    static constexpr int KS = HD / 32, DT = HD / 16;
+    static constexpr int NB = HD == 64 ? 2 : 1;
+    static constexpr int TILE = 32 * HD * 2;
+    static constexpr int NR = 4, WI = NR * CacheRows<HD>::IPR;
+    static constexpr int STREAM = kNW * 2 * NB * TILE;
+    static constexpr int MERGE_O = kNW * DT * NT * 64 * 16, MERGE = MERGE_O + kNW * NT * 64 * 8;
     static constexpr int LDS = STREAM > MERGE ? STREAM : MERGE;
 };
 
 // What a row's state (max M, sum L, both of the keys only) is multiplied by for
 // the output: the sink joins here, last, so that probabilities are relative
 // to the keys' max and keep their bits however large the sink is.
-__device__ __forceinline__ float row_weight(const PagedParams& p, int h, float M, float L) {
-    if (!p.sinks) return 1.f / L;
-    const float sk = p.sinks[h] * kLog2e, top = fmaxf(M, sk), f = fast_exp2(M - top);
-    return f / (L * f + fast_exp2(sk - top));
+// sink: in the log2 domain, -inf for none.
+__device__ __forceinline__ float row_weight(float sink, float M, float L) {
+    const float top = fmaxf(M, sink), f = fast_exp2(M - top);
+    return f / (L * f + fast_exp2(sink - top));
 }
+__device__ __forceinline__ float sink_of(const PagedParams& p, int h) { return p.sinks ? p.sinks[h] * kLog2e : -INFINITY; }
 
 // Where row rl of the piece's item goes: its output, or the partial sums of a
 // split item's piece
@@ -284,90 +309,394 @@ __device__ __forceinline__ void store_sum(const PagedParams& p, const PlanPiece&
     reinterpret_cast<float2*>(p.ws_ml)[(size_t)(z.slot * p.n_kv + kvh) * p.rows + rl] = make_float2(M, L);
 }
 
-template <int HD, int RT, int KG, bool F32, bool SC>
-__device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
-    using S = PagedShape<HD, RT, KG>;
-    constexpr int KS = S::KS, DT = S::DT, NWG = S::NWG, CPT = S::CPT, NB = S::NB;
-    constexpr int TILE = S::TILE, NR = S::NR, WI = S::WI;
+// Scores of a chunk (raw products, 16-bit or f32 queries) in the log2 domain:
+// scaled, capped, with the distance bias; v of a lane's scores at once.
+template <bool SC, typename V, int N, typename KEY>
+__device__ __forceinline__ void finish_scores(const PagedParams& p, V& s, std::integral_constant<int, N>, float slope, int pos,
+                                              KEY key) {
+    if (SC && p.cap > 0.f) {
+        // cap tanh(y / cap): tanh(y) = 1 - 2 / (1 + e^(2 y)), saturating at both
+        // ends; off by at most a few 2^-24 of the cap
+        const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[i] * f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] *= p.qscale;
+    }
+    if (SC && p.alibi) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] -= slope * fabsf((float)(pos - key(i)));
+    }
+}
+
+__device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
+    const int v = __float_as_uint(x);
+    return __uint_as_float(__builtin_amdgcn_update_dpp(v, v, 0x128, 0xF, 0xF, false));
+}
+
+// A narrow item: NT tiles of 16 rows.  v_mfma_f32_16x16x32_f16: S^T = K Q^T (a
+// lane holds 4 keys of one row from each 16), O^T += V^T P^T (the 8 scores of
+// a lane are its part of P; V's rows are read in that order).  Each wave takes
+// every fourth chunk of the piece, waits for its own loads only, and the
+// four states are merged through LDS.
+// f32 queries: PACK (at most 8 rows): hi parts in columns 0-7, lo parts in 8-15
+// of one operand, the scores added by a lane exchange, the outputs at the end;
+// otherwise two products each.
+template <int HD, int NT, bool F32, bool SC, bool PACK>
+__device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
+    static_assert(!PACK || (F32 && NT == 1), "packed hi and lo parts: f32, one tile");
+    using S_ = NarrowShape<HD, NT>;
+    using Rows = CacheRows<HD>;
+    constexpr int KS = S_::KS, DT = S_::DT, NB = S_::NB, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, c16 = lane & 15;
+    char* const kbuf = lds + wave * 2 * NB * TILE;
+    char* const vbuf = kbuf + NB * TILE;
+    Rows rows(p, z, kvh, lane);
+    const uint32_t to = lds_byte(lds) + wave * 2 * NB * TILE;
+    auto tile_chunk = [&](int t) { return z.cb + wave + kNW * t; };
+    auto fetch = [&](int t, int (&id)[NR]) {
+        const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) id[r] = rows.entry(kb + 8 * r);
+    };
+    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
+        const int c = tile_chunk(t), kb = chunk_key(c, z.n_pre, z.lo_base);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) run[r] = rows.run(kb + 8 * r, c < z.ce, id[r]);
+    };
+    auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
+        constexpr bool V = decltype(is_v)::value;
+#pragma unroll
+        for (int x = 0; x < WI; ++x)
+            rows.template load<V>(run[x / Rows::IPR], (x / Rows::IPR) & 1, x % Rows::IPR,
+                                  to + ((V ? NB : 0) + t % NB) * TILE + 1024 * x);
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
+    const int n_tiles = (z.ce - z.cb - wave + kNW - 1) / kNW;
+    // the first tiles are requested ahead of the queries, whose use waits for
+    // all that was requested before it
+    int id[NB + 1][NR];
+    typename Rows::Run run[NR];
+#pragma unroll
+    for (int t = 0; t <= NB; ++t) fetch(t, id[t]);
+#pragma unroll
+    for (int t = 0; t < NB; ++t) {
+        place(t, id[t], run);
+        load_tile(t, run, K_{});
+        load_tile(t, run, V_{});
+    }
+
+    // queries: column c16 of each tile, dims 8 g .. of every 32
+    half8 qh[NT][KS], ql[F32 && !PACK ? NT : 1][F32 && !PACK ? KS : 1];
+    int posr[NT], lor[NT];
+    unsigned span[NT];
+    bool valid[NT];
+    float slope[NT], sink[NT];
+    const bool low = PACK && c16 >= 8;  // this column holds lo parts
+    constexpr int QES = F32 ? 4 : 2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(rl, z.R - 1);
+        valid[nt] = rl < z.R;
+        const int t = r / p.hpk, h = kvh * p.hpk + r - t * p.hpk;
+        const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * g) * QES;
+        sink[nt] = z.slot < 0 ? sink_of(p, h) : -INFINITY;
+        slope[nt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (F32) {
+                const float4v a = *reinterpret_cast<const float4v*>(src + 128 * ks);
+                const float4v b = *reinterpret_cast<const float4v*>(src + 128 * ks + 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    _Float16 hi, lo;
+                    split_f16(i < 4 ? a[i % 4] : b[i % 4], hi, lo);
+                    qh[nt][ks][i] = low ? lo : hi;
+                    if constexpr (!PACK) ql[nt][ks][i] = lo;
+                }
+            } else {
+                qh[nt][ks] = load16(src + 64 * ks);
+            }
+        }
+        const int pos = z.pos0 + t;
+        posr[nt] = pos;
+        lor[nt] = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+        span[nt] = (unsigned)(pos - lor[nt]);
+        if (!valid[nt]) lor[nt] = INT32_MAX, span[nt] = 0;  // (sees none)
+    }
+    // every row sees the keys [lo_all, hi_all] and those below z.pe
+    const int hi_all = z.pos0, pos_last = z.pos0 + (z.R - 1) / p.hpk;
+    const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
+
+    float m[NT], l[NT];
+    float4v o[DT][NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][nt] = float4v{};
+    }
+    bool special = false;
+
+    // requests in order K0 V0 (K1 V1): behind a tile's stand the 2 NB - 1 tiles
+    // after it (past the last one: empty requests); table entries a tile
+    // earlier
+    constexpr int AHEAD = WI * (2 * NB - 1);
+    for (int t = 0; t < n_tiles; ++t) {
+        const int c = tile_chunk(t), kb = chunk_key(c, z.n_pre, z.lo_base);
+        const char* const kt_ = kbuf + (t % NB) * TILE;
+        char* const vt = vbuf + (t % NB) * TILE;
+        wait_loads<AHEAD>();
+        typedef float float8v __attribute__((ext_vector_type(8)));
+        float8v s[NT];
+        {
+            float4v sh[NT][2], sl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sh[nt][kt] = sl[nt][kt] = float4v{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const half8 ka = *reinterpret_cast<const half8*>(kt_ + k_slot<HD>(16 * kt + c16, 4 * ks + g));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        sh[nt][kt] = mfma16(ka, qh[nt][ks], sh[nt][kt]);
+                        if constexpr (F32 && !PACK) sl[nt][kt] = mfma16(ka, ql[nt][ks], sl[nt][kt]);
+                    }
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float x = sh[nt][i / 4][i % 4];
+                    if constexpr (PACK) x += ror8(x);
+                    else if constexpr (F32) x += sl[nt][i / 4][i % 4];
+                    s[nt][i] = x;
+                }
+        }
+        lds_done();
+        place(t + NB, id[NB], run);
+        fetch(t + NB + 1, id[NB]);
+        load_tile(t + NB, run, K_{});
+
+        auto key = [&](int i) { return kb + 16 * (i / 4) + 4 * g + i % 4; };
+        const bool all = kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all);
+        half8 ph[NT], pl[F32 && !PACK ? NT : 1];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            finish_scores<SC>(p, s[nt], std::integral_constant<int, 8>{}, slope[nt], posr[nt], key);
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[nt][i] = sees(key(i), z.pe, lor[nt], span[nt]) ? s[nt][i] : -INFINITY;
+            }
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fmaxf(s[nt][i], s[nt][4 + i]);
+            const float mn = fmaxf(m[nt], group4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
+            if (__builtin_amdgcn_ballot_w64(mn > m[nt])) {
+                const float cf = mn > m[nt] ? fast_exp2(m[nt] - mn) : 1.f;  // (0 while m was -inf)
+                l[nt] *= cf;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt][nt] *= cf;
+                m[nt] = mn;
+            }
+            const float ms = m[nt] == -INFINITY ? 0.f : m[nt];
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = fast_exp2(s[nt][i] - ms);
+                if constexpr (F32) {
+                    _Float16 hi, lo;
+                    split_f16(e[i], hi, lo);
+                    ph[nt][i] = low ? lo : hi;
+                    if constexpr (!PACK) pl[nt][i] = lo;
+                } else {
+                    ph[nt][i] = (_Float16)e[i];
+                    e[i] = (float)ph[nt][i];
+                }
+            }
+            l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        }
+        wait_loads<AHEAD>();
+        if (!all && pos_last > hi_all) special |= clean_chunk<HD>(vt, lane);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            // 4 rows' 16 dims a 16-lane group, transposed: keys 4 g .. and 16 + 4 g ..
+            const int k = 4 * g + (c16 >> 2), dim = 16 * dt + 4 * (c16 & 3);
+            const _Float16* a0 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(k, dim >> 3) + ((dim & 7) << 1));
+            const _Float16* a1 = reinterpret_cast<const _Float16*>(vt + v_slot<HD>(k + 16, dim >> 3) + ((dim & 7) << 1));
+            const half8 va = cat8(lds_read_tr(a0), lds_read_tr(a1));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                o[dt][nt] = mfma16(va, ph[nt], o[dt][nt]);
+                if constexpr (F32 && !PACK) o[dt][nt] = mfma16(va, pl[nt], o[dt][nt]);
+            }
+        }
+        lds_done();
+        load_tile(t + NB, run, V_{});
+    }
+    wait_loads<0>();
+    const bool any_bad = __syncthreads_or(rows.bad);  // (and every wave is done with the tiles)
+    if (special)
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; ++t) {
+            const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+            if (kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all)) continue;
+#pragma unroll 1
+            for (int key = kb; key < kb + 32; ++key) {
+                int first, count;
+                group_rows(key, 1, z.lo, z.kend, z.pe, first, count);
+                if (count == 0) continue;
+                const char* const src = rows.v_row(key);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const half4 x = *reinterpret_cast<const half4*>(src + 2 * (16 * dt + 4 * g));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const bool seen = !low & sees(key, z.pe, lor[nt], span[nt]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[dt][nt][i] += (seen & !is_finite(x[i])) ? (float)x[i] : 0.f;
+                    }
+                }
+            }
+        }
+
+    // the waves' states through LDS, merged in wave order: wave w takes the
+    // output tiles w, w + 4, ...
+    float4v* const so = reinterpret_cast<float4v*>(lds);
+    float2* const sml = reinterpret_cast<float2*>(lds + S_::MERGE_O);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        sml[(wave * NT + nt) * 64 + lane] = make_float2(m[nt], group4_sum(l[nt]));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) so[((wave * DT + dt) * NT + nt) * 64 + lane] = o[dt][nt];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float2 ml[kNW];
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kNW; ++w) {
+            ml[w] = sml[(w * NT + nt) * 64 + lane];
+            M = fmaxf(M, ml[w].x);
+        }
+        const float ms = M == -INFINITY ? 0.f : M;
+        float L = 0.f, wt[kNW];
+#pragma unroll
+        for (int w = 0; w < kNW; ++w) {
+            wt[w] = fast_exp2(ml[w].x - ms);  // 0 where the wave saw no key
+            L += ml[w].y * wt[w];
+        }
+        if (any_bad) L = NAN;
+        const int rl = 16 * nt + (PACK ? c16 & 7 : c16);
+        const bool stores = valid[nt] && !low;
+        const float weight = row_weight(sink[nt], M, L);
+        const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1));
+        if (stores && z.slot >= 0 && wave == 0 && g == 0) store_sum(p, z, kvh, rl, M, L);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            if ((dt * NT + nt) % kNW != wave) continue;
+            float4v x = so[(dt * NT + nt) * 64 + lane] * wt[0];
+#pragma unroll
+            for (int w = 1; w < kNW; ++w) x += so[((w * DT + dt) * NT + nt) * 64 + lane] * wt[w];
+            if constexpr (PACK) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] += ror8(x[i]);
+            }
+            if (stores) out.store(16 * dt + 4 * g, x, weight);
+        }
+    }
+}
+
+// a wide item's output: every lane's dims of its rows
+template <int HD, bool F32, int RT>
+__device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece& z, int kvh, int wave, int lane, bool bad,
+                                           const float (&m)[RT], const float (&l)[RT], const float16v (&o)[HD / 32][RT]) {
+    const int h2 = lane >> 5, c32 = lane & 31;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float L = bad ? NAN : half_sum(l[rt]);
+        const int rl = (wave * RT + rt) * 32 + c32;
+        if (z.r0 + rl >= z.R) continue;
+        if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
+        const float w = z.slot < 0 ? row_weight(sink_of(p, kvh * p.hpk + (z.r0 + rl) % p.hpk), m[rt], L) : 1.f;
+        const RowOut<HD, F32> to(p, z, kvh, rl);
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+                to.store(32 * dt + 8 * i4 + 4 * h2,
+                         float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
+    }
+}
+
+// The wide item with f32 queries: hi and lo products, a chunk at a time.
+template <int HD, bool SC>
+__device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
+    using S = WideShape<HD>;
+    constexpr int RT = S::RT, KS = S::KS, DT = S::DT, TILE = S::TILE, NR = S::NR;
     using Rows = CacheRows<HD>;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int h2 = lane >> 5, c32 = lane & 31;
-    const int kg = wave / NWG, wr = wave % NWG;
 
-    char* const kbuf = lds + kg * 2 * NB * TILE;
-    char* const vbuf = kbuf + NB * TILE;
+    char* const kbuf = lds;
+    char* const vbuf = lds + 2 * TILE;
     Rows rows(p, z, kvh, lane);
-    const uint32_t lds_at = lds_byte(lds);
-    // tile t of this key group: its first chunk
-    auto tile_chunk = [&](int t) { return KG > 1 ? z.cb + kg + KG * t : z.cb + CPT * t; };
-    // run r of this wave: its first row of a tile, its first key
-    constexpr int WR = 8 * NR;  // rows a wave fills
+    const uint32_t to = lds_byte(lds) + 16 * HD * 2 * wave;
+    // this wave fills rows 16 wave .. + 15 of a tile: two runs of one chunk
     auto run_key = [&](int t, int r) {
-        const int row = WR * wr + 8 * r;
-        return chunk_key(tile_chunk(t) + row / 32, z.n_pre, z.lo_base) + row % 32;
+        return chunk_key(z.cb + 2 * t + (wave >> 1), z.n_pre, z.lo_base) + 16 * (wave & 1) + 8 * r;
     };
     auto fetch = [&](int t, int (&id)[NR]) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t, r));
     };
-    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
+    auto load_tile = [&](int t, const int (&id)[NR]) {
+        typename Rows::Run run[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
-            run[r] = rows.run(run_key(t, r), tile_chunk(t) + (WR * wr + 8 * r) / 32 < z.ce, id[r]);
+        for (int r = 0; r < NR; ++r) run[r] = rows.run(run_key(t, r), z.cb + 2 * t + (wave >> 1) < z.ce, id[r]);
+        const uint32_t at = to + (t & 1) * TILE;
+#pragma unroll
+        for (int x = 0; x < S::WI; ++x) {
+            rows.template load<false>(run[x / Rows::IPR], (x / Rows::IPR) & 1, x % Rows::IPR, at + 1024 * x);
+            rows.template load<true>(run[x / Rows::IPR], (x / Rows::IPR) & 1, x % Rows::IPR, at + 2 * TILE + 1024 * x);
+        }
     };
-    auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
-        constexpr bool V = decltype(is_v)::value;
-        const uint32_t to = lds_at + kg * 2 * NB * TILE + (V ? NB * TILE : 0) + (t % NB) * TILE + WR * HD * 2 * wr;
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int j = 0; j < Rows::IPR; ++j) rows.template load<V>(run[r], j, to + 1024 * (Rows::IPR * r + j));
-    };
-    using K_ = std::false_type;
-    using V_ = std::true_type;
-    const int n = z.ce - z.cb;
-    const int n_tiles = KG > 1 ? (n - kg + KG - 1) / KG : (n + CPT - 1) / CPT;  // (kg <= n + KG - 1: >= 0)
-    // the first tiles are requested ahead of the queries, whose use waits for
-    // all that was requested before it
+    const int n_tiles = (z.ce - z.cb + 1) / 2;
+    // (ahead of the queries, whose use waits for all that was requested before)
     int id[NR];  // table entries of the next tile to request
-    typename Rows::Run run[NR];
     fetch(0, id);
-#pragma unroll
-    for (int t = 0; t < (KG > 1 ? NB : 1); ++t) {
-        place(t, id, run);
-        fetch(t + 1, id);
-        load_tile(t, run, K_{});
-        load_tile(t, run, V_{});
-    }
+    load_tile(0, id);
+    fetch(1, id);
 
     // rows: the queries as the B operand (column c32 of each 32-row tile)
-    half8 qh[RT][KS], ql[F32 ? RT : 1][F32 ? KS : 1];
+    half8 qh[RT][KS], ql[RT][KS];
     int posr[RT], lor[RT];  // position, first key of the window
     unsigned span[RT];      // keys behind that one that the row sees
     bool valid[RT];
     float slope[RT];
-    constexpr int QES = F32 ? 4 : 2;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = z.r0 + (wr * RT + rt) * 32 + c32;
-        valid[rt] = r < z.R && r - z.r0 < (KG > 1 ? kNarrowRows : kNW * RT * 32);
-        const int rc = min(r, z.R - 1), t = rc / p.hpk, h = kvh * p.hpk + rc % p.hpk;
-        const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * h2) * QES;
+        const int r = z.r0 + (wave * RT + rt) * 32 + c32;
+        valid[rt] = r < z.R;
+        const int rc = min(r, z.R - 1), t = rc / p.hpk, h = kvh * p.hpk + rc - t * p.hpk;
+        const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * h2) * 4;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (F32) {
-                const float4v a = *reinterpret_cast<const float4v*>(src + 64 * ks);
-                const float4v b = *reinterpret_cast<const float4v*>(src + 64 * ks + 16);
+            const float4v a = *reinterpret_cast<const float4v*>(src + 64 * ks);
+            const float4v b = *reinterpret_cast<const float4v*>(src + 64 * ks + 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    _Float16 hi, lo;
-                    split_f16(a[i], hi, lo);
-                    qh[rt][ks][i] = hi, ql[rt][ks][i] = lo;
-                    split_f16(b[i], hi, lo);
-                    qh[rt][ks][4 + i] = hi, ql[rt][ks][4 + i] = lo;
-                }
-            } else {
-                qh[rt][ks] = load16(src + 32 * ks);
+            for (int i = 0; i < 8; ++i) {
+                _Float16 hi, lo;
+                split_f16(i < 4 ? a[i % 4] : b[i % 4], hi, lo);
+                qh[rt][ks][i] = hi, ql[rt][ks][i] = lo;
             }
         }
         const int pos = z.pos0 + t;
@@ -378,7 +707,7 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
         slope[rt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
     }
     // every row sees the keys [lo_all, hi_all] and those below z.pe
-    const int r_last = min(z.R, z.r0 + (KG > 1 ? kNarrowRows : kNW * RT * 32)) - 1;
+    const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
     const int hi_all = z.pos0 + z.r0 / p.hpk, pos_last = z.pos0 + r_last / p.hpk;
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
 
@@ -404,32 +733,16 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 s[rt] = mfma32(ka, qh[rt][ks], s[rt]);
-                if constexpr (F32) s[rt] = mfma32(ka, ql[rt][ks], s[rt]);
+                s[rt] = mfma32(ka, ql[rt][ks], s[rt]);
             }
         }
     };
     auto transform = [&](int c, float16v (&s)[RT]) {
         const int kb = chunk_key(c, z.n_pre, z.lo_base);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (SC && p.cap > 0.f) {
-                // tanh(y) = 1 - 2 / (1 + e^(2 y)), saturating at both ends
-                const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[rt][i] = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[rt][i] * f));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[rt][i] *= p.qscale;
-            }
-            if (SC && p.alibi) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = kb + 8 * (i / 4) + 4 * h2 + i % 4;
-                    s[rt][i] -= slope[rt] * fabsf((float)(posr[rt] - key));
-                }
-            }
-        }
+        for (int rt = 0; rt < RT; ++rt)
+            finish_scores<SC>(p, s[rt], std::integral_constant<int, 16>{}, slope[rt], posr[rt],
+                              [&](int i) { return kb + 8 * (i / 4) + 4 * h2 + i % 4; });
         const bool all = kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all);
         if (!all) {
 #pragma unroll
@@ -461,16 +774,11 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = fast_exp2(s[rt][i] - ms);
-                if constexpr (F32) {
-                    _Float16 hi, lo;
-                    split_f16(e, hi, lo);
-                    ph[i / 8][rt][i % 8] = hi;
-                    pl[i / 8][rt][i % 8] = lo;
-                    sum += e;
-                } else {
-                    ph[i / 8][rt][i % 8] = (_Float16)e;
-                    sum += (float)ph[i / 8][rt][i % 8];
-                }
+                _Float16 hi, lo;
+                split_f16(e, hi, lo);
+                ph[i / 8][rt][i % 8] = hi;
+                pl[i / 8][rt][i % 8] = lo;
+                sum += e;
             }
             l[rt] += sum;
         }
@@ -484,7 +792,7 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     o[dt][rt] = mfma32(va, ph[w][rt], o[dt][rt]);
-                    if constexpr (F32) o[dt][rt] = mfma32(va, pl[w][rt], o[dt][rt]);
+                    o[dt][rt] = mfma32(va, pl[w][rt], o[dt][rt]);
                 }
             }
         }
@@ -497,121 +805,30 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
 
     half8 ph[2][RT], pl[2][RT];
     float16v s[RT];
-    if constexpr (KG > 1) {
-        // requests in order K0 V0 (K1 V1): ahead of a tile's wait stand the
-        // 2 NB - 1 tiles after it (past the last one: empty requests); table
-        // entries a tile earlier
-        constexpr int AHEAD = WI * (2 * NB - 1);
-        for (int t = 0; t < n_tiles; ++t) {
-            const int c = tile_chunk(t);
-            wait_loads<AHEAD>();
-            scores(kbuf + (t % NB) * TILE, 0, c, s);
-            lds_done();
-            place(t + NB, id, run);
-            fetch(t + NB + 1, id);
-            load_tile(t + NB, run, K_{});
+    for (int t = 0; t < n_tiles; ++t) {
+        wait_loads<0>();
+        __syncthreads();  // tile t is there, and no wave reads tile t - 1
+        if (t + 1 < n_tiles) {
+            load_tile(t + 1, id);
+            fetch(t + 2, id);
+        }
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            const int c = z.cb + 2 * t + sub;
+            if (c >= z.ce) break;
+            scores(kbuf + (t & 1) * TILE, sub, c, s);
             transform(c, s);
             softmax(s, ph, pl);
-            wait_loads<AHEAD>();
-            if (partly_seen(c)) special |= clean_chunk<HD>(vbuf + (t % NB) * TILE, lane);
-            pv(vbuf + (t % NB) * TILE, 0, ph, pl);
-            lds_done();
-            load_tile(t + NB, run, V_{});
-        }
-        wait_loads<0>();
-    } else {
-        for (int t = 0; t < n_tiles; ++t) {
-            wait_loads<0>();
-            __syncthreads();  // tile t is there, and no wave reads tile t - 1
-            if (t + 1 < n_tiles) {
-                place(t + 1, id, run);
-                fetch(t + 2, id);
-                load_tile(t + 1, run, K_{});
-                load_tile(t + 1, run, V_{});
-            }
-#pragma unroll
-            for (int sub = 0; sub < CPT; ++sub) {
-                const int c = tile_chunk(t) + sub;
-                if (c >= z.ce) break;
-                scores(kbuf + (t % NB) * TILE, sub, c, s);
-                transform(c, s);
-                softmax(s, ph, pl);
-                if (partly_seen(c)) special |= clean_chunk<HD>(vbuf + (t % NB) * TILE + 64 * HD * sub, lane);
-                pv(vbuf + (t % NB) * TILE, sub, ph, pl);
-            }
+            if (partly_seen(c)) special |= clean_chunk<HD>(vbuf + (t & 1) * TILE + 64 * HD * sub, lane);
+            pv(vbuf + (t & 1) * TILE, sub, ph, pl);
         }
     }
     const bool any_bad = __syncthreads_or(rows.bad);  // (and every wave is done with the tiles)
-    if (KG == 1) special = __syncthreads_or(special);
-    if (special)
+    if (__syncthreads_or(special))
 #pragma unroll 1
-        for (int t = 0; t < n_tiles; ++t)
-#pragma unroll 1
-            for (int c = tile_chunk(t); c < min(tile_chunk(t) + CPT, z.ce); ++c)
-                if (partly_seen(c))
-                    add_special<HD, RT>(p, z, rows.v, rows.table, chunk_key(c, z.n_pre, z.lo_base), h2, lor, span, o);
-
-    if constexpr (KG > 1) {
-        // the waves' states through LDS, merged in wave order: wave g takes
-        // the output tiles g, g + KG, ...
-        static_assert(RT == 1, "narrow items are one row tile");
-        float4v* const so = reinterpret_cast<float4v*>(lds);
-        float2* const sml = reinterpret_cast<float2*>(lds + kNW * DT * 64 * 64);
-        sml[wave * 64 + lane] = make_float2(m[0], half_sum(l[0]));
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-                so[((wave * DT + dt) * 4 + i4) * 64 + lane] =
-                    float4v{o[dt][0][4 * i4], o[dt][0][4 * i4 + 1], o[dt][0][4 * i4 + 2], o[dt][0][4 * i4 + 3]};
-        __syncthreads();
-        if (!valid[0]) return;
-        float2 ml[KG];
-        float M = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < KG; ++g) {
-            ml[g] = sml[g * 64 + lane];
-            M = fmaxf(M, ml[g].x);
-        }
-        const float ms = M == -INFINITY ? 0.f : M;
-        float L = 0.f, w[KG];
-#pragma unroll
-        for (int g = 0; g < KG; ++g) {
-            w[g] = fast_exp2(ml[g].x - ms);  // 0 where the wave saw no key
-            L += ml[g].y * w[g];
-        }
-        if (any_bad) L = NAN;
-        const float inv = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + c32) % p.hpk, M, L) : 1.f;
-        if (z.slot >= 0 && wave == 0 && h2 == 0) store_sum(p, z, kvh, c32, M, L);
-        const RowOut<HD, F32> to(p, z, kvh, c32);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            if (dt % KG != kg) continue;
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                float4v x = so[(dt * 4 + i4) * 64 + lane] * w[0];
-#pragma unroll
-                for (int g = 1; g < KG; ++g) x += so[((g * DT + dt) * 4 + i4) * 64 + lane] * w[g];
-                to.store(32 * dt + 8 * i4 + 4 * h2, x, inv);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float L = any_bad ? NAN : half_sum(l[rt]);
-            if (!valid[rt]) continue;
-            const int rl = (wr * RT + rt) * 32 + c32;
-            if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
-            const float w = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + rl) % p.hpk, m[rt], L) : 1.f;
-            const RowOut<HD, F32> to(p, z, kvh, rl);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4)
-                    to.store(32 * dt + 8 * i4 + 4 * h2,
-                             float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
-        }
-    }
+        for (int c = z.cb; c < z.ce; ++c)
+            if (partly_seen(c)) add_special<HD, RT>(z, rows, chunk_key(c, z.n_pre, z.lo_base), h2, lor, span, o);
+    store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o);
 }
 
 // The wide item with f16 queries, as a software pipeline over 32-key chunks:
@@ -628,10 +845,10 @@ __device__ __forceinline__ void paged_body(const PagedParams& p, const PlanPiece
 // the MFMAs (in a burst ahead of them a wave stalls at each); the barrier after
 // step 2 t orders them behind the last reads of their buffers and ahead of
 // their first.  A tile's table entries are loaded a step before its loads.
-template <int HD, int RT, bool SC>
+template <int HD, bool SC>
 __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
-    using S_ = PagedShape<HD, RT, 1>;
-    constexpr int KS = S_::KS, DT = S_::DT, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
+    using S_ = WideShape<HD>;
+    constexpr int RT = S_::RT, KS = S_::KS, DT = S_::DT, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
     using Rows = CacheRows<HD>;
     constexpr int IPR = Rows::IPR;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -656,11 +873,11 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         rv[r] = rows.run(run_key(1, r), wanted(1), rows.entry(run_key(1, r)));
     }
 #pragma unroll
-    for (int x = 0; x < WI; ++x) rows.template load<false>(rk[x / IPR], x % IPR, to_k + 1024 * x);
+    for (int x = 0; x < WI; ++x) rows.template load<false>(rk[x / IPR], (x / IPR) & 1, x % IPR, to_k + 1024 * x);
 #pragma unroll
-    for (int x = 0; x < WI; ++x) rows.template load<true>(rk[x / IPR], x % IPR, to_v + 1024 * x);
+    for (int x = 0; x < WI; ++x) rows.template load<true>(rk[x / IPR], (x / IPR) & 1, x % IPR, to_v + 1024 * x);
 #pragma unroll
-    for (int x = 0; x < WI; ++x) rows.template load<false>(rv[x / IPR], x % IPR, to_k + TILE + 1024 * x);
+    for (int x = 0; x < WI; ++x) rows.template load<false>(rv[x / IPR], (x / IPR) & 1, x % IPR, to_k + TILE + 1024 * x);
     // (the first step's empty PV product reads V tile 1's buffer)
 #pragma unroll
     for (int i = 0; i < TILE / (16 * 64 * kNW); ++i)
@@ -724,29 +941,15 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         auto load_nth = [&](auto x_) {
             constexpr int x = decltype(x_)::value;
             if constexpr (x < WI)  // K tile t + 2
-                rows.template load<false>(rk[x / IPR], x % IPR, to_k + ((PAR >> 1) & 1) * TILE + 1024 * x);
+                rows.template load<false>(rk[x / IPR], (x / IPR) & 1, x % IPR, to_k + ((PAR >> 1) & 1) * TILE + 1024 * x);
             else  // V tile t + 1
-                rows.template load<true>(rv[x / IPR - NR], x % IPR, to_v + (((PAR >> 1) + 1) & 1) * TILE + 1024 * (x - WI));
+                rows.template load<true>(rv[x / IPR - NR], (x / IPR) & 1, x % IPR, to_v + (((PAR >> 1) + 1) & 1) * TILE + 1024 * (x - WI));
         };
         if constexpr (SC) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (p.cap > 0.f) {
-                    // cap tanh(y / cap), tanh(y) = 1 - 2 / (1 + e^(2 y))
-                    const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s_cur[rt][i] = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s_cur[rt][i] * f));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s_cur[rt][i] *= p.qscale;
-                }
-                if (p.alibi) {
-                    const float d = (float)(posr[rt] - kb - 4 * h2);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s_cur[rt][i] -= slope[rt] * fabsf(d - (float)(8 * (i / 4) + i % 4));
-                }
-            }
+            for (int rt = 0; rt < RT; ++rt)
+                finish_scores<SC>(p, s_cur[rt], std::integral_constant<int, 16>{}, slope[rt], posr[rt],
+                                  [&](int i) { return kb + 8 * (i / 4) + 4 * h2 + i % 4; });
         }
         if (partly(kb)) {
 #pragma unroll
@@ -922,28 +1125,17 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     if (__syncthreads_or(special))
 #pragma unroll 1
         for (int i = 0; i < n; ++i)
-            if (partly(key_of(i))) add_special<HD, RT>(p, z, rows.v, rows.table, key_of(i), h2, lor, span, o);
-
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float L = any_bad ? NAN : half_sum(l[rt]);
-        if (!valid[rt]) continue;
-        const int rl = (wave * RT + rt) * 32 + c32;
-        if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
-        const float w = z.slot < 0 ? row_weight(p, kvh * p.hpk + (z.r0 + rl) % p.hpk, m[rt], L) : 1.f;
-        const RowOut<HD, false> to(p, z, kvh, rl);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-                to.store(32 * dt + 8 * i4 + 4 * h2,
-                         float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
-    }
+            if (partly(key_of(i))) add_special<HD, RT>(z, rows, key_of(i), h2, lor, span, o);
+    store_wide<HD, false>(p, z, kvh, wave, lane, any_bad, m, l, o);
 }
-template <int HD, bool F32, bool SC, bool WIDE>
+
+// Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more.
+enum Rows_ { kRows8, kRows16, kRows32, kRowsWide };
+
+template <int HD, bool F32, bool SC, int ROWS>
 __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedParams p) {
-    constexpr int RT = HD == 64 ? 2 : 1;
-    constexpr int LN = PagedShape<HD, 1, kNW>::LDS, LW = WIDE ? PagedShape<HD, RT, 1>::LDS : 0;
+    constexpr bool WIDE = ROWS == kRowsWide;
+    constexpr int LN = NarrowShape<HD, ROWS >= kRows32 ? 2 : 1>::LDS, LW = WIDE ? WideShape<HD>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char lds[LN > LW ? LN : LW];
     const int id = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
     // (the piece beside the header, not after it: one round trip)
@@ -952,10 +1144,18 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int n_pieces = p.head->n_pieces;
     __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces));
     if (sig != p.sig || id >= n_pieces) return;
-    if (WIDE && z.R > kNarrowRows) {
-        if constexpr (F32) paged_body<HD, RT, 1, true, SC>(p, z, kvh, lds);
-        else wide_body<HD, RT, SC>(p, z, kvh, lds);
-    } else paged_body<HD, 1, kNW, F32, SC>(p, z, kvh, lds);
+    if constexpr (WIDE) {
+        if (z.R > kNarrowRows) {
+            if constexpr (F32) wide_f32_body<HD, SC>(p, z, kvh, lds);
+            else wide_body<HD, SC>(p, z, kvh, lds);
+        } else if (z.R > 16) {
+            narrow_body<HD, 2, F32, SC, false>(p, z, kvh, lds);
+        } else {
+            narrow_body<HD, 1, F32, SC, false>(p, z, kvh, lds);
+        }
+    } else {
+        narrow_body<HD, ROWS == kRows32 ? 2 : 1, F32, SC, F32 && ROWS == kRows8>(p, z, kvh, lds);
+    }
 }
 
 // The pieces of a split item, joined with the sink: per row (M, L, O) of each
@@ -1048,7 +1248,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
         }
         if (spread ? lane >= LPR : r0 + grp >= rows) continue;
         const int rr = z.r0 + r, t = rr / p.hpk, h = kvh * p.hpk + rr - t * p.hpk;
-        o *= row_weight(p, h, m, l);
+        o *= row_weight(sink_of(p, h), m, l);
         const size_t at = (size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD + d;
         if constexpr (F32) {
             *reinterpret_cast<float4v*>(static_cast<float*>(p.out) + at) = o;
@@ -1076,13 +1276,18 @@ hipError_t launch_paged(const PagedParams& p, hipStream_t st) {
         constexpr bool F32 = decltype(f32)::value;
         const dim3 grid((unsigned)p.max_pieces * p.n_kv);
         const bool sc = p.cap > 0.f || p.alibi;
-        if (p.wide) {
-            if (sc) hipLaunchKernelGGL((paged_kernel<HD, F32, true, true>), grid, dim3(64 * kNW), 0, st, p);
-            else hipLaunchKernelGGL((paged_kernel<HD, F32, false, true>), grid, dim3(64 * kNW), 0, st, p);
-        } else {
-            if (sc) hipLaunchKernelGGL((paged_kernel<HD, F32, true, false>), grid, dim3(64 * kNW), 0, st, p);
-            else hipLaunchKernelGGL((paged_kernel<HD, F32, false, false>), grid, dim3(64 * kNW), 0, st, p);
-        }
+        auto go = [&](auto s, auto rows) {
+            hipLaunchKernelGGL((paged_kernel<HD, F32, decltype(s)::value, decltype(rows)::value>), grid, dim3(64 * kNW), 0, st, p);
+        };
+        auto by_rows = [&](auto s) {
+            // (f16 queries have no parts to pack)
+            if (p.wide) go(s, std::integral_constant<int, kRowsWide>{});
+            else if (p.rows > 16) go(s, std::integral_constant<int, kRows32>{});
+            else if (p.rows > 8 || !F32) go(s, std::integral_constant<int, kRows16>{});
+            else go(s, std::integral_constant<int, F32 ? kRows8 : kRows16>{});
+        };
+        if (sc) by_rows(std::true_type{});
+        else by_rows(std::false_type{});
         return hipGetLastError();
     });
 }
