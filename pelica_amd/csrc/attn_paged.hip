@@ -219,7 +219,10 @@ struct CacheRows {
     template <bool V>
     __device__ __forceinline__ void load(const Run& r, int odd, int j, uint32_t to) const {
         const uint64_t base = (V ? v : k) + r.off;
-        const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32), r.nrec, (uint32_t)kBufFlags};
+        // (uniform, though not where the compiler has put them in every case)
+        const u32x4 rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base),
+                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)),
+                          (uint32_t)__builtin_amdgcn_readfirstlane(r.nrec), (uint32_t)kBufFlags};
         uint32_t saved;
         __asm__ volatile(
             "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
@@ -271,10 +274,16 @@ struct NarrowShape {
     static constexpr int NB = HD == 64 ? 2 : 1;
     static constexpr int TILE = 32 * HD * 2;
     static constexpr int NR = 4, WI = NR * CacheRows<HD>::IPR;
-    static constexpr int STREAM = kNW * 2 * NB * TILE;
-    static constexpr int MERGE_O = kNW * DT * NT * 64 * 16, MERGE = MERGE_O + kNW * NT * 64 * 8;
-    static constexpr int LDS = STREAM > MERGE ? STREAM : MERGE;
+    // a wave's tiles, later its state: O, then (m, l)
+    static constexpr int MERGE_O = DT * NT * 64 * 16, MERGE = MERGE_O + NT * 64 * 8;
+    static constexpr int WAVE = 2 * NB * TILE > MERGE ? 2 * NB * TILE : MERGE;
+    static constexpr int LDS = kNW * WAVE;
 };
+
+// r / hpk (r < 2^30), as (r + 1/2) / hpk: at least 1 / (2 hpk) from a whole
+// number, hpk <= 2^16, far more than f64 is off by.  (An integer division is
+// ~25 dependent instructions ahead of the queries' and the output's addresses.)
+__device__ __forceinline__ int token_of(const PagedParams& p, int r) { return (int)(((double)r + 0.5) * p.inv_hpk); }
 
 // What a row's state (max M, sum L, both of the keys only) is multiplied by for
 // the output: the sink joins here, last, so that probabilities are relative
@@ -294,7 +303,7 @@ struct RowOut {
     bool part;
     __device__ __forceinline__ RowOut(const PagedParams& p, const PlanPiece& z, int kvh, int rl) {
         part = z.slot >= 0;
-        const int r = z.r0 + rl, t = r / p.hpk, h = kvh * p.hpk + r - t * p.hpk;
+        const int r = z.r0 + rl, t = token_of(p, r), h = kvh * p.hpk + r - t * p.hpk;
         at = part ? reinterpret_cast<char*>(p.ws_o + ((size_t)(z.slot * p.n_kv + kvh) * p.rows + rl) * HD)
                   : static_cast<char*>(p.out) + ((size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD) * (F32 ? 4 : 2);
     }
@@ -351,20 +360,39 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     constexpr int KS = S_::KS, DT = S_::DT, NB = S_::NB, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, c16 = lane & 15;
-    char* const kbuf = lds + wave * 2 * NB * TILE;
+    char* const kbuf = lds + wave * S_::WAVE;
     char* const vbuf = kbuf + NB * TILE;
     Rows rows(p, z, kvh, lane);
-    const uint32_t to = lds_byte(lds) + wave * 2 * NB * TILE;
+    const uint32_t to = lds_byte(lds) + wave * S_::WAVE;
     auto tile_chunk = [&](int t) { return z.cb + wave + kNW * t; };
+    // (a chunk in one page needs one entry)
+    const bool paged_by_32 = p.page_log2 >= 5;
     auto fetch = [&](int t, int (&id)[NR]) {
         const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+        id[0] = rows.entry(kb);
+        if (!paged_by_32) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) id[r] = rows.entry(kb + 8 * r);
+            for (int r = 1; r < NR; ++r) id[r] = rows.entry(kb + 8 * r);
+        }
     };
     auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
-        const int c = tile_chunk(t), kb = chunk_key(c, z.n_pre, z.lo_base);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) run[r] = rows.run(kb + 8 * r, c < z.ce, id[r]);
+        const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+        const bool whole = paged_by_32 & (kb >= z.lo) & (kb + 32 <= z.kend);
+        const uint32_t run_b = 8u * p.row_b;
+        run[0] = rows.run(kb, true, id[0]);
+        if (!whole) {
+            unrolled<NR - 1>([&](auto i) {
+                constexpr int r = decltype(i)::value + 1;
+                run[r] = rows.run(kb + 8 * r, true, paged_by_32 ? id[0] : id[r]);
+            });
+        } else {
+            unrolled<NR - 1>([&](auto i) {
+                constexpr int r = decltype(i)::value + 1;
+                run[r].off = run[0].off + (uint32_t)r * run_b;
+                run[r].nrec = run_b;
+                run[r].skip = 0;
+            });
+        }
     };
     auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
         constexpr bool V = decltype(is_v)::value;
@@ -384,9 +412,11 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     for (int t = 0; t <= NB; ++t) fetch(t, id[t]);
 #pragma unroll
     for (int t = 0; t < NB; ++t) {
-        place(t, id[t], run);
-        load_tile(t, run, K_{});
-        load_tile(t, run, V_{});
+        if (t < n_tiles) {
+            place(t, id[t], run);
+            load_tile(t, run, K_{});
+            load_tile(t, run, V_{});
+        }
     }
 
     // queries: column c16 of each tile, dims 8 g .. of every 32
@@ -394,17 +424,17 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     int posr[NT], lor[NT];
     unsigned span[NT];
     bool valid[NT];
-    float slope[NT], sink[NT];
+    float slope[NT], sink[NT];  // (raw: nothing here waits for a load)
     const bool low = PACK && c16 >= 8;  // this column holds lo parts
     constexpr int QES = F32 ? 4 : 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(rl, z.R - 1);
         valid[nt] = rl < z.R;
-        const int t = r / p.hpk, h = kvh * p.hpk + r - t * p.hpk;
+        const int t = token_of(p, r), h = kvh * p.hpk + r - t * p.hpk;
         const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * g) * QES;
-        sink[nt] = z.slot < 0 ? sink_of(p, h) : -INFINITY;
-        slope[nt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
+        sink[nt] = p.sinks_or_q[p.sinks ? h : 0];
+        slope[nt] = SC ? p.alibi_or_q[p.alibi ? h : 0] : 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             if constexpr (F32) {
@@ -428,7 +458,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         if (!valid[nt]) lor[nt] = INT32_MAX, span[nt] = 0;  // (sees none)
     }
     // every row sees the keys [lo_all, hi_all] and those below z.pe
-    const int hi_all = z.pos0, pos_last = z.pos0 + (z.R - 1) / p.hpk;
+    const int hi_all = z.pos0, pos_last = z.len - 1;
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
 
     float m[NT], l[NT];
@@ -442,15 +472,20 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     }
     bool special = false;
 
-    // requests in order K0 V0 (K1 V1): behind a tile's stand the 2 NB - 1 tiles
-    // after it (past the last one: empty requests); table entries a tile
-    // earlier
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) slope[nt] = SC && p.alibi ? slope[nt] * kLog2e : 0.f;
+
+    // requests in order K0 V0 (K1 V1), the next ones as their buffers become
+    // free: behind a tile's stand the 2 NB - 1 tiles after it, fewer at the end;
+    // table entries come a tile earlier
     constexpr int AHEAD = WI * (2 * NB - 1);
     for (int t = 0; t < n_tiles; ++t) {
         const int c = tile_chunk(t), kb = chunk_key(c, z.n_pre, z.lo_base);
         const char* const kt_ = kbuf + (t % NB) * TILE;
         char* const vt = vbuf + (t % NB) * TILE;
-        wait_loads<AHEAD>();
+        const int left = n_tiles - 1 - t;
+        if (left >= NB - 1) wait_loads<AHEAD>();
+        else wait_loads<WI>();
         typedef float float8v __attribute__((ext_vector_type(8)));
         float8v s[NT];
         {
@@ -480,10 +515,12 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
                     s[nt][i] = x;
                 }
         }
-        lds_done();
-        place(t + NB, id[NB], run);
-        fetch(t + NB + 1, id[NB]);
-        load_tile(t + NB, run, K_{});
+        if (left >= NB) {
+            lds_done();
+            place(t + NB, id[NB], run);
+            fetch(t + NB + 1, id[NB]);
+            load_tile(t + NB, run, K_{});
+        }
 
         auto key = [&](int i) { return kb + 16 * (i / 4) + 4 * g + i % 4; };
         const bool all = kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all);
@@ -523,7 +560,9 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             }
             l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         }
-        wait_loads<AHEAD>();
+        if (left >= NB) wait_loads<AHEAD>();
+        else if (left == NB - 1) wait_loads<2 * WI * (NB - 1)>();
+        else wait_loads<0>();
         if (!all && pos_last > hi_all) special |= clean_chunk<HD>(vt, lane);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -538,12 +577,12 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
                 if constexpr (F32 && !PACK) o[dt][nt] = mfma16(va, pl[nt], o[dt][nt]);
             }
         }
-        lds_done();
-        load_tile(t + NB, run, V_{});
+        if (left >= NB) {
+            lds_done();
+            load_tile(t + NB, run, V_{});
+        }
     }
-    wait_loads<0>();
-    const bool any_bad = __syncthreads_or(rows.bad);  // (and every wave is done with the tiles)
-    if (special)
+    if (__builtin_expect(special, 0))
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t) {
             const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
@@ -567,15 +606,17 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             }
         }
 
-    // the waves' states through LDS, merged in wave order: wave w takes the
-    // output tiles w, w + 4, ...
-    float4v* const so = reinterpret_cast<float4v*>(lds);
-    float2* const sml = reinterpret_cast<float2*>(lds + S_::MERGE_O);
+    // The waves' states through LDS, each in the room of its own tiles (which
+    // it has read), merged in wave order: wave w takes the output tiles w, w +
+    // 4, ...  A page outside the pool makes its wave's sums NaN.
+    auto so = [&](int w) { return reinterpret_cast<float4v*>(lds + w * S_::WAVE); };
+    auto sml = [&](int w) { return reinterpret_cast<float2*>(lds + w * S_::WAVE + S_::MERGE_O); };
+    lds_done();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        sml[(wave * NT + nt) * 64 + lane] = make_float2(m[nt], group4_sum(l[nt]));
+        sml(wave)[nt * 64 + lane] = make_float2(m[nt], rows.bad ? NAN : group4_sum(l[nt]));
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) so[((wave * DT + dt) * NT + nt) * 64 + lane] = o[dt][nt];
+        for (int dt = 0; dt < DT; ++dt) so(wave)[(dt * NT + nt) * 64 + lane] = o[dt][nt];
     }
     __syncthreads();
 #pragma unroll
@@ -584,7 +625,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kNW; ++w) {
-            ml[w] = sml[(w * NT + nt) * 64 + lane];
+            ml[w] = sml(w)[nt * 64 + lane];
             M = fmaxf(M, ml[w].x);
         }
         const float ms = M == -INFINITY ? 0.f : M;
@@ -594,18 +635,17 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             wt[w] = fast_exp2(ml[w].x - ms);  // 0 where the wave saw no key
             L += ml[w].y * wt[w];
         }
-        if (any_bad) L = NAN;
         const int rl = 16 * nt + (PACK ? c16 & 7 : c16);
         const bool stores = valid[nt] && !low;
-        const float weight = row_weight(sink[nt], M, L);
+        const float weight = row_weight(p.sinks ? sink[nt] * kLog2e : -INFINITY, M, L);
         const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1));
         if (stores && z.slot >= 0 && wave == 0 && g == 0) store_sum(p, z, kvh, rl, M, L);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             if ((dt * NT + nt) % kNW != wave) continue;
-            float4v x = so[(dt * NT + nt) * 64 + lane] * wt[0];
+            float4v x = so(0)[(dt * NT + nt) * 64 + lane] * wt[0];
 #pragma unroll
-            for (int w = 1; w < kNW; ++w) x += so[((w * DT + dt) * NT + nt) * 64 + lane] * wt[w];
+            for (int w = 1; w < kNW; ++w) x += so(w)[(dt * NT + nt) * 64 + lane] * wt[w];
             if constexpr (PACK) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] += ror8(x[i]);
@@ -626,7 +666,7 @@ __device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece
         const int rl = (wave * RT + rt) * 32 + c32;
         if (z.r0 + rl >= z.R) continue;
         if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
-        const float w = z.slot < 0 ? row_weight(sink_of(p, kvh * p.hpk + (z.r0 + rl) % p.hpk), m[rt], L) : 1.f;
+        const float w = z.slot < 0 ? row_weight(sink_of(p, kvh * p.hpk + z.r0 + rl - token_of(p, z.r0 + rl) * p.hpk), m[rt], L) : 1.f;
         const RowOut<HD, F32> to(p, z, kvh, rl);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
@@ -686,7 +726,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     for (int rt = 0; rt < RT; ++rt) {
         const int r = z.r0 + (wave * RT + rt) * 32 + c32;
         valid[rt] = r < z.R;
-        const int rc = min(r, z.R - 1), t = rc / p.hpk, h = kvh * p.hpk + rc - t * p.hpk;
+        const int rc = min(r, z.R - 1), t = token_of(p, rc), h = kvh * p.hpk + rc - t * p.hpk;
         const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * h2) * 4;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -708,7 +748,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     }
     // every row sees the keys [lo_all, hi_all] and those below z.pe
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
-    const int hi_all = z.pos0 + z.r0 / p.hpk, pos_last = z.pos0 + r_last / p.hpk;
+    const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
 
     float m[RT], l[RT];
@@ -893,7 +933,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     for (int rt = 0; rt < RT; ++rt) {
         const int r = z.r0 + (wave * RT + rt) * 32 + c32;
         valid[rt] = r < z.R;
-        const int rc = min(r, z.R - 1), t = rc / p.hpk, h = kvh * p.hpk + rc % p.hpk;
+        const int rc = min(r, z.R - 1), t = token_of(p, rc), h = kvh * p.hpk + rc - t * p.hpk;
         const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * h2) * 2;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qb[rt][ks] = load16(src + 32 * ks);
@@ -909,7 +949,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         for (int dt = 0; dt < DT; ++dt) o[dt][rt] = float16v{};
     }
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
-    const int hi_all = z.pos0 + z.r0 / p.hpk, pos_last = z.pos0 + r_last / p.hpk;
+    const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
 
     // a chunk that not every row sees whole; its V rows may hold infinities or
@@ -1142,7 +1182,9 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     const PlanPiece z = p.pieces[id];
     const uint32_t sig = p.head->sig;
     const int n_pieces = p.head->n_pieces;
-    __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces));
+    // (and what the end reads of the arguments: a line's first touch is a round trip)
+    __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces), "s"(p.out), "s"(p.o_tok),
+                     "s"(p.rows));
     if (sig != p.sig || id >= n_pieces) return;
     if constexpr (WIDE) {
         if (z.R > kNarrowRows) {
@@ -1247,7 +1289,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
             m = M;
         }
         if (spread ? lane >= LPR : r0 + grp >= rows) continue;
-        const int rr = z.r0 + r, t = rr / p.hpk, h = kvh * p.hpk + rr - t * p.hpk;
+        const int rr = z.r0 + r, t = token_of(p, rr), h = kvh * p.hpk + rr - t * p.hpk;
         o *= row_weight(sink_of(p, h), m, l);
         const size_t at = (size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD + d;
         if constexpr (F32) {

@@ -40,6 +40,8 @@ struct PagedParams {
     const PlanPiece* pieces;
     const int32_t* table;
     const float *sinks, *alibi;
+    const float *sinks_or_q, *alibi_or_q;  // (never NULL: a load that needs no branch)
+    double inv_hpk;             // 1 / hpk
     void* out;
     float* ws_ml;               // [slot][n_kv][rows] x (max, sum), base-2 max
     float* ws_o;                // [slot][n_kv][rows][hd]

@@ -155,6 +155,9 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, const void* q, const u
     p.table = d->page_table;
     p.sinks = sinks;
     p.alibi = d->alibi;
+    p.sinks_or_q = sinks ? sinks : static_cast<const float*>(q);
+    p.alibi_or_q = d->alibi ? d->alibi : static_cast<const float*>(q);
+    p.inv_hpk = 1.0 / x.hpk;
     p.out = out;
     p.ws_ml = x.ws_bytes ? static_cast<float*>(workspace) : nullptr;
     p.ws_o = x.ws_bytes ? reinterpret_cast<float*>(static_cast<char*>(workspace) + x.ml_bytes) : nullptr;
