@@ -4,11 +4,18 @@
 // own rows (f32 or f16), k and v rounded to f16 into the row of the token's
 // slot.
 //
-// Head slots [0, n_head) are q heads, then n_kv k heads, then n_kv v heads; a
-// lane holds 4 consecutive elements (16-byte accesses), a wave IT groups of
-// 64 / (HD / 4) heads of one token, whose (cos, sin) it loads once.
-// HBM-bound: every byte is touched once; small steps are one dependent chain
-// of loads (slot and positions, table rows beside the heads) and stores.
+// Head slots [0, n_head) are q heads, then n_kv k heads, then n_kv v heads.  A
+// lane holds 8 elements of a head, 4 from each half of the rotated part (and
+// of the rest): NeoX pairs (j, j + rot / 2) and neighbouring pairs both lie in
+// one lane, so a rotation moves nothing between lanes.  A wave takes IT groups
+// of 64 / (HD / 8) heads of one token.  The token's (cos, sin) come once a
+// wave, a pair a lane whatever axis it turns by, and through LDS to the lanes
+// that need them.
+// HBM-bound in large steps, where the instructions a value costs come next
+// (4 elements a lane, partners over lane exchanges: 4000 tokens of 32 + 8 heads
+// of 128, three axes, 36 us; four scattered table loads a lane as well: 42.9);
+// small steps are one dependent chain of loads (slot and positions, table rows
+// beside the heads) and stores.
 #include <type_traits>
 
 #include "attn_paged.hpp"
@@ -18,140 +25,202 @@ namespace pelica {
 
 namespace {
 
-// EX: rotation partners lie whole lanes away (or in the lane); else they are
-// exchanged through LDS (NeoX pairs, rot not a multiple of 8).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+
+// Sum over the N (8, 16, 32) lanes of a head, in every one of them.
+template <int N>
+__device__ __forceinline__ float head_sum(float x) {
+    x = add_dpp<0xB1>(x);   // lane ^ 1
+    x = add_dpp<0x4E>(x);   // lane ^ 2
+    x = add_dpp<0x141>(x);  // the other four of eight
+    if constexpr (N >= 16) x = add_dpp<0x140>(x);  // the other eight of sixteen
+    if constexpr (N >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return x;
+}
+
+// 1 / sqrt(x) to the last bit or two: the instruction's result (1 unit) after
+// values below its range are scaled into it.
+__device__ __forceinline__ float rsqrt_full(float x) {
+    const bool small = x < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? x * 0x1p100f : x) * (small ? 0x1p50f : 1.f);
+}
+
+__device__ __forceinline__ half4 to_half(float4v x) {
+    return {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
+
+// EX: a lane holds both values of its pairs; else (rot not a multiple of 8)
+// partners are exchanged through LDS.
 template <int HD, int IT, bool HALF, bool EX>
-__global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int wg_heads) {
-    constexpr int LPH = HD / 4, HPW = 64 / LPH;
-    __shared__ float xch[EX ? 1 : 4][EX ? 1 : HPW][EX ? 1 : HD];
+__global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int tok_waves) {
+    constexpr int LPH = HD / 8, HPW = 64 / LPH;
+    __shared__ __attribute__((aligned(16))) float turn[4][HD];  // (cos, sin) of the token's pairs
+    __shared__ __attribute__((aligned(16))) float xch[EX ? 1 : 4][EX ? 1 : HPW][EX ? 4 : HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, sub = lane / LPH, e0 = 4 * (lane % LPH);
-    const int t = blockIdx.x / wg_heads, n_slot = p.n_head + 2 * p.n_kv;
-    const int slot0 = ((blockIdx.x % wg_heads) * 4 + wave) * (HPW * IT) + sub;
-    if (slot0 - sub >= n_slot) return;
+    const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
+    const uint32_t gw = blockIdx.x * 4u + wave;  // waves follow the tokens, workgroups do not
+    const int t = (int)(gw / (uint32_t)tok_waves), n_slot = p.n_head + 2 * p.n_kv;
+    const int slot0 = (int)(gw - (uint32_t)t * tok_waves) * (HPW * IT) + sub;
+    if (t >= p.n_tokens) return;
+    const int half = p.rot / 2;
+    const bool rot = EX && l < p.rot / 8;
+    // this lane's elements: ea .. ea + 3 and eb .. eb + 3
+    const int ea = !EX ? 4 * l : rot ? 4 * l : half + 4 * l;
+    const int eb = !EX ? HD / 2 + 4 * l : rot ? half + 4 * l : HD / 2 + 4 * l;
     const int64_t row = p.slots[t];
-    float4v x[IT];
+    float4v x[IT][2];
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
         const int h = min(slot0 + HPW * it, n_slot - 1), hk = h - p.n_head, hv = hk - p.n_kv;
         const float* src = hk < 0 ? p.q + (size_t)t * p.tok_q + (size_t)h * HD
                                   : (hv < 0 ? p.k + (size_t)hk * HD : p.v + (size_t)hv * HD) + (size_t)t * p.tok_kv;
-        x[it] = *reinterpret_cast<const float4v*>(src + e0);
+        x[it][0] = *reinterpret_cast<const float4v*>(src + ea);
+        x[it][1] = *reinterpret_cast<const float4v*>(src + eb);
     }
     const float4v one = {1.f, 1.f, 1.f, 1.f};
-    const float4v wq = p.q_norm ? *reinterpret_cast<const float4v*>(p.q_norm + e0) : one;
-    const float4v wk = p.k_norm ? *reinterpret_cast<const float4v*>(p.k_norm + e0) : one;
-    // cos, sin of this lane's elements
-    const int half = p.rot / 2;
-    const bool rot = e0 < p.rot;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
-    if (rot) {
+    float4v wq[2] = {one, one}, wk[2] = {one, one};
+    if (p.q_norm) {
+        wq[0] = *reinterpret_cast<const float4v*>(p.q_norm + ea);
+        wq[1] = *reinterpret_cast<const float4v*>(p.q_norm + eb);
+    }
+    if (p.k_norm) {
+        wk[0] = *reinterpret_cast<const float4v*>(p.k_norm + ea);
+        wk[1] = *reinterpret_cast<const float4v*>(p.k_norm + eb);
+    }
+    float4v cs[2] = {one, one};  // (cos, sin) of the lane's pairs: two, two
+    if (p.rot) {
         int pos[4];
 #pragma unroll
         for (int a = 0; a < 4; ++a) pos[a] = a < p.n_axes ? p.positions[(size_t)a * p.axis_stride + t] : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = e0 + i;
-            if (e >= p.rot) continue;
-            const int j = p.neox ? (e < half ? e : e - half) : e >> 1;
+        for (int jj = 0; jj < (HD + 127) / 128; ++jj) {
+            const int j = lane + 64 * jj;
+            if (j >= half) break;
             int at = pos[0];
             if (p.n_axes > 1) {
                 uint32_t word = p.axis[0];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) word = (j >> 4) == w ? p.axis[w] : word;
+                for (int w = 1; w < HD / 32; ++w) word = (j >> 4) == w ? p.axis[w] : word;
                 const int a = (word >> (2 * (j & 15))) & 3;
                 at = a == 0 ? pos[0] : a == 1 ? pos[1] : a == 2 ? pos[2] : pos[3];
             }
-            if ((unsigned)at >= (unsigned)p.covered) {
-                c[i] = sn[i] = NAN;
-            } else if (p.table_split <= 0) {
-                const float2 v = *reinterpret_cast<const float2*>(p.table + ((size_t)at * half + j) * 2);
-                c[i] = v.x, sn[i] = v.y;
-            } else {
+            const bool there = (unsigned)at < (unsigned)p.covered;
+            const int at_ = there ? at : 0;
+            float2 v = *reinterpret_cast<const float2*>(
+                p.table + ((size_t)(p.table_split > 0 ? at_ >> 8 : at_) * half + j) * 2);
+            if (p.table_split > 0) {
                 // angle addition of the rows for pos / 256 and pos % 256
-                const float2 u = *reinterpret_cast<const float2*>(p.table + ((size_t)(at >> 8) * half + j) * 2);
-                const float2 v = *reinterpret_cast<const float2*>(
-                    p.table + ((size_t)(p.table_split + (at & 255)) * half + j) * 2);
-                c[i] = u.x * v.x - u.y * v.y;
-                sn[i] = u.y * v.x + u.x * v.y;
+                const float2 u = *reinterpret_cast<const float2*>(
+                    p.table + ((size_t)(p.table_split + (at_ & 255)) * half + j) * 2);
+                v = make_float2(v.x * u.x - v.y * u.y, v.y * u.x + v.x * u.y);
             }
+            *reinterpret_cast<float2*>(&turn[wave][2 * j]) = there ? v : make_float2(NAN, NAN);
+        }
+        // (a wave's LDS accesses complete in order)
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        if (rot) {
+            // NeoX: pairs ea .. ea + 3; else ea / 2, ea / 2 + 1 and eb / 2, eb / 2 + 1
+            cs[0] = *reinterpret_cast<const float4v*>(&turn[wave][p.neox ? 2 * ea : ea]);
+            cs[1] = *reinterpret_cast<const float4v*>(&turn[wave][p.neox ? 2 * ea + 4 : eb]);
         }
     }
     if (row < 0 || row >= p.n_slots) return;  // (uniform: a padding row)
     const int64_t base = (row >> p.page_log2) * p.page_stride + (row & ((1LL << p.page_log2) - 1)) * p.row_stride;
-    const bool hi = p.neox && e0 >= half;
-    const int partner = !rot || !p.neox ? lane : hi ? lane - half / 4 : lane + half / 4;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
         const int h = slot0 + HPW * it, hk = h - p.n_head, hv = hk - p.n_kv;
-        float4v y = x[it];
+        float4v a = x[it][0], b = x[it][1];
         if (p.q_norm || p.k_norm) {
-            float ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
-#pragma unroll
-            for (int off = LPH / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+            const float ss = head_sum<LPH>(((a[0] * a[0] + a[1] * a[1]) + (a[2] * a[2] + a[3] * a[3])) +
+                                           ((b[0] * b[0] + b[1] * b[1]) + (b[2] * b[2] + b[3] * b[3])));
             if (hk < 0 ? p.q_norm != nullptr : hv < 0 && p.k_norm) {
-                const float inv = 1.f / __builtin_sqrtf(ss / (float)HD + p.eps);
-                const float4v w = hk < 0 ? wq : wk;
+                const float inv = rsqrt_full(ss * (1.f / HD) + p.eps);
+                const float4v wa = hk < 0 ? wq[0] : wk[0], wb = hk < 0 ? wq[1] : wk[1];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = y[i] * inv * w[i];
+                for (int i = 0; i < 4; ++i) a[i] = a[i] * inv * wa[i], b[i] = b[i] * inv * wb[i];
             }
         }
-        if (p.rot) {
-            float4v z;
-            if constexpr (EX) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = p.neox ? __shfl(y[i], partner, 64) : y[i ^ 1];
-            } else {
-                // (a wave's LDS accesses complete in order)
-                *reinterpret_cast<float4v*>(&xch[wave][sub][e0]) = y;
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = e0 + i;
-                    z[i] = xch[wave][sub][e >= p.rot ? e : p.neox ? (e < half ? e + half : e - half) : e ^ 1];
-                }
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            }
+        if constexpr (EX) {
             if (rot && hv < 0) {
-                float4v r;
+                if (p.neox) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool second = p.neox ? e0 + i >= half : (i & 1) != 0;
-                    r[i] = e0 + i >= p.rot ? y[i] : second ? z[i] * sn[i] + y[i] * c[i] : y[i] * c[i] - z[i] * sn[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const float c = cs[i >> 1][2 * (i & 1)], sn = cs[i >> 1][2 * (i & 1) + 1], u = a[i], w = b[i];
+                        a[i] = u * c - w * sn;
+                        b[i] = u * sn + w * c;
+                    }
+                } else {
+                    auto turn2 = [](float4v& y, const float4v r) {
+                        const float4v u = y;
+                        y[0] = u[0] * r[0] - u[1] * r[1], y[1] = u[0] * r[1] + u[1] * r[0];
+                        y[2] = u[2] * r[2] - u[3] * r[3], y[3] = u[2] * r[3] + u[3] * r[2];
+                    };
+                    turn2(a, cs[0]);
+                    turn2(b, cs[1]);
                 }
-                y = r;
             }
+        } else {
+            *reinterpret_cast<float4v*>(&xch[wave][sub][ea]) = a;
+            *reinterpret_cast<float4v*>(&xch[wave][sub][eb]) = b;
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = (i < 4 ? ea : eb) + (i & 3);
+                const bool second = p.neox ? e >= half : (e & 1) != 0;
+                const int j = e >= p.rot ? 0 : !p.neox ? e >> 1 : second ? e - half : e;
+                const float own = i < 4 ? a[i & 3] : b[i & 3];
+                const float z = xch[wave][sub][!p.neox ? e ^ 1 : second ? j : j + half], c = turn[wave][2 * j], sn = turn[wave][2 * j + 1];
+                const float r = second ? z * sn + own * c : own * c - z * sn;
+                const float y = e < p.rot && hv < 0 ? r : own;
+                if (i < 4) a[i & 3] = y;
+                else b[i & 3] = y;
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         }
         if (h >= n_slot) break;
-        const half4 f = {(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
-        if (hk < 0) {
-            const size_t at = (size_t)t * p.tok_o + (size_t)h * HD + e0;
-            if constexpr (HALF) *reinterpret_cast<half4*>(static_cast<uint16_t*>(p.q_out) + at) = f;
-            else *reinterpret_cast<float4v*>(static_cast<float*>(p.q_out) + at) = y;
+        if (!HALF && hk < 0) {
+            float* dst = static_cast<float*>(p.q_out) + (size_t)t * p.tok_o + (size_t)h * HD;
+            *reinterpret_cast<float4v*>(dst + ea) = a;
+            *reinterpret_cast<float4v*>(dst + eb) = b;
         } else {
-            uint16_t* dst = hv < 0 ? p.k_pages + (int64_t)hk * p.head_stride : p.v_pages + (int64_t)hv * p.head_stride;
-            *reinterpret_cast<half4*>(dst + base + e0) = f;
+            uint16_t* dst = hk < 0   ? static_cast<uint16_t*>(p.q_out) + (size_t)t * p.tok_o + (size_t)h * HD
+                            : hv < 0 ? p.k_pages + base + (int64_t)hk * p.head_stride
+                                     : p.v_pages + base + (int64_t)hv * p.head_stride;
+            *reinterpret_cast<half4*>(dst + ea) = to_half(a);
+            *reinterpret_cast<half4*>(dst + eb) = to_half(b);
         }
     }
 }
 
+// Head groups a wave of a large step (4000 tokens of 32 + 8 heads of 128: one
+// group 30.1 us, two 27.0, three 28.1, five 29.0; 1000 tokens 11.2, 9.6, 9.5,
+// 9.8; the step's bytes at a copy's rate: 24.1).
+constexpr int kQkvGroups = 2;
+
 }  // namespace
 
 hipError_t launch_paged_qkv(const PagedQkvParams& p, hipStream_t st) {
-    const int hpw = 64 / (p.hd / 4), n_slot = p.n_head + 2 * p.n_kv;
+    const int hpw = 64 / (p.hd / 8), n_slot = p.n_head + 2 * p.n_kv;
     const int groups = (n_slot + hpw - 1) / hpw;
-    // one group a wave while a step waits for its one round trip, two once its
-    // bytes bound it
-    const int it = (long long)groups * p.n_tokens <= 10240 ? 1 : 2;
-    const int wg_heads = ((groups + it - 1) / it + 3) / 4;
-    const bool ex = !p.neox || p.rot % 8 == 0;
+    // one group a wave while a step waits for its one round trip (500 tokens:
+    // one and two alike, 6.7 us), two once its bytes bound it
+    const int it = (long long)groups * p.n_tokens <= 5120 ? 1 : kQkvGroups;
+    const int tok_waves = (groups + it - 1) / it;
+    const bool ex = p.rot % 8 == 0;
     ProfScope ps(kProfPagedQkv, st);
-    const dim3 grid((unsigned)p.n_tokens * wg_heads);
+    const dim3 grid((unsigned)(((int64_t)p.n_tokens * tok_waves + 3) / 4));
     auto go = [&](auto hd, auto i, auto half, auto e) {
         hipLaunchKernelGGL((paged_qkv_kernel<decltype(hd)::value, decltype(i)::value, decltype(half)::value, decltype(e)::value>),
-                           grid, dim3(256), 0, st, p, wg_heads);
+                           grid, dim3(256), 0, st, p, tok_waves);
         return hipGetLastError();
     };
     auto c = [&](auto hd, auto i, auto half) {
@@ -159,7 +228,7 @@ hipError_t launch_paged_qkv(const PagedQkvParams& p, hipStream_t st) {
     };
     auto b = [&](auto hd, auto i) { return p.half ? c(hd, i, std::true_type{}) : c(hd, i, std::false_type{}); };
     auto a = [&](auto hd) {
-        return it == 1 ? b(hd, std::integral_constant<int, 1>{}) : b(hd, std::integral_constant<int, 2>{});
+        return it == 1 ? b(hd, std::integral_constant<int, 1>{}) : b(hd, std::integral_constant<int, kQkvGroups>{});
     };
     switch (p.hd) {
         case 64: return a(std::integral_constant<int, 64>{});
