@@ -371,7 +371,7 @@ typedef struct PelicaPagedDesc {
     int64_t q_token_stride;     /* values between tokens of q; 0 = n_head * hd */
     int64_t out_token_stride;   /* values between tokens of out; 0 = n_head * hd */
     float scale;                /* 0 = 1/sqrt(hd) */
-    float softcap;              /* c > 0: scores c tanh(s / c) (ahead of the alibi term); 0 = none */
+    float softcap;              /* c > 0: scores c tanh(s / c) (ahead of the alibi term), 1e-30 .. 1e30; 0 = none */
 } PelicaPagedDesc;
 
 /* The work list of a step's attention, made on the GPU from q_start,

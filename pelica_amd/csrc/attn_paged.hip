@@ -318,17 +318,42 @@ __device__ __forceinline__ void store_sum(const PagedParams& p, const PlanPiece&
     reinterpret_cast<float2*>(p.ws_ml)[(size_t)(z.slot * p.n_kv + kvh) * p.rows + rl] = make_float2(M, L);
 }
 
+// The polynomial; times s, the capped score of a raw product up to tanh_to
+__device__ __forceinline__ float capped_small(const PagedParams& p, float s) {
+    const float u = s * s;
+    float y = __builtin_fmaf(p.tanh_c[4], u, p.tanh_c[3]);
+    y = __builtin_fmaf(y, u, p.tanh_c[2]);
+    y = __builtin_fmaf(y, u, p.tanh_c[1]);
+    return __builtin_fmaf(y, u, p.tanh_c[0]);
+}
+
+// Raw products to capped scores in the log2 domain: the polynomial, and
+// cap tanh(y) = cap - 2 cap / (1 + e^(2 y)), saturating at both ends, past it
+template <int N, typename V>
+__device__ __forceinline__ void cap_scores(const PagedParams& p, V& s) {
+    float most = 0.f;  // (NaN keeps to the polynomial, and is NaN there)
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(s[i]));
+    if (__builtin_amdgcn_ballot_w64(most > p.tanh_to)) {
+        const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float far = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[i] * f));
+            s[i] = fabsf(s[i]) <= p.tanh_to ? s[i] * capped_small(p, s[i]) : far;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] *= capped_small(p, s[i]);
+    }
+}
+
 // Scores of a chunk (raw products, 16-bit or f32 queries) in the log2 domain:
 // scaled, capped, with the distance bias; v of a lane's scores at once.
 template <bool SC, typename V, int N, typename KEY>
 __device__ __forceinline__ void finish_scores(const PagedParams& p, V& s, std::integral_constant<int, N>, float slope, int pos,
                                               KEY key) {
     if (SC && p.cap > 0.f) {
-        // cap tanh(y / cap): tanh(y) = 1 - 2 / (1 + e^(2 y)), saturating at both
-        // ends; off by at most a few 2^-24 of the cap
-        const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[i] * f));
+        cap_scores<N>(p, s);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] *= p.qscale;
@@ -871,6 +896,9 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o);
 }
 
+// Scores: scaled; capped; with a distance bias, capped or not.
+enum ScoreMode { kPlain, kCapped, kBiased };
+
 // The wide item with f16 queries, as a software pipeline over 32-key chunks:
 // while the softmax of chunk c runs on the vector ALUs, the matrix cores take
 // QK^T of chunk c + 1 and PV of chunk c - 1, one MFMA at a time between the
@@ -885,7 +913,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
 // the MFMAs (in a burst ahead of them a wave stalls at each); the barrier after
 // step 2 t orders them behind the last reads of their buffers and ahead of
 // their first.  A tile's table entries are loaded a step before its loads.
-template <int HD, bool SC>
+template <int HD, int MODE>
 __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S_ = WideShape<HD>;
     constexpr int RT = S_::RT, KS = S_::KS, DT = S_::DT, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
@@ -942,7 +970,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         lor[rt] = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
         span[rt] = (unsigned)(pos - lor[rt]);
         if (!valid[rt]) lor[rt] = INT32_MAX, span[rt] = 0;  // (sees none)
-        slope[rt] = SC && p.alibi ? p.alibi[h] * kLog2e : 0.f;
+        slope[rt] = MODE == kBiased ? p.alibi[h] * kLog2e : 0.f;
         m[rt] = valid[rt] ? -INFINITY : 0.f;
         l[rt] = 0.f;
 #pragma unroll
@@ -963,7 +991,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 
     float16v s_a[RT], s_b[RT];
     half8 p_a[2][RT], p_b[2][RT];
-    const float qs = SC ? 1.f : p.qscale;
+    const float qs = MODE == kCapped || (MODE == kBiased && p.cap > 0.f) ? 1.f : p.qscale;
 
     auto step = [&](auto par, int c, float16v (&s_cur)[RT], float16v (&s_nxt)[RT], const half8 (&p_prv)[2][RT],
                     half8 (&p_cur)[2][RT]) {
@@ -985,11 +1013,9 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
             else  // V tile t + 1
                 rows.template load<true>(rv[x / IPR - NR], (x / IPR) & 1, x % IPR, to_v + (((PAR >> 1) + 1) & 1) * TILE + 1024 * (x - WI));
         };
-        if constexpr (SC) {
+        if (MODE == kCapped || (MODE == kBiased && p.cap > 0.f)) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                finish_scores<SC>(p, s_cur[rt], std::integral_constant<int, 16>{}, slope[rt], posr[rt],
-                                  [&](int i) { return kb + 8 * (i / 4) + 4 * h2 + i % 4; });
+            for (int rt = 0; rt < RT; ++rt) cap_scores<16>(p, s_cur[rt]);
         }
         if (partly(kb)) {
 #pragma unroll
@@ -1026,14 +1052,20 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         static_assert(NS % NM == 0, "whole scores a slot");
         constexpr int NLD = (PAR & 1) ? 2 * WI : 0;
         constexpr int LSL = HD == 128 ? NM : NM / 2;  // slots the loads go out in
-        float ms[RT], acc[RT][2], e[NS];
+        float ms[RT], acc[RT][2], e[NS], ahead[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             ms[rt] = m[rt] == -INFINITY ? 0.f : m[rt];
             acc[rt][0] = acc[rt][1] = 0.f;
+            if (MODE == kBiased) ahead[rt] = (float)(posr[rt] - kb - 4 * h2);
         }
         auto op_fma = [&](int i) {
-            if (i < NS) s_cur[i / 16][i % 16] = __builtin_fmaf(s_cur[i / 16][i % 16], qs, -ms[i / 16]);
+            if (i >= NS) return;
+            const int rt = i / 16;
+            float x = __builtin_fmaf(s_cur[rt][i % 16], qs, -ms[rt]);
+            if constexpr (MODE == kBiased)
+                x = __builtin_fmaf(-slope[rt], fabsf(ahead[rt] - (float)(8 * (i % 16 / 4) + i % 4)), x);
+            s_cur[rt][i % 16] = x;
         };
         auto op_exp = [&](int i) {
             if (i < NS) e[i] = fast_exp2(s_cur[i / 16][i % 16]);
@@ -1172,9 +1204,9 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 // Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more.
 enum Rows_ { kRows8, kRows16, kRows32, kRowsWide };
 
-template <int HD, bool F32, bool SC, int ROWS>
+template <int HD, bool F32, int MODE, int ROWS>
 __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedParams p) {
-    constexpr bool WIDE = ROWS == kRowsWide;
+    constexpr bool WIDE = ROWS == kRowsWide, SC = MODE != kPlain;
     constexpr int LN = NarrowShape<HD, ROWS >= kRows32 ? 2 : 1>::LDS, LW = WIDE ? WideShape<HD>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char lds[LN > LW ? LN : LW];
     const int id = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
@@ -1189,7 +1221,7 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     if constexpr (WIDE) {
         if (z.R > kNarrowRows) {
             if constexpr (F32) wide_f32_body<HD, SC>(p, z, kvh, lds);
-            else wide_body<HD, SC>(p, z, kvh, lds);
+            else wide_body<HD, MODE>(p, z, kvh, lds);
         } else if (z.R > 16) {
             narrow_body<HD, 2, F32, SC, false>(p, z, kvh, lds);
         } else {
@@ -1317,7 +1349,6 @@ hipError_t launch_paged(const PagedParams& p, hipStream_t st) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool F32 = decltype(f32)::value;
         const dim3 grid((unsigned)p.max_pieces * p.n_kv);
-        const bool sc = p.cap > 0.f || p.alibi;
         auto go = [&](auto s, auto rows) {
             hipLaunchKernelGGL((paged_kernel<HD, F32, decltype(s)::value, decltype(rows)::value>), grid, dim3(64 * kNW), 0, st, p);
         };
@@ -1328,8 +1359,10 @@ hipError_t launch_paged(const PagedParams& p, hipStream_t st) {
             else if (p.rows > 8 || !F32) go(s, std::integral_constant<int, kRows16>{});
             else go(s, std::integral_constant<int, F32 ? kRows8 : kRows16>{});
         };
-        if (sc) by_rows(std::true_type{});
-        else by_rows(std::false_type{});
+        // (all but the wide items of f16 queries take either score by one path)
+        if (p.cap > 0.f && !p.alibi && p.wide) go(std::integral_constant<int, F32 ? kBiased : kCapped>{}, std::integral_constant<int, kRowsWide>{});
+        else if (p.cap > 0.f || p.alibi) by_rows(std::integral_constant<int, kBiased>{});
+        else by_rows(std::integral_constant<int, kPlain>{});
         return hipGetLastError();
     });
 }

@@ -1,6 +1,8 @@
 // Launch parameters of the paged kernels (attn_pages.hip, attn_paged.hip,
 // attn_paged_qkv.hip).
 #pragma once
+#include <cmath>
+
 #include "attn_common.hpp"
 #include "attn_paged_plan.hpp"
 
@@ -51,10 +53,30 @@ struct PagedParams {
     uint32_t row_b, sig;        // bytes between rows of a page
     int n_kv, hpk, n_pages, max_pages, page_log2, window, rows;
     float qscale, cap;          // scale * log2 e; softcap (0: none)
+    // of raw products up to tanh_to: the capped score (log2 domain) as s times a
+    // polynomial in s^2
+    float tanh_c[5], tanh_to;
     // host side only
     int hd, max_pieces, max_joins;
     bool f32, wide;
 };
+// cap tanh(y), y = s scale / cap, for |y| <= 0.55: tanh(y) / y as the polynomial
+// in y^2 that interpolates it at the Chebyshev nodes of [0, 0.55^2], 2^-22.7
+// relative with every rounding counted.  (1 - 2 / (1 + e^2y) is off by 2^-23 of
+// the cap, however small the score is.)
+inline void capped_poly(PagedParams& p) {
+    constexpr double c[5] = {0.999999967298071, -0.333327914802321, 0.133188187804409, -0.05258626003574007, 0.01631040386184039};
+    if (!(p.cap > 0.f)) return;
+    const double f = (double)p.qscale / kLog2e / p.cap;  // y = f s
+    double g = (double)p.cap * kLog2e * f;
+    p.tanh_to = (float)(0.55 / f);
+    for (int i = 0; i < 5; ++i, g *= f * f) {
+        p.tanh_c[i] = (float)(c[i] * g);
+        // (a tiny cap: all scores take the other form)
+        if (!(std::fabs(c[i] * g) < 1e30)) p.tanh_to = -1.f;
+    }
+}
+
 hipError_t launch_paged(const PagedParams& p, hipStream_t st);
 hipError_t launch_paged_join(const PagedParams& p, hipStream_t st);
 

@@ -78,6 +78,8 @@ int check_paged(const PelicaPagedDesc* d) {
     if (d->window < 0) return fail(PELICA_ATTN_EINVAL, "window %d must be >= 0", d->window);
     if (!(d->scale >= 0.f) || std::isinf(d->scale)) return fail(PELICA_ATTN_EINVAL, "scale must be finite, >= 0");
     if (!(d->softcap >= 0.f) || std::isinf(d->softcap)) return fail(PELICA_ATTN_EINVAL, "softcap must be finite, >= 0");
+    if (d->softcap > 0.f && (d->softcap < 1e-30f || d->softcap > 1e30f))
+        return fail(PELICA_ATTN_EUNSUPPORTED, "softcap %g (0, or 1e-30 .. 1e30)", (double)d->softcap);
     if ((int64_t)d->n_tokens * d->n_head > (1 << 30))
         return fail(PELICA_ATTN_EUNSUPPORTED, "n_tokens x n_head above 2^30");
     if (!d->q_start || !d->seq_kv_len || !d->page_table)
@@ -176,6 +178,7 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, const void* q, const u
     p.rows = x.rows;
     p.qscale = (d->scale > 0.f ? d->scale : 1.f / std::sqrt((float)d->hd)) * pelica::kLog2e;
     p.cap = d->softcap;
+    pelica::capped_poly(p);
     p.hd = d->hd;
     p.max_pieces = (int)x.max_pieces;
     p.max_joins = x.max_joins;

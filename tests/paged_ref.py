@@ -10,7 +10,7 @@ U16, U32 = 2.0 ** -11, 2.0 ** -24  # half a step of f16 / f32, relative
 
 
 def attention(q, k_pages, v_pages, table, lens, new, *, page, window=0, prefix=None, sinks=None, slopes=None, cap=0.0,
-              scale=None):
+              scale=None, cap_off=2 ** -21):
     """q [rows, n_head, hd], pages [n_pages, page, n_kv, hd], table a list of
     page lists, in f64.  Returns (out, bound): the rows of requests with
     tokens, NaN elsewhere, and how far a kernel may be off per value, split
@@ -63,7 +63,7 @@ def attention(q, k_pages, v_pages, table, lens, new, *, page, window=0, prefix=N
             # of its scaling, bias and cap, and q's hi + lo parts (2^-22)
             dot = (qq.abs() @ kh.abs().T * scale).amax(1, keepdim=True)
             big = torch.where(seen, x, torch.zeros_like(x)).abs().amax(1, keepdim=True)
-            dx = dot * ((hd + 4) * U32 + 2 ** -22) + big * 8 * U32 + cap * 2 ** -21
+            dx = dot * ((hd + 4) * U32 + 2 ** -22) + big * 8 * U32 + cap * cap_off
             # weights are off by that twice (numerator, denominator), 2^-22 of
             # exp2 and of p's parts, and every f32 sum by a rounding a key
             f32[row:row + t, h] = a * (2 * dx + 2 ** -20 + 2 * n * U32)

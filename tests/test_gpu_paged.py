@@ -96,15 +96,15 @@ class Case:
                               softcap=self.cap, scale=self.scale, out=out, **kw)
         return out
 
-    def reference(self):
+    def reference(self, **kw):
         names = [[self.live.get(p, -1) for p in r] for r in self.table]
         return ref.attention(self.q, self.k, self.v, names, self.lens, self.new, page=self.page, window=self.window,
-                             prefix=self.prefix, sinks=self.sinks, slopes=self.slopes, cap=self.cap, scale=self.scale)
+                             prefix=self.prefix, sinks=self.sinks, slopes=self.slopes, cap=self.cap, scale=self.scale, **kw)
 
-    def check(self, out=None):
+    def check(self, out=None, **kw):
         out = self.device().run() if out is None else out
         torch.cuda.synchronize()
-        want, f32, f16 = self.reference()
+        want, f32, f16 = self.reference(**kw)
         ref.check(out, want, f32, f16 if self.half else None)
         idle = want.isnan()
         assert (out.cpu()[idle] == 123.0).all(), "a row of no request was written"
@@ -168,6 +168,22 @@ def test_scores(cap, slopes, hd):
     Case([300, 40, 130], [1, 3, 1], seed=9, q_scale=8.0, **kw).check()
     Case([300, 40, 130], [90, 3, 130], seed=10, half=True, window=64, prefix=[50, 40, 0], **kw).check()
     Case([300, 40, 130], [90, 3, 130], seed=11, n_head=5, n_kv=1, **kw).check()
+
+
+@pytest.mark.parametrize("cap", [50.0, 1000.0, 1e6])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_far_below_the_cap(cap, hd):
+    # up to 0.55 of the cap a capped score is off by a part of itself, not of the cap
+    Case([300, 40, 130], [1, 3, 1], seed=40, cap=cap, hd=hd).check(cap_off=0)
+    Case([300, 40, 130], [90, 3, 130], seed=41, cap=cap, hd=hd, slopes=True).check(cap_off=0)
+    Case([300, 40, 130], [90, 3, 130], seed=42, cap=cap, hd=hd, half=True).check(cap_off=0)
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e-20])
+def test_scores_far_above_the_cap(cap):
+    # (all scores are the cap's: a mean of the values)
+    Case([300, 40, 130], [1, 3, 1], seed=43, cap=cap, hd=64).check()
+    Case([300, 40, 130], [90, 3, 130], seed=44, cap=cap, hd=128, half=True).check()
 
 
 def test_scores_far_below_and_above():

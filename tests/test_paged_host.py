@@ -62,7 +62,8 @@ BAD = [
     (dict(max_pages=(1 << 26) + 1), attn.EINVAL, "max_pages"), (dict(window=-1), attn.EINVAL, "window"),
     (dict(scale=-1.0), attn.EINVAL, "scale"), (dict(scale=float("nan")), attn.EINVAL, "scale"),
     (dict(scale=float("inf")), attn.EINVAL, "scale"), (dict(softcap=-1.0), attn.EINVAL, "softcap"),
-    (dict(softcap=float("nan")), attn.EINVAL, "softcap"), (dict(row_stride=60), attn.EINVAL, "strides"),
+    (dict(softcap=float("nan")), attn.EINVAL, "softcap"), (dict(softcap=1e-35), attn.EUNSUPPORTED, "softcap"),
+    (dict(softcap=1e35), attn.EUNSUPPORTED, "softcap"), (dict(row_stride=60), attn.EINVAL, "strides"),
     (dict(row_stride=132), attn.EINVAL, "strides"), (dict(head_stride=4), attn.EINVAL, "strides"),
     (dict(page_stride=-8), attn.EINVAL, "strides"), (dict(row_stride=1 << 24), attn.EUNSUPPORTED, "strides"),
     (dict(q_start=None), attn.EINVAL, "NULL"), (dict(seq_kv_len=None), attn.EINVAL, "NULL"),
