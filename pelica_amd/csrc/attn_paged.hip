@@ -896,6 +896,9 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o);
 }
 
+// MFMAs between a wide step's LDS reads and their use (4, 6: alike, and more registers)
+constexpr int kAhead = 2;
+
 // Scores: scaled; capped; with a distance bias, capped or not.
 enum ScoreMode { kPlain, kCapped, kBiased };
 
@@ -985,6 +988,12 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     auto key_of = [&](int c) { return chunk_key(z.cb + c, z.n_pre, z.lo_base); };
     auto partly = [&](int kb) { return !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all)); };
     bool special = false;
+    // Chunks [w0, w0 + w_n] that every row sees whole (of a prefix's only those
+    // that run into them), one compare a step; the others are looked at closer.
+    const int w_end = z.n_pre + ((hi_all + 1 - z.lo_base) >> 5) - z.cb;
+    int w0 = z.n_pre + ((imax(lo_all - z.lo_base, 0) + 31) >> 5) - z.cb;
+    if (z.n_pre == 0 && z.lo_base == 0 && (z.pe >> 5) >= w0 + z.cb) w0 = -z.cb;
+    const unsigned w_n = (unsigned)imax(w_end - w0 - 1, 0);
 
     // S^T of the first chunk
     auto v_chunk = [&](int c) { return vbuf + ((c >> 1) & 1) * TILE + 64 * HD * (c & 1); };
@@ -1005,7 +1014,6 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 #pragma unroll
             for (int r = 0; r < NR; ++r) rk[r] = rows.run(run_key(t + 2, r), wanted(t + 2), id[r]);
         }
-        if (c > 0 && pos_last > hi_all && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
         auto load_nth = [&](auto x_) {
             constexpr int x = decltype(x_)::value;
             if constexpr (x < WI)  // K tile t + 2
@@ -1017,17 +1025,20 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) cap_scores<16>(p, s_cur[rt]);
         }
-        if (partly(kb)) {
+        if ((unsigned)(c - 1 - w0) >= w_n) {  // this chunk or the one before
+            if (c > 0 && pos_last > hi_all && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
+            if (partly(kb)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = kb + 8 * (i / 4) + 4 * h2 + i % 4;
+                for (int i = 0; i < 16; ++i) {
+                    const int key = kb + 8 * (i / 4) + 4 * h2 + i % 4;
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    s_cur[rt][i] = sees(key, z.pe, lor[rt], span[rt]) ? s_cur[rt][i] : -INFINITY;
+                    for (int rt = 0; rt < RT; ++rt)
+                        s_cur[rt][i] = sees(key, z.pe, lor[rt], span[rt]) ? s_cur[rt][i] : -INFINITY;
+                }
             }
         }
         // operands: KS pieces of K (chunk c + 1), then 2 DT of V^T (chunk
-        // c - 1), each read two ahead of its first MFMA
+        // c - 1), each read kAhead MFMAs ahead of its first
         constexpr int NOPD = KS + 2 * DT, NM = KS * RT + 2 * DT * RT;
         half8 opd[NOPD];
         const char* const kt = kbuf + (((PAR + 1) >> 1) & 1) * TILE;
@@ -1042,8 +1053,8 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
                 opd[r] = v_operand<HD>(vt, 32 * ((PAR + 3) & 1) + 16 * w, dt, lane);
             }
         };
-        read_opd(std::integral_constant<int, 0>{});
-        read_opd(std::integral_constant<int, 1>{});
+        constexpr int AHEAD = kAhead / RT;
+        unrolled<AHEAD>([&](auto i) { read_opd(i); });
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s_nxt[rt] = float16v{};
         // The softmax's stages (x - m, exp2, f16 pairs, row sum) are skewed by a
@@ -1088,7 +1099,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
             constexpr int u = decltype(u_)::value;
             constexpr bool of_k = u < KS * RT;
             constexpr int r = u / RT, rt = u % RT;
-            if constexpr (rt == 0 && r + 2 < NOPD) read_opd(std::integral_constant<int, r + 2>{});
+            if constexpr (rt == 0 && r + AHEAD < NOPD) read_opd(std::integral_constant<int, r + AHEAD>{});
             unrolled<NLD>([&](auto i) {
                 if constexpr (decltype(i)::value * LSL / NLD == u) load_nth(i);
             });
@@ -1172,8 +1183,21 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     using P1 = std::integral_constant<int, 1>;
     using P2 = std::integral_constant<int, 2>;
     using P3 = std::integral_constant<int, 3>;
+    // Of the waves of two workgroups on a SIMD the older one's instructions go
+    // first: it would end well ahead of the other, which then has the SIMD
+    // alone.  Of long pieces the wave with more to do goes first instead (512
+    // tokens over 30000 keys: 322 -> 308 us; short ones leave their slots to
+    // the next pieces: 2000 tokens took 81 us instead of 77).
+    auto priority = [&](int left) {
+        if (n <= 64) return;
+        if (left > 64) __builtin_amdgcn_s_setprio(3);
+        else if (left > 24) __builtin_amdgcn_s_setprio(2);
+        else if (left > 8) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+    };
     int c = 0;
     for (; c + 4 <= n; c += 4) {
+        priority(n - c);
         step(P0{}, c, s_a, s_b, p_b, p_a);
         step(P1{}, c + 1, s_b, s_a, p_a, p_b);
         step(P2{}, c + 2, s_a, s_b, p_b, p_a);
