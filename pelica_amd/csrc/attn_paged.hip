@@ -680,25 +680,52 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     }
 }
 
-// a wide item's output: every lane's dims of its rows
+// A wide item's output.  A lane holds 4 dims of every 8 of its row: a wave's 32
+// rows go through its part of the tiles' LDS (16-byte slots, their number
+// xor the row's last bits: no bank twice), so that each store covers whole rows.
 template <int HD, bool F32, int RT>
 __device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece& z, int kvh, int wave, int lane, bool bad,
-                                           const float (&m)[RT], const float (&l)[RT], const float16v (&o)[HD / 32][RT]) {
+                                           const float (&m)[RT], const float (&l)[RT], const float16v (&o)[HD / 32][RT],
+                                           char* lds) {
     const int h2 = lane >> 5, c32 = lane & 31;
+    float4v* const mine = reinterpret_cast<float4v*>(lds) + wave * (32 * HD / 4);
+    const bool part = z.slot >= 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float L = bad ? NAN : half_sum(l[rt]);
-        const int rl = (wave * RT + rt) * 32 + c32;
-        if (z.r0 + rl >= z.R) continue;
-        if (z.slot >= 0 && h2 == 0) store_sum(p, z, kvh, rl, m[rt], L);
-        const float w = z.slot < 0 ? row_weight(sink_of(p, kvh * p.hpk + z.r0 + rl - token_of(p, z.r0 + rl) * p.hpk), m[rt], L) : 1.f;
-        const RowOut<HD, F32> to(p, z, kvh, rl);
+        const int rl = (wave * RT + rt) * 32 + c32, r = min(z.r0 + rl, z.R - 1);
+        if (part && h2 == 0 && z.r0 + rl < z.R) store_sum(p, z, kvh, rl, m[rt], L);
+        const float w = part ? 1.f : row_weight(sink_of(p, kvh * p.hpk + r - token_of(p, r) * p.hpk), m[rt], L);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4)
-                to.store(32 * dt + 8 * i4 + 4 * h2,
-                         float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]}, w);
+                mine[c32 * (HD / 4) + ((8 * dt + 2 * i4 + h2) ^ (c32 & 7))] =
+                    float4v{o[dt][rt][4 * i4], o[dt][rt][4 * i4 + 1], o[dt][rt][4 * i4 + 2], o[dt][rt][4 * i4 + 3]} * w;
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        auto rows = [&](auto dims) {  // of a lane
+            constexpr int D = decltype(dims)::value, LPR = HD / D, RPI = 64 / LPR;
+#pragma unroll
+            for (int j = 0; j < 32 / RPI; ++j) {
+                const int rr = j * RPI + lane / LPR, d4 = (lane % LPR) * (D / 4), at = (wave * RT + rt) * 32 + rr;
+                const float4v x = mine[rr * (HD / 4) + (d4 ^ (rr & 7))];
+                float4v y = x;
+                if constexpr (D == 8) y = mine[rr * (HD / 4) + ((d4 + 1) ^ (rr & 7))];
+                if (z.r0 + at < z.R) {
+                    const RowOut<HD, F32> to(p, z, kvh, at);
+                    if constexpr (D == 8)
+                        *reinterpret_cast<half8*>(to.at + 8 * d4) =
+                            half8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
+                                  (_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+                    else *reinterpret_cast<float4v*>(to.at + 16 * d4) = x;
+                }
+            }
+        };
+        if (F32 || part) rows(std::integral_constant<int, 4>{});
+        else rows(std::integral_constant<int, 8>{});
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }
 }
 
@@ -893,7 +920,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
 #pragma unroll 1
         for (int c = z.cb; c < z.ce; ++c)
             if (partly_seen(c)) add_special<HD, RT>(z, rows, chunk_key(c, z.n_pre, z.lo_base), h2, lor, span, o);
-    store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o);
+    store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o, lds);
 }
 
 // MFMAs between a wide step's LDS reads and their use (4, 6: alike, and more registers)
@@ -1222,7 +1249,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 #pragma unroll 1
         for (int i = 0; i < n; ++i)
             if (partly(key_of(i))) add_special<HD, RT>(z, rows, key_of(i), h2, lor, span, o);
-    store_wide<HD, false>(p, z, kvh, wave, lane, any_bad, m, l, o);
+    store_wide<HD, false>(p, z, kvh, wave, lane, any_bad, m, l, o, lds);
 }
 
 // Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more.
