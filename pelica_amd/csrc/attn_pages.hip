@@ -297,7 +297,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     __shared__ int q0[kPagedMaxSeq + 1], kv[kPagedMaxSeq], pre[kPagedMaxSeq];  // q_start, kv_len, prefix
     __shared__ int costs[kPlanItems];
     __shared__ int part[4][kPlanWaves];
-    __shared__ float est[2][kPlanWaves], limit[2][kPlanWaves];
+    __shared__ float est[kPlanWaves], limit[kPlanWaves];
     __shared__ int at_bucket[kBuckets], hist[kPlanWaves][64];
     __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -412,67 +412,62 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         float total = 0.f;
         for (int i = lane; i < n_items; i += 64) total += (float)abs(costs[i]);
         const float share = fmaxf(wave_sum(total) / (float)p.fill, (float)kMinPiece);
-        // wave w's limit: 0.5 .. 3 shares, the last wave's none; then finer about
-        // the best
-        float step = 2.58f / (kPlanWaves - 2);
-        float mine = wave == kPlanWaves - 1 ? 1e9f : share * 0.5f * fast_exp2((float)wave * step);
-#pragma unroll 1
-        for (int round = 0; round < 2; ++round) {
-            mine = fmaxf(mine, (float)kMinPiece);
-            const float inv = 1.f / mine;
-            float time = 0.f, longest = 0.f;
-            int pieces = 0, slots = 0;
+        // wave w's limit: 0.72 .. 2.26 shares, the last wave's none (0.5 .. 3 and a
+        // second round about the best: 3 us more, and steps as long)
+        const float mine = wave == kPlanWaves - 1
+                               ? 1e9f
+                               : fmaxf(share * 0.72f * fast_exp2((float)wave * (1.65f / (kPlanWaves - 2))), (float)kMinPiece);
+        const float inv = 1.f / mine;
+        float time = 0.f, longest = 0.f;
+        int pieces = 0, slots = 0;
+        for (int i = lane; i < n_items; i += 64) {
+            const int c = abs(costs[i]);
+            const bool wide = costs[i] < 0;
+            const int chunks = wide ? c / kWideCost : c;
+            const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
+            time += PlanCost::share(wide, m, k > 1) * (float)k;
+            longest = fmaxf(longest, PlanCost::piece(wide, m));
+            pieces += k;
+            slots += k > 1 ? k : 0;
+        }
+        time = wave_sum(time);
+        longest = wave_fold(longest, [](float a, float b) { return fmaxf(a, b); });
+        pieces = wave_sum(pieces);
+        slots = wave_sum(slots);
+        float last = longest;
+        if (pieces > p.fill) {
+            // Of more than g `fill` pieces, the g + 1 that share a slot are
+            // at least as long as number g `fill` + 1 (longest first).  A
+            // histogram of the lengths, in 64ths of the longest, finds it.
+            hist[wave][lane] = 0;
+            const float scale = 63.99f / longest;
             for (int i = lane; i < n_items; i += 64) {
                 const int c = abs(costs[i]);
                 const bool wide = costs[i] < 0;
                 const int chunks = wide ? c / kWideCost : c;
                 const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-                time += PlanCost::share(wide, m, k > 1) * (float)k;
-                longest = fmaxf(longest, PlanCost::piece(wide, m));
-                pieces += k;
-                slots += k > 1 ? k : 0;
+                atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m) * scale)], k);
             }
-            time = wave_sum(time);
-            longest = wave_fold(longest, [](float a, float b) { return fmaxf(a, b); });
-            pieces = wave_sum(pieces);
-            slots = wave_sum(slots);
-            float last = longest;
-            if (pieces > p.fill) {
-                // Of more than g `fill` pieces, the g + 1 that share a slot are
-                // at least as long as number g `fill` + 1 (longest first).  A
-                // histogram of the lengths, in 64ths of the longest, finds it.
-                hist[wave][lane] = 0;
-                const float scale = 63.99f / longest;
-                for (int i = lane; i < n_items; i += 64) {
-                    const int c = abs(costs[i]);
-                    const bool wide = costs[i] < 0;
-                    const int chunks = wide ? c / kWideCost : c;
-                    const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-                    atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m) * scale)], k);
-                }
-                __builtin_amdgcn_wave_barrier();
-                const int have = hist[wave][lane], longer = pieces - wave_scan(have) + have;  // as long as this bucket's
-                for (int g = 1; g <= 3 && pieces > g * p.fill; ++g) {
-                    const int b = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(longer > g * p.fill) | 1);
-                    last = fmaxf(last, (float)(g + 1) * ((float)b + 0.5f) / scale);
-                }
+            __builtin_amdgcn_wave_barrier();
+            const int have = hist[wave][lane], longer = pieces - wave_scan(have) + have;  // as long as this bucket's
+            for (int g = 1; g <= 3 && pieces > g * p.fill; ++g) {
+                const int b = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(longer > g * p.fill) | 1);
+                last = fmaxf(last, (float)(g + 1) * ((float)b + 0.5f) / scale);
             }
-            if (lane == 0) {
-                est[round][wave] = slots <= p.max_slots ? PlanCost::step(time / (float)p.fill, last) : INFINITY;
-                limit[round][wave] = mine;
-            }
-            __syncthreads();
-            float best = INFINITY, l0 = 1e9f;
-#pragma unroll
-            for (int w = 0; w < kPlanWaves; ++w) {
-                const float e = est[round][w];
-                l0 = e < best ? limit[round][w] : l0;
-                best = fminf(best, e);
-            }
-            // (the last wave's limit splits nothing, and is always one to take)
-            if (round == 0) mine = l0 >= 1e9f ? l0 : l0 * fast_exp2(step * (2.f / kPlanWaves) * (float)(wave - kPlanWaves / 2));
-            else inv_limit = 1.f / l0;
         }
+        if (lane == 0) {
+            est[wave] = slots <= p.max_slots ? PlanCost::step(time / (float)p.fill, last) : INFINITY;
+            limit[wave] = mine;
+        }
+        __syncthreads();
+        float best = INFINITY, l0 = 1e9f;
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) {
+            const float e = est[w];
+            l0 = e < best ? limit[w] : l0;
+            best = fminf(best, e);
+        }
+        inv_limit = 1.f / l0;  // (the last wave's splits nothing, and is always one to take)
     }
 
     // where each bucket's pieces begin
