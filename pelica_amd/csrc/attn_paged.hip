@@ -319,31 +319,34 @@ __device__ __forceinline__ void store_sum(const PagedParams& p, const PlanPiece&
 }
 
 // The polynomial; times s, the capped score of a raw product up to tanh_to
+template <bool F16>
 __device__ __forceinline__ float capped_small(const PagedParams& p, float s) {
     const float u = s * s;
+    if constexpr (F16) return __builtin_fmaf(__builtin_fmaf(p.tanh_h[2], u, p.tanh_h[1]), u, p.tanh_h[0]);
     float y = __builtin_fmaf(p.tanh_c[4], u, p.tanh_c[3]);
     y = __builtin_fmaf(y, u, p.tanh_c[2]);
     y = __builtin_fmaf(y, u, p.tanh_c[1]);
     return __builtin_fmaf(y, u, p.tanh_c[0]);
 }
 
-// Raw products to capped scores in the log2 domain: the polynomial, and
+// Raw products to capped scores in the log2 domain, minus m: the polynomial, and
 // cap tanh(y) = cap - 2 cap / (1 + e^(2 y)), saturating at both ends, past it
-template <int N, typename V>
-__device__ __forceinline__ void cap_scores(const PagedParams& p, V& s) {
+template <int N, bool F16, typename V>
+__device__ __forceinline__ void cap_scores(const PagedParams& p, V& s, float m = 0.f) {
     float most = 0.f;  // (NaN keeps to the polynomial, and is NaN there)
+    const float to = p.tanh_to[F16];
 #pragma unroll
     for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(s[i]));
-    if (__builtin_amdgcn_ballot_w64(most > p.tanh_to)) {
+    if (__builtin_amdgcn_ballot_w64(most > to)) {
         const float c2 = p.cap * kLog2e, f = 2.f * p.qscale / p.cap;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float far = c2 - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[i] * f));
-            s[i] = fabsf(s[i]) <= p.tanh_to ? s[i] * capped_small(p, s[i]) : far;
+            const float far = c2 - m - 2.f * c2 * __builtin_amdgcn_rcpf(1.f + fast_exp2(s[i] * f));
+            s[i] = fabsf(s[i]) <= to ? __builtin_fmaf(s[i], capped_small<F16>(p, s[i]), -m) : far;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] *= capped_small(p, s[i]);
+        for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(s[i], capped_small<F16>(p, s[i]), -m);
     }
 }
 
@@ -353,7 +356,7 @@ template <bool SC, typename V, int N, typename KEY>
 __device__ __forceinline__ void finish_scores(const PagedParams& p, V& s, std::integral_constant<int, N>, float slope, int pos,
                                               KEY key) {
     if (SC && p.cap > 0.f) {
-        cap_scores<N>(p, s);
+        cap_scores<N, false>(p, s);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] *= p.qscale;
@@ -1027,7 +1030,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 
     float16v s_a[RT], s_b[RT];
     half8 p_a[2][RT], p_b[2][RT];
-    const float qs = MODE == kCapped || (MODE == kBiased && p.cap > 0.f) ? 1.f : p.qscale;
+    const float qs = MODE == kBiased && p.cap > 0.f ? 1.f : p.qscale;
 
     auto step = [&](auto par, int c, float16v (&s_cur)[RT], float16v (&s_nxt)[RT], const half8 (&p_prv)[2][RT],
                     half8 (&p_cur)[2][RT]) {
@@ -1048,9 +1051,12 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
             else  // V tile t + 1
                 rows.template load<true>(rv[x / IPR - NR], (x / IPR) & 1, x % IPR, to_v + (((PAR >> 1) + 1) & 1) * TILE + 1024 * (x - WI));
         };
-        if (MODE == kCapped || (MODE == kBiased && p.cap > 0.f)) {
+        float ms[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) cap_scores<16>(p, s_cur[rt]);
+        for (int rt = 0; rt < RT; ++rt) {
+            ms[rt] = m[rt] == -INFINITY ? 0.f : m[rt];
+            if (MODE == kCapped) cap_scores<16, true>(p, s_cur[rt], ms[rt]);
+            if (MODE == kBiased && p.cap > 0.f) cap_scores<16, true>(p, s_cur[rt]);
         }
         if ((unsigned)(c - 1 - w0) >= w_n) {  // this chunk or the one before
             if (c > 0 && pos_last > hi_all && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
@@ -1090,15 +1096,14 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         static_assert(NS % NM == 0, "whole scores a slot");
         constexpr int NLD = (PAR & 1) ? 2 * WI : 0;
         constexpr int LSL = HD == 128 ? NM : NM / 2;  // slots the loads go out in
-        float ms[RT], acc[RT][2], e[NS], ahead[RT];
+        float acc[RT][2], e[NS], ahead[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            ms[rt] = m[rt] == -INFINITY ? 0.f : m[rt];
             acc[rt][0] = acc[rt][1] = 0.f;
             if (MODE == kBiased) ahead[rt] = (float)(posr[rt] - kb - 4 * h2);
         }
         auto op_fma = [&](int i) {
-            if (i >= NS) return;
+            if (MODE == kCapped || i >= NS) return;
             const int rt = i / 16;
             float x = __builtin_fmaf(s_cur[rt][i % 16], qs, -ms[rt]);
             if constexpr (MODE == kBiased)

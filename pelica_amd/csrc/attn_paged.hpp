@@ -53,28 +53,36 @@ struct PagedParams {
     uint32_t row_b, sig;        // bytes between rows of a page
     int n_kv, hpk, n_pages, max_pages, page_log2, window, rows;
     float qscale, cap;          // scale * log2 e; softcap (0: none)
-    // of raw products up to tanh_to: the capped score (log2 domain) as s times a
-    // polynomial in s^2
-    float tanh_c[5], tanh_to;
+    // of raw products up to tanh_to[i]: the capped score (log2 domain) as s times
+    // a polynomial in s^2, of f32 and of f16 queries
+    float tanh_c[5], tanh_h[3], tanh_to[2];
     // host side only
     int hd, max_pieces, max_joins;
     bool f32, wide;
 };
-// cap tanh(y), y = s scale / cap, for |y| <= 0.55: tanh(y) / y as the polynomial
-// in y^2 that interpolates it at the Chebyshev nodes of [0, 0.55^2], 2^-22.7
-// relative with every rounding counted.  (1 - 2 / (1 + e^2y) is off by 2^-23 of
-// the cap, however small the score is.)
+// cap tanh(y), y = s scale / cap, of small y: tanh(y) / y as the polynomial in
+// y^2 that interpolates it at the Chebyshev nodes of [0, y_max^2].  Up to 0.55:
+// 2^-22.7 relative with every rounding counted.  (1 - 2 / (1 + e^2y) is off by
+// 2^-23 of the cap, however small the score is.)  Of f16 queries
+// three terms, up to 0.3: 1.2e-6 relative, less than the roundings of a large
+// score's own products; at cap 50 a weight is off by 2^-16 at most, where f16
+// rounds it by 2^-11.  (2000 tokens of head dim 64: five terms 97 us, three 83.)
 inline void capped_poly(PagedParams& p) {
-    constexpr double c[5] = {0.999999967298071, -0.333327914802321, 0.133188187804409, -0.05258626003574007, 0.01631040386184039};
     if (!(p.cap > 0.f)) return;
     const double f = (double)p.qscale / kLog2e / p.cap;  // y = f s
-    double g = (double)p.cap * kLog2e * f;
-    p.tanh_to = (float)(0.55 / f);
-    for (int i = 0; i < 5; ++i, g *= f * f) {
-        p.tanh_c[i] = (float)(c[i] * g);
-        // (a tiny cap: all scores take the other form)
-        if (!(std::fabs(c[i] * g) < 1e30)) p.tanh_to = -1.f;
-    }
+    auto scaled = [&](const double* c, int n, double most, float* to, float& limit) {
+        double g = (double)p.cap * kLog2e * f;
+        limit = (float)(most / f);
+        for (int i = 0; i < n; ++i, g *= f * f) {
+            to[i] = (float)(c[i] * g);
+            // (a tiny cap: all scores take the other form)
+            if (!(std::fabs(c[i] * g) < 1e30)) limit = -1.f;
+        }
+    };
+    constexpr double c[5] = {0.999999967298071, -0.333327914802321, 0.133188187804409, -0.05258626003574007, 0.01631040386184039};
+    constexpr double h[3] = {0.9999988351337193, -0.33309988804316676, 0.1263358239158045};
+    scaled(c, 5, 0.55, p.tanh_c, p.tanh_to[0]);
+    scaled(h, 3, 0.3, p.tanh_h, p.tanh_to[1]);
 }
 
 hipError_t launch_paged(const PagedParams& p, hipStream_t st);
