@@ -380,8 +380,10 @@ typedef struct PelicaPagedDesc {
  * descriptor has the same n_head, n_kv, hd, n_seq, n_tokens, max_q, page
  * sizes and counts, window and (NULL or not) prefix_len; calls with another
  * one write nothing.  Make it again when lengths change (the same buffer
- * will do).  plan: 16-byte aligned, pelica_attn_paged_plan_bytes bytes (0 on
- * an invalid descriptor). */
+ * will do).  q_start must not decrease: the plan of one that does is empty,
+ * and calls with it write nothing.  plan: 16-byte aligned,
+ * pelica_attn_paged_plan_bytes bytes (0 on an invalid descriptor); each call
+ * is told how many the buffer has. */
 size_t pelica_attn_paged_plan_bytes(const PelicaPagedDesc* desc);
 int pelica_attn_paged_plan(const PelicaPagedDesc* desc, void* plan, size_t plan_bytes, void* stream);
 
@@ -394,12 +396,12 @@ int pelica_attn_paged_plan(const PelicaPagedDesc* desc, void* plan, size_t plan_
  * initialisation; calls that share one must be ordered on one stream, in
  * captured graphs too. */
 size_t pelica_attn_paged_workspace_bytes(const PelicaPagedDesc* desc);
-int pelica_attn_paged(const PelicaPagedDesc* desc, const void* plan, const uint16_t* q, const uint16_t* k_pages,
-                      const uint16_t* v_pages, const float* sinks, uint16_t* out, void* workspace,
-                      size_t workspace_bytes, void* stream);
-int pelica_attn_paged_f32(const PelicaPagedDesc* desc, const void* plan, const float* q, const uint16_t* k_pages,
-                          const uint16_t* v_pages, const float* sinks, float* out, void* workspace,
-                          size_t workspace_bytes, void* stream);
+int pelica_attn_paged(const PelicaPagedDesc* desc, const void* plan, size_t plan_bytes, const uint16_t* q,
+                      const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, uint16_t* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int pelica_attn_paged_f32(const PelicaPagedDesc* desc, const void* plan, size_t plan_bytes, const float* q,
+                          const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, float* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* The step before attention over pages: n_tokens rows of q ([n_head][hd]
  * f32), k and v ([n_kv][hd] f32), row i's heads at i * token_stride (0: dense
@@ -409,8 +411,9 @@ int pelica_attn_paged_f32(const PelicaPagedDesc* desc, const void* plan, const f
  * axis_stride; axis_stride 0: one for all).  q goes to q_out (f32, may be q;
  * or f16 when q_half is set) at i * q_out_stride, k and v rows rounded to f16
  * into row slots[i] of the pages.  Rows whose slot is negative or past the
- * pool are skipped and write nothing.  A position outside the rotary table
- * gives NaN.  Of the descriptor: n_head, n_kv, hd (64, 128, 256), n_tokens,
+ * pool are skipped and write nothing; of two rows with one slot either's
+ * values stay there.  A position outside the rotary table gives NaN.  q_out
+ * may be q where their strides are one.  Of the descriptor: n_head, n_kv, hd (64, 128, 256), n_tokens,
  * page_size, n_pages and the three strides. */
 typedef struct PelicaPagedRope {
     int32_t rot;            /* rotated dims at the start of each head: even, <= hd; 0 = no rope */

@@ -240,7 +240,7 @@ def load_library() -> ctypes.CDLL:
     lib.pelica_attn_paged_workspace_bytes.argtypes = [gd]
     for fn in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
         fn.restype = ctypes.c_int
-        fn.argtypes = [gd, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        fn.argtypes = [gd, vp, sz, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.pelica_attn_paged_qkv.restype = ctypes.c_int
     lib.pelica_attn_paged_qkv.argtypes = [gd, ctypes.POINTER(PagedRope), vp, vp, vp, ctypes.c_int64, vp, vp,
                                           ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]

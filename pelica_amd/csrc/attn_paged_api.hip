@@ -84,6 +84,9 @@ int check_paged(const PelicaPagedDesc* d) {
         return fail(PELICA_ATTN_EUNSUPPORTED, "n_tokens x n_head above 2^30");
     if (!d->q_start || !d->seq_kv_len || !d->page_table)
         return fail(PELICA_ATTN_EINVAL, "q_start, seq_kv_len and page_table must be non-NULL");
+    if (misaligned(d->q_start, 4) || misaligned(d->seq_kv_len, 4) || misaligned(d->page_table, 4) ||
+        misaligned(d->prefix_len, 4) || misaligned(d->alibi, 4))
+        return fail(PELICA_ATTN_EINVAL, "arrays of the descriptor must be aligned to their values");
     return PELICA_ATTN_OK;
 }
 
@@ -127,7 +130,7 @@ PagedPlan plan_of(const PelicaPagedDesc* d) {
     return x;
 }
 
-int run_paged(const PelicaPagedDesc* d, const void* plan, const void* q, const uint16_t* k, const uint16_t* v,
+int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const void* q, const uint16_t* k, const uint16_t* v,
               const float* sinks, void* out, void* workspace, size_t workspace_bytes, bool f32, void* stream) {
     pelica::clear_error();
     int rc = check_paged(d);
@@ -141,7 +144,10 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, const void* q, const u
         if (st != 0 && (st < row || (st * es) % 16 || st >= 1LL << 31))
             return fail(PELICA_ATTN_EINVAL, "token stride %lld: 0, or >= n_head*hd (%lld), < 2^31 and a whole number of "
                         "16-byte pieces", (long long)st, (long long)row);
+    if (misaligned(sinks, 4)) return fail(PELICA_ATTN_EINVAL, "sinks must be aligned to its values");
     const PagedPlan x = plan_of(d);
+    // (kernels read pieces beside the header that says whether they are theirs)
+    if (plan_bytes < x.bytes) return fail(PELICA_ATTN_EWORKSPACE, "plan of %zu bytes needed, %zu given", x.bytes, plan_bytes);
     if (x.ws_bytes && (!workspace || workspace_bytes < x.ws_bytes))
         return fail(PELICA_ATTN_EWORKSPACE, "workspace of %zu bytes needed, %zu given", x.ws_bytes,
                     workspace ? workspace_bytes : (size_t)0);
@@ -307,16 +313,16 @@ size_t pelica_attn_paged_workspace_bytes(const PelicaPagedDesc* d) {
     return plan_of(d).ws_bytes;
 }
 
-int pelica_attn_paged(const PelicaPagedDesc* d, const void* plan, const uint16_t* q, const uint16_t* k_pages,
-                      const uint16_t* v_pages, const float* sinks, uint16_t* out, void* workspace,
-                      size_t workspace_bytes, void* stream) {
-    return run_paged(d, plan, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
+int pelica_attn_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const uint16_t* q,
+                      const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, uint16_t* out,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+    return run_paged(d, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
 }
 
-int pelica_attn_paged_f32(const PelicaPagedDesc* d, const void* plan, const float* q, const uint16_t* k_pages,
-                          const uint16_t* v_pages, const float* sinks, float* out, void* workspace,
-                          size_t workspace_bytes, void* stream) {
-    return run_paged(d, plan, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
+int pelica_attn_paged_f32(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const float* q,
+                          const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, float* out,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    return run_paged(d, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
 }
 
 int pelica_attn_paged_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope, const float* q, const float* k,
@@ -337,7 +343,8 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope,
         return fail(PELICA_ATTN_EINVAL, "token_stride %lld: 0, or at least a token's heads and a multiple of 4", (long long)token_stride);
     if (q_out_stride && (q_out_stride < wq || q_out_stride % 4))
         return fail(PELICA_ATTN_EINVAL, "q_out_stride %lld: 0, or >= n_head*hd and a multiple of 4", (long long)q_out_stride);
-    if (q_half && q_out == (const void*)q) return fail(PELICA_ATTN_EINVAL, "f16 q_out must not be q");
+    if (q_out == (const void*)q && (q_half || (q_out_stride ? q_out_stride : wq) != (token_stride ? token_stride : wq)))
+        return fail(PELICA_ATTN_EINVAL, "q_out may be q in f32 only, and at its stride");
     if (!(eps >= 0.f)) return fail(PELICA_ATTN_EINVAL, "eps must be >= 0");
     pelica::PagedQkvParams p{};
     if (rope && rope->rot) {

@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     __shared__ int item0[kPagedMaxSeq + 1];  // first item of each request
     __shared__ int q0[kPagedMaxSeq + 1], kv[kPagedMaxSeq], pre[kPagedMaxSeq];  // q_start, kv_len, prefix
     __shared__ int costs[kPlanItems];
-    __shared__ int part[4][kPlanWaves];
+    __shared__ int part[4][kPlanWaves], decreasing;
     __shared__ float est[kPlanWaves], limit[kPlanWaves];
     __shared__ int at_bucket[kBuckets], hist[kPlanWaves][64];
     __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads];
@@ -310,6 +310,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         }
     }
     if (tid < kBuckets) at_bucket[tid] = 0;
+    if (tid == 0) decreasing = 0;
     __syncthreads();
 
     // tokens of a request; 0: no item (none, or lengths that do not fit together)
@@ -325,7 +326,11 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     const int per = (p.n_seq + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(tid * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
     int n = 0, n_items;
-    for (int s = s0; s < s1; ++s) n += items_of(tokens(s));
+    for (int s = s0; s < s1; ++s) {
+        n += items_of(tokens(s));
+        // (rows of two requests: their items could be more than there is room for)
+        if (q0[s + 1] < q0[s]) decreasing = 1;
+    }
     int at = block_scan<kPlanThreads>(n, part[0], n_items);
     for (int s = s0; s < s1; ++s) {
         item0[s] = at;
@@ -333,6 +338,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     }
     if (tid == 0) item0[p.n_seq] = n_items;
     __syncthreads();
+    if (decreasing) n_items = 0;
 
     // r / hpk (r < 2^30), as (r + 1/2) / hpk in f64: at least 1 / (2 hpk) from
     // a whole number, hpk <= 2^16

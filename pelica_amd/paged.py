@@ -237,6 +237,7 @@ class PagedPlan:
         self._page_shape = (n_pages, page_size, n_kv, hd)
         with _on(stream):
             self.buffer = torch.empty(n, dtype=torch.uint8, device=self.device)
+        self._buffer, self._bytes = self.buffer.data_ptr(), n
         self.workspace_bytes = lib.pelica_attn_paged_workspace_bytes(ctypes.byref(self.desc))
         self.update(stream)
 
@@ -245,7 +246,7 @@ class PagedPlan:
         if _device() != self._dev:
             raise AttnError(EINVAL, f"the plan is on device {self._dev}, the current device is {_device()}")
         rc = (attn._lib or attn.load_library()).pelica_attn_paged_plan(
-            ctypes.byref(self.desc), self.buffer.data_ptr(), self.buffer.numel(), attn._stream_ptr(stream))
+            ctypes.byref(self.desc), self._buffer, self._bytes, attn._stream_ptr(stream))
         if rc:
             attn._check(rc)
         return self
@@ -312,7 +313,7 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
         x.softcap = softcap
     lib = attn._lib
     rc = (lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged)(
-        ctypes.byref(x), plan.buffer.data_ptr(), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        ctypes.byref(x), plan._buffer, plan._bytes, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
         None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws, ws_bytes, attn._stream_ptr(stream))
     if rc:
         attn._check(rc)

@@ -336,3 +336,36 @@ def test_captured_step_follows_new_lengths():
         eager = torch.full_like(a.qd, 123.0)
         paged.paged_attention(a.qd, a.kd, a.vd, plan.update(), sinks=sinks, out=eager, workspace=ws)
         assert torch.equal(eager, out)
+
+
+def test_first_rows_that_decrease():
+    # rows of two requests: nothing is planned, nothing written
+    c = Case([200, 90, 140], [2, 40, 3], n_head=16, n_kv=2, seed=31, half=True).device()
+    for start in ([0, 45, 5, 45], [0, 2, 1, 45], [45, 0, 45, 0]):
+        c.start.copy_(torch.tensor(start, dtype=torch.int32))
+        out = c.run(c.plan())
+        torch.cuda.synchronize()
+        assert (out == 123.0).all()
+    c.start.copy_(torch.tensor([0, 2, 42, 45], dtype=torch.int32))
+    c.check(c.run(c.plan()))
+
+
+def test_two_steps_at_once():
+    # two plans, workspaces and streams: split items of single tokens beside a chunk's
+    a = Case([9000, 4000], [1, 1], n_head=16, n_kv=2, sinks=True, seed=32).device()
+    b = Case([1500, 900], [200, 1], n_head=16, n_kv=2, hd=128, half=True, seed=33).device()
+    runs = []
+    torch.cuda.synchronize()
+    for c in (a, b):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            plan = c.plan(stream=st)
+            runs.append((c, st, plan, plan.new_workspace(), torch.full_like(c.qd, 123.0), c.dev(c.sinks)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, st, plan, ws, out, sinks in runs:
+            plan.update(stream=st)
+            paged.paged_attention(c.qd, c.kd, c.vd, plan, sinks=sinks, out=out, workspace=ws, stream=st)
+    torch.cuda.synchronize()
+    for c, _, _, _, out, _ in runs:
+        c.check(out)

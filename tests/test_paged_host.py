@@ -68,6 +68,9 @@ BAD = [
     (dict(page_stride=-8), attn.EINVAL, "strides"), (dict(row_stride=1 << 24), attn.EUNSUPPORTED, "strides"),
     (dict(q_start=None), attn.EINVAL, "NULL"), (dict(seq_kv_len=None), attn.EINVAL, "NULL"),
     (dict(page_table=None), attn.EINVAL, "NULL"),
+    (dict(q_start=A + 2), attn.EINVAL, "aligned"), (dict(seq_kv_len=A + 1), attn.EINVAL, "aligned"),
+    (dict(page_table=A + 2), attn.EINVAL, "aligned"), (dict(prefix_len=A + 2), attn.EINVAL, "aligned"),
+    (dict(alibi=A + 2), attn.EINVAL, "aligned"),
 ]
 
 
@@ -79,7 +82,7 @@ def test_bad_descriptors(kw, code, word):
     assert lib.pelica_attn_paged_workspace_bytes(ctypes.byref(d)) == 0
     _error(lib.pelica_attn_paged_plan(ctypes.byref(d), A, 1 << 30, None), code, word)
     for f in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
-        _error(f(ctypes.byref(d), A, A, A, A, None, A, A, 1 << 40, None), code, word)
+        _error(f(ctypes.byref(d), A, 1 << 40, A, A, A, None, A, A, 1 << 40, None), code, word)
 
 
 def test_null_and_misaligned_arguments():
@@ -92,13 +95,15 @@ def test_null_and_misaligned_arguments():
     _error(lib.pelica_attn_paged_plan(None, A, need, None), attn.EINVAL, "desc")
     ws = lib.pelica_attn_paged_workspace_bytes(ref)
     assert ws > 0
-    good = [A, A, A, A, None, A, A, ws, None]
+    good = [A, need, A, A, A, None, A, A, ws, None]
     for f in (lib.pelica_attn_paged, lib.pelica_attn_paged_f32):
-        for i in (0, 1, 2, 3, 5):
+        for i in (0, 2, 3, 4, 6):
             _error(f(ref, *[None if j == i else x for j, x in enumerate(good)]), attn.EINVAL, "NULL")
             _error(f(ref, *[A + 8 if j == i else x for j, x in enumerate(good)]), attn.EINVAL, "aligned")
-        _error(f(ref, *[None if j == 6 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
-        _error(f(ref, *[ws - 1 if j == 7 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
+        _error(f(ref, *[None if j == 7 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
+        _error(f(ref, *[ws - 1 if j == 8 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "workspace")
+        _error(f(ref, *[need - 1 if j == 1 else x for j, x in enumerate(good)]), attn.EWORKSPACE, "plan")
+        _error(f(ref, *[A + 2 if j == 5 else x for j, x in enumerate(good)]), attn.EINVAL, "sinks")
     for kw in (dict(q_token_stride=8), dict(out_token_stride=511), dict(q_token_stride=516), dict(out_token_stride=1 << 31)):
         d = _desc(max_q=16, **kw)
         _error(lib.pelica_attn_paged(ctypes.byref(d), *good), attn.EINVAL, "stride")
@@ -149,6 +154,7 @@ def test_qkv_arguments():
     _error(call(a3=1026), attn.EINVAL, "token_stride")
     _error(call(a10=1000), attn.EINVAL, "q_out_stride")
     _error(call(a8=A, a9=1), attn.EINVAL, "q_out")
+    _error(call(a8=A, a3=1536), attn.EINVAL, "q_out")
     _error(call(a6=float("nan")), attn.EINVAL, "eps")
     _error(call(_desc(hd=96)), attn.EUNSUPPORTED, "hd")
     _error(call(_desc(hd=128, page_size=7)), attn.EUNSUPPORTED, "page_size")
