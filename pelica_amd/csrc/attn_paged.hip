@@ -9,22 +9,35 @@
 // starts them at (sink, 1).  Query rows are (token, head) pairs of one kv
 // head's group, so a key row in LDS serves the whole group.
 //
-// A workgroup (four waves) takes one piece of the work list for one kv head:
-// narrow (an item of at most 32 rows): the waves take 32-key chunks in turn,
-// each with K and V buffers of its own, no barrier until their states are
-// merged through LDS; wide: the waves hold RT tiles of 32 rows each and walk
-// 64-key tiles together, double-buffered, one barrier a tile.
+// A workgroup (four waves, two a CU) takes one piece of the work list for one kv
+// head: narrow (an item of at most 32 rows: tokens, drafts), whose waves take
+// 32-key chunks in turn and are merged at the end, or wide (a chunk's 256 rows
+// of head dim 64, 128 of 128), whose waves share the keys.  Neighbouring
+// workgroups are the kv heads of one piece: with 8 kv heads an XCD's L2 holds
+// one head's keys for all the pieces that read them.
 //
-// v_mfma_f32_32x32x16_f16, S^T = K Q^T (K from LDS as A, the queries in
-// registers as B: a lane holds 16 scores of one row), O^T += V^T P^T (V by
-// transposing LDS reads, P straight from the score registers).  f32 queries:
-// q and p as f16 hi + lo parts, two products each, so that the output keeps
-// f32's precision (the cache's f16 rows are exact).
+// S^T = K Q^T (K from LDS as A, the queries in registers as B: a lane's scores
+// are all of one row), O^T += V^T P^T (V by transposing LDS reads, P straight
+// from the score registers).  f32 queries: q and p as f16 hi + lo parts, two
+// products each, so that the output keeps f32's precision (2^-22; the cache's
+// f16 rows are exact).  f16 queries: p is rounded to f16 (2^-11) in the sum as in
+// the product; the output's rounding is as large.
 //
-// Cache rows go HBM -> LDS by buffer loads, one resource per group of 8 (head
-// dim 64) or 4 rows: they lie in one page, whose base is scalar arithmetic on
-// its table entry, in 64 bits.  The resource ends with the rows the item may
-// see: what lies behind is not touched and reads as zeros.
+// Cache rows go HBM -> LDS by buffer loads, one resource per run of 8 rows: they
+// lie in one page, whose base is scalar arithmetic on its table entry, in 64
+// bits.  The resource ends with the rows the item may see: what lies behind is
+// not touched and reads as zeros.
+//
+// Measured (floors: bytes at a copy's 5.1 TB/s, or operations at a large f16
+// product's 1.13 PFLOP/s):
+//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   116 us (118)
+//   16 tokens with a bias over 300 - 6000, 16 / 16 of 128   96 us (99)
+//   one token over 32768, 64 / 8 of 64                      16 us + join 3.8 (13)
+//   64 tokens on windows of 128, 64 / 8 of 64              8.8 us (3.7: latency)
+//   512 tokens over 30512, 64 / 8 of 64                    291 us (224)
+//   4001 tokens, 32 / 4 of 128                             161 us (116)
+//   3 chunks of 700 and 28 drafts, 64 / 8 of 64            201 us + join 12.7 (114)
+//   2000 tokens, capped, 600 of prefix, 32 / 4 of 128       73 us + join 6.7 (31.5)
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -380,6 +393,12 @@ __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
 // f32 queries: PACK (at most 8 rows): hi parts in columns 0-7, lo parts in 8-15
 // of one operand, the scores added by a lane exchange, the outputs at the end;
 // otherwise two products each.
+// HBM-bound over long keys (32 ragged requests at the copy's rate: 116 us);
+// short ones are a chain of latencies: 64 windows of 128 keys are 8.8 us, of
+// which 1.5 until the piece and its table entries are there, 1 to request the
+// tiles, 2 until they land, 1.3 for the chunks, 2.4 for merge and store.  With
+// 32-row tiles, every tile requested and two merge barriers they were 11.4;
+// with a pack of 8 rows in a tile of 16, a 32768-key token went from 17.5 to 16.
 template <int HD, int NT, bool F32, bool SC, bool PACK>
 __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     static_assert(!PACK || (F32 && NT == 1), "packed hi and lo parts: f32, one tile");
@@ -732,7 +751,9 @@ __device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece
     }
 }
 
-// The wide item with f32 queries: hi and lo products, a chunk at a time.
+// The wide item with f32 queries: hi and lo products, a chunk at a time (bound by
+// its products, twice f16's, and not pipelined: prompts come in f16; 2000 tokens
+// of 32 / 4 heads of 128, capped: 117 us against 73).
 template <int HD, bool SC>
 __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S = WideShape<HD>;
@@ -929,7 +950,9 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
 // MFMAs between a wide step's LDS reads and their use (4, 6: alike, and more registers)
 constexpr int kAhead = 2;
 
-// Scores: scaled; capped; with a distance bias, capped or not.
+// Scores: scaled; capped; with a distance bias, capped or not.  (A cap between
+// the MFMAs as well: 76 us instead of 77 at head dim 128, 122 instead of 107 at
+// 64, for its registers.)
 enum ScoreMode { kPlain, kCapped, kBiased };
 
 // The wide item with f16 queries, as a software pipeline over 32-key chunks:
@@ -946,6 +969,13 @@ enum ScoreMode { kPlain, kCapped, kBiased };
 // the MFMAs (in a burst ahead of them a wave stalls at each); the barrier after
 // step 2 t orders them behind the last reads of their buffers and ahead of
 // their first.  A tile's table entries are loaded a step before its loads.
+//
+// Bound by issue and clock: of a step's ~1900 cycles (two waves a SIMD, 1.7 -
+// 1.9 GHz under load) the matrix cores are busy 1024; at head dim 64 the exp2s
+// and their VALU work take as long, at 128 the LDS operands (16 rows' tile a
+// wave, each read once).  4001 tokens of 32 / 4 heads of 128: 0.81 PFLOP/s; 512
+// over 30512 keys of 64 / 8 of 64: 0.87.  A simple loop over tiles took 239
+// and 467 us for these calls, which now take 162 and 278.
 template <int HD, int MODE>
 __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S_ = WideShape<HD>;
@@ -1014,7 +1044,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
 
     // a chunk that not every row sees whole; its V rows may hold infinities or
-    // NaN that some rows do not see (see paged_body)
+    // NaN that some rows do not see (see clean_chunk)
     auto key_of = [&](int c) { return chunk_key(z.cb + c, z.n_pre, z.lo_base); };
     auto partly = [&](int kb) { return !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all)); };
     bool special = false;
@@ -1258,7 +1288,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
 }
 
 // Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more.
-enum Rows_ { kRows8, kRows16, kRows32, kRowsWide };
+enum RowLimit { kRows8, kRows16, kRows32, kRowsWide };
 
 template <int HD, bool F32, int MODE, int ROWS>
 __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedParams p) {
@@ -1292,8 +1322,9 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // slot, weights 2^(M_i - M).  HD / 4 lanes hold a row's dims, 4 each; a wave's
 // lane groups (and WPR waves) take one row's slots in turn and meet through
 // lane exchanges and LDS in a fixed order, or, where the slots are few, a
-// row each.  Bound by the partials' bytes, and for single tokens by its two
-// round trips (plan, partials) behind the attention kernel.
+// row each.  Bound by the partials' bytes (a mixed step's 48 MB: 12.7 us, 3.8
+// TB/s), and for single tokens by its two round trips (plan, partials) behind
+// the attention kernel: 3.8 - 4.8 us.
 template <int HD, bool F32, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     constexpr int LPR = HD / 4, GPW = 64 / LPR, U = 4;

@@ -23,9 +23,12 @@ constexpr int kNarrowRows = 32;
 PELICA_HD constexpr int wide_rows(int hd) { return hd == 64 ? 256 : 128; }
 
 // Costs of the work list, in the time a narrow workgroup's wave takes for a
-// chunk of 32 keys (~0.45 us): a wide workgroup's chunk (1.3 us at both head
-// dims, two workgroups a CU), the least cost of a piece, a piece's start and
-// end, and the partials that a split item's piece writes and the join reads.
+// chunk of 32 keys (~0.45 us): a wide workgroup's chunk (1.0 - 1.4 us at both
+// head dims, two workgroups a CU), the least cost of a piece, a piece's start
+// and end, and the partials that a split item's piece writes and the join
+// reads.  (Pieces cut at the limit with the rest behind, instead of equal ones,
+// fill the slots better by this model, and on the chip 3% better to 2% worse:
+// two workgroups of a CU share what one of them leaves.)
 constexpr int kWideCost = 3;
 constexpr int kMinPiece = 4;
 struct PlanCost {

@@ -8,6 +8,8 @@
 // pages_append runs as many workgroups as its rows fill; each scans all
 // requests by itself (8 bytes a request from L2), which costs less than a
 // second launch or a wait between workgroups.
+// Measured: 8 requests 3.7 us, 500 with prompts of up to 600 tokens 6.2, the
+// release of 31 of them 4.4.
 #include "attn_paged.hpp"
 #include "attn_prof.hpp"
 
@@ -291,7 +293,10 @@ constexpr int kBuckets = 128;     // of pieces' costs, four to a doubling, narro
 // The work list.  Items (requests' blocks of query rows) cost the chunks they
 // walk; an item of k pieces is cut into equal ranges of them by a limit on a
 // piece's cost.  Limits are weighed, a wave each, by the time that the step
-// would take (PlanCost).
+// would take (PlanCost).  Latency-bound, one workgroup: the lengths' round
+// trip, the scan, the limits, the pieces: 3.5 us for a step that is not split,
+// 7.6 for one long request's token, 9 - 11 for 32 requests or a prompt's 250
+// items; once a step, for all its layers.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) {
     __shared__ int item0[kPagedMaxSeq + 1];  // first item of each request
     __shared__ int q0[kPagedMaxSeq + 1], kv[kPagedMaxSeq], pre[kPagedMaxSeq];  // q_start, kv_len, prefix
