@@ -79,10 +79,11 @@ __device__ __forceinline__ int k_slot(int k, int p) {
     return k * (HD * 2) + ((p ^ k_swizzle<HD>(k)) << 4);
 }
 // ... and of a V tile, whose transposing reads take 4 rows' 16 dims a 16-lane
-// group, the groups rows 4 apart (or dims 16 apart).
+// group, 32 lanes at once: two groups rows 4 apart (narrow) or dims 16 apart
+// (wide).
 template <int HD>
 __device__ __forceinline__ constexpr int v_swizzle(int k) {
-    return HD == 64 ? ((k & 3) ^ ((k >> 2) & 1)) << 1 : (k & 7) << 1;
+    return HD == 64 ? ((k & 3) ^ ((k >> 2) & 1)) << 1 : ((k & 3) << 2) | ((k >> 1) & 2);
 }
 template <int HD>
 __device__ __forceinline__ int v_slot(int k, int p) {

@@ -1,7 +1,7 @@
 // The C entry points over a paged cache (include/pelica_attn.h): checks of
 // descriptors and arguments, sizes, launches.
+#include <algorithm>
 #include <cmath>
-#include <cstring>
 
 #include "../../include/pelica_attn.h"
 #include "attn_error.hpp"
