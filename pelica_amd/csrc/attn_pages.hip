@@ -71,7 +71,26 @@ __device__ __forceinline__ int block_scan(int x, int* part, int& total) {
     return (wave > 0 ? __builtin_amdgcn_readlane(waves, wave > 0 ? wave - 1 : 0) : 0) + sum - x;
 }
 
-// The same where a wave's sum fits 32 bits and the workgroup's may not.
+// Of three values at once, one barrier for all; part: 3 NT / 64 values.
+template <int NT>
+__device__ __forceinline__ void block_scan3(int (&x)[3], int* part, int (&total)[3]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int sum[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        sum[i] = wave_scan(x[i]);
+        if (lane == 63) part[i * (NT / 64) + wave] = sum[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const int waves = wave_scan(lane < NT / 64 ? part[i * (NT / 64) + lane] : 0);
+        total[i] = __builtin_amdgcn_readlane(waves, NT / 64 - 1);
+        x[i] = (wave > 0 ? __builtin_amdgcn_readlane(waves, wave > 0 ? wave - 1 : 0) : 0) + sum[i] - x[i];
+    }
+}
+
+// One where a wave's sum fits 32 bits and the workgroup's may not.
 template <int NT>
 __device__ __forceinline__ int64_t block_scan_long(int x, int* part, int64_t& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -301,10 +320,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     __shared__ int item0[kPagedMaxSeq + 1];  // first item of each request
     __shared__ int q0[kPagedMaxSeq + 1], kv[kPagedMaxSeq], pre[kPagedMaxSeq];  // q_start, kv_len, prefix
     __shared__ int costs[kPlanItems];
-    __shared__ int part[4][kPlanWaves], decreasing;
+    __shared__ int part[kPlanWaves], part3[3 * kPlanWaves], decreasing;
     __shared__ float est[kPlanWaves], limit[kPlanWaves];
     __shared__ int at_bucket[kBuckets], hist[kPlanWaves][64];
-    __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads];
+    __shared__ int piece0[kPlanThreads + 1], place[kPlanThreads], slot0[kPlanThreads], seq_of[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int W = wide_rows(p.hd);
     for (int s = tid; s <= p.n_seq; s += kPlanThreads) {
@@ -336,7 +355,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         // (rows of two requests: their items could be more than there is room for)
         if (q0[s + 1] < q0[s]) decreasing = 1;
     }
-    int at = block_scan<kPlanThreads>(n, part[0], n_items);
+    int at = block_scan<kPlanThreads>(n, part, n_items);
     for (int s = s0; s < s1; ++s) {
         item0[s] = at;
         at += items_of(tokens(s));
@@ -353,11 +372,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         int s, T, r0, R, cost;
         ItemKeys k;
     };
-    auto item = [&](int i) {
+    auto item_of = [&](int i, int s) {
         Item x;
-        // (requests without items share their first item with the next one:
-        // the last of them is the one that has it)
-        x.s = find_last(item0, p.n_seq, i);
+        x.s = s;
         x.T = tokens(x.s);
         x.R = x.T * p.hpk;
         const bool narrow = x.R <= kNarrowRows;
@@ -368,6 +385,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         x.cost = x.k.n_chunks * (narrow ? 1 : kWideCost);
         return x;
     };
+    // (requests without items share their first item with the next one: the
+    // last of them is the one that has it)
+    auto item = [&](int i) { return item_of(i, find_last(item0, p.n_seq, i)); };
     // this thread's first item, the only one of most steps
     const Item own = tid < n_items ? item(tid) : Item{};
     auto item_at = [&](int i) { return i < kPlanThreads ? own : item(i); };
@@ -506,26 +526,26 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
             k = item_pieces(x.cost, x.k.n_chunks, inv_limit);
         }
         // pieces of the items before, and split items' pieces and items
-        int all, slots, joins;
-        const int pc = block_scan<kPlanThreads>(k, part[1], all);
-        const int sl = base_slot + block_scan<kPlanThreads>(k > 1 ? k : 0, part[2], slots);
-        const int jn = base_join + block_scan<kPlanThreads>(k > 1 ? 1 : 0, part[3], joins);
-        piece0[tid] = pc;
+        int before[3] = {k, k > 1 ? k : 0, k > 1 ? 1 : 0}, all[3];
+        block_scan3<kPlanThreads>(before, part3, all);
+        const int sl = base_slot + before[1], jn = base_join + before[2];
+        piece0[tid] = before[0];
+        seq_of[tid] = x.s;
         place[tid] = k > 0 ? atomicAdd(&at_bucket[bucket_of(x, k)], k) : 0;
         slot0[tid] = k > 1 ? sl : -1;
         if (k > 1 && jn < p.max_joins) p.joins[jn] = PlanJoin{q0[x.s], x.R, x.r0, sl, k, {}};
         __syncthreads();
         const int n_here = min(kPlanThreads, n_items - b);
-        for (int j = tid; j < all; j += kPlanThreads) {
+        for (int j = tid; j < all[0]; j += kPlanThreads) {
             const int t = find_last(piece0, n_here, j);
-            const Item y = item(b + t);
+            const Item y = item_of(b + t, seq_of[t]);
             const int of = item_pieces(y.cost, y.k.n_chunks, inv_limit), nth = j - piece0[t];
             if (place[t] + nth < p.max_pieces)
                 p.pieces[place[t] + nth] = piece(y, of, nth, slot0[t] < 0 ? -1 : slot0[t] + nth);
         }
-        n_pieces += all;
-        base_slot += slots;
-        base_join += joins;
+        n_pieces += all[0];
+        base_slot += all[1];
+        base_join += all[2];
         __syncthreads();
     }
     if (tid == 0) *p.head = header(n_pieces, base_join);
