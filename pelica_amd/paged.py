@@ -48,7 +48,8 @@ def _start():
     global _torch, _device
     import torch
 
-    _device = torch._C._cuda_getDevice if torch.cuda.is_available() else lambda: -1
+    # (without a GPU: a device no tensor is on; those of the host are on -1)
+    _device = torch._C._cuda_getDevice if torch.cuda.is_available() else lambda: -2
     _torch = torch
     return torch
 
@@ -180,10 +181,10 @@ def pages_release(ended, cached_len, page_table, free_list, free_state, *, page_
 
 
 def _pools(k_pages, v_pages, dev):
-    """The strides of both pools of pages: (page, row, head)."""
-    st = k_pages.stride()
+    """The strides of both pools of pages and their shape: page, row, head, shape."""
+    st, shape = k_pages.stride(), k_pages.shape
     if not (k_pages.dtype is _torch.float16 and v_pages.dtype is _torch.float16 and len(st) == 4 and st[3] == 1
-            and v_pages.stride() == st and k_pages.shape == v_pages.shape and k_pages.get_device() == dev
+            and v_pages.stride() == st and shape == v_pages.shape and k_pages.get_device() == dev
             and v_pages.get_device() == dev):
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             _check(name, t, _torch.float16, 4, dense=False)
@@ -191,7 +192,15 @@ def _pools(k_pages, v_pages, dev):
                                 f"one layout for both; got {tuple(k_pages.shape)} strides {tuple(st)} and "
                                 f"{tuple(v_pages.shape)} strides {tuple(v_pages.stride())}")
     # (a dim of one has no stride of its own)
-    return st[0] if k_pages.shape[0] > 1 else 0, st[1], st[2] if k_pages.shape[2] > 1 else 0
+    return st[0] if shape[0] > 1 else 0, st[1], st[2] if shape[2] > 1 else 0, shape
+
+
+def _weights(name, t, n, dev):
+    """The address of a norm's ``n`` weights."""
+    if not (t.dtype is _torch.float32 and t.get_device() == dev and t.shape == (n,) and t.is_contiguous()):
+        _check(name, t, _torch.float32, 1)
+        raise AttnError(EINVAL, f"{name}: {n} weights")
+    return t.data_ptr()
 
 
 def _rows(name, t):
@@ -275,8 +284,8 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
         _check("q", q, dtype, 3, dense=False)
         _need(q.shape == shape, f"q: {shape} as planned, got {tuple(q.shape)}")
         raise AttnError(EINVAL, f"the plan is on device {dev}, q on {q.device}")
-    page, row, head = _pools(k_pages, v_pages, dev)
-    if k_pages.shape != plan._page_shape:
+    page, row, head, pool = _pools(k_pages, v_pages, dev)
+    if pool != plan._page_shape:
         raise AttnError(EINVAL, f"k_pages: {plan._page_shape} as planned, got {tuple(k_pages.shape)}")
     if out is None:
         with _on(stream):
@@ -346,6 +355,7 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
         _start()
     f32, dev = _torch.float32, _device()
     shape, kv_shape = q.shape, k.shape
+    at_q, at_k, at_v = q.stride(), k.stride(), v.stride()
     if not (q.dtype is f32 and k.dtype is f32 and v.dtype is f32 and len(shape) == 3 and len(kv_shape) == 3
             and v.shape == kv_shape and kv_shape[0] == shape[0] and kv_shape[2] == shape[2]
             and q.get_device() == dev and k.get_device() == dev and v.get_device() == dev):
@@ -355,15 +365,16 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
                                 f"{tuple(v.shape)}")
     T, n_head, hd = shape
     n_kv = kv_shape[1]
-    page, row, head = _pools(k_pages, v_pages, dev)
-    n_pages, page_size, heads, dims = k_pages.shape
+    page, row, head, (n_pages, page_size, heads, dims) = _pools(k_pages, v_pages, dev)
     if heads != n_kv or dims != hd:
         raise AttnError(EINVAL, f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
-    stride = _rows("q", q)
-    if _rows("k", k) != stride or _rows("v", v) != stride:
-        raise AttnError(EINVAL, "q, k and v: all contiguous, or views into rows of one stride")
-    if not (slots.dtype is _torch.int64 and slots.get_device() == dev and slots.dim() == 1 and slots.numel() == T
-            and slots.is_contiguous()):
+    stride = at_q[0] if T > 1 else 0
+    if not (at_q[2] == 1 and (at_q[1] == hd or n_head == 1) and at_k[2] == 1 and (at_k[1] == hd or n_kv == 1)
+            and at_v[2] == 1 and (at_v[1] == hd or n_kv == 1) and (T == 1 or at_k[0] == at_v[0] == stride)):
+        stride = _rows("q", q)
+        if _rows("k", k) != stride or _rows("v", v) != stride:
+            raise AttnError(EINVAL, "q, k and v: all contiguous, or views into rows of one stride")
+    if not (slots.dtype is _torch.int64 and slots.get_device() == dev and slots.shape == (T,) and slots.is_contiguous()):
         _check("slots", slots, _torch.int64, 1)
         raise AttnError(EINVAL, f"slots: one for each of the {T} rows")
     if out is None:
@@ -374,21 +385,24 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
         _need(out.dtype in (_torch.float16, f32), f"out: f16 or f32, got {out.dtype}")
         _check("out", out, out.dtype, 3, dense=False)
         raise AttnError(EINVAL, f"out: {tuple(shape)}, got {tuple(out.shape)}")
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None and not (t.dtype is f32 and t.get_device() == dev and t.numel() == hd and t.is_contiguous()):
-            _check(name, t, f32, 1)
-            raise AttnError(EINVAL, f"{name}: {hd} weights")
+    wq, wk = q_norm, k_norm
+    if wq is not None:
+        wq = _weights("q_norm", wq, hd, dev)
+    if wk is not None:
+        wk = _weights("k_norm", wk, hd, dev)
     rp = None
     if table is not None:
-        rot = rot or 2 * table.shape[1]
-        if not (table.dtype is f32 and table.get_device() == dev and table.dim() == 3 and 2 * table.shape[1] == rot
-                and table.shape[2] == 2 and table.is_contiguous()):
+        size = table.shape
+        if not (table.dtype is f32 and table.get_device() == dev and len(size) == 3 and size[2] == 2
+                and (rot == 0 or rot == 2 * size[1]) and table.is_contiguous()):
             _check("table", table, f32, 3)
-            raise AttnError(EINVAL, f"table: [rows, {rot // 2}, 2], got {tuple(table.shape)}")
+            raise AttnError(EINVAL, f"table: [rows, {rot // 2 or 'rot / 2'}, 2], got {tuple(table.shape)}")
+        rot = 2 * size[1]
         _need(positions is not None, "positions are needed with a table")
-        n_axes = positions.shape[0] if positions.dim() == 2 else 1
-        if not (positions.dtype is _torch.int32 and positions.get_device() == dev and positions.numel() == n_axes * T
-                and positions.shape[-1] == T and positions.is_contiguous()):
+        at = positions.shape
+        n_axes = at[0] if len(at) == 2 else 1
+        if not (positions.dtype is _torch.int32 and positions.get_device() == dev and 1 <= len(at) <= 2 and at[-1] == T
+                and positions.is_contiguous()):
             _check("positions", positions, _torch.int32)
             raise AttnError(EINVAL, f"positions: [{T}] or [n_axes, {T}], got {tuple(positions.shape)}")
         axes = None
@@ -399,15 +413,14 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
                 raise AttnError(EINVAL, f"pair_axis: an axis below {n_axes} for each pair: {e}") from None
             _need(len(axes) == rot // 2, f"pair_axis: an axis for each of the {rot // 2} pairs")
         _need(n_axes == 1 or axes is not None, "pair_axis is needed with more than one axis")
-        rp = ctypes.byref(PagedRope(rot, 1 if neox else 0, table_split, table.shape[0], table.data_ptr(), n_axes, axes,
+        rp = ctypes.byref(PagedRope(rot, 1 if neox else 0, table_split, size[0], table.data_ptr(), n_axes, axes,
                                     positions.data_ptr(), T))
     # (in the order of PagedDesc._fields_)
     d = PagedDesc(n_head, n_kv, hd, 0, T, 0, page_size, n_pages, 0, 0, None, None, None, None, None, page, row, head)
     lib = attn._lib or attn.load_library()
     rc = lib.pelica_attn_paged_qkv(
         ctypes.byref(d), rp, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride,
-        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-        slots.data_ptr(), out.data_ptr(), half, _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(),
+        wq, wk, eps, slots.data_ptr(), out.data_ptr(), half, _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(),
         attn._stream_ptr(stream))
     if rc:
         attn._check(rc)

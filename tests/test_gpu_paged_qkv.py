@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import oracle as orc
-from pelica_amd import paged
+from pelica_amd import attn, paged
 from tests import paged_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -200,3 +200,35 @@ def test_steps_of_an_engine(half):
                                            window=32 if layer == 0 else 0, sinks=sinks.cpu())
             ref.check(out, want, f32, f16 if half else None)
         cached = total
+
+
+def test_refusals_of_the_binding():
+    """What the checks of q, k, v, slots, norms, tables and positions refuse,
+    before anything is launched."""
+    T, H, hd = 3, 2, 64
+    dev = dict(device="cuda")
+    x = torch.zeros(T, 4 * H * hd, **dev)
+    q, k, v = (x[:, i * H * hd:(i + 1) * H * hd].view(T, H, hd) for i in range(3))
+    pages = torch.zeros(4, 16, H, hd, dtype=torch.float16, **dev)
+    slots = torch.arange(T, **dev)
+    table = torch.zeros(8, hd // 2, 2, **dev)
+    pos = torch.zeros(T, dtype=torch.int32, **dev)
+    good = dict(q=q, k=k, v=v, k_pages=pages, v_pages=pages, slots=slots, positions=pos, table=table)
+    paged.paged_qkv(**good)
+    bad = [
+        dict(q=q.half()), dict(k=k.cpu()), dict(v=v[:2]), dict(v=v[:, :1]), dict(q=q[..., :32]),
+        dict(q=q.contiguous()), dict(k=k.contiguous()), dict(v=v.contiguous()),
+        dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), dict(q=torch.zeros(T, H, 2 * hd, **dev)[..., ::2]),
+        dict(q=q[0]), dict(k_pages=pages.float()), dict(v_pages=pages[:2]), dict(k_pages=pages[:, :, :1]),
+        dict(k_pages=pages.transpose(1, 2)), dict(slots=slots.int()), dict(slots=slots[:2]), dict(slots=slots.cpu()),
+        dict(slots=torch.zeros(T, 1, dtype=torch.int64, **dev)), dict(q_norm=torch.ones(hd + 1, **dev)),
+        dict(k_norm=torch.ones(hd, 1, **dev)), dict(q_norm=torch.ones(hd)), dict(table=table.half()),
+        dict(table=table[:, :4, :1]), dict(table=table, rot=32), dict(table=table[0]), dict(positions=None),
+        dict(positions=pos.long()), dict(positions=pos[:2]), dict(positions=torch.zeros(2, T, dtype=torch.int32, **dev)),
+        dict(positions=torch.zeros(1, 1, T, dtype=torch.int32, **dev)), dict(pair_axis=[0] * 5), dict(pair_axis=[1] * (hd // 2)),
+        dict(out=torch.zeros(T, H, 32, **dev)), dict(out=torch.zeros(T, H, hd, dtype=torch.bfloat16, **dev)),
+        dict(out=torch.zeros(T, H, hd)),
+    ]
+    for kw in bad:
+        with pytest.raises(attn.AttnError):
+            paged.paged_qkv(**{**good, **kw})

@@ -179,6 +179,13 @@ def test_the_binding_refuses_cpu_tensors_and_wrong_types():
         assert e.value.code == attn.EINVAL
 
 
+def test_rows_of_the_host_are_refused():
+    x, pages = torch.zeros(2, 1, 64), torch.zeros(4, 16, 1, 64, dtype=torch.float16)
+    with pytest.raises(attn.AttnError) as e:
+        paged.paged_qkv(x, x, x, pages, pages, torch.zeros(2, dtype=torch.int64), out=x)
+    assert e.value.code == attn.EINVAL and "device" in str(e.value)
+
+
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     so = tmp_path_factory.mktemp("plan") / "plan.so"
