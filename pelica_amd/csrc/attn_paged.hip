@@ -976,7 +976,7 @@ enum ScoreMode { kPlain, kCapped, kBiased };
 // and their VALU work take as long, at 128 the LDS operands (16 rows' tile a
 // wave, each read once).  4001 tokens of 32 / 4 heads of 128: 0.81 PFLOP/s; 512
 // over 30512 keys of 64 / 8 of 64: 0.87.  A simple loop over tiles took 239
-// and 467 us for these calls, which now take 162 and 278.
+// and 467 us for these calls, which now take 165 and 284.
 template <int HD, int MODE>
 __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S_ = WideShape<HD>;
