@@ -389,7 +389,9 @@ int pelica_attn_paged_plan(const PelicaPagedDesc* desc, void* plan, size_t plan_
 
 /* Attention of each request's new tokens over its pages: f16 queries and
  * output, or f32 (_f32), whose products keep f32's precision (queries and
- * probabilities as f16 hi + lo parts).  Softmax and sums in f32.  sinks:
+ * probabilities as f16 hi + lo parts: a query's value is kept to 2^-22 of
+ * itself or 2^-25, the larger, and one past 65504 gives NaN).  Softmax and
+ * sums in f32.  sinks:
  * [n_head] natural-log logits or NULL.  Rows of skipped requests and behind
  * the last one are left as they were.  Workspace (partials of key ranges;
  * pelica_attn_paged_workspace_bytes, 0 if none is needed): contents need no

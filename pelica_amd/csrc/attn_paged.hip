@@ -381,6 +381,11 @@ __device__ __forceinline__ void finish_scores(const PagedParams& p, V& s, std::i
     }
 }
 
+// The running max is kept 14 below the largest score: p up to 2^14 in f16, or as
+// hi + lo parts, whose last step is 2^-24 of 2^14 then.  (With p up to 1, of
+// 20000 keys 2^-20 of one other each can be 2^-25 off, and their sum 2^-11.)
+constexpr float kAbove = 14.f;
+
 __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
     const int v = __float_as_uint(x);
     return __uint_as_float(__builtin_amdgcn_update_dpp(v, v, 0x128, 0xF, 0xF, false));
@@ -583,7 +588,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = fmaxf(s[nt][i], s[nt][4 + i]);
-            const float mn = fmaxf(m[nt], group4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
+            const float mn = fmaxf(m[nt], group4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) - kAbove);
             if (__builtin_amdgcn_ballot_w64(mn > m[nt])) {
                 const float cf = mn > m[nt] ? fast_exp2(m[nt] - mn) : 1.f;  // (0 while m was -inf)
                 l[nt] *= cf;
@@ -676,6 +681,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             ml[w] = sml(w)[nt * 64 + lane];
             M = fmaxf(M, ml[w].x);
         }
+        M += kAbove;  // (p up to 1 from here on)
         const float ms = M == -INFINITY ? 0.f : M;
         float L = 0.f, wt[kNW];
 #pragma unroll
@@ -878,7 +884,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
             float x = s[rt][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) x = fmaxf(x, s[rt][i]);
-            const float mn = fmaxf(m[rt], half_max(x));
+            const float mn = fmaxf(m[rt], half_max(x) - kAbove);
             if (__builtin_amdgcn_ballot_w64(mn > m[rt])) {
                 const float cf = mn > m[rt] ? fast_exp2(m[rt] - mn) : 1.f;  // (0 while m was -inf)
                 l[rt] *= cf;
@@ -945,6 +951,14 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
 #pragma unroll 1
         for (int c = z.cb; c < z.ce; ++c)
             if (partly_seen(c)) add_special<HD, RT>(z, rows, chunk_key(c, z.n_pre, z.lo_base), h2, lor, span, o);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float down = fast_exp2(-kAbove);  // (p up to 1 from here on)
+        m[rt] += kAbove;
+        l[rt] *= down;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt][rt] *= down;
+    }
     store_wide<HD, true>(p, z, kvh, wave, lane, any_bad, m, l, o, lds);
 }
 

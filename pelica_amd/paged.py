@@ -271,7 +271,7 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
                     scale: Optional[float] = None, out=None, workspace=None, stream=None):
     """Attention of every request's new tokens over its pages.  q: f16
     (pelica_attn_paged) or f32 (pelica_attn_paged_f32, products to f32's
-    precision) [n_tokens, n_head, hd], contiguous or token rows of a wider
+    precision; values up to 65504) [n_tokens, n_head, hd], contiguous or token rows of a wider
     buffer; ``sinks`` f32 [n_head]; ``alibi`` f32 [n_head] slopes of the
     distance bias; ``softcap`` c: scores c tanh(s / c).  Returns q's type;
     rows of requests without tokens or with lengths that do not fit, and rows

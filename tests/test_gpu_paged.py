@@ -369,3 +369,22 @@ def test_two_steps_at_once():
     torch.cuda.synchronize()
     for c, _, _, _, out, _ in runs:
         c.check(out)
+
+
+@pytest.mark.parametrize("new", [[1], [5], [200]], ids=["token", "draft", "chunk"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_equal_keys_far_below_one(new, hd):
+    """Key 0 scores s, 20000 others 0, all values 1: the result is 1 to the
+    roundings of sums, however the small weights are rounded on their way."""
+    n, s = 20000, 13.3  # e^-13.3 = 1.75 x 2^-20
+    c = Case([n], new, n_head=8, n_kv=1, hd=hd, page=64, seed=34)
+    c.k[:], c.v[:] = 0, 1
+    first = c.table[0][0]
+    c.k[c.live[first], 0, 0, 0] = 4
+    c.q[:] = 0
+    c.q[..., 0] = s / 4 * math.sqrt(hd)
+    out = c.device().run().double().cpu()
+    # one rounding for each 32-key chunk a wave walks alone (a quarter of them)
+    # and a few for the trees, in the sum and in the product
+    tol = 2 * (n // 128 + 16) * ref.U32 if new[0] * 8 <= 32 else 2 * (n // 32 + 16) * ref.U32
+    assert (out - 1).abs().max() <= tol
