@@ -385,6 +385,9 @@ __device__ __forceinline__ void finish_scores(const PagedParams& p, V& s, std::i
 // hi + lo parts, whose last step is 2^-24 of 2^14 then.  (With p up to 1, of
 // 20000 keys 2^-20 of one other each can be 2^-25 off, and their sum 2^-11.)
 constexpr float kAbove = 14.f;
+// ... and 8 below a wide item's of f16 queries, whose max moves only when a
+// chunk's weights sum to more than 2^14
+constexpr float kAboveWide = 8.f;
 
 __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
     const int v = __float_as_uint(x);
@@ -975,7 +978,8 @@ enum ScoreMode { kPlain, kCapped, kBiased };
 // QK^T of chunk c + 1 and PV of chunk c - 1, one MFMA at a time between the
 // softmax's instructions.  P = 2^(x - m) with a max m that moves only when a
 // chunk's row sum passes 2^14 (below it nothing overflowed f16, and keys far
-// below m are negligible beside the one m was taken from), or is not set yet:
+// enough below m to lose bits are negligible beside the one m was taken from,
+// 2^8 in weight), or is not set yet:
 // then the wave takes the chunk's max, rescales O and the sum, and
 // recomputes P.
 //
@@ -1213,7 +1217,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
                 float x = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x = fmaxf(x, s_cur[rt][i]);
-                const float mn = fmaxf(m[rt], half_max(x) + ms[rt]);
+                const float mn = fmaxf(m[rt], half_max(x) + ms[rt] - kAboveWide);
                 if (mn > m[rt]) {
                     const float cf = fast_exp2(m[rt] - mn);  // 0 while m was -inf
                     l[rt] *= cf;

@@ -388,3 +388,22 @@ def test_many_equal_keys_far_below_one(new, hd):
     # and a few for the trees, in the sum and in the product
     tol = 2 * (n // 128 + 16) * ref.U32 if new[0] * 8 <= 32 else 2 * (n // 32 + 16) * ref.U32
     assert (out - 1).abs().max() <= tol
+
+
+@pytest.mark.parametrize("new", [[1], [200]], ids=["token", "chunk"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_equal_f16_weights_far_below_one(new, hd):
+    """f16 queries, the same keys, of which key 0 has the value 0: the others'
+    share of the weights, 29.6 x 2^-24 each beside 1, is off by their one
+    rounding (all alike) and the output's."""
+    n, s = 20000, 13.25
+    c = Case([n], new, n_head=8, n_kv=1, hd=hd, page=64, half=True, seed=35)
+    c.k[:], c.v[:] = 0, 1
+    at = c.live[c.table[0][0]]
+    c.k[at, 0, 0, 0], c.v[at, 0] = 4, 0
+    c.q[:] = 0
+    c.q[..., 0] = s / 4 * math.sqrt(hd)
+    want = c.reference()[0]
+    out = c.device().run().double().cpu()
+    tol = want * (2 * ref.U16 + ref.U16 ** 2 + 2 * (n // 32 + 16) * ref.U32)
+    assert ((out - want).abs() <= tol).all()
