@@ -142,7 +142,11 @@ __device__ __forceinline__ half8 v_operand(const char* vt, int key, int dt, int 
 // taken out of the tile (clean_chunk: whether any were there) and added after
 // the last chunk to the rows that see them (add_special).  The waves of a wide
 // workgroup may clean a chunk at once: each has written zeros over what it
-// found before it reads the chunk.
+// found before it reads the chunk.  Such rows are the keys of the item's later
+// tokens, and keys between a prefix and a window that share a run with both.
+__device__ __forceinline__ bool may_hide(const PlanPiece& z, int hi_all, int pos_last) {
+    return pos_last > hi_all || gap_in_run(z.lo, z.pe);
+}
 __device__ __forceinline__ bool is_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; }
 
 // Whether a row sees a key: its own span of keys from lo on, or the prefix
@@ -516,6 +520,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     // every row sees the keys [lo_all, hi_all] and those below z.pe
     const int hi_all = z.pos0, pos_last = z.len - 1;
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
+    const bool hide = may_hide(z, hi_all, pos_last);
 
     float m[NT], l[NT];
     float4v o[DT][NT];
@@ -619,7 +624,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         if (left >= NB) wait_loads<AHEAD>();
         else if (left == NB - 1) wait_loads<2 * WI * (NB - 1)>();
         else wait_loads<0>();
-        if (!all && pos_last > hi_all) special |= clean_chunk<HD>(vt, lane);
+        if (!all && hide) special |= clean_chunk<HD>(vt, lane);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             // 4 rows' 16 dims a 16-lane group, transposed: keys 4 g .. and 16 + 4 g ..
@@ -836,6 +841,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
     const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
+    const bool hide = may_hide(z, hi_all, pos_last);
 
     float m[RT], l[RT];
     float16v o[DT][RT];
@@ -925,7 +931,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     };
     auto partly_seen = [&](int c) {
         const int kb = chunk_key(c, z.n_pre, z.lo_base);
-        return pos_last > hi_all && !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all));
+        return hide && !(kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all));
     };
     bool special = false;
 
@@ -1061,6 +1067,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
     const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
+    const bool hide = may_hide(z, hi_all, pos_last);
 
     // a chunk that not every row sees whole; its V rows may hold infinities or
     // NaN that some rows do not see (see clean_chunk)
@@ -1108,7 +1115,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
             if (MODE == kBiased && p.cap > 0.f) cap_scores<16, true>(p, s_cur[rt]);
         }
         if ((unsigned)(c - 1 - w0) >= w_n) {  // this chunk or the one before
-            if (c > 0 && pos_last > hi_all && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
+            if (c > 0 && hide && partly(key_of(c - 1))) special |= clean_chunk<HD>(v_chunk(c - 1), lane);
             if (partly(kb)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -1289,7 +1296,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     if (rem >= 2) step(P1{}, c + 1, s_b, s_a, p_a, p_b);
     if (rem >= 3) step(P2{}, c + 2, s_a, s_b, p_b, p_a);
     wait_loads<0>();  // (what was requested past the last tile)
-    if (pos_last > hi_all && partly(key_of(n - 1))) special |= clean_chunk<HD>(v_chunk(n - 1), lane);
+    if (hide && partly(key_of(n - 1))) special |= clean_chunk<HD>(v_chunk(n - 1), lane);
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll

@@ -80,9 +80,6 @@ PELICA_HD ItemKeys item_keys(int pos_first, int pos_last, int len, int window, i
 // first key of chunk c
 PELICA_HD int chunk_key(int c, int n_pre, int lo_base) { return c < n_pre ? 32 * c : lo_base + 32 * (c - n_pre); }
 
-// Of n consecutive keys from kg (all in one page), the rows [first, first +
-// count) that some row of the item may see: a load touches no others (they may
-// lie in a page that was given away, or hold anything).
 // x between 0 and n, on the scalar unit: as a minimum of a maximum the compiler
 // makes it a vector instruction, and every address that follows with it
 PELICA_HD int clamp_to(int x, int n) {
@@ -94,6 +91,10 @@ PELICA_HD int clamp_to(int x, int n) {
     return imin(imax(x, 0), n);
 #endif
 }
+// Of n consecutive keys from kg (all in one page), the rows [first, first +
+// count) that a load touches: those that some row of the item sees, and, where
+// the prefix ends and the window begins within them, what lies between
+// (gap_in_run).  No others: they may lie in a page that was given away.
 PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, int& count) {
     const int a = clamp_to(pe - kg, n);  // of the prefix: [0, a)
     const int b0 = clamp_to(lo - kg, n), b1 = clamp_to(kend - kg, n);
@@ -101,6 +102,9 @@ PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, i
     const int end = b1 > b0 ? imax(a, b1) : a;
     count = imax(end - first, 0);
 }
+// Whether a run of 8 rows holds keys [pe, lo) between a prefix and a window,
+// which no row of the item sees, beside keys of both
+PELICA_HD bool gap_in_run(int lo, int pe) { return pe > 0 && pe < lo && (pe - 1) >> 3 == lo >> 3; }
 
 // Pieces of an item of `cost` where a piece's may be 1 / inv_limit
 PELICA_HD int item_pieces(int cost, int n_chunks, float inv_limit) {

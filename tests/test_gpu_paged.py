@@ -407,3 +407,26 @@ def test_many_equal_f16_weights_far_below_one(new, hd):
     out = c.device().run().double().cpu()
     tol = want * (2 * ref.U16 + ref.U16 ** 2 + 2 * (n // 32 + 16) * ref.U32)
     assert ((out - want).abs() <= tol).all()
+
+
+# one token of each request, (lens, window, prefix): the prefix ends a few keys
+# before the window, within one run of 8 rows; the keys between hold NaN
+GAPS = {
+    "first_chunk": ([130], 100, [26]),
+    "only_chunk": ([31], 3, [26]),
+    "last_chunk": ([300, 275, 64], 24, [275, 250, 33]),
+    "one_key": ([300], 24, [275]),
+}
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_head,n_kv", [(8, 2), (20, 1), (40, 1)], ids=["rows8", "rows32", "wide"])
+def test_keys_between_a_prefix_and_a_window(n_head, n_kv, hd, half, gap):
+    lens, window, prefix = GAPS[gap]
+    kw = dict(n_head=n_head, n_kv=n_kv, hd=hd, half=half, window=window, prefix=prefix, page=8)
+    Case(lens, [1] * len(lens), seed=45, **kw).check()
+    Case(lens, [1] * len(lens), seed=46, cap=5.0, sinks=True, **kw).check()
+    Case(lens, [1] * len(lens), seed=47, slopes=True, **kw).check()
+    Case(lens, [min(n, 3) for n in lens], seed=48, **kw).check()

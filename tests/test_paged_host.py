@@ -236,6 +236,30 @@ def test_an_items_chunks_hold_every_key_its_rows_see_once(rules):
         assert len(got) == len(set(got)) and set(got) == want
 
 
+def test_rows_that_one_token_loads_and_does_not_see_are_told(rules):
+    """An item whose rows share one position: its loads touch a key that it does
+    not see where, and only where, gap_in_run says so."""
+    r = random.Random(4)
+    out6, out2 = (ctypes.c_int * 6)(), (ctypes.c_int * 2)()
+    told = 0
+    for _ in range(6000):
+        length = r.randint(1, 200)
+        window = r.choice((0, 1, 3, 24, 100))
+        begin = max(0, length - window)
+        prefix = max(0, r.choice((0, 5, begin - 1, begin - 2, begin - 7, begin - 8, begin, begin + 3)))
+        rules.item_keys_of(length - 1, length - 1, length, window, prefix, out6)
+        n_pre, lo_base, n_chunks, lo, kend, pe = out6
+        unseen = set()
+        for c in range(n_chunks):
+            key = rules.chunk_key_of(c, n_pre, lo_base)
+            for kg in range(key, key + 32, 8):  # runs of 8, as the kernels address them
+                rules.group_rows_of(kg, 8, lo, kend, pe, out2)
+                unseen |= set(range(kg + out2[0], kg + sum(out2))) - _seen(length - 1, window, pe)
+        assert bool(unseen) == bool(rules.gap_in_run_of(lo, pe)), (length, window, prefix, unseen)
+        told += bool(unseen)
+    assert 300 < told < 3000
+
+
 def test_pieces_of_an_item(rules):
     rules.item_pieces_of.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_float]
     r = random.Random(3)
