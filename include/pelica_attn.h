@@ -324,8 +324,10 @@ typedef struct PelicaPageDesc {
  * seq_kv_len is 0 (attention skips it) and its rows' slots are -1 (the qkv
  * step skips them).  When pages run out, every later request that needs one
  * gets PELICA_ATTN_PAGES_NONE.  A page id outside the pool, from the table
- * or the list, gives slot -1.  free_out must not overlap free_in: workgroups
- * read the one while another writes the other. */
+ * or the list, gives slot -1.  No array that is written (page_table among
+ * them) may overlap another one: workgroups read all the inputs while others
+ * write.  So cached_len is not this call's seq_kv_len; a caller that passes on
+ * lengths takes two sets of outputs in turn. */
 int pelica_attn_pages_append(const PelicaPageDesc* desc, const int32_t* cached_len, const int32_t* new_len,
                              int32_t* page_table, const int32_t* free_list, const int64_t* free_in,
                              int64_t* free_out, int32_t* q_start, int32_t* seq_kv_len, int64_t* slots,
@@ -336,7 +338,7 @@ int pelica_attn_pages_append(const PelicaPageDesc* desc, const int32_t* cached_l
  * page_size)), which must be pages of the pool.  The table is not changed
  * (set the request's cached length to 0).  When the list would hold more
  * than n_pages nothing is given back.  n_tokens of the descriptor is not
- * used.  free_out must not overlap free_in. */
+ * used.  free_list and free_out may overlap no other array. */
 int pelica_attn_pages_release(const PelicaPageDesc* desc, const int32_t* ended, const int32_t* cached_len,
                               const int32_t* page_table, int32_t* free_list, const int64_t* free_in,
                               int64_t* free_out, void* stream);

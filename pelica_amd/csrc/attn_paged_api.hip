@@ -42,6 +42,30 @@ int check_pages(const PelicaPageDesc* d) {
     return PELICA_ATTN_OK;
 }
 
+// The arrays of a call over pages.  Every workgroup reads all of the inputs
+// while others write, so an output shares no byte with another array.
+struct Array {
+    const char* name;
+    const void* at;
+    int64_t n;
+    int size;
+    bool out;
+};
+template <int N>
+int check_arrays(const char* call, const Array (&a)[N]) {
+    for (const Array& x : a)
+        if (!x.at) return fail(PELICA_ATTN_EINVAL, "every array of %s must be non-NULL", call);
+    for (const Array& x : a)
+        if (misaligned(x.at, x.size)) return fail(PELICA_ATTN_EINVAL, "arrays of %s must be aligned to their values", call);
+    for (const Array& x : a)
+        for (const Array& y : a) {
+            const uintptr_t p = reinterpret_cast<uintptr_t>(x.at), q = reinterpret_cast<uintptr_t>(y.at);
+            if (x.out && &x != &y && p < q + (uint64_t)y.n * y.size && q < p + (uint64_t)x.n * x.size)
+                return fail(PELICA_ATTN_EINVAL, "%s: %s overlaps %s", call, x.name, y.name);
+        }
+    return PELICA_ATTN_OK;
+}
+
 int64_t row_stride(const PelicaPagedDesc* d) { return d->row_stride ? d->row_stride : (int64_t)d->n_kv * d->hd; }
 int64_t head_stride(const PelicaPagedDesc* d) { return d->head_stride ? d->head_stride : d->hd; }
 int64_t page_stride(const PelicaPagedDesc* d) { return d->page_stride ? d->page_stride : (int64_t)d->page_size * row_stride(d); }
@@ -209,14 +233,16 @@ int pelica_attn_pages_append(const PelicaPageDesc* d, const int32_t* cached_len,
     int rc = check_pages(d);
     if (rc) return rc;
     if (d->n_tokens <= 0 || d->n_tokens > kMaxTokens) return fail(PELICA_ATTN_EINVAL, "n_tokens %d (1 .. %d)", d->n_tokens, kMaxTokens);
-    if (!cached_len || !new_len || !page_table || !free_list || !free_in || !free_out || !q_start || !seq_kv_len ||
-        !slots || !positions || !token_seq || !status)
-        return fail(PELICA_ATTN_EINVAL, "every array of pages_append must be non-NULL");
-    if (free_in < free_out + 2 && free_out < free_in + 2) return fail(PELICA_ATTN_EINVAL, "free_out overlaps free_in");
-    if (misaligned(cached_len, 4) || misaligned(new_len, 4) || misaligned(page_table, 4) || misaligned(free_list, 4) ||
-        misaligned(free_in, 8) || misaligned(free_out, 8) || misaligned(q_start, 4) || misaligned(seq_kv_len, 4) ||
-        misaligned(slots, 8) || misaligned(positions, 4) || misaligned(token_seq, 4) || misaligned(status, 4))
-        return fail(PELICA_ATTN_EINVAL, "arrays of pages_append must be aligned to their values");
+    const int64_t cells = (int64_t)d->n_seq * d->max_pages;
+    const Array arrays[] = {
+        {"cached_len", cached_len, d->n_seq, 4, false}, {"new_len", new_len, d->n_seq, 4, false},
+        {"page_table", page_table, cells, 4, true},     {"free_list", free_list, d->n_pages, 4, false},
+        {"free_in", free_in, 2, 8, false},              {"free_out", free_out, 2, 8, true},
+        {"q_start", q_start, d->n_seq + 1, 4, true},    {"seq_kv_len", seq_kv_len, d->n_seq, 4, true},
+        {"slots", slots, d->n_tokens, 8, true},         {"positions", positions, d->n_tokens, 4, true},
+        {"token_seq", token_seq, d->n_tokens, 4, true}, {"status", status, d->n_seq, 4, true}};
+    rc = check_arrays("pages_append", arrays);
+    if (rc) return rc;
     pelica::PagesParams p{};
     p.cached = cached_len;
     p.fresh = new_len;
@@ -246,12 +272,12 @@ int pelica_attn_pages_release(const PelicaPageDesc* d, const int32_t* ended, con
     pelica::clear_error();
     int rc = check_pages(d);
     if (rc) return rc;
-    if (!ended || !cached_len || !page_table || !free_list || !free_in || !free_out)
-        return fail(PELICA_ATTN_EINVAL, "every array of pages_release must be non-NULL");
-    if (free_in < free_out + 2 && free_out < free_in + 2) return fail(PELICA_ATTN_EINVAL, "free_out overlaps free_in");
-    if (misaligned(ended, 4) || misaligned(cached_len, 4) || misaligned(page_table, 4) || misaligned(free_list, 4) ||
-        misaligned(free_in, 8) || misaligned(free_out, 8))
-        return fail(PELICA_ATTN_EINVAL, "arrays of pages_release must be aligned to their values");
+    const int64_t cells = (int64_t)d->n_seq * d->max_pages;
+    const Array arrays[] = {{"ended", ended, d->n_seq, 4, false},   {"cached_len", cached_len, d->n_seq, 4, false},
+                            {"page_table", page_table, cells, 4, false}, {"free_list", free_list, d->n_pages, 4, true},
+                            {"free_in", free_in, 2, 8, false},      {"free_out", free_out, 2, 8, true}};
+    rc = check_arrays("pages_release", arrays);
+    if (rc) return rc;
     pelica::PagesParams p{};
     p.ended = ended;
     p.cached = cached_len;

@@ -79,7 +79,9 @@ class PageStep:
     """What ``pages_append`` writes: ``q_start`` [n_seq + 1], ``seq_kv_len``
     and ``status`` [n_seq] int32, ``slots`` [n_tokens] int64, ``positions`` and
     ``token_seq`` [n_tokens] int32, ``free_state`` [2] int64.  Keep it over the
-    steps (its addresses stay, for a captured step)."""
+    steps (its addresses stay, for a captured step).  None of them may be an
+    input of the call that writes them: to pass ``seq_kv_len`` on as the next
+    call's ``cached_len``, take two PageSteps in turn."""
 
     def __init__(self, n_seq: int, n_tokens: int, device="cuda"):
         import torch
@@ -129,7 +131,7 @@ def pages_append(cached_len, new_len, page_table, free_list, free_state, *, page
     ``page_table`` [n_seq, max_pages] (appended to), int32 ``free_list``
     [n_pages] and its queue ends ``free_state`` int64 [2].  Returns ``step``, or
     a new PageStep of ``n_tokens`` rows; its ``free_state`` is the next call's
-    (of another PageStep: a call's may not be its own input)."""
+    (of another PageStep: a call's outputs may not be its inputs)."""
     if _torch is None:
         _start()
     _need(page_table.dim() == 2, "page_table: [n_seq, max_pages]")

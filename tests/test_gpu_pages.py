@@ -1,9 +1,11 @@
 """Page bookkeeping on the GPU against a plain Python walk of the requests: whole
 numbers, equal or wrong."""
+import ctypes
+
 import pytest
 import torch
 
-from pelica_amd import paged
+from pelica_amd import attn, paged
 from tests import paged_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -180,3 +182,54 @@ def test_append_in_a_graph():
         torch.cuda.synchronize()
         assert tab.tolist() == want["table"] and step.slots.tolist() == want["slots"]
         assert step.free_state.tolist() == want["free_state"] and step.q_start.tolist() == want["q_start"]
+
+
+def test_lengths_of_the_last_step_are_the_next_ones():
+    """Two PageSteps in turn, the one's seq_kv_len the other's cached_len, in
+    steps of many workgroups; the same PageStep is refused."""
+    n_seq, page, n_pages, most = 300, 8, 2500, 20
+    g = torch.Generator().manual_seed(10)
+    lens = torch.randint(0, 40, (n_seq,), generator=g).tolist()
+    table, queue, state = _pool(lens, page, n_pages, most, 11)
+    tab, lst, fs, cached = i32(table), i32(queue), i64(state), i32(lens)
+    steps = [paged.PageStep(n_seq, 2000), paged.PageStep(n_seq, 2000)]
+    for i in range(6):
+        new = torch.randint(0, 7, (n_seq,), generator=g).tolist()
+        want = ref.pages_append(lens, new, table, queue, state, page, 2000, most)
+        step = paged.pages_append(cached, i32(new), tab, lst, fs, page_size=page, step=steps[i % 2])
+        torch.cuda.synchronize()
+        for name in ("q_start", "seq_kv_len", "status", "slots", "positions", "token_seq", "free_state"):
+            assert getattr(step, name).tolist() == want[name], (i, name)
+        assert tab.tolist() == want["table"]
+        cached, fs, table, state, lens = step.seq_kv_len, step.free_state, want["table"], want["free_state"], want["seq_kv_len"]
+        with pytest.raises(attn.AttnError, match="overlaps cached_len"):
+            paged.pages_append(cached, i32(new), tab, lst, steps[(i + 1) % 2].free_state, page_size=page, step=step)
+
+
+def test_arrays_one_behind_the_other():
+    # no gap between them, and none overlaps
+    cached, new, page, n_tokens = [5, 30, 0, 7], [1, 2, 20, 700], 16, 1000
+    table, queue, state = _pool(cached, page, 90, 50, 12)
+    want = ref.pages_append(cached, new, table, queue, state, page, n_tokens, 50)
+    parts = {"free_in": i64(state), "free_out": i64([0, 0]), "slots": i64([0] * n_tokens), "cached": i32(cached),
+             "new": i32(new), "table": i32(table), "list": i32(queue), "q_start": i32([0] * 5), "len": i32([0] * 4),
+             "positions": i32([0] * n_tokens), "token_seq": i32([0] * n_tokens), "status": i32([0] * 4)}
+    buf = torch.cat([t.reshape(-1).view(torch.int32) for t in parts.values()])
+    at, views = 0, {}
+    for name, t in parts.items():
+        n = t.numel() * t.element_size() // 4
+        views[name] = buf[at:at + n].view(t.dtype)
+        at += n
+    order = ("cached", "new", "table", "list", "free_in", "free_out", "q_start", "len", "slots", "positions", "token_seq",
+             "status")
+    desc = attn.PageDesc(4, n_tokens, page, 90, 50)
+    rc = attn.load_library().pelica_attn_pages_append(ctypes.byref(desc), *[views[n].data_ptr() for n in order],
+                                                      attn._stream_ptr(None))
+    torch.cuda.synchronize()
+    assert rc == 0
+    for name, key in (("q_start", "q_start"), ("len", "seq_kv_len"), ("slots", "slots"), ("positions", "positions"),
+                      ("token_seq", "token_seq"), ("status", "status"), ("free_out", "free_state")):
+        assert views[name].tolist() == want[key], name
+    assert views["table"].view(4, 50).tolist() == want["table"]
+    for name in ("cached", "new", "list", "free_in"):
+        assert torch.equal(views[name], parts[name].view(-1)), name

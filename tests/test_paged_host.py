@@ -137,6 +137,42 @@ def test_pages_arguments():
         _error(lib.pelica_attn_pages_append(ctypes.byref(d), *args), attn.EINVAL, "n_tokens")
 
 
+def _apart(counts):
+    """An address for each array of so many values, one behind the other."""
+    at, out = 1 << 20, []
+    for n, size in counts:
+        out.append(at)
+        at += -(-n * size // 64) * 64 + 64
+    return out
+
+
+def test_pages_outputs_may_not_overlap_another_array():
+    # workgroups read the inputs while another writes the outputs (lengths
+    # updated in place went wrong in steps of more than one workgroup)
+    lib = attn.load_library()
+    n_seq, n_tokens, n_pages, most = 4, 1000, 100, 10
+    d = ctypes.byref(attn.PageDesc(n_seq, n_tokens, 16, n_pages, most))
+    sizes = [(n_seq, 4), (n_seq, 4), (n_seq * most, 4), (n_pages, 4), (2, 8), (2, 8), (n_seq + 1, 4), (n_seq, 4),
+             (n_tokens, 8), (n_tokens, 4), (n_tokens, 4), (n_seq, 4)]
+    at = _apart(sizes)
+    for o in (2, *range(5, 12)):  # outputs: page_table, free_out, q_start ... status
+        for i in range(12):
+            if i == o:
+                continue
+            (n, size), (m, width) = sizes[i], sizes[o]
+            # on it, its last value, and the output's last value on its first
+            for x in (at[i], (at[i] + n * size - 1) // 8 * 8, (at[i] - m * width) // 8 * 8 + 8):
+                args = [x if j == o else a for j, a in enumerate(at)]
+                _error(lib.pelica_attn_pages_append(d, *args, None), attn.EINVAL, "overlaps")
+    sizes = [(n_seq, 4), (n_seq, 4), (n_seq * most, 4), (n_pages, 4), (2, 8), (2, 8)]
+    at = _apart(sizes)
+    for o in (3, 5):  # free_list, free_out
+        for i in range(6):
+            if i != o:
+                args = [at[i] if j == o else a for j, a in enumerate(at)]
+                _error(lib.pelica_attn_pages_release(d, *args, None), attn.EINVAL, "overlaps")
+
+
 def test_qkv_arguments():
     lib = attn.load_library()
     args = [A, A, A, 0, None, None, 1e-6, A, 128, 0, 0, A, A, None]
