@@ -13,7 +13,8 @@ A step of an engine, all of it on the GPU:
 
 Pages are f16 tensors [n_pages, page_size, n_kv, hd], in any layout whose hd
 values are contiguous (a transposed [n_pages, n_kv, page_size, hd], or K and V
-side by side in one buffer).  Every call runs on the current device, on
+side by side in one buffer); an expanded dim (stride 0) is refused, of token
+rows too.  Every call runs on the current device, on
 ``stream`` or the current stream; errors are ``AttnError``.
 """
 from __future__ import annotations
@@ -187,11 +188,11 @@ def _pools(k_pages, v_pages, dev):
     st, shape = k_pages.stride(), k_pages.shape
     if not (k_pages.dtype is _torch.float16 and v_pages.dtype is _torch.float16 and len(st) == 4 and st[3] == 1
             and v_pages.stride() == st and shape == v_pages.shape and k_pages.get_device() == dev
-            and v_pages.get_device() == dev):
+            and v_pages.get_device() == dev and (0 not in st or all(s or n == 1 for s, n in zip(st, shape)))):
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             _check(name, t, _torch.float16, 4, dense=False)
         raise AttnError(EINVAL, "k_pages and v_pages: [n_pages, page_size, n_kv, hd] pages whose hd values are contiguous, "
-                                f"one layout for both; got {tuple(k_pages.shape)} strides {tuple(st)} and "
+                                f"no stride of 0, one layout for both; got {tuple(k_pages.shape)} strides {tuple(st)} and "
                                 f"{tuple(v_pages.shape)} strides {tuple(v_pages.stride())}")
     # (a dim of one has no stride of its own)
     return st[0] if shape[0] > 1 else 0, st[1], st[2] if shape[2] > 1 else 0, shape
@@ -210,8 +211,8 @@ def _rows(name, t):
     if t.is_contiguous():
         return 0
     st = t.stride()
-    _need(st[2] == 1 and (t.shape[1] == 1 or st[1] == t.shape[2]),
-          f"{name}: token rows need contiguous heads, got strides {tuple(st)}")
+    _need(st[2] == 1 and (t.shape[1] == 1 or st[1] == t.shape[2]) and st[0] > 0,
+          f"{name}: token rows need contiguous heads and rows of their own, got strides {tuple(st)}")
     return st[0]
 
 
@@ -372,7 +373,7 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
         raise AttnError(EINVAL, f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
     stride = at_q[0] if T > 1 else 0
     if not (at_q[2] == 1 and (at_q[1] == hd or n_head == 1) and at_k[2] == 1 and (at_k[1] == hd or n_kv == 1)
-            and at_v[2] == 1 and (at_v[1] == hd or n_kv == 1) and (T == 1 or at_k[0] == at_v[0] == stride)):
+            and at_v[2] == 1 and (at_v[1] == hd or n_kv == 1) and (T == 1 or at_k[0] == at_v[0] == stride > 0)):
         stride = _rows("q", q)
         if _rows("k", k) != stride or _rows("v", v) != stride:
             raise AttnError(EINVAL, "q, k and v: all contiguous, or views into rows of one stride")

@@ -222,6 +222,61 @@ def test_rows_of_the_host_are_refused():
     assert e.value.code == attn.EINVAL and "device" in str(e.value)
 
 
+def test_strides_of_zero_are_refused(monkeypatch):
+    """To the C calls 0 means dense; of a tensor it is one row for all, and the
+    rows that a dense tensor would have lie behind its storage.  (Host tensors,
+    and no call: whatever passes the checks ends in the recorder.)"""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name) or 0
+
+    paged._start()
+    monkeypatch.setattr(paged, "_device", lambda: -1)
+    monkeypatch.setattr(attn, "_lib", Lib())
+    monkeypatch.setattr(attn, "_stream_ptr", lambda s: None)
+    n, page, heads, hd = 3, 16, 4, 64
+    pool = torch.zeros(n, page, heads, hd, dtype=torch.float16)
+    one = [pool[:1].expand(n, -1, -1, -1), pool[:, :1].expand(-1, page, -1, -1), pool[:, :, :1].expand(-1, -1, heads, -1)]
+    T = 5
+    rows = torch.zeros(T, heads, hd)
+    slots = torch.arange(T)
+    few = rows[:1].expand(T, -1, -1)
+    good = dict(q=rows, k=rows, v=rows, k_pages=pool, v_pages=pool, slots=slots, out=rows)
+    # dims of one have any stride: a single page, head, token
+    fine = [{}, dict(k_pages=pool[:1].expand(1, -1, -1, -1), v_pages=pool[:1])]
+    single = torch.zeros(1, page, 1, hd, dtype=torch.float16)
+    x = torch.zeros(1, 1, hd)
+    fine.append(dict(q=x, k=x, v=x, k_pages=single, v_pages=single, slots=slots[:1], out=x))
+    x = torch.as_strided(torch.zeros(hd), (1, 1, hd), (0, 0, 1))
+    fine.append(dict(q=x, k=x, v=x, k_pages=torch.as_strided(single, single.shape, (0, hd, 0, 1)),
+                     v_pages=torch.as_strided(single, single.shape, (0, hd, 0, 1)), slots=slots[:1], out=x))
+    for kw in fine:
+        paged.paged_qkv(**{**good, **kw})
+    assert len(calls) == len(fine)
+    bad = [dict(k_pages=p, v_pages=p) for p in one]
+    bad += [dict(q=few, k=few, v=few), dict(q=few), dict(k=few), dict(v=few), dict(k=few, v=few), dict(out=few)]
+    bad += [dict(q=rows[:, :1].expand(-1, heads, -1)), dict(k=rows[:, :1].expand(-1, heads, -1))]
+    for kw in bad:
+        with pytest.raises(attn.AttnError) as e:
+            paged.paged_qkv(**{**good, **kw})
+        assert e.value.code == attn.EINVAL and "stride" in str(e.value)
+    assert len(calls) == len(fine)
+
+    plan = paged.PagedPlan.__new__(paged.PagedPlan)
+    plan._dev, plan._q_shape, plan._page_shape = -1, (T, heads, hd), (n, page, heads, hd)
+    plan.workspace_bytes, plan.desc, plan._buffer, plan._bytes = 0, attn.PagedDesc(), None, 0
+    good = dict(q=rows, k_pages=pool, v_pages=pool, plan=plan, out=rows)
+    paged.paged_attention(**good)
+    assert len(calls) == len(fine) + 1
+    for kw in [dict(k_pages=p, v_pages=p) for p in one] + [dict(q=few), dict(out=few)]:
+        with pytest.raises(attn.AttnError) as e:
+            paged.paged_attention(**{**good, **kw})
+        assert e.value.code == attn.EINVAL and "stride" in str(e.value)
+    assert len(calls) == len(fine) + 1
+
+
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     so = tmp_path_factory.mktemp("plan") / "plan.so"
