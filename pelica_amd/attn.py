@@ -300,6 +300,8 @@ def token_stride(t) -> int:
     if t.stride(3) != 1 or (n_head > 1 and t.stride(2) != hd):
         raise AttnError(EINVAL, f"token rows need contiguous heads, got strides {tuple(t.stride())}")
     st = t.stride(1) if T > 1 else t.stride(0)
+    if st == 0:  # (an expanded tensor: to the call, dense)
+        raise AttnError(EINVAL, f"tokens need rows of their own, got strides {tuple(t.stride())}")
     if n_seq > 1 and T > 1 and t.stride(0) != T * st:
         raise AttnError(EINVAL, f"tokens of all sequences need one stride, got strides {tuple(t.stride())}")
     return st

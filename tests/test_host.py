@@ -301,3 +301,16 @@ def test_recorded_traffic_follows_the_kernel_sources(tmp_path, monkeypatch):
     stale.write_text("traffic c3_gptoss_decode_full 123 src=000000000000\n")
     monkeypatch.setattr(bench, "TRAFFIC_PROFILE", str(stale))
     assert bench.recorded_traffic("c3_gptoss_decode_full")[0] is None
+
+
+def test_a_token_stride_of_zero_is_no_dense_tensor():
+    # the descriptor's 0 means dense; tokens expanded from one have no rows behind it
+    import torch
+
+    x = torch.zeros(1, 1, 4, 64)
+    for t in (x.expand(1, 5, -1, -1), x.expand(3, 1, -1, -1), x.expand(3, 5, -1, -1)):
+        with pytest.raises(attn.AttnError, match="stride"):
+            attn.token_stride(t)
+    assert attn.token_stride(x) == 0 and attn.token_stride(torch.as_strided(x, x.shape, (0, 0, 64, 1))) == 0
+    wide = torch.zeros(3, 5, 6, 64)[:, :, :4]
+    assert attn.token_stride(wide) == 6 * 64
