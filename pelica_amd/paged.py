@@ -263,11 +263,13 @@ class PagedPlan:
             attn._check(rc)
         return self
 
-    def new_workspace(self):
-        """A workspace for calls with this plan (uninitialised)."""
+    def new_workspace(self, stream=None):
+        """A workspace (uninitialised) for calls with this plan on ``stream`` or
+        the current stream."""
         import torch
 
-        return torch.empty(max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device)
+        with _on(stream):
+            return torch.empty(max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device)
 
 
 def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=None, softcap: float = 0.0,

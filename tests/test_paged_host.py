@@ -277,6 +277,30 @@ def test_strides_of_zero_are_refused(monkeypatch):
     assert len(calls) == len(fine) + 1
 
 
+def test_a_workspace_belongs_to_its_stream(monkeypatch):
+    """Memory of the stream that the calls run on: another's may be in use."""
+    import contextlib
+
+    on = []
+
+    @contextlib.contextmanager
+    def _on(stream):
+        on.append(stream)
+        yield
+        on.append("made")
+
+    plan = paged.PagedPlan.__new__(paged.PagedPlan)
+    plan.device, plan.workspace_bytes = torch.device("cpu"), 100
+    monkeypatch.setattr(paged, "_on", _on)
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: on.append("empty") or empty(*a, **kw))
+    st = object()
+    assert plan.new_workspace(st).numel() == plan.new_workspace(stream=st).numel() == 100
+    assert on == [st, "empty", "made"] * 2
+    plan.new_workspace()
+    assert on[6:] == [None, "empty", "made"]
+
+
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     so = tmp_path_factory.mktemp("plan") / "plan.so"
