@@ -315,8 +315,8 @@ typedef struct PelicaPageDesc {
 /* Takes free pages for every request's new tokens, in request order, and
  * appends them to its row of page_table (entries of pages it had stay as they
  * are).  Writes q_start[n_seq + 1] (first row of each request's new tokens,
- * packed in request order; requests with a negative length count none, and
- * no entry passes n_tokens), seq_kv_len[n_seq] = cached + new, per row the
+ * packed in request order; a negative new_len counts none, and no entry
+ * passes n_tokens), seq_kv_len[n_seq] = cached + new, per row the
  * slot (page * page_size + row in it), the position and the request
  * (slots[n_tokens], positions[n_tokens], token_seq[n_tokens]; rows behind
  * the last request: -1, 0, -1), status[n_seq], and free_out[2].
@@ -392,8 +392,11 @@ int pelica_attn_paged_plan(const PelicaPagedDesc* desc, void* plan, size_t plan_
 /* Attention of each request's new tokens over its pages: f16 queries and
  * output, or f32 (_f32), whose products keep f32's precision (queries and
  * probabilities as f16 hi + lo parts: a query's value is kept to 2^-22 of
- * itself or 2^-25, the larger, and one past 65504 gives NaN).  Softmax and
- * sums in f32.  sinks:
+ * itself or 2^-25, the larger, and one past 65504 gives NaN).  Scores, running
+ * maxima and sums are f32 in both; with f16 queries each probability is rounded
+ * to f16 (2^-11) for the product with V and for the sum alike, as in
+ * pelica_attn_prefill, so an output is off by two such roundings instead of
+ * one, its own.  sinks:
  * [n_head] natural-log logits or NULL.  Rows of skipped requests and behind
  * the last one are left as they were.  Workspace (partials of key ranges;
  * pelica_attn_paged_workspace_bytes, 0 if none is needed): contents need no

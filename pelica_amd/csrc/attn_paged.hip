@@ -28,16 +28,16 @@
 // bits.  The resource ends with the rows the item may see: what lies behind is
 // not touched and reads as zeros.
 //
-// Measured (floors: bytes at a copy's 5.1 TB/s, or operations at a large f16
-// product's 1.13 PFLOP/s):
+// Measured, medians of warm traced launches (floors: bytes at a copy's 5.13 TB/s,
+// or operations at a large f16 product's 1.17 PFLOP/s):
 //   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   116 us (118)
 //   16 tokens with a bias over 300 - 6000, 16 / 16 of 128   96 us (99)
-//   one token over 32768, 64 / 8 of 64                      16 us + join 3.8 (13)
-//   64 tokens on windows of 128, 64 / 8 of 64              8.8 us (3.7: latency)
-//   512 tokens over 30512, 64 / 8 of 64                    291 us (224)
-//   4001 tokens, 32 / 4 of 128                             161 us (116)
-//   3 chunks of 700 and 28 drafts, 64 / 8 of 64            201 us + join 12.7 (114)
-//   2000 tokens, capped, 600 of prefix, 32 / 4 of 128       73 us + join 6.7 (31.5)
+//   one token over 32768, 64 / 8 of 64                      16 us + join 3.9 (13)
+//   64 tokens on windows of 128, 64 / 8 of 64              8.6 us (3.7: latency)
+//   512 tokens over 30512, 64 / 8 of 64                    291 us + join 7.9 (217)
+//   4001 tokens, 32 / 4 of 128                             165 us + join 4.8 (112)
+//   3 chunks of 700 and 28 drafts, 64 / 8 of 64            208 us + join 12.6 (111)
+//   2000 tokens, capped, 600 of prefix, 32 / 4 of 128       73 us + join 7.0 (30.5)
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -407,7 +407,7 @@ __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
 // of one operand, the scores added by a lane exchange, the outputs at the end;
 // otherwise two products each.
 // HBM-bound over long keys (32 ragged requests at the copy's rate: 116 us);
-// short ones are a chain of latencies: 64 windows of 128 keys are 8.8 us, of
+// short ones are a chain of latencies: 64 windows of 128 keys are 8.6 us, of
 // which 1.5 until the piece and its table entries are there, 1 to request the
 // tiles, 2 until they land, 1.3 for the chunks, 2.4 for merge and store.  With
 // 32-row tiles, every tile requested and two merge barriers they were 11.4;
@@ -766,9 +766,11 @@ __device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece
     }
 }
 
-// The wide item with f32 queries: hi and lo products, a chunk at a time (bound by
-// its products, twice f16's, and not pipelined: prompts come in f16; 2000 tokens
-// of 32 / 4 heads of 128, capped: 117 us against 73).
+// The wide item with f32 queries: hi and lo products, a chunk at a time: loads run
+// ahead, but scores, softmax and PV follow one another, where the f16 item's
+// overlap (a prompt's queries may be had in f16 from the step before).  2000
+// tokens of 32 / 4 heads of 128: a whole call 110 us, f16 69; the products, twice
+// f16's, at a large product's rate 56.
 template <int HD, bool SC>
 __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S = WideShape<HD>;
@@ -998,9 +1000,9 @@ enum ScoreMode { kPlain, kCapped, kBiased };
 // Bound by issue and clock: of a step's ~1900 cycles (two waves a SIMD, 1.7 -
 // 1.9 GHz under load) the matrix cores are busy 1024; at head dim 64 the exp2s
 // and their VALU work take as long, at 128 the LDS operands (16 rows' tile a
-// wave, each read once).  4001 tokens of 32 / 4 heads of 128: 0.81 PFLOP/s; 512
+// wave, each read once).  4001 tokens of 32 / 4 heads of 128: 0.80 PFLOP/s; 512
 // over 30512 keys of 64 / 8 of 64: 0.87.  A simple loop over tiles took 239
-// and 467 us for these calls, which now take 165 and 284.
+// and 467 us for these calls, plan and join included, which now take 167 and 293.
 template <int HD, int MODE>
 __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S_ = WideShape<HD>;
@@ -1350,7 +1352,7 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // lane exchanges and LDS in a fixed order, or, where the slots are few, a
 // row each.  Bound by the partials' bytes (a mixed step's 48 MB: 12.7 us, 3.8
 // TB/s), and for single tokens by its two round trips (plan, partials) behind
-// the attention kernel: 3.8 - 4.8 us.
+// the attention kernel: 3.9 - 4.8 us.
 template <int HD, bool F32, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     constexpr int LPR = HD / 4, GPW = 64 / LPR, U = 4;

@@ -65,8 +65,8 @@ struct PagedParams {
 // 2^-22.7 relative with every rounding counted.  (1 - 2 / (1 + e^2y) is off by
 // 2^-23 of the cap, however small the score is.)  Of f16 queries
 // three terms, up to 0.3: 1.2e-6 relative, less than the roundings of a large
-// score's own products; at cap 50 a weight is off by 2^-16 at most, where f16
-// rounds it by 2^-11.  (2000 tokens of head dim 64: five terms 97 us, three 83.)
+// score's own products; at cap 50 a weight is off by 1.7e-5 (2^-15.8) at most,
+// where f16 rounds it by 2^-11.  (2000 tokens of head dim 64: five terms 97 us, three 83.)
 inline void capped_poly(PagedParams& p) {
     if (!(p.cap > 0.f)) return;
     const double f = (double)p.qscale / kLog2e / p.cap;  // y = f s

