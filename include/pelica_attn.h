@@ -439,6 +439,43 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* desc, const PelicaPagedRope* ro
                           const int64_t* slots, void* q_out, int32_t q_half, int64_t q_out_stride, uint16_t* k_pages,
                           uint16_t* v_pages, void* stream);
 
+/* ---- an 8-bit paged cache ------------------------------------------------- */
+
+/* A row of one head as hd integers n in -127 .. 127 (int8, where the f16 row
+ * would be: the descriptor's strides count them) and, for each 32 values, an
+ * f16 scale s beside them: it stands for the f16 numbers n s (rounded to
+ * nearest).  Head h's hd / 32 scales of row r of page p start at p *
+ * page_stride + r * row_stride + h * head_stride, the same for K's and V's.
+ * The qkv step takes the smallest f16 number s with 127 s >= the group's
+ * largest magnitude and n = x / s to nearest, so a value is kept to s / 2 (1 +
+ * 2^-14).  A group that holds an infinity, a NaN or a magnitude above 127 *
+ * 65504 reads as NaN, a value above 65468 may read as infinity.
+ * Rows of one head that lie side by side ([page][head][row][...]) are read in
+ * whole cache lines, scales among them. */
+typedef struct PelicaPagedQ8 {
+    uint16_t* k_scales;   /* device */
+    uint16_t* v_scales;
+    int64_t page_stride;  /* f16 values; 0 = page_size * row_stride */
+    int64_t row_stride;   /* 0 = n_kv * hd / 32 */
+    int64_t head_stride;  /* 0 = hd / 32 */
+} PelicaPagedQ8;
+
+/* pelica_attn_paged_qkv into 8-bit pages (16-byte aligned, as are their strides). */
+int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* desc, const PelicaPagedRope* rope, const PelicaPagedQ8* q8,
+                             const float* q, const float* k, const float* v, int64_t token_stride,
+                             const float* q_norm, const float* k_norm, float eps, const int64_t* slots, void* q_out,
+                             int32_t q_half, int64_t q_out_stride, int8_t* k_pages, int8_t* v_pages, void* stream);
+
+/* n_tokens rows of the pages as f16 rows: row slots[i] of every kv head to
+ * k_out and v_out [n_kv][hd] at i * out_stride values (0 = n_kv * hd), from 8-bit pages,
+ * or f16 ones (q8 NULL): what attention reads, for the calls over dense
+ * rows and for requests that leave the pool.  Rows whose slot is negative or
+ * past the pool are left as they were.  Of the descriptor: n_head and n_kv
+ * (alike will do), hd (64, 128, 256), n_tokens, page_size, n_pages and the strides of pages. */
+int pelica_attn_pages_read(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8, const int64_t* slots,
+                           const void* k_pages, const void* v_pages, uint16_t* k_out, uint16_t* v_out,
+                           int64_t out_stride, void* stream);
+
 /* ---- per-kernel GPU timing ------------------------------------------- */
 
 /* kernel ids of PelicaAttnProfRecord */
@@ -452,6 +489,7 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* desc, const PelicaPagedRope* ro
 #define PELICA_ATTN_PROF_PAGED 8
 #define PELICA_ATTN_PROF_PAGED_JOIN 9
 #define PELICA_ATTN_PROF_PAGED_QKV 10
+#define PELICA_ATTN_PROF_PAGES_READ 11
 
 typedef struct PelicaAttnProfRecord {
     int32_t kernel; /* PELICA_ATTN_PROF_* */

@@ -56,13 +56,15 @@ EXPORTS = (
     "pelica_attn_paged",
     "pelica_attn_paged_f32",
     "pelica_attn_paged_qkv",
+    "pelica_attn_paged_qkv_q8",
+    "pelica_attn_pages_read",
     "pelica_attn_prof_enable",
     "pelica_attn_prof_read",
 )
 
 #: kernel ids of the per-kernel timing records
 PROF_KERNELS = {1: "decode_split", 2: "decode_combine", 3: "prefill", 4: "partials_merge", 5: "qkv_rope_cache",
-                6: "pages", 7: "paged_plan", 8: "paged", 9: "paged_join", 10: "paged_qkv"}
+                6: "pages", 7: "paged_plan", 8: "paged", 9: "paged_join", 10: "paged_qkv", 11: "pages_read"}
 
 
 class AttnError(RuntimeError):
@@ -168,6 +170,18 @@ class PagedRope(ctypes.Structure):
     ]
 
 
+class PagedQ8(ctypes.Structure):
+    """``PelicaPagedQ8`` (field meanings in include/pelica_attn.h)."""
+
+    _fields_ = [
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -244,6 +258,12 @@ def load_library() -> ctypes.CDLL:
     lib.pelica_attn_paged_qkv.restype = ctypes.c_int
     lib.pelica_attn_paged_qkv.argtypes = [gd, ctypes.POINTER(PagedRope), vp, vp, vp, ctypes.c_int64, vp, vp,
                                           ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
+    q8 = ctypes.POINTER(PagedQ8)
+    lib.pelica_attn_paged_qkv_q8.restype = ctypes.c_int
+    lib.pelica_attn_paged_qkv_q8.argtypes = [gd, ctypes.POINTER(PagedRope), q8, vp, vp, vp, ctypes.c_int64, vp, vp,
+                                             ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
+    lib.pelica_attn_pages_read.restype = ctypes.c_int
+    lib.pelica_attn_pages_read.argtypes = [gd, q8, vp, vp, vp, vp, vp, ctypes.c_int64, vp]
     lib.pelica_attn_prof_enable.restype = ctypes.c_int
     lib.pelica_attn_prof_enable.argtypes = [ctypes.c_int]
     lib.pelica_attn_prof_read.restype = ctypes.c_int

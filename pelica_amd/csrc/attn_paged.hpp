@@ -85,6 +85,11 @@ inline void capped_poly(PagedParams& p) {
     scaled(h, 3, 0.3, p.tanh_h, p.tanh_to[1]);
 }
 
+constexpr int kQ8Group = 32;  // values that share a scale
+struct Q8Strides {
+    int64_t page, row, head;  // f16 values
+};
+
 hipError_t launch_paged(const PagedParams& p, hipStream_t st);
 hipError_t launch_paged_join(const PagedParams& p, hipStream_t st);
 
@@ -93,15 +98,29 @@ struct PagedQkvParams {
     const int64_t* slots;
     const int32_t* positions;
     void* q_out;
-    uint16_t *k_pages, *v_pages;
+    uint16_t *k_pages, *v_pages;      // (f16 values, or 8-bit ones with scales)
+    uint16_t *k_scales, *v_scales;
+    Q8Strides sc;
     int64_t tok_q, tok_kv, tok_o, axis_stride;
     int64_t page_stride, row_stride, head_stride, n_slots;
     int n_head, n_kv, n_tokens, rot, neox, table_split, covered, page_log2, n_axes;
     float eps;
     uint32_t axis[8];  // 2 bits a pair
     int hd;            // host side only
-    bool half;
+    bool half, q8;
 };
 hipError_t launch_paged_qkv(const PagedQkvParams& p, hipStream_t st);
+
+struct PagesReadParams {
+    const int64_t* slots;
+    const char *k, *v;
+    const uint16_t *k_scales, *v_scales;  // NULL: f16 pages
+    uint16_t *k_out, *v_out;
+    int64_t page_b, row_b, head_b;        // bytes
+    Q8Strides sc;
+    int64_t out_stride, n_slots;
+    int n_tokens, n_kv, page_log2, hd;
+};
+hipError_t launch_pages_read(const PagesReadParams& p, hipStream_t st);
 
 }  // namespace pelica

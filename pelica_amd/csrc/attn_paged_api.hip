@@ -70,7 +70,8 @@ int64_t row_stride(const PelicaPagedDesc* d) { return d->row_stride ? d->row_str
 int64_t head_stride(const PelicaPagedDesc* d) { return d->head_stride ? d->head_stride : d->hd; }
 int64_t page_stride(const PelicaPagedDesc* d) { return d->page_stride ? d->page_stride : (int64_t)d->page_size * row_stride(d); }
 
-// The pool's shape; attention reads 16-byte pieces (8 values), the qkv step writes 8-byte ones (4)
+// The pool's shape; attention reads 16-byte pieces (8 values), the qkv step writes 8-byte ones (4);
+// 8-bit rows are read in pieces of up to 16 values
 int check_pool(const PelicaPagedDesc* d, int piece) {
     if (!d) return fail(PELICA_ATTN_EINVAL, "desc is NULL");
     if (d->n_head <= 0 || d->n_kv <= 0 || d->n_head % d->n_kv || d->n_head > 65536)
@@ -81,12 +82,38 @@ int check_pool(const PelicaPagedDesc* d, int piece) {
     if (d->n_pages <= 0) return fail(PELICA_ATTN_EINVAL, "n_pages %d must be positive", d->n_pages);
     const int64_t rs = row_stride(d), hs = head_stride(d), ps = page_stride(d);
     if (rs < d->hd || hs < d->hd || ps < d->hd || rs % piece || hs % piece || ps % piece)
-        return fail(PELICA_ATTN_EINVAL, "page, row and head strides (%lld, %lld, %lld): at least hd, whole %d-byte pieces",
-                    (long long)ps, (long long)rs, (long long)hs, 2 * piece);
+        return fail(PELICA_ATTN_EINVAL, "page, row and head strides (%lld, %lld, %lld): at least hd, multiples of %d",
+                    (long long)ps, (long long)rs, (long long)hs, piece);
     // (a page's rows are addressed with 32-bit byte offsets, a page with 64)
     if (rs >= 1 << 24 || rs * d->page_size >= 1LL << 31 || hs >= 1LL << 40 || ps >= 1LL << 40)
         return fail(PELICA_ATTN_EUNSUPPORTED, "page, row and head strides (%lld, %lld, %lld) too large", (long long)ps,
                     (long long)rs, (long long)hs);
+    return PELICA_ATTN_OK;
+}
+
+int64_t scale_row(const PelicaPagedDesc* d, const PelicaPagedQ8* x) {
+    return x->row_stride ? x->row_stride : (int64_t)d->n_kv * (d->hd / pelica::kQ8Group);
+}
+pelica::Q8Strides scale_strides(const PelicaPagedDesc* d, const PelicaPagedQ8* x) {
+    const int64_t row = scale_row(d, x);
+    return {x->page_stride ? x->page_stride : d->page_size * row, row, x->head_stride ? x->head_stride : d->hd / pelica::kQ8Group};
+}
+
+// Scales beside 8-bit pages (whose strides are whole 16-byte pieces)
+int check_q8(const PelicaPagedDesc* d, const PelicaPagedQ8* x) {
+    const int rc = check_pool(d, 16);
+    if (rc) return rc;
+    if (!x) return fail(PELICA_ATTN_EINVAL, "q8 is NULL");
+    if (!x->k_scales || !x->v_scales || misaligned(x->k_scales, 2) || misaligned(x->v_scales, 2))
+        return fail(PELICA_ATTN_EINVAL, "k_scales and v_scales must be non-NULL and aligned to their values");
+    const pelica::Q8Strides st = scale_strides(d, x);
+    const int64_t g = d->hd / pelica::kQ8Group;
+    if (st.row < g || st.head < g || st.page < g)
+        return fail(PELICA_ATTN_EINVAL, "page, row and head strides of scales (%lld, %lld, %lld): at least hd / 32",
+                    (long long)st.page, (long long)st.row, (long long)st.head);
+    if (st.row >= 1 << 24 || st.row * d->page_size >= 1LL << 30 || st.head >= 1LL << 40 || st.page >= 1LL << 40)
+        return fail(PELICA_ATTN_EUNSUPPORTED, "page, row and head strides of scales (%lld, %lld, %lld) too large",
+                    (long long)st.page, (long long)st.row, (long long)st.head);
     return PELICA_ATTN_OK;
 }
 
@@ -218,6 +245,87 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, con
     hipError_t e = pelica::launch_paged(p, st);
     if (e == hipSuccess && x.split) e = pelica::launch_paged_join(p, st);
     if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged attention launch: %s", hipGetErrorString(e));
+    return PELICA_ATTN_OK;
+}
+
+// (q8: NULL for f16 pages)
+int run_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope, const PelicaPagedQ8* q8, const float* q, const float* k,
+            const float* v, int64_t token_stride, const float* q_norm, const float* k_norm, float eps,
+            const int64_t* slots, void* q_out, int32_t q_half, int64_t q_out_stride, void* k_pages, void* v_pages,
+            void* stream) {
+    if (d->hd != 64 && d->hd != 128 && d->hd != 256) return fail(PELICA_ATTN_EUNSUPPORTED, "hd %d (64, 128 or 256)", d->hd);
+    if (!q || !k || !v || !slots || !q_out || !k_pages || !v_pages)
+        return fail(PELICA_ATTN_EINVAL, "q, k, v, slots, q_out and the pages must be non-NULL");
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out, q_half ? 8 : 16) || misaligned(q_norm) ||
+        misaligned(k_norm) || misaligned(k_pages, q8 ? 16 : 8) || misaligned(v_pages, q8 ? 16 : 8) || misaligned(slots, 8))
+        return fail(PELICA_ATTN_EINVAL, "q, k, v, f32 q_out, norms and 8-bit pages must be 16-byte aligned, f16 q_out, slots and f16 pages 8");
+    const int64_t wq = (int64_t)d->n_head * d->hd, wkv = (int64_t)d->n_kv * d->hd;
+    if (token_stride && (token_stride < wq || token_stride < wkv || token_stride % 4))
+        return fail(PELICA_ATTN_EINVAL, "token_stride %lld: 0, or at least a token's heads and a multiple of 4", (long long)token_stride);
+    if (q_out_stride && (q_out_stride < wq || q_out_stride % 4))
+        return fail(PELICA_ATTN_EINVAL, "q_out_stride %lld: 0, or >= n_head*hd and a multiple of 4", (long long)q_out_stride);
+    if (q_out == (const void*)q && (q_half || (q_out_stride ? q_out_stride : wq) != (token_stride ? token_stride : wq)))
+        return fail(PELICA_ATTN_EINVAL, "q_out may be q in f32 only, and at its stride");
+    if (!(eps >= 0.f)) return fail(PELICA_ATTN_EINVAL, "eps must be >= 0");
+    pelica::PagedQkvParams p{};
+    if (rope && rope->rot) {
+        if (rope->rot < 0 || rope->rot % 2 || rope->rot > d->hd) return fail(PELICA_ATTN_EINVAL, "rot %d", rope->rot);
+        if (!rope->table || misaligned(rope->table, 8) || rope->table_split < 0 || rope->table_rows <= 0)
+            return fail(PELICA_ATTN_EINVAL, "rope table missing, or not 8-byte aligned");
+        if (rope->table_split && rope->table_rows < (int64_t)rope->table_split + 256)
+            return fail(PELICA_ATTN_EINVAL, "a two-level rope table needs %lld rows", (long long)rope->table_split + 256);
+        if (rope->n_axes < 1 || rope->n_axes > 4) return fail(PELICA_ATTN_EINVAL, "n_axes %d (1 .. 4)", rope->n_axes);
+        if (!rope->positions || misaligned(rope->positions, 4)) return fail(PELICA_ATTN_EINVAL, "positions missing");
+        if (rope->axis_stride != 0 && rope->axis_stride < d->n_tokens)
+            return fail(PELICA_ATTN_EINVAL, "axis_stride %lld: 0, or >= n_tokens", (long long)rope->axis_stride);
+        if (rope->pair_axis)
+            for (int j = 0; j < rope->rot / 2; ++j) {
+                if (rope->pair_axis[j] >= rope->n_axes)
+                    return fail(PELICA_ATTN_EINVAL, "pair %d turns by axis %d of %d", j, rope->pair_axis[j], rope->n_axes);
+                p.axis[j / 16] |= (uint32_t)rope->pair_axis[j] << (2 * (j % 16));
+            }
+        p.table = rope->table;
+        p.positions = rope->positions;
+        p.axis_stride = rope->axis_stride;
+        p.rot = rope->rot;
+        p.neox = rope->neox ? 1 : 0;
+        p.table_split = rope->table_split;
+        p.covered = (int)std::min<int64_t>(rope->table_split ? 256LL * rope->table_split : rope->table_rows, INT32_MAX);
+        p.n_axes = rope->n_axes;
+    }
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.q_norm = q_norm;
+    p.k_norm = k_norm;
+    p.slots = slots;
+    p.q_out = q_out;
+    p.k_pages = static_cast<uint16_t*>(k_pages);
+    p.v_pages = static_cast<uint16_t*>(v_pages);
+    if (q8) {
+        p.q8 = true;
+        p.k_scales = q8->k_scales;
+        p.v_scales = q8->v_scales;
+        p.sc = scale_strides(d, q8);
+    }
+    p.tok_q = token_stride ? token_stride : wq;
+    p.tok_kv = token_stride ? token_stride : wkv;
+    p.tok_o = q_out_stride ? q_out_stride : wq;
+    p.page_stride = page_stride(d);
+    p.row_stride = row_stride(d);
+    p.head_stride = head_stride(d);
+    p.page_log2 = log2_of(d->page_size);
+    p.n_slots = (int64_t)d->n_pages << p.page_log2;
+    p.n_head = d->n_head;
+    p.n_kv = d->n_kv;
+    p.n_tokens = d->n_tokens;
+    p.eps = eps;
+    p.hd = d->hd;
+    p.half = q_half != 0;
+    if ((int64_t)d->n_tokens * ((d->n_head + 2 * d->n_kv) * (d->hd / 4) / 256 + 1) >= 1 << 24)
+        return fail(PELICA_ATTN_EUNSUPPORTED, "more than 2^24 workgroups");
+    const hipError_t e = pelica::launch_paged_qkv(p, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_qkv launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;
 }
 
@@ -356,75 +464,61 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope,
                           const int64_t* slots, void* q_out, int32_t q_half, int64_t q_out_stride, uint16_t* k_pages,
                           uint16_t* v_pages, void* stream) {
     pelica::clear_error();
-    int rc = check_pool(d, 4);
+    const int rc = check_pool(d, 4);
+    if (rc) return rc;
+    return run_qkv(d, rope, nullptr, q, k, v, token_stride, q_norm, k_norm, eps, slots, q_out, q_half, q_out_stride, k_pages,
+                   v_pages, stream);
+}
+
+int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* d, const PelicaPagedRope* rope, const PelicaPagedQ8* q8, const float* q,
+                             const float* k, const float* v, int64_t token_stride, const float* q_norm,
+                             const float* k_norm, float eps, const int64_t* slots, void* q_out, int32_t q_half,
+                             int64_t q_out_stride, int8_t* k_pages, int8_t* v_pages, void* stream) {
+    pelica::clear_error();
+    const int rc = check_q8(d, q8);
+    if (rc) return rc;
+    return run_qkv(d, rope, q8, q, k, v, token_stride, q_norm, k_norm, eps, slots, q_out, q_half, q_out_stride, k_pages,
+                   v_pages, stream);
+}
+
+int pelica_attn_pages_read(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const int64_t* slots, const void* k_pages,
+                           const void* v_pages, uint16_t* k_out, uint16_t* v_out, int64_t out_stride, void* stream) {
+    pelica::clear_error();
+    const int rc = q8 ? check_q8(d, q8) : check_pool(d, 8);
     if (rc) return rc;
     if (d->hd != 64 && d->hd != 128 && d->hd != 256) return fail(PELICA_ATTN_EUNSUPPORTED, "hd %d (64, 128 or 256)", d->hd);
-    if (!q || !k || !v || !slots || !q_out || !k_pages || !v_pages)
-        return fail(PELICA_ATTN_EINVAL, "q, k, v, slots, q_out and the pages must be non-NULL");
-    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(q_out, q_half ? 8 : 16) || misaligned(q_norm) ||
-        misaligned(k_norm) || misaligned(k_pages, 8) || misaligned(v_pages, 8) || misaligned(slots, 8))
-        return fail(PELICA_ATTN_EINVAL, "q, k, v, f32 q_out and norms must be 16-byte aligned, f16 q_out, slots and pages 8");
-    const int64_t wq = (int64_t)d->n_head * d->hd, wkv = (int64_t)d->n_kv * d->hd;
-    if (token_stride && (token_stride < wq || token_stride < wkv || token_stride % 4))
-        return fail(PELICA_ATTN_EINVAL, "token_stride %lld: 0, or at least a token's heads and a multiple of 4", (long long)token_stride);
-    if (q_out_stride && (q_out_stride < wq || q_out_stride % 4))
-        return fail(PELICA_ATTN_EINVAL, "q_out_stride %lld: 0, or >= n_head*hd and a multiple of 4", (long long)q_out_stride);
-    if (q_out == (const void*)q && (q_half || (q_out_stride ? q_out_stride : wq) != (token_stride ? token_stride : wq)))
-        return fail(PELICA_ATTN_EINVAL, "q_out may be q in f32 only, and at its stride");
-    if (!(eps >= 0.f)) return fail(PELICA_ATTN_EINVAL, "eps must be >= 0");
-    pelica::PagedQkvParams p{};
-    if (rope && rope->rot) {
-        if (rope->rot < 0 || rope->rot % 2 || rope->rot > d->hd) return fail(PELICA_ATTN_EINVAL, "rot %d", rope->rot);
-        if (!rope->table || misaligned(rope->table, 8) || rope->table_split < 0 || rope->table_rows <= 0)
-            return fail(PELICA_ATTN_EINVAL, "rope table missing, or not 8-byte aligned");
-        if (rope->table_split && rope->table_rows < (int64_t)rope->table_split + 256)
-            return fail(PELICA_ATTN_EINVAL, "a two-level rope table needs %lld rows", (long long)rope->table_split + 256);
-        if (rope->n_axes < 1 || rope->n_axes > 4) return fail(PELICA_ATTN_EINVAL, "n_axes %d (1 .. 4)", rope->n_axes);
-        if (!rope->positions || misaligned(rope->positions, 4)) return fail(PELICA_ATTN_EINVAL, "positions missing");
-        if (rope->axis_stride != 0 && rope->axis_stride < d->n_tokens)
-            return fail(PELICA_ATTN_EINVAL, "axis_stride %lld: 0, or >= n_tokens", (long long)rope->axis_stride);
-        if (rope->pair_axis)
-            for (int j = 0; j < rope->rot / 2; ++j) {
-                if (rope->pair_axis[j] >= rope->n_axes)
-                    return fail(PELICA_ATTN_EINVAL, "pair %d turns by axis %d of %d", j, rope->pair_axis[j], rope->n_axes);
-                p.axis[j / 16] |= (uint32_t)rope->pair_axis[j] << (2 * (j % 16));
-            }
-        p.table = rope->table;
-        p.positions = rope->positions;
-        p.axis_stride = rope->axis_stride;
-        p.rot = rope->rot;
-        p.neox = rope->neox ? 1 : 0;
-        p.table_split = rope->table_split;
-        p.covered = (int)std::min<int64_t>(rope->table_split ? 256LL * rope->table_split : rope->table_rows, INT32_MAX);
-        p.n_axes = rope->n_axes;
-    }
-    p.q = q;
-    p.k = k;
-    p.v = v;
-    p.q_norm = q_norm;
-    p.k_norm = k_norm;
+    if (!slots || !k_pages || !v_pages || !k_out || !v_out)
+        return fail(PELICA_ATTN_EINVAL, "slots, the pages, k_out and v_out must be non-NULL");
+    if (misaligned(k_pages) || misaligned(v_pages) || misaligned(k_out) || misaligned(v_out) || misaligned(slots, 8))
+        return fail(PELICA_ATTN_EINVAL, "pages, k_out and v_out must be 16-byte aligned, slots 8");
+    const int64_t row = (int64_t)d->n_kv * d->hd;
+    if (out_stride && (out_stride < row || out_stride % 8 || out_stride >= 1LL << 31))
+        return fail(PELICA_ATTN_EINVAL, "out_stride %lld: 0, or >= n_kv*hd (%lld), < 2^31 and a multiple of 8", (long long)out_stride,
+                    (long long)row);
+    if (d->n_tokens * row > 1LL << 33) return fail(PELICA_ATTN_EUNSUPPORTED, "more than 2^33 values");
+    pelica::PagesReadParams p{};
+    const int size = q8 ? 1 : 2;
     p.slots = slots;
-    p.q_out = q_out;
-    p.k_pages = k_pages;
-    p.v_pages = v_pages;
-    p.tok_q = token_stride ? token_stride : wq;
-    p.tok_kv = token_stride ? token_stride : wkv;
-    p.tok_o = q_out_stride ? q_out_stride : wq;
-    p.page_stride = page_stride(d);
-    p.row_stride = row_stride(d);
-    p.head_stride = head_stride(d);
+    p.k = static_cast<const char*>(k_pages);
+    p.v = static_cast<const char*>(v_pages);
+    if (q8) {
+        p.k_scales = q8->k_scales;
+        p.v_scales = q8->v_scales;
+        p.sc = scale_strides(d, q8);
+    }
+    p.k_out = k_out;
+    p.v_out = v_out;
+    p.page_b = page_stride(d) * size;
+    p.row_b = row_stride(d) * size;
+    p.head_b = head_stride(d) * size;
+    p.out_stride = out_stride ? out_stride : row;
     p.page_log2 = log2_of(d->page_size);
     p.n_slots = (int64_t)d->n_pages << p.page_log2;
-    p.n_head = d->n_head;
-    p.n_kv = d->n_kv;
     p.n_tokens = d->n_tokens;
-    p.eps = eps;
+    p.n_kv = d->n_kv;
     p.hd = d->hd;
-    p.half = q_half != 0;
-    if ((int64_t)d->n_tokens * ((d->n_head + 2 * d->n_kv) * (d->hd / 4) / 256 + 1) >= 1 << 24)
-        return fail(PELICA_ATTN_EUNSUPPORTED, "more than 2^24 workgroups");
-    const hipError_t e = pelica::launch_paged_qkv(p, static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_qkv launch: %s", hipGetErrorString(e));
+    const hipError_t e = pelica::launch_pages_read(p, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "pages_read launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;
 }
 

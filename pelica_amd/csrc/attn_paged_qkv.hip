@@ -2,7 +2,8 @@
 // (x w / sqrt(mean x^2 + eps)), rotary embedding with a position per axis
 // (pair j turns by the angle of row positions[axis(j)] of the table), q to its
 // own rows (f32 or f16), k and v rounded to f16 into the row of the token's
-// slot.
+// slot; or to 8-bit integers and a scale for each 32 values (Q8): s the smallest
+// f16 number with 127 s >= the group's largest magnitude, n = x / s to nearest.
 //
 // Head slots [0, n_head) are q heads, then n_kv k heads, then n_kv v heads.  A
 // lane holds 8 elements of a head, 4 from each half of the rotated part (and
@@ -55,13 +56,56 @@ __device__ __forceinline__ half4 to_half(float4v x) {
     return {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
 }
 
+// max over lanes l, l ^ 1, l ^ 2, l ^ 3
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));
+}
+
+// Eight consecutive values of a lane, a group in four lanes, as 8-bit integers
+// and their scale's bits.  Magnitudes are compared as integers: an infinity
+// or a NaN is larger than all numbers.
+__device__ __forceinline__ u32x2 quantise8(const float4v& a, const float4v& b, uint16_t& scale) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        top = max(top, max(__float_as_uint(a[i]) & 0x7FFFFFFFu, __float_as_uint(b[i]) & 0x7FFFFFFFu));
+    const float most = __uint_as_float(quad_max(top));
+    _Float16 s = (_Float16)(most * (1.f / 127.f));
+    uint16_t bits = __builtin_bit_cast(uint16_t, s);
+    // (off by a last bit of the quotient s is still one of the two f16 numbers
+    // around it; 127 s is exact in f32)
+    if ((float)s * 127.f < most) ++bits;
+    if (!(most < INFINITY)) bits = 0x7E00;
+    const float f = (float)__builtin_bit_cast(_Float16, bits);
+    const float inv = f > 0.f ? __builtin_amdgcn_rcpf(f) : 0.f;
+    scale = bits;
+    // the sum's last byte is n: 2^23 takes the places behind the point.  Of a
+    // quotient next to a border the remainder, exact by the fma, decides.
+    uint32_t n[8];
+    const float half = 0.5f * f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = i < 4 ? a[i & 3] : b[i & 3];
+        float t = __builtin_fmaf(x, inv, 12582912.f);
+        const float r = __builtin_fmaf(12582912.f - t, f, x);
+        t += r > half ? 1.f : r < -half ? -1.f : 0.f;
+        n[i] = __float_as_uint(t);
+    }
+    auto pack = [&](int i) {
+        const uint32_t lo = __builtin_amdgcn_perm(n[i + 1], n[i], 0x0C0C0400u), hi = __builtin_amdgcn_perm(n[i + 3], n[i + 2], 0x04000C0Cu);
+        return lo | hi;
+    };
+    return u32x2{pack(0), pack(4)};
+}
+
 // EX: a lane holds both values of its pairs; else (rot not a multiple of 8)
 // partners are exchanged through LDS.
-template <int HD, int IT, bool HALF, bool EX>
+template <int HD, int IT, bool HALF, bool EX, bool Q8>
 __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int tok_waves) {
     constexpr int LPH = HD / 8, HPW = 64 / LPH;
     __shared__ __attribute__((aligned(16))) float turn[4][HD];  // (cos, sin) of the token's pairs
-    __shared__ __attribute__((aligned(16))) float xch[EX ? 1 : 4][EX ? 1 : HPW][EX ? 4 : HD];
+    __shared__ __attribute__((aligned(16))) float xch[EX && !Q8 ? 1 : 4][EX && !Q8 ? 1 : HPW][EX && !Q8 ? 4 : HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
     const uint32_t gw = blockIdx.x * 4u + wave;  // waves follow the tokens, workgroups do not
@@ -186,6 +230,30 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int to
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         }
+        if constexpr (Q8) {
+            // a group's 32 values into four lanes, eight each
+            if (hk >= 0) {
+                *reinterpret_cast<float4v*>(&xch[wave][sub][ea]) = a;
+                *reinterpret_cast<float4v*>(&xch[wave][sub][eb]) = b;
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            if (hk >= 0 && h < n_slot) {
+                const float4v x0 = *reinterpret_cast<const float4v*>(&xch[wave][sub][8 * l]);
+                const float4v x1 = *reinterpret_cast<const float4v*>(&xch[wave][sub][8 * l + 4]);
+                uint16_t s;
+                const u32x2 n = quantise8(x0, x1, s);
+                const bool is_k = hv < 0;
+                const int hc = is_k ? hk : hv;
+                int8_t* const pages = reinterpret_cast<int8_t*>(is_k ? p.k_pages : p.v_pages);
+                *reinterpret_cast<u32x2*>(pages + base + (int64_t)hc * p.head_stride + 8 * l) = n;
+                const int64_t at = (row >> p.page_log2) * p.sc.page + (row & ((1LL << p.page_log2) - 1)) * p.sc.row + (int64_t)hc * p.sc.head;
+                if (l % 4 == 0) (is_k ? p.k_scales : p.v_scales)[at + l / 4] = s;
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            if (hk >= 0) continue;
+        }
         if (h >= n_slot) break;
         if (!HALF && hk < 0) {
             float* dst = static_cast<float*>(p.q_out) + (size_t)t * p.tok_o + (size_t)h * HD;
@@ -219,8 +287,9 @@ hipError_t launch_paged_qkv(const PagedQkvParams& p, hipStream_t st) {
     ProfScope ps(kProfPagedQkv, st);
     const dim3 grid((unsigned)(((int64_t)p.n_tokens * tok_waves + 3) / 4));
     auto go = [&](auto hd, auto i, auto half, auto e) {
-        hipLaunchKernelGGL((paged_qkv_kernel<decltype(hd)::value, decltype(i)::value, decltype(half)::value, decltype(e)::value>),
-                           grid, dim3(256), 0, st, p, tok_waves);
+        auto kernel = p.q8 ? paged_qkv_kernel<decltype(hd)::value, decltype(i)::value, decltype(half)::value, decltype(e)::value, true>
+                           : paged_qkv_kernel<decltype(hd)::value, decltype(i)::value, decltype(half)::value, decltype(e)::value, false>;
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, tok_waves);
         return hipGetLastError();
     };
     auto c = [&](auto hd, auto i, auto half) {

@@ -10,7 +10,7 @@ namespace pelica {
 
 enum ProfKernel {
     kProfDecodeSplit = 1, kProfDecodeCombine = 2, kProfPrefill = 3, kProfMerge = 4, kProfQkv = 5,
-    kProfPages = 6, kProfPagedPlan = 7, kProfPaged = 8, kProfPagedJoin = 9, kProfPagedQkv = 10
+    kProfPages = 6, kProfPagedPlan = 7, kProfPaged = 8, kProfPagedJoin = 9, kProfPagedQkv = 10, kProfPagesRead = 11
 };
 
 bool prof_enabled();

@@ -24,12 +24,16 @@ import ctypes
 from typing import Optional, Sequence
 
 from . import attn
-from .attn import EINVAL, AttnError, PagedDesc, PagedRope, PageDesc
+from .attn import EINVAL, AttnError, PagedDesc, PagedQ8, PagedRope, PageDesc
 
-__all__ = ["PagedPlan", "PageStep", "paged_attention", "paged_qkv", "pages_append", "pages_release", "pair_axes"]
+__all__ = ["PagedPlan", "PageStep", "new_q8_pages", "paged_attention", "paged_qkv", "pages_append", "pages_read",
+           "pages_release", "pair_axes"]
 
 #: most requests of one step (PELICA_ATTN_PAGED_MAX_SEQ)
 MAX_SEQ = 4096
+
+#: values of an 8-bit row that share a scale
+GROUP = 32
 
 #: values of PageStep.status
 PAGES_OK, PAGES_NONE, PAGES_TABLE, PAGES_ROWS, PAGES_LENGTH = range(5)
@@ -184,19 +188,32 @@ def pages_release(ended, cached_len, page_table, free_list, free_state, *, page_
     return free_out
 
 
-def _pools(k_pages, v_pages, dev):
+def _pools(k_pages, v_pages, dev, dtype=None, names=("k_pages", "v_pages"), last="hd"):
     """The strides of both pools of pages and their shape: page, row, head, shape."""
     st, shape = k_pages.stride(), k_pages.shape
-    if not (k_pages.dtype is _torch.float16 and v_pages.dtype is _torch.float16 and len(st) == 4 and st[3] == 1
+    dtype = dtype or _torch.float16
+    if not (k_pages.dtype is dtype and v_pages.dtype is dtype and len(st) == 4 and st[3] == 1
             and v_pages.stride() == st and shape == v_pages.shape and k_pages.get_device() == dev
             and v_pages.get_device() == dev and (0 not in st or all(s or n == 1 for s, n in zip(st, shape)))):
-        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            _check(name, t, _torch.float16, 4, dense=False)
-        raise AttnError(EINVAL, "k_pages and v_pages: [n_pages, page_size, n_kv, hd] pages whose hd values are contiguous, "
-                                f"no stride of 0, one layout for both; got {tuple(k_pages.shape)} strides {tuple(st)} and "
-                                f"{tuple(v_pages.shape)} strides {tuple(v_pages.stride())}")
+        for name, t in zip(names, (k_pages, v_pages)):
+            _check(name, t, dtype, 4, dense=False)
+        raise AttnError(EINVAL, f"{names[0]} and {names[1]}: [n_pages, page_size, n_kv, {last}] pages whose {last} values are "
+                                f"contiguous, no stride of 0, one layout for both; got {tuple(k_pages.shape)} strides "
+                                f"{tuple(st)} and {tuple(v_pages.shape)} strides {tuple(v_pages.stride())}")
     # (a dim of one has no stride of its own)
     return st[0] if shape[0] > 1 else 0, st[1], st[2] if shape[2] > 1 else 0, shape
+
+
+def _q8(k_pages, k_scales, v_scales, dev):
+    """The scales of 8-bit pages, and their strides (None: f16 pages)."""
+    if k_scales is None and v_scales is None:
+        return None
+    _need(k_scales is not None and v_scales is not None, "k_scales and v_scales come together")
+    page, row, head, size = _pools(k_scales, v_scales, dev, None, ("k_scales", "v_scales"), "hd / 32")
+    pool = k_pages.shape
+    if k_pages.dim() != 4 or size[:3] != pool[:3] or size[3] * GROUP != pool[3]:
+        raise AttnError(EINVAL, f"k_scales: one for each {GROUP} values of the pages {tuple(pool)}, got {tuple(size)}")
+    return PagedQ8(k_scales.data_ptr(), v_scales.data_ptr(), page, row, head)
 
 
 def _weights(name, t, n, dev):
@@ -346,7 +363,54 @@ def pair_axes(sections: Sequence[int], interleaved: bool = False) -> list:
     return [j % n if j // n < sections[j % n] else 0 for j in range(half)]
 
 
-def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, rot: int = 0, neox: bool = True,
+def new_q8_pages(n_pages: int, page_size: int, n_kv: int, hd: int, device="cuda"):
+    """Empty 8-bit pages, ``(k_pages, v_pages, k_scales, v_scales)``: int8
+    [n_pages, page_size, n_kv, hd] and f16 [n_pages, page_size, n_kv, hd / 32]
+    (PelicaPagedQ8), zeros, a head's rows side by side, as attention reads them."""
+    import torch
+
+    _need(n_pages > 0 and page_size > 0 and n_kv > 0 and hd > 0 and hd % GROUP == 0,
+          f"pages of [{n_pages}, {page_size}, {n_kv}, {hd}]: positive, hd a multiple of {GROUP}")
+    pool = lambda n, t: torch.zeros(n_pages, n_kv, page_size, n, dtype=t, device=device).transpose(1, 2)  # noqa: E731
+    return (pool(hd, torch.int8), pool(hd, torch.int8), pool(hd // GROUP, torch.float16), pool(hd // GROUP, torch.float16))
+
+
+def pages_read(k_pages, v_pages, slots, *, k_scales=None, v_scales=None, out=None, stream=None):
+    """Rows of the pages as f16 rows (pelica_attn_pages_read): ``slots`` int64
+    [n] (negative or past the pool: the row is left as it was).  8-bit pages
+    (int8, with ``k_scales`` and ``v_scales``) or f16 ones.  Returns ``out``, (k_rows,
+    v_rows) of f16 [n, n_kv, hd], contiguous or rows of wider buffers of one
+    stride, by default new ones (skipped rows undefined)."""
+    if _torch is None:
+        _start()
+    dev, f16 = _device(), _torch.float16
+    q8 = _q8(k_pages, k_scales, v_scales, dev)
+    page, row, head, (n_pages, page_size, n_kv, hd) = _pools(k_pages, v_pages, dev, None if q8 is None else _torch.int8)
+    if not (slots.dtype is _torch.int64 and slots.get_device() == dev and slots.dim() == 1 and slots.is_contiguous()):
+        _check("slots", slots, _torch.int64, 1)
+    shape = (slots.numel(), n_kv, hd)
+    if out is None:
+        with _on(stream):
+            out = (_torch.empty(shape, dtype=f16, device=k_pages.device), _torch.empty(shape, dtype=f16, device=k_pages.device))
+    k_out, v_out = out
+    for t in (k_out, v_out):
+        if not (t.dtype is f16 and t.shape == shape and t.get_device() == dev):
+            _check("out", t, f16, 3, dense=False)
+            raise AttnError(EINVAL, f"out: two of {shape}, got {tuple(t.shape)}")
+    stride = _rows("out", k_out)
+    if _rows("out", v_out) != stride:
+        raise AttnError(EINVAL, "out: both contiguous, or rows of one stride")
+    d = PagedDesc(n_kv, n_kv, hd, 0, shape[0], 0, page_size, n_pages, 0, 0, None, None, None, None, None, page, row, head)
+    lib = attn._lib or attn.load_library()
+    rc = lib.pelica_attn_pages_read(ctypes.byref(d), None if q8 is None else ctypes.byref(q8), slots.data_ptr(),
+                                    k_pages.data_ptr(), v_pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), stride,
+                                    attn._stream_ptr(stream))
+    if rc:
+        attn._check(rc)
+    return out
+
+
+def paged_qkv(q, k, v, k_pages, v_pages, slots, *, k_scales=None, v_scales=None, positions=None, table=None, rot: int = 0, neox: bool = True,
               table_split: int = 0, pair_axis: Optional[Sequence[int]] = None, q_norm=None, k_norm=None,
               eps: float = 1e-6, out=None, stream=None):
     """The step before attention over pages (pelica_attn_paged_qkv): per-head
@@ -354,7 +418,8 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
     (int32 [n_tokens], or [n_axes, n_tokens] with ``pair_axis``: the axis of
     each pair, see ``pair_axes``) with the f32 cos/sin ``table`` [rows, rot/2,
     2], k and v rows to f16 rows ``slots`` (int64 [n_tokens]; negative: the row
-    is skipped) of the pages.  q: f32 [n_tokens, n_head, hd], k, v: f32
+    is skipped) of the pages; 8-bit pages (int8, with ``k_scales`` and
+    ``v_scales``) take the rows quantised (pelica_attn_paged_qkv_q8).  q: f32 [n_tokens, n_head, hd], k, v: f32
     [n_tokens, n_kv, hd], contiguous or views into one buffer of token rows.
     Returns ``out`` (f32, may be q; or f16), by default a new f32 tensor (its
     skipped rows undefined)."""
@@ -372,7 +437,8 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
                                 f"{tuple(v.shape)}")
     T, n_head, hd = shape
     n_kv = kv_shape[1]
-    page, row, head, (n_pages, page_size, heads, dims) = _pools(k_pages, v_pages, dev)
+    q8 = _q8(k_pages, k_scales, v_scales, dev)
+    page, row, head, (n_pages, page_size, heads, dims) = _pools(k_pages, v_pages, dev, None if q8 is None else _torch.int8)
     if heads != n_kv or dims != hd:
         raise AttnError(EINVAL, f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
     stride = at_q[0] if T > 1 else 0
@@ -425,10 +491,12 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, positions=None, table=None, r
     # (in the order of PagedDesc._fields_)
     d = PagedDesc(n_head, n_kv, hd, 0, T, 0, page_size, n_pages, 0, 0, None, None, None, None, None, page, row, head)
     lib = attn._lib or attn.load_library()
-    rc = lib.pelica_attn_paged_qkv(
-        ctypes.byref(d), rp, q.data_ptr(), k.data_ptr(), v.data_ptr(), stride,
-        wq, wk, eps, slots.data_ptr(), out.data_ptr(), half, _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(),
-        attn._stream_ptr(stream))
+    tail = (q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, wq, wk, eps, slots.data_ptr(), out.data_ptr(), half,
+            _rows("out", out), k_pages.data_ptr(), v_pages.data_ptr(), attn._stream_ptr(stream))
+    if q8 is None:
+        rc = lib.pelica_attn_paged_qkv(ctypes.byref(d), rp, *tail)
+    else:
+        rc = lib.pelica_attn_paged_qkv_q8(ctypes.byref(d), rp, ctypes.byref(q8), *tail)
     if rc:
         attn._check(rc)
     return out
