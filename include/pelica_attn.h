@@ -466,6 +466,13 @@ int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* desc, const PelicaPagedRope*
                              const float* q_norm, const float* k_norm, float eps, const int64_t* slots, void* q_out,
                              int32_t q_half, int64_t q_out_stride, int8_t* k_pages, int8_t* v_pages, void* stream);
 
+/* pelica_attn_paged (half != 0: f16 q and out) or pelica_attn_paged_f32 over
+ * 8-bit pages, with the same plans and workspaces: attention over the f16 numbers that the
+ * rows stand for. */
+int pelica_attn_paged_q8(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8, const void* plan, size_t plan_bytes,
+                         const void* q, int32_t half, const int8_t* k_pages, const int8_t* v_pages, const float* sinks,
+                         void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* n_tokens rows of the pages as f16 rows: row slots[i] of every kv head to
  * k_out and v_out [n_kv][hd] at i * out_stride values (0 = n_kv * hd), from 8-bit pages,
  * or f16 ones (q8 NULL): what attention reads, for the calls over dense

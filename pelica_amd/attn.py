@@ -57,6 +57,7 @@ EXPORTS = (
     "pelica_attn_paged_f32",
     "pelica_attn_paged_qkv",
     "pelica_attn_paged_qkv_q8",
+    "pelica_attn_paged_q8",
     "pelica_attn_pages_read",
     "pelica_attn_prof_enable",
     "pelica_attn_prof_read",
@@ -262,6 +263,8 @@ def load_library() -> ctypes.CDLL:
     lib.pelica_attn_paged_qkv_q8.restype = ctypes.c_int
     lib.pelica_attn_paged_qkv_q8.argtypes = [gd, ctypes.POINTER(PagedRope), q8, vp, vp, vp, ctypes.c_int64, vp, vp,
                                              ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
+    lib.pelica_attn_paged_q8.restype = ctypes.c_int
+    lib.pelica_attn_paged_q8.argtypes = [gd, q8, vp, sz, vp, ctypes.c_int32, vp, vp, vp, vp, vp, sz, vp]
     lib.pelica_attn_pages_read.restype = ctypes.c_int
     lib.pelica_attn_pages_read.argtypes = [gd, q8, vp, vp, vp, vp, vp, ctypes.c_int64, vp]
     lib.pelica_attn_prof_enable.restype = ctypes.c_int

@@ -56,6 +56,10 @@ struct PagedParams {
     // of raw products up to tanh_to[i]: the capped score (log2 domain) as s times
     // a polynomial in s^2, of f32 and of f16 queries
     float tanh_c[5], tanh_h[3], tanh_to[2];
+    // 8-bit pages: scales, bytes between pages, heads, rows of theirs
+    const uint16_t *ks, *vs;
+    int64_t spage_b, shead_b;
+    uint32_t srow_b;
     // host side only
     int hd, max_pieces, max_joins;
     bool f32, wide;
@@ -91,6 +95,7 @@ struct Q8Strides {
 };
 
 hipError_t launch_paged(const PagedParams& p, hipStream_t st);
+hipError_t launch_paged_q8(const PagedParams& p, hipStream_t st);
 hipError_t launch_paged_join(const PagedParams& p, hipStream_t st);
 
 struct PagedQkvParams {

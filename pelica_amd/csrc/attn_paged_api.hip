@@ -181,11 +181,9 @@ PagedPlan plan_of(const PelicaPagedDesc* d) {
     return x;
 }
 
-int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const void* q, const uint16_t* k, const uint16_t* v,
-              const float* sinks, void* out, void* workspace, size_t workspace_bytes, bool f32, void* stream) {
-    pelica::clear_error();
-    int rc = check_paged(d);
-    if (rc) return rc;
+// (q8: NULL for f16 pages)
+int run_paged(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* plan, size_t plan_bytes, const void* q, const void* k,
+              const void* v, const float* sinks, void* out, void* workspace, size_t workspace_bytes, bool f32, void* stream) {
     if (!plan || !q || !k || !v || !out) return fail(PELICA_ATTN_EINVAL, "plan, q, k_pages, v_pages and out must be non-NULL");
     if (misaligned(plan) || misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(workspace))
         return fail(PELICA_ATTN_EINVAL, "plan, q, k_pages, v_pages, out and workspace must be 16-byte aligned");
@@ -205,8 +203,8 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, con
     if (x.max_pieces * d->n_kv >= 1 << 24) return fail(PELICA_ATTN_EUNSUPPORTED, "more than 2^24 workgroups");
     pelica::PagedParams p{};
     p.q = q;
-    p.k = k;
-    p.v = v;
+    p.k = static_cast<const uint16_t*>(k);
+    p.v = static_cast<const uint16_t*>(v);
     const char* pl = static_cast<const char*>(plan);
     p.head = reinterpret_cast<const pelica::PlanHeader*>(pl);
     p.joins = reinterpret_cast<const pelica::PlanJoin*>(pl + x.join_at);
@@ -220,9 +218,18 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, con
     p.out = out;
     p.ws_ml = x.ws_bytes ? static_cast<float*>(workspace) : nullptr;
     p.ws_o = x.ws_bytes ? reinterpret_cast<float*>(static_cast<char*>(workspace) + x.ml_bytes) : nullptr;
-    p.page_b = page_stride(d) * 2;
-    p.head_b = head_stride(d) * 2;
-    p.row_b = (uint32_t)(row_stride(d) * 2);
+    const int size = q8 ? 1 : 2;
+    p.page_b = page_stride(d) * size;
+    p.head_b = head_stride(d) * size;
+    p.row_b = (uint32_t)(row_stride(d) * size);
+    if (q8) {
+        const pelica::Q8Strides s = scale_strides(d, q8);
+        p.ks = q8->k_scales;
+        p.vs = q8->v_scales;
+        p.spage_b = s.page * 2;
+        p.shead_b = s.head * 2;
+        p.srow_b = (uint32_t)(s.row * 2);
+    }
     p.q_tok = d->q_token_stride ? d->q_token_stride : row;
     p.o_tok = d->out_token_stride ? d->out_token_stride : row;
     p.sig = x.sig;
@@ -242,7 +249,7 @@ int run_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, con
     p.f32 = f32;
     p.wide = x.wide;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipError_t e = pelica::launch_paged(p, st);
+    hipError_t e = q8 ? pelica::launch_paged_q8(p, st) : pelica::launch_paged(p, st);
     if (e == hipSuccess && x.split) e = pelica::launch_paged_join(p, st);
     if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged attention launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;
@@ -450,13 +457,19 @@ size_t pelica_attn_paged_workspace_bytes(const PelicaPagedDesc* d) {
 int pelica_attn_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const uint16_t* q,
                       const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, uint16_t* out,
                       void* workspace, size_t workspace_bytes, void* stream) {
-    return run_paged(d, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
+    pelica::clear_error();
+    const int rc = check_paged(d);
+    if (rc) return rc;
+    return run_paged(d, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
 }
 
 int pelica_attn_paged_f32(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const float* q,
                           const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks, float* out,
                           void* workspace, size_t workspace_bytes, void* stream) {
-    return run_paged(d, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
+    pelica::clear_error();
+    const int rc = check_paged(d);
+    if (rc) return rc;
+    return run_paged(d, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
 }
 
 int pelica_attn_paged_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope, const float* q, const float* k,
@@ -479,6 +492,16 @@ int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* d, const PelicaPagedRope* ro
     if (rc) return rc;
     return run_qkv(d, rope, q8, q, k, v, token_stride, q_norm, k_norm, eps, slots, q_out, q_half, q_out_stride, k_pages,
                    v_pages, stream);
+}
+
+int pelica_attn_paged_q8(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* plan, size_t plan_bytes, const void* q,
+                         int32_t half, const int8_t* k_pages, const int8_t* v_pages, const float* sinks, void* out,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+    pelica::clear_error();
+    int rc = check_paged(d);
+    if (!rc) rc = check_q8(d, q8);
+    if (rc) return rc;
+    return run_paged(d, q8, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, half == 0, stream);
 }
 
 int pelica_attn_pages_read(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const int64_t* slots, const void* k_pages,

@@ -89,7 +89,9 @@ __device__ __forceinline__ u32x2 quantise8(const float4v& a, const float4v& b, u
         const float x = i < 4 ? a[i & 3] : b[i & 3];
         float t = __builtin_fmaf(x, inv, 12582912.f);
         const float r = __builtin_fmaf(12582912.f - t, f, x);
-        t += r > half ? 1.f : r < -half ? -1.f : 0.f;
+        // (of two as near the even one, as elsewhere: an odd n gives way at half)
+        const float most_r = __uint_as_float(__float_as_uint(half) - (__float_as_uint(t) & 1u));
+        t += r > most_r ? 1.f : r < -most_r ? -1.f : 0.f;
         n[i] = __float_as_uint(t);
     }
     auto pack = [&](int i) {

@@ -290,13 +290,14 @@ class PagedPlan:
             return torch.empty(max(self.workspace_bytes, 16), dtype=torch.uint8, device=self.device)
 
 
-def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=None, softcap: float = 0.0,
+def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_scales=None, sinks=None, alibi=None, softcap: float = 0.0,
                     scale: Optional[float] = None, out=None, workspace=None, stream=None):
     """Attention of every request's new tokens over its pages.  q: f16
     (pelica_attn_paged, probabilities rounded to f16 too) or f32
     (pelica_attn_paged_f32, products to f32's precision; values up to 65504)
     [n_tokens, n_head, hd], contiguous or token rows of a wider buffer; ``sinks`` f32 [n_head]; ``alibi`` f32 [n_head] slopes of the
-    distance bias; ``softcap`` c: scores c tanh(s / c); ``scale`` None or 0:
+    distance bias; 8-bit pages (int8) come with ``k_scales`` and ``v_scales``
+    (pelica_attn_paged_q8); ``softcap`` c: scores c tanh(s / c); ``scale`` None or 0:
     1/sqrt(hd).  Returns q's type;
     rows of requests without tokens or with lengths that do not fit, and rows
     behind the last, are left as they were (undefined in a new ``out``)."""
@@ -308,7 +309,8 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
         _check("q", q, dtype, 3, dense=False)
         _need(q.shape == shape, f"q: {shape} as planned, got {tuple(q.shape)}")
         raise AttnError(EINVAL, f"the plan is on device {dev}, q on {q.device}")
-    page, row, head, pool = _pools(k_pages, v_pages, dev)
+    q8 = _q8(k_pages, k_scales, v_scales, dev)
+    page, row, head, pool = _pools(k_pages, v_pages, dev, None if q8 is None else torch.int8)
     if pool != plan._page_shape:
         raise AttnError(EINVAL, f"k_pages: {plan._page_shape} as planned, got {tuple(k_pages.shape)}")
     if out is None:
@@ -345,9 +347,13 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, sinks=None, alibi=N
     if softcap:
         x.softcap = softcap
     lib = attn._lib
-    rc = (lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged)(
-        ctypes.byref(x), plan._buffer, plan._bytes, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws, ws_bytes, attn._stream_ptr(stream))
+    tail = (k_pages.data_ptr(), v_pages.data_ptr(), None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws,
+            ws_bytes, attn._stream_ptr(stream))
+    if q8 is not None:
+        rc = lib.pelica_attn_paged_q8(ctypes.byref(x), ctypes.byref(q8), plan._buffer, plan._bytes, q.data_ptr(), not f32, *tail)
+    else:
+        rc = (lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged)(ctypes.byref(x), plan._buffer, plan._bytes,
+                                                                           q.data_ptr(), *tail)
     if rc:
         attn._check(rc)
     return out
