@@ -483,6 +483,40 @@ int pelica_attn_pages_read(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8,
                            const void* k_pages, const void* v_pages, uint16_t* k_out, uint16_t* v_out,
                            int64_t out_stride, void* stream);
 
+/* ---- requests that share their first keys -------------------------------- */
+
+/* most groups of one step */
+#define PELICA_ATTN_PAGED_MAX_GROUPS 1024
+
+/* Group g is the requests group_start[g] .. group_start[g + 1) (which must not
+ * decrease, 0 .. n_seq): their first shared_len[g] keys lie in the same pages,
+ * the entries for them in the rows of page_table are alike.  Requests of a group of one, of a
+ * group whose shared_len is 0 or less, or of none share nothing.  The plan walks
+ * such keys once for the tokens of the whole group: a multiple of 32 of them,
+ * at most shared_len and what each request had ahead of its new tokens, through
+ * the row of page_table of the group's first request that has tokens.
+ * Every token sees what it sees without groups.  No window, prefix_len
+ * or alibi. */
+typedef struct PelicaPagedShared {
+    int32_t n_groups;            /* 1 .. PELICA_ATTN_PAGED_MAX_GROUPS, <= n_seq */
+    const int32_t* group_start;  /* device [n_groups + 1] */
+    const int32_t* shared_len;   /* device [n_groups] */
+} PelicaPagedShared;
+
+/* pelica_attn_paged_plan, _workspace_bytes and the attention itself (f16 q
+ * and out where half != 0, else f32; 8-bit pages with q8, else f16 ones) for
+ * such requests.  A plan serves calls with the same n_groups; its group_start
+ * and shared_len are read when it is made.  A group_start or q_start that decreases
+ * gives an empty plan. */
+size_t pelica_attn_paged_shared_plan_bytes(const PelicaPagedDesc* desc, const PelicaPagedShared* shared);
+int pelica_attn_paged_shared_plan(const PelicaPagedDesc* desc, const PelicaPagedShared* shared, void* plan,
+                                  size_t plan_bytes, void* stream);
+size_t pelica_attn_paged_shared_workspace_bytes(const PelicaPagedDesc* desc, const PelicaPagedShared* shared);
+int pelica_attn_paged_shared(const PelicaPagedDesc* desc, const PelicaPagedShared* shared, const PelicaPagedQ8* q8,
+                             const void* plan, size_t plan_bytes, const void* q, int32_t half, const void* k_pages,
+                             const void* v_pages, const float* sinks, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 /* ---- per-kernel GPU timing ------------------------------------------- */
 
 /* kernel ids of PelicaAttnProfRecord */

@@ -59,6 +59,10 @@ EXPORTS = (
     "pelica_attn_paged_qkv_q8",
     "pelica_attn_paged_q8",
     "pelica_attn_pages_read",
+    "pelica_attn_paged_shared_plan_bytes",
+    "pelica_attn_paged_shared_plan",
+    "pelica_attn_paged_shared_workspace_bytes",
+    "pelica_attn_paged_shared",
     "pelica_attn_prof_enable",
     "pelica_attn_prof_read",
 )
@@ -183,6 +187,12 @@ class PagedQ8(ctypes.Structure):
     ]
 
 
+class PagedShared(ctypes.Structure):
+    """``PelicaPagedShared`` (field meanings in include/pelica_attn.h)."""
+
+    _fields_ = [("n_groups", ctypes.c_int32), ("group_start", ctypes.c_void_p), ("shared_len", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -265,6 +275,14 @@ def load_library() -> ctypes.CDLL:
                                              ctypes.c_float, vp, vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
     lib.pelica_attn_paged_q8.restype = ctypes.c_int
     lib.pelica_attn_paged_q8.argtypes = [gd, q8, vp, sz, vp, ctypes.c_int32, vp, vp, vp, vp, vp, sz, vp]
+    sh = ctypes.POINTER(PagedShared)
+    for fn in (lib.pelica_attn_paged_shared_plan_bytes, lib.pelica_attn_paged_shared_workspace_bytes):
+        fn.restype = sz
+        fn.argtypes = [gd, sh]
+    lib.pelica_attn_paged_shared_plan.restype = ctypes.c_int
+    lib.pelica_attn_paged_shared_plan.argtypes = [gd, sh, vp, sz, vp]
+    lib.pelica_attn_paged_shared.restype = ctypes.c_int
+    lib.pelica_attn_paged_shared.argtypes = [gd, sh, q8, vp, sz, vp, ctypes.c_int32, vp, vp, vp, vp, vp, sz, vp]
     lib.pelica_attn_pages_read.restype = ctypes.c_int
     lib.pelica_attn_pages_read.argtypes = [gd, q8, vp, vp, vp, vp, vp, ctypes.c_int64, vp]
     lib.pelica_attn_prof_enable.restype = ctypes.c_int

@@ -12,19 +12,35 @@ namespace {
 // row each.  Bound by the partials' bytes (a mixed step's 48 MB: 12.7 us, 3.8
 // TB/s), and for single tokens by its two round trips (plan, partials) behind
 // the attention kernel: 3.9 - 4.8 us.
-template <int HD, bool F32, int WPR>
+template <int HD, bool F32, int WPR, bool SHARED>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     constexpr int LPR = HD / 4, GPW = 64 / LPR, U = 4;
     __shared__ float st[WPR > 1 ? WPR : 1][64][6];
     const int j = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
-    const PlanJoin z = p.joins[j];
+    const std::conditional_t<SHARED, SharedJoin, PlanJoin> z = [&] {
+        if constexpr (SHARED) return p.shared_joins[j];
+        else return p.joins[j];
+    }();
     const uint32_t sig = p.head->sig;
     const int n_joins = p.head->n_joins;
-    __asm__ volatile("" ::"s"(z.q0), "s"(z.slot0), "s"(sig), "s"(n_joins));
+    __asm__ volatile("" ::"s"(z.q0), "s"(z.r0), "s"(sig), "s"(n_joins));
     if (sig != p.sig || j >= n_joins) return;
+    int rows, n_slots;
+    if constexpr (SHARED) rows = z.rows, n_slots = z.k + z.g_k;
+    else rows = min(z.R - z.r0, p.rows), n_slots = z.n_slots;
+    // row r of partial sl
+    auto partial = [&](int sl, int r) -> size_t {
+        if constexpr (SHARED) {
+            if (sl < z.k) return (size_t)(z.at + sl * z.rows) * p.n_kv + (size_t)kvh * z.rows + r;
+            constexpr int W = wide_rows(HD);
+            const int gr = z.g_row + r, b = gr / W, of = min(W, z.g_R - b * W);
+            return (size_t)(z.g_at + b * W * z.g_k + (sl - z.k) * of) * p.n_kv + (size_t)kvh * of + (gr - b * W);
+        } else {
+            return ((size_t)(z.slot0 + sl) * p.n_kv + kvh) * p.rows + r;
+        }
+    };
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, d = 4 * (lane % LPR), grp = lane / LPR;
-    const int rows = min(z.R - z.r0, p.rows);
-    const bool spread = WPR > 1 || z.n_slots > 8;  // a row's slots over the lane groups
+    const bool spread = WPR > 1 || n_slots > 8;  // a row's slots over the lane groups
     const int ph = WPR > 1 ? wave * GPW + grp : spread ? grp : 0, n_ph = WPR > 1 ? GPW * WPR : spread ? GPW : 1;
     const int per_wave = spread ? 1 : GPW;  // rows
     const int step = WPR > 1 ? (int)gridDim.y : (int)gridDim.y * 4 * per_wave;
@@ -32,7 +48,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
         const int r = min(r0 + (spread ? 0 : grp), rows - 1);
         float m = -INFINITY, l = 0.f;
         float4v o = {};
-        for (int s0 = 0; s0 < z.n_slots; s0 += n_ph * U) {
+        for (int s0 = 0; s0 < n_slots; s0 += n_ph * U) {
             float2 ml[U];
             float4v v[U];
 #pragma unroll
@@ -40,8 +56,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
                 const int sl = s0 + ph + n_ph * u;
                 ml[u] = make_float2(-INFINITY, 0.f);
                 v[u] = float4v{};
-                if (sl < z.n_slots) {
-                    const size_t at = ((size_t)(z.slot0 + sl) * p.n_kv + kvh) * p.rows + r;
+                if (sl < n_slots) {
+                    const size_t at = partial(sl, r);
                     ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[at];
                     v[u] = *reinterpret_cast<const float4v*>(p.ws_o + at * HD + d);
                 }
@@ -117,8 +133,14 @@ hipError_t launch_paged_join(const PagedParams& p, hipStream_t st) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool F32 = decltype(f32)::value;
         const unsigned x = (unsigned)p.max_joins * p.n_kv;
-        if (p.wide) hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1>), dim3(x, 16), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((paged_join_kernel<HD, F32, 4>), dim3(x, std::min(p.rows, 32)), dim3(256), 0, st, p);
+        if (p.shared_joins) {
+            const unsigned y = (unsigned)std::min((p.max_rows + 3) / 4, 16);
+            hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1, true>), dim3(x, y), dim3(256), 0, st, p);
+        } else if (p.wide) {
+            hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1, false>), dim3(x, 16), dim3(256), 0, st, p);
+        } else {
+            hipLaunchKernelGGL((paged_join_kernel<HD, F32, 4, false>), dim3(x, std::min(p.rows, 32)), dim3(256), 0, st, p);
+        }
         return hipGetLastError();
     });
 }

@@ -30,10 +30,20 @@ struct PlanParams {
     int64_t max_keys;
     int max_joins, max_pieces;
     int max_slots;  // most pieces of split items
+    int rows;       // partial rows of a kv head and piece
     bool split;     // no: every item is one piece
     uint32_t sig;
 };
 hipError_t launch_paged_plan(const PlanParams& p, hipStream_t st);
+
+constexpr int kSharedMaxGroups = 1024;
+struct SharedPlanParams {
+    PlanParams plan;
+    const int32_t *group_start, *shared_len;
+    SharedJoin* joins;
+    int n_groups;
+};
+hipError_t launch_paged_shared_plan(const SharedPlanParams& p, hipStream_t st);
 
 struct PagedParams {
     const void* q;
@@ -45,9 +55,10 @@ struct PagedParams {
     const float *sinks_or_q, *alibi_or_q;  // (never NULL: a load that needs no branch)
     double inv_hpk;             // 1 / hpk
     void* out;
-    float* ws_ml;               // [slot][n_kv][rows] x (max, sum), base-2 max
-    float* ws_o;                // [slot][n_kv][rows][hd]
+    float* ws_ml;               // of a piece [n_kv][its rows] x (max, sum), base-2 max
+    float* ws_o;                // [n_kv][its rows][hd]
     const PlanJoin* joins;
+    const SharedJoin* shared_joins;  // (not NULL: a plan of shared keys)
     int64_t page_b, head_b;     // bytes between pages, between kv heads of a row
     int64_t q_tok, o_tok;       // values between tokens
     uint32_t row_b, sig;        // bytes between rows of a page
@@ -61,7 +72,7 @@ struct PagedParams {
     int64_t spage_b, shead_b;
     uint32_t srow_b;
     // host side only
-    int hd, max_pieces, max_joins;
+    int hd, max_pieces, max_joins, max_rows;  // (of a request's item)
     bool f32, wide;
 };
 // cap tanh(y), y = s scale / cap, of small y: tanh(y) / y as the polynomial in

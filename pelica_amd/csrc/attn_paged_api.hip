@@ -141,48 +141,97 @@ int check_paged(const PelicaPagedDesc* d) {
     return PELICA_ATTN_OK;
 }
 
+// Keys that requests share: what such a plan takes of the descriptor, and its groups
+int check_shared(const PelicaPagedDesc* d, const PelicaPagedShared* x) {
+    const int rc = check_paged(d);
+    if (rc) return rc;
+    if (!x) return fail(PELICA_ATTN_EINVAL, "shared is NULL");
+    if (x->n_groups <= 0 || x->n_groups > PELICA_ATTN_PAGED_MAX_GROUPS || x->n_groups > d->n_seq)
+        return fail(PELICA_ATTN_EINVAL, "n_groups %d (1 .. %d, and at most n_seq %d)", x->n_groups, PELICA_ATTN_PAGED_MAX_GROUPS, d->n_seq);
+    if (!x->group_start || !x->shared_len || misaligned(x->group_start, 4) || misaligned(x->shared_len, 4))
+        return fail(PELICA_ATTN_EINVAL, "group_start and shared_len must be non-NULL and aligned to their values");
+    if (d->window) return fail(PELICA_ATTN_EUNSUPPORTED, "shared keys and a window (such layers take a plain plan)");
+    if (d->prefix_len) return fail(PELICA_ATTN_EUNSUPPORTED, "shared keys and prefix_len");
+    if (d->alibi) return fail(PELICA_ATTN_EUNSUPPORTED, "shared keys and alibi: rows of one position each have their own bias");
+    if ((int64_t)d->n_tokens * d->n_head > 1 << 28) return fail(PELICA_ATTN_EUNSUPPORTED, "shared keys and n_tokens x n_head above 2^28");
+    return PELICA_ATTN_OK;
+}
+
 struct PagedPlan {
-    int hpk, fill, rows, max_joins;
+    int hpk, fill, rows, max_joins, max_rows;
     int64_t max_pieces;
     bool wide, split;
     size_t join_at, piece_at, bytes, ml_bytes, ws_bytes;
     uint32_t sig;
 };
 
-PagedPlan plan_of(const PelicaPagedDesc* d) {
+PagedPlan plan_of(const PelicaPagedDesc* d, const PelicaPagedShared* shared = nullptr) {
     PagedPlan x;
     x.hpk = d->n_head / d->n_kv;
-    x.wide = (int64_t)d->max_q * x.hpk > pelica::kNarrowRows;
+    // (the rows of a group are one item's)
+    x.wide = (int64_t)(shared ? d->n_tokens : d->max_q) * x.hpk > pelica::kNarrowRows;
     x.fill = pelica::plan_fill(d->n_kv, device_cus());
-    const int64_t items = x.wide ? pelica::plan_items(d->n_seq, d->n_tokens, x.hpk, d->hd)
-                                 : std::min(d->n_seq, d->n_tokens);
+    int64_t items = x.wide ? pelica::plan_items(d->n_seq, d->n_tokens, x.hpk, d->hd)
+                           : std::min(d->n_seq, d->n_tokens);
+    x.max_joins = shared ? (int)items : 0;  // (of requests; groups have none)
+    if (shared) items += x.wide ? pelica::plan_items(shared->n_groups, d->n_tokens, x.hpk, d->hd) : shared->n_groups;
     x.rows = x.wide ? pelica::wide_rows(d->hd)
-                    : std::min(pelica::kNarrowRows, d->max_q * x.hpk);
+                    : std::min(pelica::kNarrowRows, (shared ? d->n_tokens : d->max_q) * x.hpk);
+    x.max_rows = std::min((int64_t)d->max_q * x.hpk, (int64_t)x.rows);
     // a step whose items are at most two chunks a wave (window layers) is not
     // split, and has no second kernel
     const int64_t keys = (int64_t)d->max_pages * d->page_size;
     const int64_t span = d->window > 0 && !d->prefix_len ? std::min(keys, (int64_t)d->window + d->max_q - 1) : keys;
-    x.split = x.wide || span / 32 + 2 > 8;
+    x.split = shared || x.wide || span / 32 + 2 > 8;
     x.max_pieces = x.split ? pelica::plan_pieces(items, x.fill) : items;
-    x.max_joins = x.split ? (int)std::min<int64_t>(items, pelica::plan_slots(x.fill) / 2) : 0;
+    if (!shared) x.max_joins = x.split ? (int)std::min<int64_t>(items, pelica::plan_slots(x.fill) / 2) : 0;
     auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
     x.join_at = 64;
-    x.piece_at = 64 + (((size_t)x.max_joins * sizeof(pelica::PlanJoin) + 63) & ~(size_t)63);
+    x.piece_at = 64 + (((size_t)x.max_joins * (shared ? sizeof(pelica::SharedJoin) : sizeof(pelica::PlanJoin)) + 63) & ~(size_t)63);
     x.bytes = x.piece_at + (size_t)x.max_pieces * sizeof(pelica::PlanPiece);
-    const size_t slots = x.split ? (size_t)pelica::plan_slots(x.fill) * d->n_kv * x.rows : 0;
+    // (rows of partials; with shared keys each row has one of its request's and one of its group's at least)
+    const size_t slots = x.split ? ((size_t)pelica::plan_slots(x.fill) * x.rows + (shared ? 2 * (size_t)d->n_tokens * x.hpk : 0)) * d->n_kv : 0;
     x.ml_bytes = al(slots * 8);
     x.ws_bytes = x.split ? x.ml_bytes + al(slots * d->hd * 4) : 0;
     // what a plan depends on (FNV-1a)
     const int32_t parts[] = {d->n_head, d->n_kv, d->hd, d->n_seq, d->n_tokens, d->max_q, d->page_size, d->n_pages,
                              d->max_pages, d->window, d->prefix_len ? 1 : 0, x.fill};
-    x.sig = 2166136261u;
+    x.sig = 2166136261u ^ (shared ? (uint32_t)shared->n_groups : 0u);
     for (int32_t v : parts)
         for (int b = 0; b < 4; ++b) x.sig = (x.sig ^ ((uint32_t)v >> (8 * b) & 255)) * 16777619u;
     return x;
 }
 
+// The work list's parameters; 0 where the buffer will do
+int plan_params(const PelicaPagedDesc* d, const PagedPlan& x, void* plan, size_t plan_bytes, pelica::PlanParams& p) {
+    if (!plan || misaligned(plan)) return fail(PELICA_ATTN_EINVAL, "plan must be non-NULL and 16-byte aligned");
+    if (plan_bytes < x.bytes) return fail(PELICA_ATTN_EWORKSPACE, "plan of %zu bytes needed, %zu given", x.bytes, plan_bytes);
+    char* pl = static_cast<char*>(plan);
+    p.q_start = d->q_start;
+    p.kv_len = d->seq_kv_len;
+    p.prefix = d->prefix_len;
+    p.head = reinterpret_cast<pelica::PlanHeader*>(pl);
+    p.joins = reinterpret_cast<pelica::PlanJoin*>(pl + x.join_at);
+    p.pieces = reinterpret_cast<pelica::PlanPiece*>(pl + x.piece_at);
+    p.n_seq = d->n_seq;
+    p.n_tokens = d->n_tokens;
+    p.max_q = d->max_q;
+    p.hpk = x.hpk;
+    p.hd = d->hd;
+    p.window = d->window;
+    p.fill = x.fill;
+    p.max_keys = (int64_t)d->max_pages * d->page_size;
+    p.max_joins = x.max_joins;
+    p.max_pieces = (int)x.max_pieces;
+    p.sig = x.sig;
+    p.split = x.split;
+    p.max_slots = pelica::plan_slots(x.fill);
+    p.rows = x.rows;
+    return PELICA_ATTN_OK;
+}
+
 // (q8: NULL for f16 pages)
-int run_paged(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* plan, size_t plan_bytes, const void* q, const void* k,
+int run_paged(const PelicaPagedDesc* d, const PelicaPagedShared* shared, const PelicaPagedQ8* q8, const void* plan, size_t plan_bytes, const void* q, const void* k,
               const void* v, const float* sinks, void* out, void* workspace, size_t workspace_bytes, bool f32, void* stream) {
     if (!plan || !q || !k || !v || !out) return fail(PELICA_ATTN_EINVAL, "plan, q, k_pages, v_pages and out must be non-NULL");
     if (misaligned(plan) || misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(workspace))
@@ -194,7 +243,7 @@ int run_paged(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* pla
             return fail(PELICA_ATTN_EINVAL, "token stride %lld: 0, or >= n_head*hd (%lld), < 2^31 and a whole number of "
                         "16-byte pieces", (long long)st, (long long)row);
     if (misaligned(sinks, 4)) return fail(PELICA_ATTN_EINVAL, "sinks must be aligned to its values");
-    const PagedPlan x = plan_of(d);
+    const PagedPlan x = plan_of(d, shared);
     // (kernels read pieces beside the header that says whether they are theirs)
     if (plan_bytes < x.bytes) return fail(PELICA_ATTN_EWORKSPACE, "plan of %zu bytes needed, %zu given", x.bytes, plan_bytes);
     if (x.ws_bytes && (!workspace || workspace_bytes < x.ws_bytes))
@@ -208,6 +257,7 @@ int run_paged(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* pla
     const char* pl = static_cast<const char*>(plan);
     p.head = reinterpret_cast<const pelica::PlanHeader*>(pl);
     p.joins = reinterpret_cast<const pelica::PlanJoin*>(pl + x.join_at);
+    p.shared_joins = shared ? reinterpret_cast<const pelica::SharedJoin*>(pl + x.join_at) : nullptr;
     p.pieces = reinterpret_cast<const pelica::PlanPiece*>(pl + x.piece_at);
     p.table = d->page_table;
     p.sinks = sinks;
@@ -246,6 +296,7 @@ int run_paged(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const void* pla
     p.hd = d->hd;
     p.max_pieces = (int)x.max_pieces;
     p.max_joins = x.max_joins;
+    p.max_rows = x.max_rows;
     p.f32 = f32;
     p.wide = x.wide;
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -419,30 +470,9 @@ int pelica_attn_paged_plan(const PelicaPagedDesc* d, void* plan, size_t plan_byt
     pelica::clear_error();
     int rc = check_paged(d);
     if (rc) return rc;
-    const PagedPlan x = plan_of(d);
-    if (!plan || misaligned(plan)) return fail(PELICA_ATTN_EINVAL, "plan must be non-NULL and 16-byte aligned");
-    if (plan_bytes < x.bytes) return fail(PELICA_ATTN_EWORKSPACE, "plan of %zu bytes needed, %zu given", x.bytes, plan_bytes);
-    char* pl = static_cast<char*>(plan);
     pelica::PlanParams p{};
-    p.q_start = d->q_start;
-    p.kv_len = d->seq_kv_len;
-    p.prefix = d->prefix_len;
-    p.head = reinterpret_cast<pelica::PlanHeader*>(pl);
-    p.joins = reinterpret_cast<pelica::PlanJoin*>(pl + x.join_at);
-    p.pieces = reinterpret_cast<pelica::PlanPiece*>(pl + x.piece_at);
-    p.n_seq = d->n_seq;
-    p.n_tokens = d->n_tokens;
-    p.max_q = d->max_q;
-    p.hpk = x.hpk;
-    p.hd = d->hd;
-    p.window = d->window;
-    p.fill = x.fill;
-    p.max_keys = (int64_t)d->max_pages * d->page_size;
-    p.max_joins = x.max_joins;
-    p.max_pieces = (int)x.max_pieces;
-    p.sig = x.sig;
-    p.split = x.split;
-    p.max_slots = pelica::plan_slots(x.fill);
+    rc = plan_params(d, plan_of(d), plan, plan_bytes, p);
+    if (rc) return rc;
     const hipError_t e = pelica::launch_paged_plan(p, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_plan launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;
@@ -460,7 +490,7 @@ int pelica_attn_paged(const PelicaPagedDesc* d, const void* plan, size_t plan_by
     pelica::clear_error();
     const int rc = check_paged(d);
     if (rc) return rc;
-    return run_paged(d, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
+    return run_paged(d, nullptr, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, false, stream);
 }
 
 int pelica_attn_paged_f32(const PelicaPagedDesc* d, const void* plan, size_t plan_bytes, const float* q,
@@ -469,7 +499,7 @@ int pelica_attn_paged_f32(const PelicaPagedDesc* d, const void* plan, size_t pla
     pelica::clear_error();
     const int rc = check_paged(d);
     if (rc) return rc;
-    return run_paged(d, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
+    return run_paged(d, nullptr, nullptr, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, true, stream);
 }
 
 int pelica_attn_paged_qkv(const PelicaPagedDesc* d, const PelicaPagedRope* rope, const float* q, const float* k,
@@ -501,7 +531,47 @@ int pelica_attn_paged_q8(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, cons
     int rc = check_paged(d);
     if (!rc) rc = check_q8(d, q8);
     if (rc) return rc;
-    return run_paged(d, q8, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, half == 0, stream);
+    return run_paged(d, nullptr, q8, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, half == 0, stream);
+}
+
+size_t pelica_attn_paged_shared_plan_bytes(const PelicaPagedDesc* d, const PelicaPagedShared* shared) {
+    pelica::clear_error();
+    if (check_shared(d, shared)) return 0;
+    return plan_of(d, shared).bytes;
+}
+
+int pelica_attn_paged_shared_plan(const PelicaPagedDesc* d, const PelicaPagedShared* shared, void* plan, size_t plan_bytes,
+                                  void* stream) {
+    pelica::clear_error();
+    int rc = check_shared(d, shared);
+    if (rc) return rc;
+    const PagedPlan x = plan_of(d, shared);
+    pelica::SharedPlanParams p{};
+    rc = plan_params(d, x, plan, plan_bytes, p.plan);
+    if (rc) return rc;
+    p.group_start = shared->group_start;
+    p.shared_len = shared->shared_len;
+    p.joins = reinterpret_cast<pelica::SharedJoin*>(static_cast<char*>(plan) + x.join_at);
+    p.n_groups = shared->n_groups;
+    const hipError_t e = pelica::launch_paged_shared_plan(p, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_shared_plan launch: %s", hipGetErrorString(e));
+    return PELICA_ATTN_OK;
+}
+
+size_t pelica_attn_paged_shared_workspace_bytes(const PelicaPagedDesc* d, const PelicaPagedShared* shared) {
+    pelica::clear_error();
+    if (check_shared(d, shared)) return 0;
+    return plan_of(d, shared).ws_bytes;
+}
+
+int pelica_attn_paged_shared(const PelicaPagedDesc* d, const PelicaPagedShared* shared, const PelicaPagedQ8* q8, const void* plan,
+                             size_t plan_bytes, const void* q, int32_t half, const void* k_pages, const void* v_pages,
+                             const float* sinks, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    pelica::clear_error();
+    int rc = check_shared(d, shared);
+    if (!rc && q8) rc = check_q8(d, q8);
+    if (rc) return rc;
+    return run_paged(d, shared, q8, plan, plan_bytes, q, k_pages, v_pages, sinks, out, workspace, workspace_bytes, half == 0, stream);
 }
 
 int pelica_attn_pages_read(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, const int64_t* slots, const void* k_pages,

@@ -433,6 +433,11 @@ __device__ __forceinline__ float row_weight(float sink, float M, float L) {
 }
 __device__ __forceinline__ float sink_of(const PagedParams& p, int h) { return p.sinks ? p.sinks[h] * kLog2e : -INFINITY; }
 
+// Row rl of a piece's partials
+__device__ __forceinline__ size_t partial_row(const PagedParams& p, const PlanPiece& z, int kvh, int rl) {
+    return (size_t)z.slot * p.n_kv + (size_t)kvh * z.rows + rl;
+}
+
 // Where row rl of the piece's item goes: its output, or the partial sums of a
 // split item's piece
 template <int HD, bool F32>
@@ -442,7 +447,7 @@ struct RowOut {
     __device__ __forceinline__ RowOut(const PagedParams& p, const PlanPiece& z, int kvh, int rl) {
         part = z.slot >= 0;
         const int r = z.r0 + rl, t = token_of(p, r), h = kvh * p.hpk + r - t * p.hpk;
-        at = part ? reinterpret_cast<char*>(p.ws_o + ((size_t)(z.slot * p.n_kv + kvh) * p.rows + rl) * HD)
+        at = part ? reinterpret_cast<char*>(p.ws_o + partial_row(p, z, kvh, rl) * HD)
                   : static_cast<char*>(p.out) + ((size_t)(z.q0 + t) * p.o_tok + (size_t)h * HD) * (F32 ? 4 : 2);
     }
     // 4 dims from d on
@@ -453,7 +458,7 @@ struct RowOut {
     }
 };
 __device__ __forceinline__ void store_sum(const PagedParams& p, const PlanPiece& z, int kvh, int rl, float M, float L) {
-    reinterpret_cast<float2*>(p.ws_ml)[(size_t)(z.slot * p.n_kv + kvh) * p.rows + rl] = make_float2(M, L);
+    reinterpret_cast<float2*>(p.ws_ml)[partial_row(p, z, kvh, rl)] = make_float2(M, L);
 }
 
 // The polynomial; times s, the capped score of a raw product up to tanh_to
@@ -1547,7 +1552,7 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int n_pieces = p.head->n_pieces;
     // (and what the end reads of the arguments: a line's first touch is a round trip)
     __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces), "s"(p.out), "s"(p.o_tok),
-                     "s"(p.rows));
+                     "s"(z.rows));
     if (sig != p.sig || id >= n_pieces) return;
     if constexpr (WIDE) {
         if (z.R > kNarrowRows) {

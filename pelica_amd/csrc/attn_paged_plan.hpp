@@ -135,12 +135,22 @@ struct PlanHeader {
 struct PlanPiece {
     int seq, q0, R, r0;        // request, its first row of q, its query rows, the item's first
     int pos0, len, cb, ce;     // position of its first token, its keys; chunks [cb, ce)
-    int slot, n_pre, lo_base;  // partial slot, or -1: the item's only piece
-    int lo, kend, pe, pad[2];
+    int slot, n_pre, lo_base;  // first partial row of kv head 0 / n_kv, or -1: the output is written
+    int lo, kend, pe;
+    int rows, pad;             // partial rows of a kv head
 };
 struct PlanJoin {
     int q0, R, r0, slot0, n_slots, pad[3];
 };
+// Where requests share their first keys: of an item of a request with
+// partials.  Its `k` pieces' rows lie at `at` on, each `rows`; its group's
+// first R rows are cut into blocks of wide_rows, each block's k pieces after one another.
+struct SharedJoin {
+    int q0, r0, rows, at, k;      // the request's first row of q, the item's first row, its rows, pieces
+    int g_at, g_k, g_row, g_R;    // the group's partials, pieces (0: none), the item's first row in it, its rows
+    int pad[3];
+};
+static_assert(sizeof(SharedJoin) == 48, "plan layout");
 static_assert(sizeof(PlanHeader) == 64 && sizeof(PlanPiece) == 64 && sizeof(PlanJoin) == 32, "plan layout");
 
 }  // namespace pelica

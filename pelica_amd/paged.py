@@ -24,7 +24,7 @@ import ctypes
 from typing import Optional, Sequence
 
 from . import attn
-from .attn import EINVAL, AttnError, PagedDesc, PagedQ8, PagedRope, PageDesc
+from .attn import EINVAL, AttnError, PagedDesc, PagedQ8, PagedRope, PagedShared, PageDesc
 
 __all__ = ["PagedPlan", "PageStep", "new_q8_pages", "paged_attention", "paged_qkv", "pages_append", "pages_read",
            "pages_release", "pair_axes"]
@@ -240,10 +240,19 @@ class PagedPlan:
     [n_seq, max_pages] and ``prefix_len`` [n_seq] or None (int32): ``update``
     makes it again when these have new contents.  Layers that differ in
     ``window`` need a plan each.  ``n_tokens``: rows of q; ``max_q``: most new
-    tokens of one request."""
+    tokens of one request.
+
+    ``group_start`` [n_groups + 1] and ``shared_len`` [n_groups] (int32,
+    together): requests ``group_start[g]`` .. ``group_start[g + 1]`` share their
+    first ``shared_len[g]`` keys, which lie in the same pages (PelicaPagedShared):
+    the plan walks those once for the whole group (no ``window``, ``prefix_len``
+    or alibi)."""
+
+    _shared = None
 
     def __init__(self, q_start, seq_kv_len, page_table, *, n_head: int, n_kv: int, hd: int, page_size: int,
-                 n_pages: int, n_tokens: int, max_q: int, window: int = 0, prefix_len=None, stream=None):
+                 n_pages: int, n_tokens: int, max_q: int, window: int = 0, prefix_len=None, group_start=None, shared_len=None,
+                 stream=None):
         import torch
 
         n_seq = page_table.shape[0]
@@ -257,8 +266,17 @@ class PagedPlan:
         self.desc = PagedDesc(n_head, n_kv, hd, n_seq, n_tokens, max_q, page_size, n_pages, page_table.shape[1],
                               window, q_start.data_ptr(), seq_kv_len.data_ptr(), page_table.data_ptr(),
                               attn._ptr(prefix_len))
+        if group_start is not None or shared_len is not None:
+            _need(group_start is not None and shared_len is not None, "group_start and shared_len come together")
+            _check("group_start", group_start, torch.int32, 1)
+            _check("shared_len", shared_len, torch.int32, 1)
+            _need(group_start.numel() == shared_len.numel() + 1,
+                  f"group_start: {shared_len.numel() + 1} values for {shared_len.numel()} groups, got {group_start.numel()}")
+            self._keep += (group_start, shared_len)
+            self._shared = PagedShared(shared_len.numel(), group_start.data_ptr(), shared_len.data_ptr())
         lib = attn.load_library()
-        n = lib.pelica_attn_paged_plan_bytes(ctypes.byref(self.desc))
+        args = (ctypes.byref(self.desc),) if self._shared is None else (ctypes.byref(self.desc), ctypes.byref(self._shared))
+        n = (lib.pelica_attn_paged_plan_bytes if self._shared is None else lib.pelica_attn_paged_shared_plan_bytes)(*args)
         if n == 0:
             raise AttnError(EINVAL, lib.pelica_attn_last_error().decode(errors="replace"))
         self.device = page_table.device
@@ -268,15 +286,20 @@ class PagedPlan:
         with _on(stream):
             self.buffer = torch.empty(n, dtype=torch.uint8, device=self.device)
         self._buffer, self._bytes = self.buffer.data_ptr(), n
-        self.workspace_bytes = lib.pelica_attn_paged_workspace_bytes(ctypes.byref(self.desc))
+        self.workspace_bytes = (lib.pelica_attn_paged_workspace_bytes if self._shared is None
+                                else lib.pelica_attn_paged_shared_workspace_bytes)(*args)
         self.update(stream)
 
     def update(self, stream=None) -> "PagedPlan":
         """Make the work list from the arrays' present contents."""
         if _device() != self._dev:
             raise AttnError(EINVAL, f"the plan is on device {self._dev}, the current device is {_device()}")
-        rc = (attn._lib or attn.load_library()).pelica_attn_paged_plan(
-            ctypes.byref(self.desc), self._buffer, self._bytes, attn._stream_ptr(stream))
+        lib = attn._lib or attn.load_library()
+        tail = (self._buffer, self._bytes, attn._stream_ptr(stream))
+        if self._shared is None:
+            rc = lib.pelica_attn_paged_plan(ctypes.byref(self.desc), *tail)
+        else:
+            rc = lib.pelica_attn_paged_shared_plan(ctypes.byref(self.desc), ctypes.byref(self._shared), *tail)
         if rc:
             attn._check(rc)
         return self
@@ -349,7 +372,10 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_sc
     lib = attn._lib
     tail = (k_pages.data_ptr(), v_pages.data_ptr(), None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws,
             ws_bytes, attn._stream_ptr(stream))
-    if q8 is not None:
+    if plan._shared is not None:
+        rc = lib.pelica_attn_paged_shared(ctypes.byref(x), ctypes.byref(plan._shared), None if q8 is None else ctypes.byref(q8),
+                                          plan._buffer, plan._bytes, q.data_ptr(), not f32, *tail)
+    elif q8 is not None:
         rc = lib.pelica_attn_paged_q8(ctypes.byref(x), ctypes.byref(q8), plan._buffer, plan._bytes, q.data_ptr(), not f32, *tail)
     else:
         rc = (lib.pelica_attn_paged_f32 if f32 else lib.pelica_attn_paged)(ctypes.byref(x), plan._buffer, plan._bytes,
