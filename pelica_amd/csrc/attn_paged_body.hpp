@@ -145,8 +145,9 @@ __device__ __forceinline__ half8 v_operand(const char* vt, int key, int dt, int 
 // workgroup may clean a chunk at once: each has written zeros over what it
 // found before it reads the chunk.  Such rows are the keys of the item's later
 // tokens, and keys between a prefix and a window that share a run with both.
+template <int RUN = 8>
 __device__ __forceinline__ bool may_hide(const PlanPiece& z, int hi_all, int pos_last) {
-    return pos_last > hi_all || gap_in_run(z.lo, z.pe);
+    return pos_last > hi_all || gap_in_run<RUN>(z.lo, z.pe);
 }
 __device__ __forceinline__ bool is_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; }
 
@@ -272,7 +273,7 @@ struct Q8Rows {
     uint32_t dlane, slane;    // bytes from a run's first row and scale
     uint32_t kto, vto;        // bytes from a run's place in an even run's tile
 
-    struct Run {
+    struct Run {             // 8 rows, or 16 of a page that holds them
         uint64_t off, soff;  // bytes to the run's first row and scales
         int first, count;    // the rows wanted
     };
@@ -295,10 +296,11 @@ struct Q8Rows {
         vto = (uint32_t)v_slot<HD>(row, PARTS * part);
     }
     __device__ __forceinline__ int entry(int key) const { return table_entry(table, imin(key, last) >> p.page_log2); }
-    // keys key .. key + 7; none are wanted unless `any`
+    // N keys from key on; none are wanted unless `any`
+    template <int N = 8>
     __device__ __forceinline__ Run run(int key, bool any, int id) {
         int first, count;
-        group_rows(key, 8, z.lo, z.kend, z.pe, first, count);
+        group_rows(key, N, z.lo, z.kend, z.pe, first, count);
         count = any ? count : 0;
         bad |= count > 0 ? (unsigned)id >= (unsigned)p.n_pages : 0;
         const unsigned page = min((unsigned)id, (unsigned)p.n_pages - 1u);
@@ -317,22 +319,38 @@ struct Q8Rows {
         return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0,
                                                  __builtin_amdgcn_readfirstlane(bytes), kBufFlags);
     }
+    // from the first row wanted on: a lane ahead of it is past the end, too
     template <bool V>
-    __device__ __forceinline__ Regs fetch(const Run& r) const {
-        // (from the first row wanted on: a lane ahead of it is past the end, too)
-        const uint32_t skip = (uint32_t)r.first * p.row_b, sskip = (uint32_t)r.first * p.srow_b;
-        const __amdgpu_buffer_rsrc_t d = resource((V ? v : k) + r.off + skip, (uint32_t)r.count * p.row_b);
-        const __amdgpu_buffer_rsrc_t s = resource((V ? vs : ks) + r.soff + sskip, (uint32_t)r.count * p.srow_b);
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t data(const Run& r) const {
+        return resource((V ? v : k) + r.off + (uint32_t)r.first * p.row_b, (uint32_t)r.count * p.row_b);
+    }
+    template <bool V>
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t scales(const Run& r) const {
+        return resource((V ? vs : ks) + r.soff + (uint32_t)r.first * p.srow_b, (uint32_t)r.count * p.srow_b);
+    }
+    // the run's rows 8 half .. + 7
+    __device__ __forceinline__ Regs load(__amdgpu_buffer_rsrc_t d, __amdgpu_buffer_rsrc_t s, const Run& r, int half) const {
+        const uint32_t at = dlane + (uint32_t)(8 * half - r.first) * p.row_b, sat = slane + (uint32_t)(8 * half - r.first) * p.srow_b;
         Regs x;
         if constexpr (WORDS == 4) {
-            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, dlane - skip, 0, 0));
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, at, 0, 0));
             x.w[0] = w[0], x.w[1] = w[1], x.w[2] = w[2], x.w[3] = w[3];
         } else {
-            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(d, dlane - skip, 0, 0));
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(d, at, 0, 0));
             x.w[0] = w[0], x.w[1] = w[1];
         }
-        x.s = __builtin_amdgcn_raw_buffer_load_b16(s, slane - sskip, 0, 0);
+        x.s = __builtin_amdgcn_raw_buffer_load_b16(s, sat, 0, 0);
         return x;
+    }
+    template <bool V>
+    __device__ __forceinline__ Regs fetch(const Run& r) const {
+        return load(data<V>(r), scales<V>(r), r, 0);
+    }
+    template <bool V>
+    __device__ __forceinline__ void fetch16(const Run& r, Regs (&x)[2]) const {
+        const __amdgpu_buffer_rsrc_t d = data<V>(r), s = scales<V>(r);
+        x[0] = load(d, s, r, 0);
+        x[1] = load(d, s, r, 1);
     }
     // part i of a lane's values, run `run` of the tile
     template <bool V>
@@ -967,15 +985,23 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     typename Q8Rows<HD>::Regs regs[2][NR];  // of the tile after
     auto load_tile = [&](int t, const int (&id)[NR]) {
         typename Rows::Run run[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) run[r] = rows.run(run_key(t, r), z.cb + 2 * t + (wave >> 1) < z.ce, id[r]);
+        const bool any = z.cb + 2 * t + (wave >> 1) < z.ce;
         if constexpr (Q8) {
+            if (p.page_log2 >= 4) {
+                run[0] = rows.template run<16>(run_key(t, 0), any, id[0]);
+                rows.template fetch16<false>(run[0], regs[0]);
+                rows.template fetch16<true>(run[0], regs[1]);
+            } else {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                regs[0][r] = rows.template fetch<false>(run[r]);
-                regs[1][r] = rows.template fetch<true>(run[r]);
+                for (int r = 0; r < NR; ++r) {
+                    run[r] = rows.run(run_key(t, r), any, id[r]);
+                    regs[0][r] = rows.template fetch<false>(run[r]);
+                    regs[1][r] = rows.template fetch<true>(run[r]);
+                }
             }
         } else {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) run[r] = rows.run(run_key(t, r), any, id[r]);
             const uint32_t at = to + (t & 1) * TILE;
 #pragma unroll
             for (int x = 0; x < S::WI; ++x) {
@@ -1034,7 +1060,7 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
     const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
-    const bool hide = may_hide(z, hi_all, pos_last);
+    const bool hide = may_hide<Q8 ? 16 : 8>(z, hi_all, pos_last);
 
     float m[RT], l[RT];
     float16v o[DT][RT];
@@ -1216,24 +1242,56 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     };
     auto wanted = [&](int t) { return 2 * t + (wave >> 1) < n; };
     // the first tiles, then the queries beside them
-    int id[NR];                            // table entries of the next K tile to request
+    int id[NR], vid[NR];                   // table entries of the next K tile to request (8-bit rows: and V tile)
     typename Rows::Run rk[NR], rv[NR];     // runs of the K tile and the V tile to request
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-        rk[r] = rows.run(run_key(0, r), wanted(0), rows.entry(run_key(0, r)));
-        rv[r] = rows.run(run_key(1, r), wanted(1), rows.entry(run_key(1, r)));
+        vid[r] = rows.entry(run_key(1, r));
+        if constexpr (!Q8) {
+            rk[r] = rows.run(run_key(0, r), wanted(0), rows.entry(run_key(0, r)));
+            rv[r] = rows.run(run_key(1, r), wanted(1), vid[r]);
+        }
     }
-    // 8-bit rows wait in registers: V tile 0 and K tile 1, written in step 0
+    // 8-bit rows wait in registers: V tile 0 and K tile 1, written in step 0.
+    // rk[0]: the 16 rows of the last K tile requested, which are the next V
+    // tile's; pages of 8 rows take two runs, made again.
     typename Q8Rows<HD>::Regs kr[NR], vr[NR];
+    const bool pages16 = p.page_log2 >= 4;
+    auto load_k8 = [&](int t, const int (&ids)[NR]) {
+        if constexpr (Q8) {
+            int key = run_key(t, 0);
+            // (a run is made here and now: made ahead, it would take the scalar registers of all else)
+            __asm__ volatile("" : "+s"(key));
+            if (pages16) {
+                rk[0] = rows.template run<16>(key, wanted(t), ids[0]);
+                rows.template fetch16<false>(rk[0], kr);
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) kr[r] = rows.template fetch<false>(rows.run(key + 8 * r, wanted(t), ids[r]));
+            }
+        }
+    };
+    auto load_v8 = [&](int t, const int (&ids)[NR]) {
+        if constexpr (Q8) {
+            int key = run_key(t, 0);
+            __asm__ volatile("" : "+s"(key));
+            if (pages16) {
+                rows.template fetch16<true>(rk[0], vr);
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) vr[r] = rows.template fetch<true>(rows.run(key + 8 * r, wanted(t), ids[r]));
+            }
+        }
+    };
     if constexpr (Q8) {
+        int first[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) kr[r] = rows.template fetch<false>(rk[r]);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) vr[r] = rows.template fetch<true>(rk[r]);
+        for (int r = 0; r < NR; ++r) first[r] = rows.entry(run_key(0, r));
+        load_k8(0, first);
+        load_v8(0, first);
 #pragma unroll
         for (int r = 0; r < NR; ++r) rows.template put<false>(kr[r], kbuf + 16 * HD * 2 * wave, r);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) kr[r] = rows.template fetch<false>(rv[r]);
+        load_k8(1, vid);
     } else {
 #pragma unroll
         for (int x = 0; x < WI; ++x) rows.template load<false>(rk[x / IPR], (x / IPR) & 1, x % IPR, to_k + 1024 * x);
@@ -1275,7 +1333,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     const int r_last = min(z.R, z.r0 + kNW * RT * 32) - 1;
     const int hi_all = z.pos0 + token_of(p, z.r0), pos_last = z.pos0 + token_of(p, r_last);
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
-    const bool hide = may_hide(z, hi_all, pos_last);
+    const bool hide = may_hide<Q8 ? 16 : 8>(z, hi_all, pos_last);
 
     // a chunk that not every row sees whole; its V rows may hold infinities or
     // NaN that some rows do not see (see clean_chunk)
@@ -1306,13 +1364,14 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
             for (int r = 0; r < NR; ++r) id[r] = rows.entry(run_key(t + 2, r));
         } else {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) rk[r] = rows.run(run_key(t + 2, r), wanted(t + 2), id[r]);
+            for (int r = 0; r < NR; ++r)
+                if constexpr (!Q8) rk[r] = rows.run(run_key(t + 2, r), wanted(t + 2), id[r]);
         }
         auto load_nth = [&](auto x_) {
             constexpr int x = decltype(x_)::value;
             if constexpr (Q8) {
-                if constexpr (x < NR) kr[x] = rows.template fetch<false>(rk[x]);
-                else vr[x - NR] = rows.template fetch<true>(rv[x - NR]);
+                if constexpr (x == 0) load_v8(t + 1, vid);  // (ahead of K's, whose run it takes)
+                else load_k8(t + 2, id);
             } else if constexpr (x < WI)  // K tile t + 2
                 rows.template load<false>(rk[x / IPR], (x / IPR) & 1, x % IPR, to_k + ((PAR >> 1) & 1) * TILE + 1024 * x);
             else  // V tile t + 1
@@ -1371,7 +1430,7 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         // slot (an MFMA) each, NS / NM scores a slot.
         constexpr int NS = 16 * RT, NP = NS / 2, S = NS / NM;
         static_assert(NS % NM == 0, "whole scores a slot");
-        constexpr int NLD = (PAR & 1) ? 2 * (Q8 ? NR : WI) : 0;
+        constexpr int NLD = (PAR & 1) ? 2 * (Q8 ? 1 : WI) : 0;
         constexpr int LSL = HD == 128 ? NM : NM / 2;  // slots the loads go out in
         float acc[RT][2], e[NS], ahead[RT];
 #pragma unroll
@@ -1470,7 +1529,10 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
         for (int rt = 0; rt < RT; ++rt) l[rt] += ls[rt];
         if constexpr (PAR & 1) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) rv[r] = rk[r];
+            for (int r = 0; r < NR; ++r) {
+                if constexpr (Q8) vid[r] = id[r];
+                else rv[r] = rk[r];
+            }
         } else {
             if (!Q8) wait_loads<0>();
             __syncthreads();

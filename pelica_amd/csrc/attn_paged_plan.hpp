@@ -102,9 +102,10 @@ PELICA_HD void group_rows(int kg, int n, int lo, int kend, int pe, int& first, i
     const int end = b1 > b0 ? imax(a, b1) : a;
     count = imax(end - first, 0);
 }
-// Whether a run of 8 rows holds keys [pe, lo) between a prefix and a window,
-// which no row of the item sees, beside keys of both
-PELICA_HD bool gap_in_run(int lo, int pe) { return pe > 0 && pe < lo && (pe - 1) >> 3 == lo >> 3; }
+// Whether a run of 8 (or 16) rows holds keys [pe, lo) between a prefix and a
+// window, which no row of the item sees, beside keys of both
+template <int RUN = 8>
+PELICA_HD bool gap_in_run(int lo, int pe) { return pe > 0 && pe < lo && (pe - 1) / RUN == lo / RUN; }
 
 // Pieces of an item of `cost` where a piece's may be 1 / inv_limit
 PELICA_HD int item_pieces(int cost, int n_chunks, float inv_limit) {
