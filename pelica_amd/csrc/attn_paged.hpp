@@ -41,7 +41,7 @@ struct SharedPlanParams {
     PlanParams plan;
     const int32_t *group_start, *shared_len;
     SharedJoin* joins;
-    int n_groups;
+    int n_groups, wide_cost;
 };
 hipError_t launch_paged_shared_plan(const SharedPlanParams& p, hipStream_t st);
 

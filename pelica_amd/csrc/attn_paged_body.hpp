@@ -578,49 +578,72 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             for (int r = 1; r < NR; ++r) id[r] = rows.entry(kb + 8 * r);
         }
     };
-    // (8-bit rows, whose resources leave no scalar registers: a lane's run, by
-    // vector loads behind K's, taken apart when the tile is requested)
-    int entries = 0;
-    auto fetch_lanes = [&](int t) {
-        const int key = chunk_key(tile_chunk(t), z.n_pre, z.lo_base) + 8 * (lane & 3);
-        entries = rows.table[imin(key, rows.last) >> p.page_log2];
-    };
-    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR], bool any = true) {
-        const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
-        const bool whole = paged_by_32 & (kb >= z.lo) & (kb + 32 <= z.kend);
-        const uint32_t run_b = 8u * p.row_b;
-        run[0] = rows.run(kb, any, id[0]);
-        if (!whole) {
-            unrolled<NR - 1>([&](auto i) {
-                constexpr int r = decltype(i)::value + 1;
-                run[r] = rows.run(kb + 8 * r, any, paged_by_32 ? id[0] : id[r]);
-            });
-        } else {
-            unrolled<NR - 1>([&](auto i) {
-                constexpr int r = decltype(i)::value + 1;
-                run[r].off = run[0].off + (uint32_t)r * run_b;
-                if constexpr (Q8) {
-                    run[r].soff = run[0].soff + (uint32_t)r * 8u * p.srow_b;
-                    run[r].first = 0;
-                    run[r].count = run[0].count;
-                } else {
+    auto place = [&](int t, const int (&id)[NR], typename Rows::Run (&run)[NR]) {
+        if constexpr (Q8) return;
+        else {
+            const int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+            const bool whole = paged_by_32 & (kb >= z.lo) & (kb + 32 <= z.kend);
+            const uint32_t run_b = 8u * p.row_b;
+            run[0] = rows.run(kb, true, id[0]);
+            if (!whole) {
+                unrolled<NR - 1>([&](auto i) {
+                    constexpr int r = decltype(i)::value + 1;
+                    run[r] = rows.run(kb + 8 * r, true, paged_by_32 ? id[0] : id[r]);
+                });
+            } else {
+                unrolled<NR - 1>([&](auto i) {
+                    constexpr int r = decltype(i)::value + 1;
+                    run[r].off = run[0].off + (uint32_t)r * run_b;
                     run[r].nrec = run_b;
                     run[r].skip = 0;
-                }
-            });
+                });
+            }
         }
     };
-    typename Q8Rows<HD>::Regs regs[Q8 ? 2 : 1][NR];  // of the next chunk: K's, V's
     auto load_tile = [&](int t, const typename Rows::Run (&run)[NR], auto is_v) {
         constexpr bool V = decltype(is_v)::value;
+        if constexpr (Q8) return;
+        else
+#pragma unroll
+        for (int x = 0; x < WI; ++x)
+            rows.template load<V>(run[x / Rows::IPR], (x / Rows::IPR) & 1, x % Rows::IPR,
+                                  to + ((V ? NB : 0) + t % NB) * TILE + 1024 * x);
+    };
+    using K_ = std::false_type;
+    using V_ = std::true_type;
+    const int n_tiles = (z.ce - z.cb - wave + kNW - 1) / kNW;
+    // 8-bit rows: the next chunk's in registers, K's and V's, in runs as long as a page
+    // allows; lane r's table entry is run r's, of the chunk after
+    typename Q8Rows<HD>::Regs regs[Q8 ? 2 : 1][NR];
+    typename Q8Rows<HD>::Run run32;
+    auto entries_of = [&](int t) {
+        const int key = chunk_key(tile_chunk(t), z.n_pre, z.lo_base) + 8 * (lane & 3);
+        return rows.table[imin(key, rows.last) >> p.page_log2];
+    };
+    auto request = [&](auto is_v, int t, bool any, int entries) {
+        constexpr bool V = decltype(is_v)::value;
         if constexpr (Q8) {
+            int kb = chunk_key(tile_chunk(t), z.n_pre, z.lo_base);
+            auto of_runs = [&](auto len) {
+                constexpr int N = decltype(len)::value;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) regs[V][r] = rows.template fetch<V>(run[r]);
-        } else {
+                for (int x = 0; x < 32 / N; ++x) {
+                    typename Rows::Run r;
+                    if (V && N == 32) {
+                        r = run32;  // (K's; several are made again, for want of scalar registers)
+                    } else {
+                        __asm__ volatile("" : "+s"(kb));
+                        r = rows.template run<N>(kb + N * x, any, __builtin_amdgcn_readlane(entries, x * (N / 8)));
+                    }
+                    if (N == 32) run32 = r;
+                    const auto d = rows.template data<V>(r), sc = rows.template scales<V>(r);
 #pragma unroll
-            for (int x = 0; x < WI; ++x)
-                rows.template load<V>(run[x / Rows::IPR], (x / Rows::IPR) & 1, x % Rows::IPR,
-                                      to + ((V ? NB : 0) + t % NB) * TILE + 1024 * x);
+                    for (int y = 0; y < N / 8; ++y) regs[V][x * (N / 8) + y] = rows.load(d, sc, r, y);
+                }
+            };
+            if (p.page_log2 >= 5) of_runs(std::integral_constant<int, 32>{});
+            else if (p.page_log2 == 4) of_runs(std::integral_constant<int, 16>{});
+            else of_runs(std::integral_constant<int, 8>{});
         }
     };
     auto put_tile = [&](char* tile, auto is_v) {
@@ -630,25 +653,29 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             for (int r = 0; r < NR; ++r) rows.template put<V>(regs[V][r], tile, r);
         }
     };
-    using K_ = std::false_type;
-    using V_ = std::true_type;
-    const int n_tiles = (z.ce - z.cb - wave + kNW - 1) / kNW;
     // the first tiles are requested ahead of the queries, whose use waits for
     // all that was requested before it
     int id[NB + 1][NR];
     typename Rows::Run run[NR];
+    int entries = 0, next_entries = 0;  // of the chunk requested last, of the one after
     if constexpr (Q8) {
-        fetch_lanes(NB);
-        __asm__ volatile("" ::: "memory");  // (ahead of V's: those are not waited for with it)
-    }
+        entries = entries_of(0);
+        next_entries = entries_of(1);
+        __asm__ volatile("" : "+v"(entries), "+v"(next_entries)::"memory");  // (ahead of the tiles: not waited for with them)
+        if (n_tiles > 0) {
+            request(K_{}, 0, true, entries);
+            request(V_{}, 0, true, entries);
+        }
+    } else {
 #pragma unroll
-    for (int t = 0; t <= (Q8 ? NB - 1 : NB); ++t) fetch(t, id[t]);
+        for (int t = 0; t <= NB; ++t) fetch(t, id[t]);
 #pragma unroll
-    for (int t = 0; t < NB; ++t) {
-        if (t < n_tiles) {
-            place(t, id[t], run);
-            load_tile(t, run, K_{});
-            load_tile(t, run, V_{});
+        for (int t = 0; t < NB; ++t) {
+            if (t < n_tiles) {
+                place(t, id[t], run);
+                load_tile(t, run, K_{});
+                load_tile(t, run, V_{});
+            }
         }
     }
     // queries: column c16 of each tile, dims 8 g .. of every 32
@@ -692,7 +719,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     // every row sees the keys [lo_all, hi_all] and those below z.pe
     const int hi_all = z.pos0, pos_last = z.len - 1;
     const int lo_all = p.window > 0 && pos_last >= p.window ? pos_last - p.window + 1 : 0;
-    const bool hide = may_hide(z, hi_all, pos_last);
+    const bool hide = may_hide<Q8 ? 32 : 8>(z, hi_all, pos_last);
 
     float m[NT], l[NT];
     float4v o[DT][NT];
@@ -718,14 +745,12 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         char* const vt = vbuf + (t % NB) * TILE;
         const int left = n_tiles - 1 - t;
         if constexpr (Q8) {
-            // (8-bit rows: behind the last chunk's the loads fetch nothing; skipped,
-            // the compiler would wait for V's with K's)
+            // (behind the last chunk's the loads fetch nothing; skipped, the
+            // compiler would wait for V's with K's)
             put_tile(kbuf, K_{});
-#pragma unroll
-            for (int r = 0; r < NR; ++r) id[NB][r] = __builtin_amdgcn_readlane(entries, r);
-            place(t + NB, id[NB], run, left >= NB);
-            load_tile(t + NB, run, K_{});
-            fetch_lanes(t + NB + 1);
+            entries = next_entries;
+            request(K_{}, t + 1, left >= 1, entries);
+            next_entries = entries_of(t + 2);
         } else if (left >= NB - 1) {
             wait_loads<AHEAD>();
         } else {
@@ -760,12 +785,13 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
                     s[nt][i] = x;
                 }
         }
-        if (!Q8 && left >= NB) {
-            lds_done();
-            place(t + NB, id[NB], run);
-            fetch(t + NB + 1, id[NB]);
-            load_tile(t + NB, run, K_{});
-        }
+        if constexpr (!Q8)
+            if (left >= NB) {
+                lds_done();
+                place(t + NB, id[NB], run);
+                fetch(t + NB + 1, id[NB]);
+                load_tile(t + NB, run, K_{});
+            }
 
         auto key = [&](int i) { return kb + 16 * (i / 4) + 4 * g + i % 4; };
         const bool all = kb + 31 < z.pe || (kb >= lo_all && kb + 31 <= hi_all);
@@ -807,7 +833,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         }
         if constexpr (Q8) {
             put_tile(vbuf, V_{});
-            load_tile(t + NB, run, V_{});
+            request(V_{}, t + 1, left >= 1, entries);
         } else if (left >= NB) {
             wait_loads<AHEAD>();
         } else if (left == NB - 1) {
@@ -829,10 +855,11 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
                 if constexpr (F32 && !PACK) o[dt][nt] = mfma16(va, pl[nt], o[dt][nt]);
             }
         }
-        if (!Q8 && left >= NB) {
-            lds_done();
-            load_tile(t + NB, run, V_{});
-        }
+        if constexpr (!Q8)
+            if (left >= NB) {
+                lds_done();
+                load_tile(t + NB, run, V_{});
+            }
     }
     if (__builtin_expect(special, 0))
 #pragma unroll 1

@@ -33,11 +33,11 @@ constexpr int kWideCost = 3;
 constexpr int kMinPiece = 4;
 struct PlanCost {
     // a piece's own time, and what it takes of the whole chip's
-    static PELICA_HD float piece(bool wide, int chunks) {
-        return (float)(wide ? kWideCost * chunks + 10 : ((chunks + 3) & ~3) + 10);  // (four waves share a narrow one's)
+    static PELICA_HD float piece(bool wide, int chunks, int wide_cost = kWideCost) {
+        return (float)(wide ? wide_cost * chunks + 10 : ((chunks + 3) & ~3) + 10);  // (four waves share a narrow one's)
     }
-    static PELICA_HD float share(bool wide, int chunks, bool split) {
-        return piece(wide, chunks) + (split ? wide ? 20.f : 1.f : 0.f);
+    static PELICA_HD float share(bool wide, int chunks, bool split, int wide_cost = kWideCost) {
+        return piece(wide, chunks, wide_cost) + (split ? wide ? 20.f : 1.f : 0.f);
     }
     // the step: the chip's mean, or a slot with `last` to do (its one piece, or
     // the pieces that have to share a slot), which runs faster once its

@@ -114,7 +114,8 @@ struct PlanWeighLds {
 // item's is negative, kWideCost a chunk, and a multiple.  SHARED: items that
 // are one piece write partials, too.
 template <bool SHARED>
-__device__ __forceinline__ float plan_limit(const int* costs, int n_items, int fill, int max_slots, PlanWeighLds& x) {
+__device__ __forceinline__ float plan_limit(const int* costs, int n_items, int fill, int max_slots, PlanWeighLds& x,
+                                            int wide_cost = kWideCost) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto& est = x.est;
     auto& limit = x.limit;
@@ -133,10 +134,10 @@ __device__ __forceinline__ float plan_limit(const int* costs, int n_items, int f
     for (int i = lane; i < n_items; i += 64) {
         const int c = abs(costs[i]);
         const bool wide = costs[i] < 0;
-        const int chunks = wide ? c / kWideCost : c;
+        const int chunks = wide ? c / wide_cost : c;
         const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-        time += PlanCost::share(wide, m, SHARED || k > 1) * (float)k;
-        longest = fmaxf(longest, PlanCost::piece(wide, m));
+        time += PlanCost::share(wide, m, SHARED || k > 1, wide_cost) * (float)k;
+        longest = fmaxf(longest, PlanCost::piece(wide, m, wide_cost));
         pieces += k;
         slots += k > 1 ? k : 0;
     }
@@ -154,9 +155,9 @@ __device__ __forceinline__ float plan_limit(const int* costs, int n_items, int f
         for (int i = lane; i < n_items; i += 64) {
             const int c = abs(costs[i]);
             const bool wide = costs[i] < 0;
-            const int chunks = wide ? c / kWideCost : c;
+            const int chunks = wide ? c / wide_cost : c;
             const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-            atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m) * scale)], k);
+            atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m, wide_cost) * scale)], k);
         }
         __builtin_amdgcn_wave_barrier();
         const int have = hist[wave][lane], longer = pieces - wave_scan(have) + have;  // as long as this bucket's

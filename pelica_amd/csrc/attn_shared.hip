@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
         x.lo = e;
         x.kend = x.shared ? ge[owner] : pos0 + token(x.r0 + x.rows - 1) + 1;
         x.n_chunks = (x.kend - x.lo + 31) >> 5;
-        x.cost = x.n_chunks * (narrow ? 1 : kWideCost);
+        x.cost = x.n_chunks * (narrow ? 1 : sp.wide_cost);
         return x;
     };
     auto owner_of = [&](int i) { return i < n_group_items ? find_last(gitem0, sp.n_groups, i) : find_last(item0, p.n_seq, i); };
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
             costs[i] = x.R <= kNarrowRows ? x.cost : -x.cost;
         }
         __syncthreads();
-        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh);
+        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh, sp.wide_cost);
     }
 
     auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, x.R <= kNarrowRows, k); };
