@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     __asm__ volatile("" ::"s"(z.q0), "s"(z.r0), "s"(sig), "s"(n_joins));
     if (sig != p.sig || j >= n_joins) return;
     int rows, n_slots;
-    if constexpr (SHARED) rows = z.rows, n_slots = z.k + z.g_k;
+    if constexpr (SHARED) rows = z.rows, n_slots = z.k + max(z.g_k, z.g_k2);
     else rows = min(z.R - z.r0, p.rows), n_slots = z.n_slots;
     // row r of partial sl
     auto partial = [&](int sl, int r) -> size_t {
@@ -34,7 +34,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
             if (sl < z.k) return (size_t)(z.at + sl * z.rows) * p.n_kv + (size_t)kvh * z.rows + r;
             constexpr int W = wide_rows(HD);
             const int gr = z.g_row + r, b = gr / W, of = min(W, z.g_R - b * W);
-            return (size_t)(z.g_at + b * W * z.g_k + (sl - z.k) * of) * p.n_kv + (size_t)kvh * of + (gr - b * W);
+            const bool last = (b + 1) * W >= z.g_R;
+            if (sl - z.k >= (last ? z.g_k2 : z.g_k)) return ~(size_t)0;  // (the other block's)
+            const int at = last ? z.g_at2 : z.g_at + b * W * z.g_k;
+            return (size_t)(at + (sl - z.k) * of) * p.n_kv + (size_t)kvh * of + (gr - b * W);
         } else {
             return ((size_t)(z.slot0 + sl) * p.n_kv + kvh) * p.rows + r;
         }
@@ -56,8 +59,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
                 const int sl = s0 + ph + n_ph * u;
                 ml[u] = make_float2(-INFINITY, 0.f);
                 v[u] = float4v{};
-                if (sl < n_slots) {
-                    const size_t at = partial(sl, r);
+                const size_t at = sl < n_slots ? partial(sl, r) : ~(size_t)0;
+                if (at != ~(size_t)0) {
                     ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[at];
                     v[u] = *reinterpret_cast<const float4v*>(p.ws_o + at * HD + d);
                 }
@@ -134,8 +137,14 @@ hipError_t launch_paged_join(const PagedParams& p, hipStream_t st) {
         constexpr bool F32 = decltype(f32)::value;
         const unsigned x = (unsigned)p.max_joins * p.n_kv;
         if (p.shared_joins) {
-            const unsigned y = (unsigned)std::min((p.max_rows + 3) / 4, 16);
-            hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1, true>), dim3(x, y), dim3(256), 0, st, p);
+            // a row a wave, or, of rows that leave most of the chip idle, a workgroup
+            // (8 chats of 32 heads: 5.9 -> 3.9 us)
+            if (p.all_rows <= 2048) {
+                hipLaunchKernelGGL((paged_join_kernel<HD, F32, 4, true>), dim3(x, std::min(p.max_rows, 32)), dim3(256), 0, st, p);
+            } else {
+                const unsigned y = (unsigned)std::min((p.max_rows + 3) / 4, 16);
+                hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1, true>), dim3(x, y), dim3(256), 0, st, p);
+            }
         } else if (p.wide) {
             hipLaunchKernelGGL((paged_join_kernel<HD, F32, 1, false>), dim3(x, 16), dim3(256), 0, st, p);
         } else {

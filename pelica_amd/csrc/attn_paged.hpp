@@ -41,7 +41,7 @@ struct SharedPlanParams {
     PlanParams plan;
     const int32_t *group_start, *shared_len;
     SharedJoin* joins;
-    int n_groups, wide_cost;
+    int n_groups;
 };
 hipError_t launch_paged_shared_plan(const SharedPlanParams& p, hipStream_t st);
 
@@ -73,6 +73,7 @@ struct PagedParams {
     uint32_t srow_b;
     // host side only
     int hd, max_pieces, max_joins, max_rows;  // (of a request's item)
+    int all_rows;                             // n_tokens n_head
     bool f32, wide;
 };
 // cap tanh(y), y = s scale / cap, of small y: tanh(y) / y as the polynomial in

@@ -297,6 +297,7 @@ int run_paged(const PelicaPagedDesc* d, const PelicaPagedShared* shared, const P
     p.max_pieces = (int)x.max_pieces;
     p.max_joins = x.max_joins;
     p.max_rows = x.max_rows;
+    p.all_rows = d->n_tokens * d->n_head;
     p.f32 = f32;
     p.wide = x.wide;
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -553,7 +554,6 @@ int pelica_attn_paged_shared_plan(const PelicaPagedDesc* d, const PelicaPagedSha
     p.shared_len = shared->shared_len;
     p.joins = reinterpret_cast<pelica::SharedJoin*>(static_cast<char*>(plan) + x.join_at);
     p.n_groups = shared->n_groups;
-    p.wide_cost = getenv("PELICA_WC") ? atoi(getenv("PELICA_WC")) : pelica::kWideCost;
     const hipError_t e = pelica::launch_paged_shared_plan(p, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(PELICA_ATTN_EHIP, "paged_shared_plan launch: %s", hipGetErrorString(e));
     return PELICA_ATTN_OK;

@@ -688,8 +688,8 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     constexpr int QES = F32 ? 4 : 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(rl, z.R - 1);
-        valid[nt] = rl < z.R;
+        const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(z.r0 + rl, z.R - 1);
+        valid[nt] = z.r0 + rl < z.R;
         const int t = token_of(p, r), h = kvh * p.hpk + r - t * p.hpk;
         const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * g) * QES;
         sink[nt] = p.sinks_or_q[p.sinks ? h : 0];
@@ -918,7 +918,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         const int rl = 16 * nt + (PACK ? c16 & 7 : c16);
         const bool stores = valid[nt] && !low;
         const float weight = row_weight(p.sinks ? sink[nt] * kLog2e : -INFINITY, M, L);
-        const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1));
+        const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1 - z.r0));
         if (stores && z.slot >= 0 && wave == 0 && g == 0) store_sum(p, z, kvh, rl, M, L);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -1644,10 +1644,10 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
                      "s"(z.rows));
     if (sig != p.sig || id >= n_pieces) return;
     if constexpr (WIDE) {
-        if (z.R > kNarrowRows) {
+        if (z.R > kNarrowRows && !z.narrow) {
             if constexpr (F32) wide_f32_body<HD, SC, Q8>(p, z, kvh, lds);
             else wide_body<HD, MODE, Q8>(p, z, kvh, lds);
-        } else if (z.R > 16) {
+        } else if (z.R - z.r0 > 16) {
             narrow_body<HD, 2, F32, SC, false, Q8>(p, z, kvh, lds);
         } else {
             narrow_body<HD, 1, F32, SC, false, Q8>(p, z, kvh, lds);

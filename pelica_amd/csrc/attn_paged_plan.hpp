@@ -30,6 +30,11 @@ PELICA_HD constexpr int wide_rows(int hd) { return hd == 64 ? 256 : 128; }
 // fill the slots better by this model, and on the chip 3% better to 2% worse:
 // two workgroups of a CU share what one of them leaves.)
 constexpr int kWideCost = 3;
+// Where requests share keys, few wide items stand beside many narrow ones, each
+// often alone on its CU, and f32 queries take twice the products: longer pieces end
+// last (64 readers of 16384 keys at a cost of 3, 5, 7, 10: f32 91, 82, 80, 73 us, f16
+// 55, 52, 52, 50; three prompts' 60 requests, f16: 49, 48, 52, 55 and f32 61, 52, 51, 53).
+constexpr int kSharedWideCost = 5;
 constexpr int kMinPiece = 4;
 struct PlanCost {
     // a piece's own time, and what it takes of the whole chip's
@@ -138,18 +143,20 @@ struct PlanPiece {
     int pos0, len, cb, ce;     // position of its first token, its keys; chunks [cb, ce)
     int slot, n_pre, lo_base;  // first partial row of kv head 0 / n_kv, or -1: the output is written
     int lo, kend, pe;
-    int rows, pad;             // partial rows of a kv head
+    int rows;                  // partial rows of a kv head
+    int narrow;                // of shared keys: the item's rows, at most kNarrowRows, as a narrow item's
 };
 struct PlanJoin {
     int q0, R, r0, slot0, n_slots, pad[3];
 };
 // Where requests share their first keys: of an item of a request with
 // partials.  Its `k` pieces' rows lie at `at` on, each `rows`; its group's
-// first R rows are cut into blocks of wide_rows, each block's k pieces after one another.
+// rows are cut into blocks of wide_rows, each block's g_k pieces after one another
+// (the last block's, which may be narrow, g_k2 of them at g_at2).
 struct SharedJoin {
     int q0, r0, rows, at, k;      // the request's first row of q, the item's first row, its rows, pieces
     int g_at, g_k, g_row, g_R;    // the group's partials, pieces (0: none), the item's first row in it, its rows
-    int pad[3];
+    int g_at2, g_k2, pad;         // of its last block
 };
 static_assert(sizeof(SharedJoin) == 48, "plan layout");
 static_assert(sizeof(PlanHeader) == 64 && sizeof(PlanPiece) == 64 && sizeof(PlanJoin) == 32, "plan layout");

@@ -319,7 +319,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         z.lo = y.k.lo;
         z.kend = y.k.kend;
         z.pe = y.k.pe;
-        z.pad = 0;
+        z.narrow = 0;
         return z;
     };
     auto header = [&](int pieces, int joins) {

@@ -30,7 +30,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
     __shared__ int gstart[kSharedMaxGroups + 1], gitem0[kSharedMaxGroups + 1];
     __shared__ int ge[kSharedMaxGroups];      // shared keys that are walked once
     __shared__ int gcount[kSharedMaxGroups], gfirst[kSharedMaxGroups], glast[kSharedMaxGroups];  // requests with tokens
-    __shared__ int gat[kSharedMaxGroups], gk[kSharedMaxGroups];  // partials: first row, pieces of a block
+    __shared__ int gat[kSharedMaxGroups], gk[kSharedMaxGroups];    // partials: first row, pieces of a block
+    __shared__ int gat2[kSharedMaxGroups], gk2[kSharedMaxGroups];  // of the last block
     __shared__ int costs[kPlanItems];
     __shared__ int part[kPlanWaves], part3[3 * kPlanWaves], bad;
     __shared__ PlanWeighLds weigh;
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
             ge[g] = sp.shared_len[g];
             gcount[g] = 0;
             gfirst[g] = kPagedMaxSeq;
-            glast[g] = gat[g] = gk[g] = 0;
+            glast[g] = gat[g] = gk[g] = gat2[g] = gk2[g] = 0;
         }
     }
     if (tid < kBuckets) at_bucket[tid] = 0;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
     auto token = [&](int r) { return (int)(((double)r + 0.5) * inv_hpk); };
     struct Item {
         int group, s;      // the group it is of (a request's: its own, or -1), its (first) request
-        bool shared;       // of the group's shared keys
+        bool shared, narrow;  // of the group's shared keys; at most kNarrowRows rows
         int T, r0, R, rows, cost;
         int n_chunks, lo, kend;
     };
@@ -147,13 +148,16 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
             pos0 = kv[owner] - x.T;
             e = x.group >= 0 ? ge[x.group] : 0;
         }
-        const bool narrow = x.R <= kNarrowRows;
-        x.r0 = narrow ? 0 : (i - (x.shared ? gitem0[owner] : item0[owner])) * W;
-        x.rows = narrow ? x.R : imin(W, x.R - x.r0);
+        x.narrow = x.R <= kNarrowRows;
+        x.r0 = x.narrow ? 0 : (i - (x.shared ? gitem0[owner] : item0[owner])) * W;
+        x.rows = x.narrow ? x.R : imin(W, x.R - x.r0);
+        // (a group's last block may be as small as a request's item: 17 requests of
+        // 8 heads a kv head, head dim 128: 128 rows and 8)
+        if (x.shared && x.rows <= kNarrowRows) x.narrow = true;
         x.lo = e;
         x.kend = x.shared ? ge[owner] : pos0 + token(x.r0 + x.rows - 1) + 1;
         x.n_chunks = (x.kend - x.lo + 31) >> 5;
-        x.cost = x.n_chunks * (narrow ? 1 : sp.wide_cost);
+        x.cost = x.n_chunks * (x.narrow ? 1 : kSharedWideCost);
         return x;
     };
     auto owner_of = [&](int i) { return i < n_group_items ? find_last(gitem0, sp.n_groups, i) : find_last(item0, p.n_seq, i); };
@@ -168,13 +172,13 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
     if (n_items > 0 && n_items <= kPlanItems) {
         for (int i = tid; i < n_items; i += kPlanThreads) {
             const Item x = item_at(i);
-            costs[i] = x.R <= kNarrowRows ? x.cost : -x.cost;
+            costs[i] = x.narrow ? x.cost : -x.cost;
         }
         __syncthreads();
-        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh, sp.wide_cost);
+        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh, kSharedWideCost);
     }
 
-    auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, x.R <= kNarrowRows, k); };
+    auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, x.narrow, k); };
     for (int i = tid; i < n_items; i += kPlanThreads) {
         const Item x = item_at(i);
         const int k = item_pieces(x.cost, x.n_chunks, inv_limit);
@@ -207,10 +211,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
         owner[tid] = x.shared ? x.group : x.s;
         place[tid] = k > 0 ? atomicAdd(&at_bucket[bucket_of(x, k)], k) : 0;
         row0[tid] = parts ? row : -1;
-        // (a group's blocks are cut alike: equal chunks, and all but the last whole)
-        if (k > 0 && x.shared && x.r0 == 0) {
-            gat[x.group] = row;
-            gk[x.group] = k;
+        // (all but a group's last block are whole, and cut alike)
+        if (k > 0 && x.shared) {
+            if (x.r0 == 0) gat[x.group] = row, gk[x.group] = k;
+            if (x.r0 + x.rows == x.R) gat2[x.group] = row, gk2[x.group] = k;
         }
         __syncthreads();
         if (joined && jn < p.max_joins) {
@@ -227,6 +231,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
                 j.g_k = gk[g];
                 j.g_row = (q0[x.s] - q0[gfirst[g]]) * p.hpk + x.r0;
                 j.g_R = group_rows_of(g);
+                j.g_at2 = gat2[g];
+                j.g_k2 = gk2[g];
             }
             sp.joins[jn] = j;
         }
@@ -251,7 +257,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
             z.kend = y.kend;
             z.pe = 0;
             z.rows = y.rows;
-            z.pad = 0;
+            z.narrow = y.shared && y.narrow;
             p.pieces[place[t] + nth] = z;
         }
         n_pieces += all[0];
