@@ -57,48 +57,87 @@ __device__ __forceinline__ half4 to_half(float4v x) {
 }
 
 // max over lanes l, l ^ 1, l ^ 2, l ^ 3
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));
-    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));
+__device__ __forceinline__ double quad_max(double x) {
+    auto with = [&](auto moved) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint64_t v = (uint64_t)(uint32_t)moved((int)(u >> 32)) << 32 | (uint32_t)moved((int)u);
+        x = fmax(x, __builtin_bit_cast(double, v));
+    };
+    with([](int v) { return __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false); });
+    with([](int v) { return __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false); });
+    return x;
 }
 
-// Eight consecutive values of a lane, a group in four lanes, as 8-bit integers
-// and their scale's bits.  Magnitudes are compared as integers: an infinity
-// or a NaN is larger than all numbers.
-__device__ __forceinline__ u32x2 quantise8(const float4v& a, const float4v& b, uint16_t& scale) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        top = max(top, max(__float_as_uint(a[i]) & 0x7FFFFFFFu, __float_as_uint(b[i]) & 0x7FFFFFFFu));
-    const float most = __uint_as_float(quad_max(top));
-    _Float16 s = (_Float16)(most * (1.f / 127.f));
-    uint16_t bits = __builtin_bit_cast(uint16_t, s);
-    // (off by a last bit of the quotient s is still one of the two f16 numbers
-    // around it; 127 s is exact in f32)
-    if ((float)s * 127.f < most) ++bits;
-    if (!(most < INFINITY)) bits = 0x7E00;
-    const float f = (float)__builtin_bit_cast(_Float16, bits);
-    const float inv = f > 0.f ? __builtin_amdgcn_rcpf(f) : 0.f;
-    scale = bits;
-    // the sum's last byte is n: 2^23 takes the places behind the point.  Of a
-    // quotient next to a border the remainder, exact by the fma, decides.
-    uint32_t n[8];
-    const float half = 0.5f * f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = i < 4 ? a[i & 3] : b[i & 3];
-        float t = __builtin_fmaf(x, inv, 12582912.f);
-        const float r = __builtin_fmaf(12582912.f - t, f, x);
-        // (of two as near the even one, as elsewhere: an odd n gives way at half)
-        const float most_r = __uint_as_float(__float_as_uint(half) - (__float_as_uint(t) & 1u));
-        t += r > most_r ? 1.f : r < -most_r ? -1.f : 0.f;
-        n[i] = __float_as_uint(t);
-    }
+// the last bytes of eight words
+__device__ __forceinline__ u32x2 last_bytes(const uint32_t (&n)[8]) {
     auto pack = [&](int i) {
         const uint32_t lo = __builtin_amdgcn_perm(n[i + 1], n[i], 0x0C0C0400u), hi = __builtin_amdgcn_perm(n[i + 3], n[i + 2], 0x04000C0Cu);
         return lo | hi;
     };
     return u32x2{pack(0), pack(4)};
+}
+
+// Eight consecutive values of a lane, a group in four lanes, as 8-bit integers
+// and their scale's bits.  Of v, whose values are given: the quotient's integer,
+// put right by its remainder.
+__device__ __forceinline__ u32x2 quantise8(const float4v& a, const float4v& b, uint16_t& scale) {
+    // (as integers an infinity or a NaN is larger than all numbers)
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        top = max(top, max(__float_as_uint(a[i]) & 0x7FFFFFFFu, __float_as_uint(b[i]) & 0x7FFFFFFFu));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xF, 0xF, false));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xF, 0xF, false));
+    const float most = __uint_as_float(top);
+    uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)(most * (1.f / 127.f)));
+    // (that is one of the two f16 numbers around the quotient; 127 s is exact in f32)
+    if ((float)__builtin_bit_cast(_Float16, bits) * 127.f < most) ++bits;
+    if (!(most < INFINITY)) bits = 0x7E00;
+    const float f = (float)__builtin_bit_cast(_Float16, bits);
+    const float inv = f > 0.f ? __builtin_amdgcn_rcpf(f) : 0.f, half = 0.5f * f;
+    scale = bits;
+    // the sum's last byte is n: 2^23 takes the places behind the point.  The
+    // remainder is exact by the fma; of two integers as near the even one is taken.
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = i < 4 ? a[i & 3] : b[i & 3];
+        float t = __builtin_fmaf(x, inv, 12582912.f);
+        const float r = __builtin_fmaf(12582912.f - t, f, x);
+        const float most_r = __uint_as_float(__float_as_uint(half) - (__float_as_uint(t) & 1u));
+        t += r > most_r ? 1.f : r < -most_r ? -1.f : 0.f;
+        n[i] = __float_as_uint(t);
+    }
+    return last_bytes(n);
+}
+
+// Of k, in 64 bits as its norm and turn are: an integer next to a border is
+// decided by a value's last bits (in f32 1 of 30000 was the other one; 4000 tokens
+// of 32 + 4 heads of 128 took 26.6 us, and take 29.8).
+__device__ __forceinline__ u32x2 quantise8(const double (&x)[8], uint16_t& scale) {
+    double top = 0;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        top = fmax(top, fabs(x[i]));
+        bad |= !(fabs(x[i]) < INFINITY);
+    }
+    top = quad_max(bad ? INFINITY : top);
+    uint16_t bits = __builtin_bit_cast(uint16_t, (_Float16)((float)top * (1.f / 127.f)));
+    // (that is one of the two f16 numbers around the quotient)
+    if ((double)__builtin_bit_cast(_Float16, bits) * 127 < top) ++bits;
+    if (!(top < INFINITY)) bits = 0x7E00;
+    const double s = (double)__builtin_bit_cast(_Float16, bits);
+    const double inv = s > 0 ? 1 / s : 0;
+    scale = bits;
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // the quotient, rounded once, and 2^52: the sum's last byte is n
+        const double y = x[i] * inv, q = fma(fma(-y, s, x[i]), inv, y);
+        n[i] = (uint32_t)__builtin_bit_cast(uint64_t, q + 6755399441055744.0);
+    }
+    return last_bytes(n);
 }
 
 // EX: a lane holds both values of its pairs; else (rot not a multiple of 8)
@@ -107,7 +146,8 @@ template <int HD, int IT, bool HALF, bool EX, bool Q8>
 __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int tok_waves) {
     constexpr int LPH = HD / 8, HPW = 64 / LPH;
     __shared__ __attribute__((aligned(16))) float turn[4][HD];  // (cos, sin) of the token's pairs
-    __shared__ __attribute__((aligned(16))) float xch[EX && !Q8 ? 1 : 4][EX && !Q8 ? 1 : HPW][EX && !Q8 ? 4 : HD];
+    __shared__ __attribute__((aligned(16))) float xch[EX ? 1 : 4][EX ? 1 : HPW][EX ? 4 : HD];
+    __shared__ __attribute__((aligned(16))) double rows8[Q8 ? 4 : 1][Q8 ? HPW : 1][Q8 ? HD : 2];  // k and v heads, normed
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
     const uint32_t gw = blockIdx.x * 4u + wave;  // waves follow the tokens, workgroups do not
@@ -183,6 +223,81 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int to
     for (int it = 0; it < IT; ++it) {
         const int h = slot0 + HPW * it, hk = h - p.n_head, hv = hk - p.n_kv;
         float4v a = x[it][0], b = x[it][1];
+        if constexpr (Q8) {
+            // k and v heads through LDS: a group's 32 values to four lanes, eight each
+            double* const row8 = rows8[wave][sub];
+            float* const row4 = reinterpret_cast<float*>(row8);
+            if (hk >= 0 && hv < 0) {
+                double inv = 1;
+                if (p.k_norm) {
+                    double ss = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ss = fma((double)a[i], (double)a[i], fma((double)b[i], (double)b[i], ss));
+#pragma unroll
+                    for (int off = 1; off < LPH; off <<= 1) ss += __shfl_xor(ss, off, 64);
+                    inv = 1 / sqrt(ss / HD + (double)p.eps);
+                }
+                double u[4], w[4];  // (wk: ones without a norm)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] = (double)a[i] * inv * (double)wk[0][i], w[i] = (double)b[i] * inv * (double)wk[1][i];
+                if (EX && rot) {
+                    auto turn2 = [](double& x, double& y, float c, float sn) {
+                        const double t = fma(-y, (double)sn, x * (double)c);
+                        y = fma(x, (double)sn, y * (double)c);
+                        x = t;
+                    };
+                    if (p.neox) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) turn2(u[i], w[i], cs[i >> 1][2 * (i & 1)], cs[i >> 1][2 * (i & 1) + 1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            turn2(u[i], u[i + 1], cs[0][i], cs[0][i + 1]);
+                            turn2(w[i], w[i + 1], cs[1][i], cs[1][i + 1]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) row8[ea + i] = u[i], row8[eb + i] = w[i];
+            } else if (hk >= 0) {
+                *reinterpret_cast<float4v*>(row4 + ea) = a;
+                *reinterpret_cast<float4v*>(row4 + eb) = b;
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            if (hk >= 0 && h < n_slot) {
+                uint16_t s;
+                u32x2 n;
+                if (hv < 0) {
+                    double y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = row8[8 * l + i];
+                    if constexpr (!EX) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int e = 8 * l + i;
+                            const bool second = p.neox ? e >= half : (e & 1) != 0;
+                            const int j = e >= p.rot ? 0 : !p.neox ? e >> 1 : second ? e - half : e;
+                            const double z = row8[!p.neox ? e ^ 1 : second ? j : j + half];
+                            const double c = (double)turn[wave][2 * j], sn = (double)turn[wave][2 * j + 1];
+                            const double r = fma(second ? z : -z, sn, y[i] * c);
+                            y[i] = e < p.rot ? r : y[i];
+                        }
+                    }
+                    n = quantise8(y, s);
+                } else {
+                    n = quantise8(*reinterpret_cast<const float4v*>(row4 + 8 * l), *reinterpret_cast<const float4v*>(row4 + 8 * l + 4), s);
+                }
+                const bool is_k = hv < 0;
+                const int hc = is_k ? hk : hv;
+                int8_t* const pages = reinterpret_cast<int8_t*>(is_k ? p.k_pages : p.v_pages);
+                *reinterpret_cast<u32x2*>(pages + base + (int64_t)hc * p.head_stride + 8 * l) = n;
+                const int64_t at = (row >> p.page_log2) * p.sc.page + (row & ((1LL << p.page_log2) - 1)) * p.sc.row + (int64_t)hc * p.sc.head;
+                if (l % 4 == 0) (is_k ? p.k_scales : p.v_scales)[at + l / 4] = s;
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        }
         if (p.q_norm || p.k_norm) {
             const float ss = head_sum<LPH>(((a[0] * a[0] + a[1] * a[1]) + (a[2] * a[2] + a[3] * a[3])) +
                                            ((b[0] * b[0] + b[1] * b[1]) + (b[2] * b[2] + b[3] * b[3])));
@@ -232,30 +347,7 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p, int to
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         }
-        if constexpr (Q8) {
-            // a group's 32 values into four lanes, eight each
-            if (hk >= 0) {
-                *reinterpret_cast<float4v*>(&xch[wave][sub][ea]) = a;
-                *reinterpret_cast<float4v*>(&xch[wave][sub][eb]) = b;
-            }
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            if (hk >= 0 && h < n_slot) {
-                const float4v x0 = *reinterpret_cast<const float4v*>(&xch[wave][sub][8 * l]);
-                const float4v x1 = *reinterpret_cast<const float4v*>(&xch[wave][sub][8 * l + 4]);
-                uint16_t s;
-                const u32x2 n = quantise8(x0, x1, s);
-                const bool is_k = hv < 0;
-                const int hc = is_k ? hk : hv;
-                int8_t* const pages = reinterpret_cast<int8_t*>(is_k ? p.k_pages : p.v_pages);
-                *reinterpret_cast<u32x2*>(pages + base + (int64_t)hc * p.head_stride + 8 * l) = n;
-                const int64_t at = (row >> p.page_log2) * p.sc.page + (row & ((1LL << p.page_log2) - 1)) * p.sc.row + (int64_t)hc * p.sc.head;
-                if (l % 4 == 0) (is_k ? p.k_scales : p.v_scales)[at + l / 4] = s;
-            }
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            if (hk >= 0) continue;
-        }
+        if (Q8 && hk >= 0) continue;
         if (h >= n_slot) break;
         if (!HALF && hk < 0) {
             float* dst = static_cast<float*>(p.q_out) + (size_t)t * p.tok_o + (size_t)h * HD;
