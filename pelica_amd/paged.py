@@ -204,16 +204,28 @@ def _pools(k_pages, v_pages, dev, dtype=None, names=("k_pages", "v_pages"), last
     return st[0] if shape[0] > 1 else 0, st[1], st[2] if shape[2] > 1 else 0, shape
 
 
-def _q8(k_pages, k_scales, v_scales, dev):
-    """The scales of 8-bit pages, and their strides (None: f16 pages)."""
+def _q8_pools(k_pages, v_pages, k_scales, v_scales, dev):
+    """Both pools' strides and shape as of ``_pools``, and their scales
+    (PagedQ8; None for f16 pages, which come without)."""
     if k_scales is None and v_scales is None:
-        return None
+        return (*_pools(k_pages, v_pages, dev), None)
     _need(k_scales is not None and v_scales is not None, "k_scales and v_scales come together")
-    page, row, head, size = _pools(k_scales, v_scales, dev, None, ("k_scales", "v_scales"), "hd / 32")
-    pool = k_pages.shape
-    if k_pages.dim() != 4 or size[:3] != pool[:3] or size[3] * GROUP != pool[3]:
-        raise AttnError(EINVAL, f"k_scales: one for each {GROUP} values of the pages {tuple(pool)}, got {tuple(size)}")
-    return PagedQ8(k_scales.data_ptr(), v_scales.data_ptr(), page, row, head)
+    st, shape, at, size = k_pages.stride(), k_pages.shape, k_scales.stride(), k_scales.shape
+    i8, f16 = _torch.int8, _torch.float16
+    if not (k_pages.dtype is i8 and v_pages.dtype is i8 and k_scales.dtype is f16 and v_scales.dtype is f16
+            and len(st) == 4 and len(at) == 4 and st[3] == 1 and at[3] == 1 and v_pages.stride() == st
+            and v_scales.stride() == at and v_pages.shape == shape and v_scales.shape == size
+            and size[0] == shape[0] and size[1] == shape[1] and size[2] == shape[2] and size[3] * GROUP == shape[3]
+            and k_pages.get_device() == dev and v_pages.get_device() == dev and k_scales.get_device() == dev
+            and v_scales.get_device() == dev and 0 not in st and 0 not in at):
+        # (names what is wrong; a dim of one may have a stride of 0)
+        _pools(k_pages, v_pages, dev, i8)
+        _pools(k_scales, v_scales, dev, None, ("k_scales", "v_scales"), "hd / 32")
+        if size[:3] != shape[:3] or size[3] * GROUP != shape[3]:
+            raise AttnError(EINVAL, f"k_scales: one for each {GROUP} values of the pages {tuple(shape)}, got {tuple(size)}")
+    many, heads = shape[0] > 1, shape[2] > 1
+    return (st[0] if many else 0, st[1], st[2] if heads else 0, shape,
+            PagedQ8(k_scales.data_ptr(), v_scales.data_ptr(), at[0] if many else 0, at[1], at[2] if heads else 0))
 
 
 def _weights(name, t, n, dev):
@@ -221,6 +233,14 @@ def _weights(name, t, n, dev):
     if not (t.dtype is _torch.float32 and t.get_device() == dev and t.shape == (n,) and t.is_contiguous()):
         _check(name, t, _torch.float32, 1)
         raise AttnError(EINVAL, f"{name}: {n} weights")
+    return t.data_ptr()
+
+
+def _per_head(name, t, n, dev):
+    """The address of ``n`` heads' values."""
+    if not (t.dtype is _torch.float32 and t.get_device() == dev and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
+        _check(name, t, _torch.float32, 1)
+        raise AttnError(EINVAL, f"{name}: one value for each of the {n} heads")
     return t.data_ptr()
 
 
@@ -332,8 +352,7 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_sc
         _check("q", q, dtype, 3, dense=False)
         _need(q.shape == shape, f"q: {shape} as planned, got {tuple(q.shape)}")
         raise AttnError(EINVAL, f"the plan is on device {dev}, q on {q.device}")
-    q8 = _q8(k_pages, k_scales, v_scales, dev)
-    page, row, head, pool = _pools(k_pages, v_pages, dev, None if q8 is None else torch.int8)
+    page, row, head, pool, q8 = _q8_pools(k_pages, v_pages, k_scales, v_scales, dev)
     if pool != plan._page_shape:
         raise AttnError(EINVAL, f"k_pages: {plan._page_shape} as planned, got {tuple(k_pages.shape)}")
     if out is None:
@@ -342,11 +361,10 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_sc
     elif not (out.dtype is dtype and out.shape == shape and out.get_device() == dev):
         _check("out", out, dtype, 3, dense=False)
         raise AttnError(EINVAL, f"out: {shape}, got {tuple(out.shape)}")
-    for name, t in (("sinks", sinks), ("alibi", alibi)):
-        if t is not None and not (t.dtype is torch.float32 and t.get_device() == dev and t.shape == shape[1:2]
-                                  and t.is_contiguous()):
-            _check(name, t, torch.float32, 1)
-            raise AttnError(EINVAL, f"{name}: one value for each of the {shape[1]} heads")
+    if sinks is not None:
+        sinks = _per_head("sinks", sinks, shape[1], dev)
+    if alibi is not None:
+        alibi = _per_head("alibi", alibi, shape[1], dev)
     need, ws, ws_bytes = plan.workspace_bytes, None, 0
     if need:
         ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
@@ -359,7 +377,7 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_sc
         ws = workspace.data_ptr()
     x = PagedDesc.from_buffer_copy(plan.desc)
     if alibi is not None:
-        x.alibi = alibi.data_ptr()
+        x.alibi = alibi
     x.page_stride, x.row_stride, x.head_stride = page, row, head
     if not q.is_contiguous():
         x.q_token_stride = _rows("q", q)
@@ -370,7 +388,7 @@ def paged_attention(q, k_pages, v_pages, plan: PagedPlan, *, k_scales=None, v_sc
     if softcap:
         x.softcap = softcap
     lib = attn._lib
-    tail = (k_pages.data_ptr(), v_pages.data_ptr(), None if sinks is None else sinks.data_ptr(), out.data_ptr(), ws,
+    tail = (k_pages.data_ptr(), v_pages.data_ptr(), sinks, out.data_ptr(), ws,
             ws_bytes, attn._stream_ptr(stream))
     if plan._shared is not None:
         rc = lib.pelica_attn_paged_shared(ctypes.byref(x), ctypes.byref(plan._shared), None if q8 is None else ctypes.byref(q8),
@@ -416,8 +434,7 @@ def pages_read(k_pages, v_pages, slots, *, k_scales=None, v_scales=None, out=Non
     if _torch is None:
         _start()
     dev, f16 = _device(), _torch.float16
-    q8 = _q8(k_pages, k_scales, v_scales, dev)
-    page, row, head, (n_pages, page_size, n_kv, hd) = _pools(k_pages, v_pages, dev, None if q8 is None else _torch.int8)
+    page, row, head, (n_pages, page_size, n_kv, hd), q8 = _q8_pools(k_pages, v_pages, k_scales, v_scales, dev)
     if not (slots.dtype is _torch.int64 and slots.get_device() == dev and slots.dim() == 1 and slots.is_contiguous()):
         _check("slots", slots, _torch.int64, 1)
     shape = (slots.numel(), n_kv, hd)
@@ -425,12 +442,13 @@ def pages_read(k_pages, v_pages, slots, *, k_scales=None, v_scales=None, out=Non
         with _on(stream):
             out = (_torch.empty(shape, dtype=f16, device=k_pages.device), _torch.empty(shape, dtype=f16, device=k_pages.device))
     k_out, v_out = out
-    for t in (k_out, v_out):
-        if not (t.dtype is f16 and t.shape == shape and t.get_device() == dev):
+    if not (k_out.dtype is f16 and v_out.dtype is f16 and k_out.shape == shape and v_out.shape == shape
+            and k_out.get_device() == dev and v_out.get_device() == dev):
+        for t in out:
             _check("out", t, f16, 3, dense=False)
-            raise AttnError(EINVAL, f"out: two of {shape}, got {tuple(t.shape)}")
-    stride = _rows("out", k_out)
-    if _rows("out", v_out) != stride:
+        raise AttnError(EINVAL, f"out: two of {shape}, got {tuple(k_out.shape)} and {tuple(v_out.shape)}")
+    stride = 0 if k_out.is_contiguous() else _rows("out", k_out)
+    if (0 if v_out.is_contiguous() else _rows("out", v_out)) != stride:
         raise AttnError(EINVAL, "out: both contiguous, or rows of one stride")
     d = PagedDesc(n_kv, n_kv, hd, 0, shape[0], 0, page_size, n_pages, 0, 0, None, None, None, None, None, page, row, head)
     lib = attn._lib or attn.load_library()
@@ -469,8 +487,7 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, k_scales=None, v_scales=None,
                                 f"{tuple(v.shape)}")
     T, n_head, hd = shape
     n_kv = kv_shape[1]
-    q8 = _q8(k_pages, k_scales, v_scales, dev)
-    page, row, head, (n_pages, page_size, heads, dims) = _pools(k_pages, v_pages, dev, None if q8 is None else _torch.int8)
+    page, row, head, (n_pages, page_size, heads, dims), q8 = _q8_pools(k_pages, v_pages, k_scales, v_scales, dev)
     if heads != n_kv or dims != hd:
         raise AttnError(EINVAL, f"k_pages: [n_pages, page_size, {n_kv}, {hd}], got {tuple(k_pages.shape)}")
     stride = at_q[0] if T > 1 else 0
