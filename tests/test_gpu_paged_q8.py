@@ -249,3 +249,31 @@ def test_refusals():
         args = {**dict(k_pages=c.kd, v_pages=c.vd, k_scales=c.ks, v_scales=c.vs), **kw}
         with pytest.raises(attn.AttnError):
             paged.paged_attention(c.qd, plan=plan, **args)
+
+
+# (lens, window, prefix): the prefix ends and the window begins within 16 or 32 rows that one load covers
+@pytest.mark.parametrize("lens,window,prefix", [([130], 100, [20]), ([300, 275, 64], 24, [268, 242, 33]), ([300], 30, [257]),
+                                                ([31], 3, [9]), ([420], 36, [353])])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_head,n_kv", [(8, 2), (20, 1), (40, 1)], ids=["rows8", "rows32", "wide"])
+def test_keys_between_a_prefix_and_a_window_in_longer_pages(n_head, n_kv, hd, page, lens, window, prefix):
+    for half in (False, True):
+        kw = dict(n_head=n_head, n_kv=n_kv, hd=hd, half=half, window=window, prefix=prefix, page=page)
+        Case(lens, [1] * len(lens), seed=45, **kw).check()
+        Case(lens, [min(n, 3) for n in lens], seed=48, cap=5.0, sinks=True, **kw).check()
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 128])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_random_mixes(page, hd, half):
+    g = torch.Generator().manual_seed(page + hd + half)
+    r = lambda a, b: int(torch.randint(a, b + 1, (1,), generator=g))  # noqa: E731
+    for seed in range(6):
+        n = r(1, 7)
+        lens = [r(1, 700) for _ in range(n)]
+        new = [min(a, r(1, (1, 3, 90)[r(0, 2)])) for a in lens]
+        hpk, n_kv = (1, 2, 3, 5, 8)[r(0, 4)], r(1, 3)
+        Case(lens, new, n_head=hpk * n_kv, n_kv=n_kv, hd=hd, half=half, page=page, window=(0, 0, r(1, 300))[r(0, 2)], sinks=r(0, 1) == 1,
+             layout=("hnd", "nhd", "wide", "kv")[r(0, 3)], pad=r(0, 3), seed=100 + seed).check()

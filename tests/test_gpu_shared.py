@@ -144,6 +144,33 @@ def test_many_groups():
     CASES["f16_pages"](lens, [1 + i % 2 for i in range(700)], [(0, 700, 96, 96)], n_head=4, n_kv=1, hd=64, half=True, seed=14).check()
 
 
+@f16_cases
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_random_mixes(hd, half, pages):
+    g = torch.Generator().manual_seed(hd + half + len(pages))
+    r = lambda a, b: int(torch.randint(a, b + 1, (1,), generator=g))  # noqa: E731
+    for seed in range(8):
+        page = (8, 16, 32, 64)[r(0, 3)]
+        lens, new, groups = [], [], []
+        for _ in range(r(1, 4)):
+            n, common = r(1, 6), page * r(1, 20)
+            first = len(lens)
+            for _ in range(n):
+                t = r(0, 3) if r(0, 5) else r(1, 60)
+                lens.append(common + t + r(0, 150) if r(0, 9) else t + r(0, common))
+                new.append(t)
+            least = min(a - b for a, b in zip(lens[first:], new[first:]))
+            groups.append((first, len(lens), min(common, least // page * page), r(0, common + 5) if r(0, 3) == 0 else min(common, least // page * page)))
+            if groups[-1][3] > groups[-1][2]:  # (never more keys than the tables share)
+                groups[-1] = (*groups[-1][:3], groups[-1][2])
+        if sum(new) == 0:
+            new[0], lens[0] = 1, max(lens[0], 1)
+        hpk, n_kv = (1, 2, 3, 5, 8)[r(0, 4)], r(1, 3)
+        CASES[pages](lens, new, groups, n_head=hpk * n_kv, n_kv=n_kv, hd=hd, half=half, page=page, sinks=r(0, 1) == 1, cap=(0.0, 30.0)[r(0, 1)],
+                     layout=("hnd", "nhd", "wide", "kv")[r(0, 3)], pad=r(0, 3), seed=200 + seed).check()
+
+
 def test_the_most_groups_and_empty_ones():
     n = 1100
     c = CASES["f16_pages"]([70] * n, [1] * n, [(0, n, 64, 64)], n_head=2, n_kv=1, page=16, seed=15).device()
