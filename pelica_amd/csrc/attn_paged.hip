@@ -59,8 +59,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
                 const int sl = s0 + ph + n_ph * u;
                 ml[u] = make_float2(-INFINITY, 0.f);
                 v[u] = float4v{};
-                const size_t at = sl < n_slots ? partial(sl, r) : ~(size_t)0;
-                if (at != ~(size_t)0) {
+                bool there = sl < n_slots;
+                size_t at = 0;
+                if constexpr (SHARED) {
+                    at = there ? partial(sl, r) : 0;
+                    there &= at != ~(size_t)0;
+                }
+                if (there) {
+                    if constexpr (!SHARED) at = partial(sl, r);
                     ml[u] = reinterpret_cast<const float2*>(p.ws_ml)[at];
                     v[u] = *reinterpret_cast<const float4v*>(p.ws_o + at * HD + d);
                 }

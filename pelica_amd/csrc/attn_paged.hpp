@@ -58,7 +58,6 @@ struct PagedParams {
     float* ws_ml;               // of a piece [n_kv][its rows] x (max, sum), base-2 max
     float* ws_o;                // [n_kv][its rows][hd]
     const PlanJoin* joins;
-    const SharedJoin* shared_joins;  // (not NULL: a plan of shared keys)
     int64_t page_b, head_b;     // bytes between pages, between kv heads of a row
     int64_t q_tok, o_tok;       // values between tokens
     uint32_t row_b, sig;        // bytes between rows of a page
@@ -67,14 +66,16 @@ struct PagedParams {
     // of raw products up to tanh_to[i]: the capped score (log2 domain) as s times
     // a polynomial in s^2, of f32 and of f16 queries
     float tanh_c[5], tanh_h[3], tanh_to[2];
-    // 8-bit pages: scales, bytes between pages, heads, rows of theirs
-    const uint16_t *ks, *vs;
-    int64_t spage_b, shead_b;
-    uint32_t srow_b;
     // host side only
     int hd, max_pieces, max_joins, max_rows;  // (of a request's item)
     int all_rows;                             // n_tokens n_head
     bool f32, wide;
+    // (behind what all calls read: a line of the arguments more is a round trip more)
+    const SharedJoin* shared_joins;  // (not NULL: a plan of shared keys)
+    // 8-bit pages: scales, bytes between pages, heads, rows of theirs
+    const uint16_t *ks, *vs;
+    int64_t spage_b, shead_b;
+    uint32_t srow_b;
 };
 // cap tanh(y), y = s scale / cap, of small y: tanh(y) / y as the polynomial in
 // y^2 that interpolates it at the Chebyshev nodes of [0, y_max^2].  Up to 0.55:

@@ -453,7 +453,7 @@ __device__ __forceinline__ float sink_of(const PagedParams& p, int h) { return p
 
 // Row rl of a piece's partials
 __device__ __forceinline__ size_t partial_row(const PagedParams& p, const PlanPiece& z, int kvh, int rl) {
-    return (size_t)z.slot * p.n_kv + (size_t)kvh * z.rows + rl;
+    return (uint32_t)z.slot * (uint32_t)p.n_kv + (uint32_t)(kvh * z.rows + rl);  // (below 2^31)
 }
 
 // Where row rl of the piece's item goes: its output, or the partial sums of a
@@ -555,7 +555,8 @@ __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
 // tiles, 2 until they land, 1.3 for the chunks, 2.4 for merge and store.  With
 // 32-row tiles, every tile requested and two merge barriers they were 11.4;
 // with a pack of 8 rows in a tile of 16, a 32768-key token went from 17.5 to 16.
-template <int HD, int NT, bool F32, bool SC, bool PACK, bool Q8>
+// WIDE: beside wide items, whose last small block begins at a row of its own.
+template <int HD, int NT, bool F32, bool SC, bool PACK, bool Q8, bool WIDE>
 __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     static_assert(!PACK || (F32 && NT == 1), "packed hi and lo parts: f32, one tile");
     using S_ = NarrowShape<HD, NT, Q8>;
@@ -563,6 +564,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     constexpr int KS = S_::KS, DT = S_::DT, NB = S_::NB, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, c16 = lane & 15;
+    const int r0 = WIDE ? z.r0 : 0;
     char* const kbuf = lds + wave * S_::WAVE;
     char* const vbuf = kbuf + NB * TILE;
     Rows rows(p, z, kvh, lane);
@@ -688,8 +690,8 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     constexpr int QES = F32 ? 4 : 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(z.r0 + rl, z.R - 1);
-        valid[nt] = z.r0 + rl < z.R;
+        const int rl = 16 * nt + (PACK ? c16 & 7 : c16), r = min(r0 + rl, z.R - 1);
+        valid[nt] = r0 + rl < z.R;
         const int t = token_of(p, r), h = kvh * p.hpk + r - t * p.hpk;
         const char* src = static_cast<const char*>(p.q) + ((size_t)(z.q0 + t) * p.q_tok + (size_t)h * HD + 8 * g) * QES;
         sink[nt] = p.sinks_or_q[p.sinks ? h : 0];
@@ -918,7 +920,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
         const int rl = 16 * nt + (PACK ? c16 & 7 : c16);
         const bool stores = valid[nt] && !low;
         const float weight = row_weight(p.sinks ? sink[nt] * kLog2e : -INFINITY, M, L);
-        const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1 - z.r0));
+        const RowOut<HD, F32> out(p, z, kvh, min(rl, z.R - 1 - r0));
         if (stores && z.slot >= 0 && wave == 0 && g == 0) store_sum(p, z, kvh, rl, M, L);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -1641,19 +1643,19 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int n_pieces = p.head->n_pieces;
     // (and what the end reads of the arguments: a line's first touch is a round trip)
     __asm__ volatile("" ::"s"(z.seq), "s"(z.cb), "s"(z.slot), "s"(z.kend), "s"(sig), "s"(n_pieces), "s"(p.out), "s"(p.o_tok),
-                     "s"(z.rows));
+                     "s"(p.qscale), "s"(z.rows));
     if (sig != p.sig || id >= n_pieces) return;
     if constexpr (WIDE) {
         if (z.R > kNarrowRows && !z.narrow) {
             if constexpr (F32) wide_f32_body<HD, SC, Q8>(p, z, kvh, lds);
             else wide_body<HD, MODE, Q8>(p, z, kvh, lds);
         } else if (z.R - z.r0 > 16) {
-            narrow_body<HD, 2, F32, SC, false, Q8>(p, z, kvh, lds);
+            narrow_body<HD, 2, F32, SC, false, Q8, true>(p, z, kvh, lds);
         } else {
-            narrow_body<HD, 1, F32, SC, false, Q8>(p, z, kvh, lds);
+            narrow_body<HD, 1, F32, SC, false, Q8, true>(p, z, kvh, lds);
         }
     } else {
-        narrow_body<HD, ROWS == kRows32 ? 2 : 1, F32, SC, F32 && ROWS == kRows8, Q8>(p, z, kvh, lds);
+        narrow_body<HD, ROWS == kRows32 ? 2 : 1, F32, SC, F32 && ROWS == kRows8, Q8, false>(p, z, kvh, lds);
     }
 }
 
