@@ -91,6 +91,15 @@ __device__ __forceinline__ int v_slot(int k, int p) {
     return k * (HD * 2) + ((p ^ v_swizzle<HD>(k)) << 4);
 }
 
+// split_f16 of two values: two packed conversions and, between them, a mixed
+// multiply-add each (x - hi is exact in f32)
+__device__ __forceinline__ void split_pair(float x, float y, half2& hi, half2& lo) {
+    float minus = -1.f;
+    __asm__("" : "+s"(minus));  // (known, it would be a conversion and a subtraction)
+    hi = half2{(_Float16)x, (_Float16)y};
+    lo = half2{(_Float16)__builtin_fmaf((float)hi[0], minus, x), (_Float16)__builtin_fmaf((float)hi[1], minus, y)};
+}
+
 // f(0) .. f(N - 1), the indexes as types
 template <typename F, int... I>
 __device__ __forceinline__ void unrolled_(F&& f, std::integer_sequence<int, I...>) {
@@ -819,16 +828,18 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
             const float ms = m[nt] == -INFINITY ? 0.f : m[nt];
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8; i += 2) {
                 e[i] = fast_exp2(s[nt][i] - ms);
+                e[i + 1] = fast_exp2(s[nt][i + 1] - ms);
                 if constexpr (F32) {
-                    _Float16 hi, lo;
-                    split_f16(e[i], hi, lo);
-                    ph[nt][i] = low ? lo : hi;
-                    if constexpr (!PACK) pl[nt][i] = lo;
+                    half2 hi, lo;
+                    split_pair(e[i], e[i + 1], hi, lo);
+                    const half2 own = low ? lo : hi;
+                    ph[nt][i] = own[0], ph[nt][i + 1] = own[1];
+                    if constexpr (!PACK) pl[nt][i] = lo[0], pl[nt][i + 1] = lo[1];
                 } else {
-                    ph[nt][i] = (_Float16)e[i];
-                    e[i] = (float)ph[nt][i];
+                    ph[nt][i] = (_Float16)e[i], ph[nt][i + 1] = (_Float16)e[i + 1];
+                    e[i] = (float)ph[nt][i], e[i + 1] = (float)ph[nt][i + 1];
                 }
             }
             l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
@@ -1152,13 +1163,13 @@ __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPi
             const float ms = m[rt] == -INFINITY ? 0.f : m[rt];
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = fast_exp2(s[rt][i] - ms);
-                _Float16 hi, lo;
-                split_f16(e, hi, lo);
-                ph[i / 8][rt][i % 8] = hi;
-                pl[i / 8][rt][i % 8] = lo;
-                sum += e;
+            for (int i = 0; i < 16; i += 2) {
+                const float e = fast_exp2(s[rt][i] - ms), f = fast_exp2(s[rt][i + 1] - ms);
+                half2 hi, lo;
+                split_pair(e, f, hi, lo);
+                ph[i / 8][rt][i % 8] = hi[0], ph[i / 8][rt][i % 8 + 1] = hi[1];
+                pl[i / 8][rt][i % 8] = lo[0], pl[i / 8][rt][i % 8 + 1] = lo[1];
+                sum = (sum + e) + f;
             }
             l[rt] += sum;
         }
