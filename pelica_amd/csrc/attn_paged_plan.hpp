@@ -30,19 +30,14 @@ PELICA_HD constexpr int wide_rows(int hd) { return hd == 64 ? 256 : 128; }
 // fill the slots better by this model, and on the chip 3% better to 2% worse:
 // two workgroups of a CU share what one of them leaves.)
 constexpr int kWideCost = 3;
-// Where requests share keys, few wide items stand beside many narrow ones, each
-// often alone on its CU, and f32 queries take twice the products: longer pieces end
-// last (64 readers of 16384 keys at a cost of 3, 5, 7, 10: f32 91, 82, 80, 73 us, f16
-// 55, 52, 52, 50; three prompts' 60 requests, f16: 49, 48, 52, 55 and f32 61, 52, 51, 53).
-constexpr int kSharedWideCost = 5;
 constexpr int kMinPiece = 4;
 struct PlanCost {
     // a piece's own time, and what it takes of the whole chip's
-    static PELICA_HD float piece(bool wide, int chunks, int wide_cost = kWideCost) {
-        return (float)(wide ? wide_cost * chunks + 10 : ((chunks + 3) & ~3) + 10);  // (four waves share a narrow one's)
+    static PELICA_HD float piece(bool wide, int chunks) {
+        return (float)(wide ? kWideCost * chunks + 10 : ((chunks + 3) & ~3) + 10);  // (four waves share a narrow one's)
     }
-    static PELICA_HD float share(bool wide, int chunks, bool split, int wide_cost = kWideCost) {
-        return piece(wide, chunks, wide_cost) + (split ? wide ? 20.f : 1.f : 0.f);
+    static PELICA_HD float share(bool wide, int chunks, bool split) {
+        return piece(wide, chunks) + (split ? wide ? 20.f : 1.f : 0.f);
     }
     // the step: the chip's mean, or a slot with `last` to do (its one piece, or
     // the pieces that have to share a slot), which runs faster once its

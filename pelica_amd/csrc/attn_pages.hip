@@ -329,6 +329,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         h.n_joins = min(joins, p.max_joins);
         return h;
     };
+    // Narrow pieces start first, longest first: they wait for memory while the
+    // wide ones beside them keep the matrix cores busy
     auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, x.R <= kNarrowRows, k); };
     // a step that is not split: an item a piece, in order
     if (!p.split) {

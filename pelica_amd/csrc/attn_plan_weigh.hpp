@@ -97,11 +97,11 @@ constexpr int kPlanItems = 4096;  // items whose costs are weighed against each 
 
 constexpr int kBuckets = 128;     // of pieces' costs, four to a doubling, narrow and wide
 
-// Narrow pieces start first, longest first: they wait for memory while the
-// wide ones beside them keep the matrix cores busy
-__device__ __forceinline__ int plan_bucket(int cost, bool narrow, int k) {
+// The place in the launch of a piece of an item's k: of those that go `first`
+// or of the others, longest first
+__device__ __forceinline__ int plan_bucket(int cost, bool first, int k) {
     const int c = min(kBuckets / 2 - 1, max(0, (int)(__float_as_uint((float)cost / (float)k) >> 21) - (127 << 2)));
-    return (narrow ? kBuckets / 2 - 1 : kBuckets - 1) - c;
+    return (first ? kBuckets / 2 - 1 : kBuckets - 1) - c;
 }
 
 struct PlanWeighLds {
@@ -114,8 +114,7 @@ struct PlanWeighLds {
 // item's is negative, kWideCost a chunk, and a multiple.  SHARED: items that
 // are one piece write partials, too.
 template <bool SHARED>
-__device__ __forceinline__ float plan_limit(const int* costs, int n_items, int fill, int max_slots, PlanWeighLds& x,
-                                            int wide_cost = kWideCost) {
+__device__ __forceinline__ float plan_limit(const int* costs, int n_items, int fill, int max_slots, PlanWeighLds& x) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto& est = x.est;
     auto& limit = x.limit;
@@ -134,10 +133,10 @@ __device__ __forceinline__ float plan_limit(const int* costs, int n_items, int f
     for (int i = lane; i < n_items; i += 64) {
         const int c = abs(costs[i]);
         const bool wide = costs[i] < 0;
-        const int chunks = wide ? c / wide_cost : c;
+        const int chunks = wide ? c / kWideCost : c;
         const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-        time += PlanCost::share(wide, m, SHARED || k > 1, wide_cost) * (float)k;
-        longest = fmaxf(longest, PlanCost::piece(wide, m, wide_cost));
+        time += PlanCost::share(wide, m, SHARED || k > 1) * (float)k;
+        longest = fmaxf(longest, PlanCost::piece(wide, m));
         pieces += k;
         slots += k > 1 ? k : 0;
     }
@@ -155,9 +154,9 @@ __device__ __forceinline__ float plan_limit(const int* costs, int n_items, int f
         for (int i = lane; i < n_items; i += 64) {
             const int c = abs(costs[i]);
             const bool wide = costs[i] < 0;
-            const int chunks = wide ? c / wide_cost : c;
+            const int chunks = wide ? c / kWideCost : c;
             const int k = item_pieces(c, chunks, inv), m = k > 1 ? (int)ceilf((float)chunks / (float)k) : chunks;
-            atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m, wide_cost) * scale)], k);
+            atomicAdd(&hist[wave][(int)(PlanCost::piece(wide, m) * scale)], k);
         }
         __builtin_amdgcn_wave_barrier();
         const int have = hist[wave][lane], longer = pieces - wave_scan(have) + have;  // as long as this bucket's

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
         x.lo = e;
         x.kend = x.shared ? ge[owner] : pos0 + token(x.r0 + x.rows - 1) + 1;
         x.n_chunks = (x.kend - x.lo + 31) >> 5;
-        x.cost = x.n_chunks * (x.narrow ? 1 : kSharedWideCost);
+        x.cost = x.n_chunks * (x.narrow ? 1 : kWideCost);
         return x;
     };
     auto owner_of = [&](int i) { return i < n_group_items ? find_last(gitem0, sp.n_groups, i) : find_last(item0, p.n_seq, i); };
@@ -175,10 +175,16 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(SharedP
             costs[i] = x.narrow ? x.cost : -x.cost;
         }
         __syncthreads();
-        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh, kSharedWideCost);
+        inv_limit = plan_limit<true>(costs, n_items, p.fill, p.max_slots, weigh);
     }
 
-    auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, x.narrow, k); };
+    // Wide pieces first, longest first, unlike the plain plan's: a group's are few
+    // and long, about one a CU, and the requests' narrow ones, which come next, wait for
+    // memory beside them.  Narrow ones first fill both slots of every CU, and the wide ones
+    // follow alone (64 readers of 16384 keys 77 -> 57 us, drafts 66 -> 59, 60 requests of
+    // three prompts 47 -> 46; f32, three prompts 51 -> 46).  Wide chunks weighed at 4, 5, 7
+    // instead of 3: 70, 65, 68 us of the 57.
+    auto bucket_of = [&](const Item& x, int k) { return plan_bucket(x.cost, !x.narrow, k); };
     for (int i = tid; i < n_items; i += kPlanThreads) {
         const Item x = item_at(i);
         const int k = item_pieces(x.cost, x.n_chunks, inv_limit);
