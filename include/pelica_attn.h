@@ -450,8 +450,8 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* desc, const PelicaPagedRope* ro
  * largest magnitude and n = x / s to nearest, so a value is kept to s / 2 (1 +
  * 2^-14).  A group that holds an infinity, a NaN or a magnitude above 127 *
  * 65504 reads as NaN, a value above 65468 may read as infinity.
- * Rows of one head that lie side by side ([page][head][row][...]) are read in
- * whole cache lines, scales among them. */
+ * Attention and pages_read take any integers and scales.  Rows of one head that
+ * lie side by side ([page][head][row][...]) are read in whole cache lines, scales among them. */
 typedef struct PelicaPagedQ8 {
     uint16_t* k_scales;   /* device */
     uint16_t* v_scales;
@@ -460,7 +460,9 @@ typedef struct PelicaPagedQ8 {
     int64_t head_stride;  /* 0 = hd / 32 */
 } PelicaPagedQ8;
 
-/* pelica_attn_paged_qkv into 8-bit pages (16-byte aligned, as are their strides). */
+/* pelica_attn_paged_qkv into 8-bit pages (16-byte aligned, as are their strides).
+ * k's norm and turn are in 64 bits up to the integers.  No two rows of a call may have
+ * one slot: integers and scales of both could stay there. */
 int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* desc, const PelicaPagedRope* rope, const PelicaPagedQ8* q8,
                              const float* q, const float* k, const float* v, int64_t token_stride,
                              const float* q_norm, const float* k_norm, float eps, const int64_t* slots, void* q_out,
@@ -495,8 +497,10 @@ int pelica_attn_pages_read(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8,
  * such keys once for the tokens of the whole group: a multiple of 32 of them,
  * at most shared_len and what each request had ahead of its new tokens, through
  * the row of page_table of the group's first request that has tokens.
- * Every token sees what it sees without groups.  No window, prefix_len
- * or alibi. */
+ * Every token sees what it sees without groups.  (A request of
+ * the group that has fewer keys ahead of its tokens bounds them for all: one whose
+ * prompt is still being read stays out until it has them.)  No window, prefix_len
+ * or alibi: layers with a window take a plain plan. */
 typedef struct PelicaPagedShared {
     int32_t n_groups;            /* 1 .. PELICA_ATTN_PAGED_MAX_GROUPS, <= n_seq */
     const int32_t* group_start;  /* device [n_groups + 1] */

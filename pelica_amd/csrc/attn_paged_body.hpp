@@ -270,6 +270,13 @@ struct CacheRows {
 // from memory a chunk or more ahead of their use and writes them into the
 // tile as f16, in CacheRows' order.  (Eight lanes a row, one load a run: whole
 // lines where a head's rows lie side by side.)
+// Bound by HBM over long keys, by issue where keys come from L2 (7 instructions
+// take 4 values apart).  Medians of traced launches (floors: bytes at a copy's 5.04
+// TB/s, or operations at a large f16 product's 1.18 PFLOP/s):
+//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   70.6 us (64)
+//   64 tokens on windows of 128, 64 / 8 of 64               9.1 us (2.2: latency)
+//   one token over 32768, 64 / 8 of 64                     15.4 us (7.1)
+//   512 tokens over 30512, 64 / 8 of 64                     308 - 328 us (215)
 template <int HD>
 struct Q8Rows {
     static constexpr int VB = HD / 8, WORDS = VB / 4;  // bytes, words of a lane

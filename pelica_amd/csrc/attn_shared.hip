@@ -13,7 +13,11 @@
 //
 // One workgroup, latency-bound as the plain plan: groups first (their lengths'
 // minimum by LDS atomics, whose order does not matter), then items, groups'
-// ahead of requests', weighed and cut alike.
+// ahead of requests', weighed and cut alike: 9.6 us for 8 requests, 12.5 for 60 in 3
+// groups (the plain plan's 7 - 8 and what finding the groups takes).
+// A layer of 64 readers of 16384 keys, 64 / 8 heads of 64, f32: 58 us + join 5.8
+// (plain plan 154 + 4.6; the keys' bytes 26, the shared keys' products 25); 60 requests
+// of three prompts, 32 / 4 of 128, f16: 45.5 + 5.0 (56.5 + 4.9; bytes 42).
 #include "attn_paged.hpp"
 #include "attn_plan_weigh.hpp"
 #include "attn_prof.hpp"

@@ -11,7 +11,12 @@ A step of an engine, all of it on the GPU:
         paged_qkv(q, k, v, k_pages, v_pages, step.slots, positions=step.positions, table=rope_table, out=q)
         paged_attention(q, k_pages, v_pages, plan, out=attn, workspace=ws)
 
-Pages are f16 tensors [n_pages, page_size, n_kv, hd], in any layout whose hd
+With 8-bit pages (``new_q8_pages``) the last two take ``k_scales`` and
+``v_scales``, and ``pages_read`` gives rows back as f16 ones.  Requests that begin
+with the same pages are groups of their PagedPlan (``group_start``, ``shared_len``).
+
+Pages are f16 tensors [n_pages, page_size, n_kv, hd] (8-bit ones int8, with f16
+scales [n_pages, page_size, n_kv, hd / 32]), in any layout whose hd
 values are contiguous (a transposed [n_pages, n_kv, page_size, hd], or K and V
 side by side in one buffer); an expanded dim (stride 0) is refused, of token
 rows too.  Every call runs on the current device, on
@@ -469,7 +474,7 @@ def paged_qkv(q, k, v, k_pages, v_pages, slots, *, k_scales=None, v_scales=None,
     each pair, see ``pair_axes``) with the f32 cos/sin ``table`` [rows, rot/2,
     2], k and v rows to f16 rows ``slots`` (int64 [n_tokens]; negative: the row
     is skipped) of the pages; 8-bit pages (int8, with ``k_scales`` and
-    ``v_scales``) take the rows quantised (pelica_attn_paged_qkv_q8).  q: f32 [n_tokens, n_head, hd], k, v: f32
+    ``v_scales``) take the rows quantised (pelica_attn_paged_qkv_q8; no slot twice).  q: f32 [n_tokens, n_head, hd], k, v: f32
     [n_tokens, n_kv, hd], contiguous or views into one buffer of token rows.
     Returns ``out`` (f32, may be q; or f16), by default a new f32 tensor (its
     skipped rows undefined)."""
