@@ -585,6 +585,8 @@ int pelica_attn_pages_read(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, co
         return fail(PELICA_ATTN_EINVAL, "slots, the pages, k_out and v_out must be non-NULL");
     if (misaligned(k_pages) || misaligned(v_pages) || misaligned(k_out) || misaligned(v_out) || misaligned(slots, 8))
         return fail(PELICA_ATTN_EINVAL, "pages, k_out and v_out must be 16-byte aligned, slots 8");
+    if (k_out == v_out || k_out == k_pages || v_out == v_pages || k_out == v_pages || v_out == k_pages)
+        return fail(PELICA_ATTN_EINVAL, "k_out, v_out and the pages must be different arrays");
     const int64_t row = (int64_t)d->n_kv * d->hd;
     if (out_stride && (out_stride < row || out_stride % 8 || out_stride >= 1LL << 31))
         return fail(PELICA_ATTN_EINVAL, "out_stride %lld: 0, or >= n_kv*hd (%lld), < 2^31 and a multiple of 8", (long long)out_stride,

@@ -77,9 +77,10 @@ def test_null_and_misaligned_arguments():
                      (dict(out=A, half=1, q=A), "q_out"), (dict(eps=-1.0), "eps")):
         _error(lib.pelica_attn_paged_qkv_q8(*{**qkv, **kw}.values()), attn.EINVAL, word)
     _error(lib.pelica_attn_paged_qkv_q8(*{**qkv, "d": _desc(hd=96)}.values()), attn.EUNSUPPORTED, "hd")
-    read = dict(d=d, x=x, slots=A, kp=A, vp=A, ko=A, vo=A, so=0, st=None)
+    read = dict(d=d, x=x, slots=A, kp=A, vp=A, ko=2 * A, vo=3 * A, so=0, st=None)
     for kw, word in ((dict(d=None), "desc"), (dict(slots=None), "NULL"), (dict(kp=None), "NULL"), (dict(vp=None), "NULL"),
                      (dict(ko=None), "NULL"), (dict(vo=None), "NULL"), (dict(kp=A + 8), "aligned"), (dict(ko=A + 8), "aligned"),
+                     (dict(ko=3 * A), "different"), (dict(vo=A), "different"), (dict(ko=A), "different"),
                      (dict(slots=A + 4), "aligned"), (dict(so=127), "out_stride"), (dict(so=132), "out_stride"),
                      (dict(so=-128), "out_stride"), (dict(so=1 << 31), "out_stride")):
         for form in (x, None):  # 8-bit and f16 pages
