@@ -264,6 +264,25 @@ def test_write_and_read_in_a_graph():
             assert (got.cpu().double() != y).float().mean() < 1e-2
 
 
+@pytest.mark.parametrize("neox", [True, False])
+def test_a_position_outside_the_table_gives_nan(neox):
+    """k's groups that turn read as NaN, the others and the other rows as they are."""
+    T, n_kv, hd, rot = 6, 2, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = [torch.randn(T, h, hd, generator=g, device="cuda") for h in (4, n_kv, n_kv)]
+    pools = paged.new_q8_pages(2, 8, n_kv, hd)
+    sc = dict(k_scales=pools[2], v_scales=pools[3])
+    table = torch.from_numpy(orc.rope_table(100, rot)).cuda()
+    pos = torch.tensor([0, 99, 100, -1, 5, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    slots = torch.arange(T, device="cuda")
+    paged.paged_qkv(*x, *pools[:2], slots, **sc, positions=pos, table=table, neox=neox)
+    k, v = paged.pages_read(*pools[:2], slots, **sc)
+    torch.cuda.synchronize()
+    bad = torch.tensor([False, False, True, True, False, True])
+    assert k.cpu()[bad][..., :rot].isnan().all() and k.cpu()[bad][..., rot:].isfinite().all()
+    assert k.cpu()[~bad].isfinite().all() and v.isfinite().all()
+
+
 def test_refusals():
     k, v, ks, vs = paged.new_q8_pages(4, 16, 2, 64)
     slots = torch.arange(5, device="cuda")
