@@ -1008,7 +1008,9 @@ __device__ __forceinline__ void store_wide(const PagedParams& p, const PlanPiece
 // ahead, but scores, softmax and PV follow one another, where the f16 item's
 // overlap (a prompt's queries may be had in f16 from the step before).  2000
 // tokens of 32 / 4 heads of 128: a whole call 110 us, f16 69; the products, twice
-// f16's, at a large product's rate 56.
+// f16's, at a large product's rate 56.  (A pipeline over chunks has no registers left
+// at head dim 64: 512 tokens over 30512 keys 657 us instead of 634; at 128 it is alike:
+// the two waves of a SIMD overlap by themselves.)
 template <int HD, bool SC, bool Q8>
 __device__ __forceinline__ void wide_f32_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     using S = WideShape<HD>;
