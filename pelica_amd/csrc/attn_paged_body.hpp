@@ -571,8 +571,8 @@ __device__ __forceinline__ float ror8(float x) {  // lane l's from lane l ^ 8
 // tiles, 2 until they land, 1.3 for the chunks, 2.4 for merge and store.  With
 // 32-row tiles, every tile requested and two merge barriers they were 11.4;
 // with a pack of 8 rows in a tile of 16, a 32768-key token went from 17.5 to 16.
-// WIDE: beside wide items, whose last small block begins at a row of its own.
-template <int HD, int NT, bool F32, bool SC, bool PACK, bool Q8, bool WIDE>
+// SHARED: the item may be a group's last block, which begins at a row of its own.
+template <int HD, int NT, bool F32, bool SC, bool PACK, bool Q8, bool SHARED>
 __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiece& z, int kvh, char* lds) {
     static_assert(!PACK || (F32 && NT == 1), "packed hi and lo parts: f32, one tile");
     using S_ = NarrowShape<HD, NT, Q8>;
@@ -580,7 +580,7 @@ __device__ __forceinline__ void narrow_body(const PagedParams& p, const PlanPiec
     constexpr int KS = S_::KS, DT = S_::DT, NB = S_::NB, TILE = S_::TILE, NR = S_::NR, WI = S_::WI;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, c16 = lane & 15;
-    const int r0 = WIDE ? z.r0 : 0;
+    const int r0 = SHARED ? z.r0 : 0;
     char* const kbuf = lds + wave * S_::WAVE;
     char* const vbuf = kbuf + NB * TILE;
     Rows rows(p, z, kvh, lane);
@@ -1648,12 +1648,22 @@ __device__ __forceinline__ void wide_body(const PagedParams& p, const PlanPiece&
     store_wide<HD, false>(p, z, kvh, wave, lane, any_bad, m, l, o, lds);
 }
 
-// Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more.
-enum RowLimit { kRows8, kRows16, kRows32, kRowsWide };
+// Rows of the step's largest item: at most 8, 16 or 32 (narrow), or more; or more
+// and, of a plan of shared keys, a group's last block among them.
+enum RowLimit { kRows8, kRows16, kRows32, kRowsWide, kRowsShared };
+// Whether plain plans' wide steps have a kernel of their own.  Narrow items that
+// begin at a row of their own, a group's last blocks, cost the wide items beside them
+// registers where those are fewest: f16 pages, head dim 64, capped, 512 tokens over 30512
+// keys 412 us in one kernel for both plans (53 scalar spills more), 371 apart, a prompt of
+// 4001 252 and 219, uncapped alike.  Apart, the others gain nothing or lose by
+// the order that their instructions happen to fall into: a capped prompt of head dim 128 181
+// and 188, a capped f32 chunk over 8-bit pages of 64 768 and 793.
+template <int HD, bool Q8>
+constexpr bool kPlainWide = HD == 64 && !Q8;
 
 template <int HD, bool F32, int MODE, int ROWS, bool Q8>
 __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedParams p) {
-    constexpr bool WIDE = ROWS == kRowsWide, SC = MODE != kPlain;
+    constexpr bool SHARED = ROWS == kRowsShared, WIDE = ROWS == kRowsWide || SHARED, SC = MODE != kPlain;
     constexpr int LN = NarrowShape<HD, ROWS >= kRows32 ? 2 : 1, Q8>::LDS, LW = WIDE ? WideShape<HD>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char lds[LN > LW ? LN : LW];
     const int id = blockIdx.x / p.n_kv, kvh = blockIdx.x % p.n_kv;
@@ -1666,13 +1676,13 @@ __global__ __launch_bounds__(64 * kNW) __attribute__((amdgpu_waves_per_eu(2, 2))
                      "s"(p.qscale), "s"(z.rows));
     if (sig != p.sig || id >= n_pieces) return;
     if constexpr (WIDE) {
-        if (z.R > kNarrowRows && !z.narrow) {
+        if (z.R > kNarrowRows && !(SHARED && z.narrow)) {
             if constexpr (F32) wide_f32_body<HD, SC, Q8>(p, z, kvh, lds);
             else wide_body<HD, MODE, Q8>(p, z, kvh, lds);
-        } else if (z.R - z.r0 > 16) {
-            narrow_body<HD, 2, F32, SC, false, Q8, true>(p, z, kvh, lds);
+        } else if (z.R - (SHARED ? z.r0 : 0) > 16) {
+            narrow_body<HD, 2, F32, SC, false, Q8, SHARED>(p, z, kvh, lds);
         } else {
-            narrow_body<HD, 1, F32, SC, false, Q8, true>(p, z, kvh, lds);
+            narrow_body<HD, 1, F32, SC, false, Q8, SHARED>(p, z, kvh, lds);
         }
     } else {
         narrow_body<HD, ROWS == kRows32 ? 2 : 1, F32, SC, F32 && ROWS == kRows8, Q8, false>(p, z, kvh, lds);
@@ -1697,15 +1707,22 @@ hipError_t launch_paged_as(const PagedParams& p, hipStream_t st) {
         auto go = [&](auto s, auto rows) {
             hipLaunchKernelGGL((paged_kernel<HD, F32, decltype(s)::value, decltype(rows)::value, Q8>), grid, dim3(64 * kNW), 0, st, p);
         };
+        auto wide = [&](auto s) {
+            // (no distance bias over shared keys; capped f32 scores take its path)
+            constexpr bool both = decltype(s)::value != kBiased || F32;
+            if constexpr (!kPlainWide<HD, Q8>) go(s, std::integral_constant<int, kRowsShared>{});
+            else if (both && p.shared_joins) go(s, std::integral_constant<int, both ? kRowsShared : kRowsWide>{});
+            else go(s, std::integral_constant<int, kRowsWide>{});
+        };
         auto by_rows = [&](auto s) {
             // (f16 queries have no parts to pack)
-            if (p.wide) go(s, std::integral_constant<int, kRowsWide>{});
+            if (p.wide) wide(s);
             else if (p.rows > 16) go(s, std::integral_constant<int, kRows32>{});
             else if (p.rows > 8 || !F32) go(s, std::integral_constant<int, kRows16>{});
             else go(s, std::integral_constant<int, F32 ? kRows8 : kRows16>{});
         };
         // (all but the wide items of f16 queries take either score by one path)
-        if (p.cap > 0.f && !p.alibi && p.wide) go(std::integral_constant<int, F32 ? kBiased : kCapped>{}, std::integral_constant<int, kRowsWide>{});
+        if (p.cap > 0.f && !p.alibi && p.wide) wide(std::integral_constant<int, F32 ? kBiased : kCapped>{});
         else if (p.cap > 0.f || p.alibi) by_rows(std::integral_constant<int, kBiased>{});
         else by_rows(std::integral_constant<int, kPlain>{});
         return hipGetLastError();
