@@ -447,9 +447,10 @@ int pelica_attn_paged_qkv(const PelicaPagedDesc* desc, const PelicaPagedRope* ro
  * nearest).  Head h's hd / 32 scales of row r of page p start at p *
  * page_stride + r * row_stride + h * head_stride, the same for K's and V's.
  * The qkv step takes the smallest f16 number s with 127 s >= the group's
- * largest magnitude and n = x / s to nearest, so a value is kept to s / 2 (1 +
- * 2^-14).  A group that holds an infinity, a NaN or a magnitude above 127 *
- * 65504 reads as NaN, a value above 65468 may read as infinity.
+ * largest magnitude and n = x / s to nearest, so a value is off by s / 2 and half
+ * an f16 step of n s at most: 0.563 s (and 2^-25).  A group that holds an infinity, a NaN or
+ * a magnitude above 127 * 65504 reads as NaN.  n s of 65520 or more reads as an infinity:
+ * only in groups with a magnitude above 65468 (there, of values from 65520 - s / 2 on).
  * Attention and pages_read take any integers and scales.  Rows of one head that
  * lie side by side ([page][head][row][...]) are read in whole cache lines, scales among them. */
 typedef struct PelicaPagedQ8 {
