@@ -480,7 +480,10 @@ int pelica_attn_paged_q8(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8, c
  * k_out and v_out [n_kv][hd] at i * out_stride values (0 = n_kv * hd), from 8-bit pages,
  * or f16 ones (q8 NULL): what attention reads, for the calls over dense
  * rows and for requests that leave the pool.  Rows whose slot is negative or
- * past the pool are left as they were.  k_out, v_out and the pages are apart.  Of the descriptor: n_head and n_kv
+ * past the pool are left as they were.  k_out and v_out may share no byte with each
+ * other, the pages, the scales or slots: K's and V's rows may take turns in one
+ * buffer, all rows of one may lie between two pages; else another array that begins or
+ * ends among an output's rows is refused.  Of the descriptor: n_head and n_kv
  * (alike will do), hd (64, 128, 256), n_tokens, page_size, n_pages and the strides of pages. */
 int pelica_attn_pages_read(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8, const int64_t* slots,
                            const void* k_pages, const void* v_pages, uint16_t* k_out, uint16_t* v_out,

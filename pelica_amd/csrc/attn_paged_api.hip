@@ -91,6 +91,28 @@ int check_pool(const PelicaPagedDesc* d, int piece) {
     return PELICA_ATTN_OK;
 }
 
+// `n` pieces of `bytes` each, the first at `at`, `step` bytes between their beginnings
+struct Pieces {
+    const char* name;
+    const void* at;
+    int64_t n, step, bytes;
+};
+// Whether rows of an output may share a byte with another array: not where the one's
+// ends lie ahead of the other or behind it, where both have one step and their pieces
+// take turns (K's and V's rows in one buffer), or where all rows lie between two pieces.
+bool may_overlap(const Pieces& rows, const Pieces& y) {
+    typedef __int128 wide;
+    const wide p = reinterpret_cast<uintptr_t>(rows.at), q = reinterpret_cast<uintptr_t>(y.at);
+    const wide p_end = p + (wide)(rows.n - 1) * rows.step + rows.bytes, q_end = q + (wide)(y.n - 1) * y.step + y.bytes;
+    if (p >= q_end || q >= p_end) return false;
+    if (rows.step == y.step) {
+        const wide d = ((p - q) % y.step + y.step) % y.step;  // from a piece to the row after it
+        return d < y.bytes || y.step - d < rows.bytes;
+    }
+    const wide d = (p - q) % y.step;
+    return p < q || d < y.bytes || d + (p_end - p) > y.step;
+}
+
 int64_t scale_row(const PelicaPagedDesc* d, const PelicaPagedQ8* x) {
     return x->row_stride ? x->row_stride : (int64_t)d->n_kv * (d->hd / pelica::kQ8Group);
 }
@@ -592,8 +614,26 @@ int pelica_attn_pages_read(const PelicaPagedDesc* d, const PelicaPagedQ8* q8, co
         return fail(PELICA_ATTN_EINVAL, "out_stride %lld: 0, or >= n_kv*hd (%lld), < 2^31 and a multiple of 8", (long long)out_stride,
                     (long long)row);
     if (d->n_tokens * row > 1LL << 33) return fail(PELICA_ATTN_EUNSUPPORTED, "more than 2^33 values");
-    pelica::PagesReadParams p{};
+    // (other workgroups read while one writes)
     const int size = q8 ? 1 : 2;
+    const int64_t step = 2 * (out_stride ? out_stride : row);
+    const int64_t page_bytes = size * ((d->page_size - 1) * row_stride(d) + (d->n_kv - 1) * head_stride(d) + d->hd);
+    const Pieces k_rows{"k_out", k_out, d->n_tokens, step, 2 * row}, v_rows{"v_out", v_out, d->n_tokens, step, 2 * row};
+    Pieces others[6] = {v_rows, {"slots", slots, 1, 8LL * d->n_tokens, 8LL * d->n_tokens},
+                        {"k_pages", k_pages, d->n_pages, page_stride(d) * size, page_bytes},
+                        {"v_pages", v_pages, d->n_pages, page_stride(d) * size, page_bytes}};
+    int n_others = 4;
+    if (q8) {
+        const pelica::Q8Strides sc = scale_strides(d, q8);
+        const int64_t bytes = 2 * ((d->page_size - 1) * sc.row + (d->n_kv - 1) * sc.head + d->hd / pelica::kQ8Group);
+        others[n_others++] = {"k_scales", q8->k_scales, d->n_pages, 2 * sc.page, bytes};
+        others[n_others++] = {"v_scales", q8->v_scales, d->n_pages, 2 * sc.page, bytes};
+    }
+    for (int i = 0; i < n_others; ++i) {
+        if (may_overlap(k_rows, others[i])) return fail(PELICA_ATTN_EINVAL, "pages_read: k_out overlaps %s", others[i].name);
+        if (i > 0 && may_overlap(v_rows, others[i])) return fail(PELICA_ATTN_EINVAL, "pages_read: v_out overlaps %s", others[i].name);
+    }
+    pelica::PagesReadParams p{};
     p.slots = slots;
     p.k = static_cast<const char*>(k_pages);
     p.v = static_cast<const char*>(v_pages);
