@@ -462,7 +462,8 @@ typedef struct PelicaPagedQ8 {
 } PelicaPagedQ8;
 
 /* pelica_attn_paged_qkv into 8-bit pages (16-byte aligned, as are their strides).
- * k's norm and turn are in 64 bits up to the integers.  No two rows of a call may have
+ * k's norm and turn are in 64 bits up to the integers, from (cos, sin) in f32: the table's,
+ * or, of a two-level table, its two rows' product, as for q.  No two rows of a call may have
  * one slot: integers and scales of both could stay there. */
 int pelica_attn_paged_qkv_q8(const PelicaPagedDesc* desc, const PelicaPagedRope* rope, const PelicaPagedQ8* q8,
                              const float* q, const float* k, const float* v, int64_t token_stride,
@@ -504,7 +505,14 @@ int pelica_attn_pages_read(const PelicaPagedDesc* desc, const PelicaPagedQ8* q8,
  * Every token sees what it sees without groups.  (A request of
  * the group that has fewer keys ahead of its tokens bounds them for all: one whose
  * prompt is still being read stays out until it has them.)  No window, prefix_len
- * or alibi: layers with a window take a plain plan. */
+ * or alibi: layers with a window take a plain plan.
+ *
+ * When to tell groups: every group is walked as told, whether that is less time or not.  It
+ * is for single tokens and drafts from about 4000 shared keys on, or 32 requests and 1000
+ * (64 requests and 16000: 0.2 - 0.4 of the plain plan's time).  Fewer pay for
+ * the partials, up to 4 us a layer, and the plan takes 2 - 4 us more.  A request with hundreds of new
+ * tokens fills the matrix cores by itself: in a group its layer is
+ * a fifth slower. */
 typedef struct PelicaPagedShared {
     int32_t n_groups;            /* 1 .. PELICA_ATTN_PAGED_MAX_GROUPS, <= n_seq */
     const int32_t* group_start;  /* device [n_groups + 1] */
@@ -515,7 +523,9 @@ typedef struct PelicaPagedShared {
  * and out where half != 0, else f32; 8-bit pages with q8, else f16 ones) for
  * such requests.  A plan serves calls with the same n_groups; its group_start
  * and shared_len are read when it is made.  A group_start or q_start that decreases
- * gives an empty plan. */
+ * gives an empty plan.  The workspace holds two f32 partials of hd + 2 values for every one of n_tokens *
+ * n_head rows, in groups or not, beside a plain plan's: 64 tokens of 64 heads of 64 take 71
+ * MB, 4160 take 210, 32768 take 1.2 GB. */
 size_t pelica_attn_paged_shared_plan_bytes(const PelicaPagedDesc* desc, const PelicaPagedShared* shared);
 int pelica_attn_paged_shared_plan(const PelicaPagedDesc* desc, const PelicaPagedShared* shared, void* plan,
                                   size_t plan_bytes, void* stream);

@@ -30,14 +30,14 @@
 //
 // Measured, medians of warm traced launches (floors: bytes at a copy's 5.13 TB/s,
 // or operations at a large f16 product's 1.17 PFLOP/s):
-//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   116 us (118)
-//   16 tokens with a bias over 300 - 6000, 16 / 16 of 128   96 us (99)
-//   one token over 32768, 64 / 8 of 64                      16 us + join 3.9 (13)
-//   64 tokens on windows of 128, 64 / 8 of 64              8.6 us (3.7: latency)
-//   512 tokens over 30512, 64 / 8 of 64                    291 us + join 7.9 (217)
-//   4001 tokens, 32 / 4 of 128                             165 us + join 4.8 (112)
-//   3 chunks of 700 and 28 drafts, 64 / 8 of 64            208 us + join 12.6 (111)
-//   2000 tokens, capped, 600 of prefix, 32 / 4 of 128       73 us + join 7.0 (30.5)
+//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   115 us (118)
+//   16 tokens with a bias over 300 - 6000, 16 / 16 of 128   95 us (99)
+//   one token over 32768, 64 / 8 of 64                      16 - 19 us by card + join 3.9 (13)
+//   64 tokens on windows of 128, 64 / 8 of 64              8.6 - 8.9 us (3.7: latency)
+//   512 tokens over 30512, 64 / 8 of 64                    266 - 300 us by card + join 7.9 (217)
+//   4001 tokens, 32 / 4 of 128                             156 us + join 4.6 (112)
+//   3 chunks of 700 and 28 drafts, 64 / 8 of 64            205 us + join 12.6 (111)
+//   2000 tokens, capped, 600 of prefix, 32 / 4 of 128       69 us + join 6.8 (30.5)
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -273,10 +273,12 @@ struct CacheRows {
 // Bound by HBM over long keys, by issue where keys come from L2 (7 instructions
 // take 4 values apart).  Medians of traced launches (floors: bytes at a copy's 5.04
 // TB/s, or operations at a large f16 product's 1.18 PFLOP/s):
-//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   70.6 us (64)
+//   32 tokens over 512 - 16384 keys, 32 / 4 heads of 128   67.4 us (64)
 //   64 tokens on windows of 128, 64 / 8 of 64               9.1 us (2.2: latency)
-//   one token over 32768, 64 / 8 of 64                     15.4 us (7.1)
-//   512 tokens over 30512, 64 / 8 of 64                     308 - 328 us (215)
+//   one token over 32768, 64 / 8 of 64                     15.2 us (7.1)
+//   512 tokens over 30512, 64 / 8 of 64                     301 - 340 us by card (215)
+// The wide items of f16 queries spill 34 - 60 vector registers at head dim 64: the
+// same chunk capped takes 442 us (374 over f16 pages), with a distance bias 671 (512).
 template <int HD>
 struct Q8Rows {
     static constexpr int VB = HD / 8, WORDS = VB / 4;  // bytes, words of a lane

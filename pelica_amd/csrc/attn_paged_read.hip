@@ -3,8 +3,11 @@
 //
 // A lane takes 8 values of a head, of K and of V: 8 bytes and a scale in, 16
 // bytes out, each a whole line with its neighbours.  HBM-bound: 30000 rows of 4
-// heads of 128 16.7 us, 5.6 TB/s (a copy's 5.04); 333 rows of 8 heads of 64 2.8 us,
-// a launch and two round trips (slot, row).
+// heads of 128 from twelve pools in turn (94 MB a call, 1.1 GB in all: more than
+// the caches hold) 22.7 us, 4.2 TB/s with start and end (a copy as large, as cold: 4.8);
+// 300000 rows 179 us, 5.3 TB/s (a 1 GiB copy's 5.04); one pool again and again, which
+// the 256 MB cache keeps, 16.5 us.  f16 pages 26.9, 236, 19.6 us.  333 rows of 8 heads of 64
+// 2.8 us, a launch and two round trips (slot, row).
 #include "attn_paged.hpp"
 #include "attn_prof.hpp"
 #include "attn_q8.hpp"

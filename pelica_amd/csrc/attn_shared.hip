@@ -17,7 +17,10 @@
 // groups (the plain plan's 7 - 8 and what finding the groups takes).
 // A layer of 64 readers of 16384 keys, 64 / 8 heads of 64, f32: 58 us + join 5.8
 // (plain plan 154 + 4.6; the keys' bytes 26, the shared keys' products 25); 60 requests
-// of three prompts, 32 / 4 of 128, f16: 45.5 + 5.0 (56.5 + 4.9; bytes 42).
+// of three prompts, 32 / 4 of 128, f16: 45.5 + 5.0 (56.5 + 4.9; bytes 42).  Few readers gain
+// nothing, 8 of 2000 keys 11.4 + 3.8 (11.4 + 4.0), and lose below: 8 of 250 keys 12 us a
+// layer with the join (10).  Prompts' chunks lose: three of 700 tokens among 16 requests behind
+// 13000 keys 833 + 19 (676 + 7).  Every group is walked as it is told.
 #include "attn_paged.hpp"
 #include "attn_plan_weigh.hpp"
 #include "attn_prof.hpp"

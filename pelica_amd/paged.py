@@ -271,7 +271,9 @@ class PagedPlan:
     together): requests ``group_start[g]`` .. ``group_start[g + 1]`` share their
     first ``shared_len[g]`` keys, which lie in the same pages (PelicaPagedShared):
     the plan walks those once for the whole group (no ``window``, ``prefix_len``
-    or alibi)."""
+    or alibi).  Worth it for single tokens and drafts from about 4000 shared keys on,
+    or 32 requests and 1000; not for few short ones, or prompts' chunks.  Its
+    ``workspace_bytes`` grow with ``n_tokens``."""
 
     _shared = None
 
